@@ -117,8 +117,8 @@ def _encode(m, signed):
     top = 127 if signed else 255
     big = m.abs().amax(1, keepdim=True)
     whole = torch.full_like(big, float(top * top))
-    ok = big >= 2.0 ** -110
-    inv = torch.where(ok, whole / torch.where(ok, big, torch.ones_like(big)), torch.zeros_like(big))
+    tiny = big < 2.0 ** -110  # held as zeros
+    inv = torch.where(tiny, torch.zeros_like(big), whole / torch.where(tiny, torch.ones_like(big), big))
     y = m.abs() * inv
     c = torch.round(torch.sqrt(y))  # the nearest code, settled by comparisons that are exact in 32 bits
     c = c + (y >= c * c + c + 0.25)
@@ -127,8 +127,8 @@ def _encode(m, signed):
     if signed:
         c = torch.where(m < 0, -c, c).to(torch.int8)
     else:
-        c = torch.where((m > 0) & ok, c.clamp(min=1), c).to(torch.uint8)
-    return c, torch.where(ok, big, torch.zeros_like(big)) / whole
+        c = torch.where((m > 0) & ~tiny, c.clamp(min=1), c).to(torch.uint8)
+    return c, torch.where(tiny, torch.zeros_like(big), big) / whole
 
 
 def _decode(c, scale):
@@ -174,6 +174,8 @@ def prepare(case, seed):
             flat["c"] = flat["p"].to(torch.bfloat16)
         part = {k: [t[a // BLOCK:-(-(a + n) // BLOCK)] if k in ("ms", "vs") else t[a:a + n] for a, n in zip(starts, sizes)]
                 for k, t in flat.items()}
+        if case["bits"] == 8:  # a moment: its codes and their scales
+            part["m"], part["v"] = list(zip(part["m"], part["ms"])), list(zip(part["v"], part["vs"]))
         s["tensors"] = part
     s["case"] = dict(case)
     return s
@@ -294,15 +296,10 @@ def _own_adamw(s, c):
     import flash_maxsim_amd as fm
 
     f, t = s["flat"], s["tensors"]
-    eight = c["bits"] == 8
-    m = [fm.AdamW8bitState(a, b) for a, b in zip(t["m"], t["ms"])] if eight else t["m"]
-    v = [fm.AdamW8bitState(a, b) for a, b in zip(t["v"], t["vs"])] if eight else t["v"]
-    fm.adamw_step(t["p"], t["g"], m, v, s["step"], lr=LR, betas=(BETA1, BETA2), eps=EPS, weight_decay=DECAY,
+    fm.adamw_step(t["p"], t["g"], t["m"], t["v"], s["step"], lr=LR, betas=(BETA1, BETA2), eps=EPS, weight_decay=DECAY,
                   grad_scale=s["scale"], copies=t.get("c"))
-    if eight:
-        r = fm.AdamW8bitState(f["v"], f["vs"])
-        return {"p": f["p"], "m": fm.dequantize_adamw(fm.AdamW8bitState(f["m"], f["ms"])),
-                "v": fm.dequantize_adamw(r)}
+    if c["bits"] == 8:
+        return {"p": f["p"], "m": fm.dequantize_adamw((f["m"], f["ms"])), "v": fm.dequantize_adamw((f["v"], f["vs"]))}
     return {k: f[k] for k in ("p", "m", "v", "c") if k in f}
 
 

@@ -10,7 +10,8 @@ quantize_int8_packed, flash_maxsim_packed, flash_maxsim_int8_packed) and
 top-k retrieval on the GPU (topk_scores, flash_maxsim_topk,
 flash_maxsim_batched_topk, flash_maxsim_int8_topk), and training with doc
 lengths (flash_maxsim_train's doc_lengths) or several queries
-(flash_maxsim_train_batched).
+(flash_maxsim_train_batched). The layers that such training moves: layer norm
+(layer_norm) and AdamW with moments in 32 or 8 bits (AdamW, adamw_step).
 """
 
 __version__ = "0.1.0"
@@ -22,6 +23,8 @@ from .flash_maxsim_sparse import flash_maxsim_sparse, maxsim_sparse_naive
 from .flash_maxsim_packed import (PackedDocs, PackedInt8Docs, flash_maxsim_int8_packed, flash_maxsim_packed,
                                   pack_docs, quantize_int8_packed)
 from .flash_maxsim_topk import flash_maxsim_batched_topk, flash_maxsim_int8_topk, flash_maxsim_topk, topk_scores
+from .flash_maxsim_norm import layer_norm
+from .flash_maxsim_optim import AdamW, AdamW8bitState, adamw_state, adamw_step, dequantize_adamw
 
 __all__ = [
     "flash_maxsim",
@@ -44,4 +47,10 @@ __all__ = [
     "flash_maxsim_batched_topk",
     "flash_maxsim_int8_topk",
     "flash_maxsim_train_batched",
+    "layer_norm",
+    "AdamW",
+    "AdamW8bitState",
+    "adamw_state",
+    "adamw_step",
+    "dequantize_adamw",
 ]

@@ -22,6 +22,7 @@ _i64 = ctypes.c_int64
 _ptr = ctypes.c_void_p
 _int = ctypes.c_int
 _size = ctypes.c_size_t
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes)
 _SIGNATURES = {
@@ -94,6 +95,20 @@ _SIGNATURES = {
     ),
     "fmx_convert_rows": (_int, [_int, _ptr, _i64, _i64, _i64, _i64, _i64, _ptr, _int, _ptr, _i64, _ptr]),
     "fmx_bwd_batched_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64]),
+    "fmx_layer_norm": (
+        _int,
+        [_int, _ptr, _i64, _int, _ptr, _ptr, _i64, _i64, _f64, _ptr, _ptr, _ptr, _ptr],
+    ),
+    "fmx_layer_norm_bwd": (
+        _int,
+        [_int, _ptr, _i64, _ptr, _i64, _int, _ptr, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _size, _ptr],
+    ),
+    "fmx_layer_norm_bwd_workspace_bytes": (_size, [_i64, _i64]),
+    "fmx_adamw": (
+        _int,
+        [_int, _int, _int, _int, _ptr, _i64, _i64, _f64, _f64, _f64, _f64, _f64, _ptr, _ptr],
+    ),
+    "fmx_adamw_decode": (_int, [_int, _ptr, _ptr, _i64, _ptr, _ptr]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -1,0 +1,293 @@
+// AdamW (decoupled weight decay) over many tensors in one launch, with the two
+// moments held in float32 or in 8 bits.
+//
+//   g = grad * grad_scale
+//   m = beta1 m + (1 - beta1) g          v = beta2 v + (1 - beta2) g^2
+//   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+//
+// Every product and sum is rounded to float32 by itself (no contraction into
+// fma), so a new 8-bit code never depends on how the compiler fused the
+// formula; the root is the device library's sqrtf. The parameter is rounded to
+// its own type once, at the end.
+//
+// 8-bit moments: blocks of 256 elements of one tensor share a float32 scale q.
+// The first moment is c |c| q with c an int8 code, q = max |m| / 127^2; of the
+// second the root is held, c^2 q with c a uint8 code, q = max sqrt(v) / 255^2:
+// a quadratic grid, whose steps are 1.6 % (0.8 %) of the largest value at the
+// top and shrink towards zero, where most values of a block lie. A code is the
+// number of grid midpoints (c - 1/2)^2 at or below |m| / q: y = |m| (127^2 / max)
+// is compared with c^2 + c + 1/4, which float32 holds exactly. A root that is
+// not zero keeps at least code 1, so no element's step grows because its second
+// moment was rounded to nothing. A block with a value that is not finite
+// decodes to NaN.
+//
+// Bound by HBM: 28 bytes a parameter in float32, 10 with bf16 parameters and
+// 8-bit moments, against about 40 (80) vector operations.
+#include "fmx_device.h"
+#include "fmx_layers.h"
+
+#include "../../include/fmx.h"
+
+#pragma clang fp contract(off)
+
+namespace fmx {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kElems = 8;                         // per lane: 32 lanes hold a block of 256
+constexpr int kChunk = kThreads * kElems;         // elements a workgroup takes
+constexpr int kMaxTensors = 48;                   // of one launch: the table travels in the kernel's arguments
+constexpr float kTinyBlock = 0x1p-110f;           // a block below this is held as zeros (127^2 / it overflows soon after)
+
+struct Table {
+  AdamWTensor t[kMaxTensors];
+  int32_t first[kMaxTensors + 1];                 // first workgroup of each tensor
+  int32_t vec[kMaxTensors];                       // all of its arrays allow 16-byte (codes: 8-byte) accesses
+  int32_t count;
+};
+static_assert(sizeof(Table) + sizeof(AdamWScalars) <= 4096, "kernel arguments");
+
+template <typename T, int V>
+struct __attribute__((aligned(sizeof(T) * V >= 16 ? 16 : sizeof(T) * V))) Pack {
+  T v[V];
+};
+
+// Elements i0 .. i0 + 7 of an array of n; those at or past n read as zero and are not written.
+template <typename T, typename F>
+__device__ __forceinline__ void load8(const T* p, int64_t i0, int64_t n, bool whole, F&& put) {
+  if (whole) {
+    const Pack<T, kElems> x = *reinterpret_cast<const Pack<T, kElems>*>(p + i0);
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) put(i, x.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) put(i, i0 + i < n ? p[i0 + i] : T(0));
+  }
+}
+template <typename T, typename F>
+__device__ __forceinline__ void store8(T* p, int64_t i0, int64_t n, bool whole, F&& get) {
+  if (whole) {
+    Pack<T, kElems> x;
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) x.v[i] = get(i);
+    *reinterpret_cast<Pack<T, kElems>*>(p + i0) = x;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kElems; ++i)
+      if (i0 + i < n) p[i0 + i] = get(i);
+  }
+}
+
+// Largest value over the 32 lanes of each half of the wave, NaN if any is.
+__device__ __forceinline__ float half_max(float v) {
+  v = vmax(v, dpp_mov<0xB1>(v));
+  v = vmax(v, dpp_mov<0x4E>(v));
+  v = vmax(v, dpp_mov<0x141>(v));
+  v = vmax(v, dpp_mov<0x140>(v));
+  float lo, hi;
+  halves16(v, lo, hi);
+  return vmax(lo, hi);
+}
+
+// The code of y = |value| top^2 / max: see above. v_sqrt_f32 is within an ulp of
+// the root, so its nearest integer is off by one at most, next to a midpoint.
+__device__ __forceinline__ float code_of(float y, float top) {
+  float c = rintf(__builtin_amdgcn_sqrtf(y));
+  const float up = c * c + c + 0.25f;
+  const float dn = c * c - c + 0.25f;
+  c = y >= up ? c + 1.0f : (y < dn && c > 0.0f) ? c - 1.0f : c;
+  return c <= top ? c : y == y ? top : 0.0f;  // not a number: any code, its block's scale is NaN
+}
+
+template <typename P, typename G, typename C, int BITS>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(Table tab, AdamWScalars sc) {
+  // the tensor whose workgroups include this one
+  int lo = 0, hi = tab.count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if ((int)blockIdx.x >= tab.first[mid])
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const AdamWTensor t = tab.t[lo];
+  const int64_t i0 = (int64_t)((int)blockIdx.x - tab.first[lo]) * kChunk + threadIdx.x * kElems;
+  const int64_t n = t.n;
+  if (BITS == 32 && i0 >= n) return;
+  const bool whole = tab.vec[lo] && i0 + kElems <= n;
+  const float scale = sc.grad_scale ? *sc.grad_scale : 1.0f;
+
+  float p[kElems], g[kElems], m[kElems], r[kElems];
+  load8(static_cast<const P*>(t.param), i0, n, whole, [&](int i, P x) { p[i] = (float)x; });
+  load8(static_cast<const G*>(t.grad), i0, n, whole, [&](int i, G x) { g[i] = (float)x; });
+  const int64_t block = i0 / 256;
+  if constexpr (BITS == 8) {
+    const bool in = i0 < n;
+    const float qm = in ? t.ms[block] : 0.0f, qv = in ? t.vs[block] : 0.0f;
+    load8(static_cast<const int8_t*>(t.m), i0, n, whole, [&](int i, int8_t c) {
+      const float f = (float)c;
+      m[i] = (f * __builtin_fabsf(f)) * qm;
+    });
+    load8(static_cast<const uint8_t*>(t.v), i0, n, whole, [&](int i, uint8_t c) {
+      const float f = (float)c;
+      const float root = (f * f) * qv;
+      r[i] = root * root;
+    });
+  } else {
+    load8(static_cast<const float*>(t.m), i0, n, whole, [&](int i, float x) { m[i] = x; });
+    load8(static_cast<const float*>(t.v), i0, n, whole, [&](int i, float x) { r[i] = x; });
+  }
+  float v[kElems];
+#pragma unroll
+  for (int i = 0; i < kElems; ++i) {
+    const float gi = sc.grad_scale ? g[i] * scale : g[i];
+    m[i] = m[i] * sc.beta1 + gi * sc.omb1;
+    v[i] = r[i] * sc.beta2 + (gi * gi) * sc.omb2;
+    r[i] = sqrtf(v[i]);
+    // m over the denominator by the hardware's reciprocal (one ulp): of the step,
+    // not of the state
+    const float step = m[i] * __builtin_amdgcn_rcpf(r[i] * sc.root + sc.eps);
+    p[i] = p[i] * sc.keep - step * sc.rate;
+  }
+  store8(static_cast<P*>(t.param), i0, n, whole, [&](int i) { return (P)p[i]; });
+  if (t.copy) store8(static_cast<C*>(t.copy), i0, n, whole, [&](int i) { return (C)p[i]; });
+  if constexpr (BITS == 8) {
+    // elements past the end: their moments are zero, as all they were made of
+    float bm = 0.0f, bv = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) {
+      bm = vmax(bm, __builtin_fabsf(m[i]));
+      bv = vmax(bv, r[i]);
+    }
+    bm = half_max(bm);
+    bv = half_max(bv);
+    const bool zm = bm < kTinyBlock, zv = bv < kTinyBlock;
+    const float im = zm ? 0.0f : 16129.0f / bm, iv = zv ? 0.0f : 65025.0f / bv;
+    if ((threadIdx.x & 31) == 0 && i0 < n) {
+      t.ms[block] = zm ? 0.0f : bm / 16129.0f;
+      t.vs[block] = zv ? 0.0f : bv / 65025.0f;
+    }
+    store8(static_cast<int8_t*>(t.m), i0, n, whole, [&](int i) {
+      const int c = (int)code_of(__builtin_fabsf(m[i]) * im, 127.0f);
+      return (int8_t)(m[i] < 0.0f ? -c : c);
+    });
+    store8(static_cast<uint8_t*>(t.v), i0, n, whole, [&](int i) {
+      const int c = (int)code_of(r[i] * iv, 255.0f);
+      return (uint8_t)(c < 1 && r[i] > 0.0f && !zv ? 1 : c);
+    });
+  } else {
+    store8(static_cast<float*>(t.m), i0, n, whole, [&](int i) { return m[i]; });
+    store8(static_cast<float*>(t.v), i0, n, whole, [&](int i) { return v[i]; });
+  }
+}
+
+// The values of 8-bit codes: c |c| q, and for the second moment its square. One
+// lane takes eight; 10 bytes an element move.
+template <bool SECOND>
+__global__ void __launch_bounds__(kThreads) adamw_decode_kernel(const void* codes, const float* scales, int64_t n,
+                                                                float* out, int vec) {
+  using C = std::conditional_t<SECOND, uint8_t, int8_t>;
+  const int64_t i0 = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kElems;
+  if (i0 >= n) return;
+  const bool whole = vec && i0 + kElems <= n;
+  const float q = scales[i0 / 256];
+  float x[kElems];
+  load8(static_cast<const C*>(codes), i0, n, whole, [&](int i, C c) {
+    const float f = (float)c;
+    const float e = (f * __builtin_fabsf(f)) * q;
+    x[i] = SECOND ? e * e : e;
+  });
+  store8(out, i0, n, whole, [&](int i) { return x[i]; });
+}
+
+template <typename P, typename G, typename C>
+hipError_t launch_bits(int bits, int grid, const Table& tab, const AdamWScalars& sc, hipStream_t s) {
+  if (bits == 8)
+    adamw_kernel<P, G, C, 8><<<grid, kThreads, 0, s>>>(tab, sc);
+  else
+    adamw_kernel<P, G, C, 32><<<grid, kThreads, 0, s>>>(tab, sc);
+  return hipGetLastError();
+}
+
+hipError_t launch_types(int pkind, int gkind, int ckind, int bits, int grid, const Table& tab, const AdamWScalars& sc,
+                        hipStream_t s) {
+  // gradients in the parameters' type or in float32; only float32 parameters have copies
+  if (pkind == FMX_DTYPE_F16)
+    return gkind == FMX_DTYPE_F32 ? launch_bits<_Float16, float, _Float16>(bits, grid, tab, sc, s)
+                                  : launch_bits<_Float16, _Float16, _Float16>(bits, grid, tab, sc, s);
+  if (pkind == FMX_DTYPE_BF16)
+    return gkind == FMX_DTYPE_F32 ? launch_bits<__bf16, float, __bf16>(bits, grid, tab, sc, s)
+                                  : launch_bits<__bf16, __bf16, __bf16>(bits, grid, tab, sc, s);
+  if (ckind == FMX_DTYPE_F16) {
+    if (gkind == FMX_DTYPE_F16) return launch_bits<float, _Float16, _Float16>(bits, grid, tab, sc, s);
+    return launch_bits<float, float, _Float16>(bits, grid, tab, sc, s);
+  }
+  if (gkind == FMX_DTYPE_BF16) return launch_bits<float, __bf16, __bf16>(bits, grid, tab, sc, s);
+  return launch_bits<float, float, __bf16>(bits, grid, tab, sc, s);
+}
+
+bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
+
+}  // namespace
+
+hipError_t launch_adamw(int pkind, int gkind, int ckind, int bits, const AdamWTensor* t, int64_t count,
+                        const AdamWScalars& sc, hipStream_t s) {
+  Table tab;
+  tab.count = 0;
+  int64_t grid = 0;
+  auto flush = [&]() -> hipError_t {
+    if (tab.count == 0) return hipSuccess;
+    const hipError_t e = launch_types(pkind, gkind, ckind, bits, (int)grid, tab, sc, s);
+    tab.count = 0;
+    grid = 0;
+    return e;
+  };
+  for (int64_t k = 0; k < count; ++k) {
+    // a tensor of more workgroups than a launch's tail may hold goes on in pieces
+    constexpr int64_t kPiece = (int64_t)1 << 20;  // workgroups
+    for (int64_t at = 0; at < t[k].n; at += kPiece * kChunk) {
+      const int64_t n = t[k].n - at < kPiece * kChunk ? t[k].n - at : kPiece * kChunk;
+      if (tab.count == kMaxTensors || grid > kPiece) {
+        const hipError_t e = flush();
+        if (e != hipSuccess) return e;
+      }
+      const int ps = pkind == FMX_DTYPE_F32 ? 4 : 2, gs = gkind == FMX_DTYPE_F32 ? 4 : 2, ms = bits == 8 ? 1 : 4;
+      AdamWTensor& x = tab.t[tab.count];
+      x.param = static_cast<char*>(t[k].param) + at * ps;
+      x.grad = static_cast<const char*>(t[k].grad) + at * gs;
+      x.m = static_cast<char*>(t[k].m) + at * ms;
+      x.v = static_cast<char*>(t[k].v) + at * ms;
+      x.ms = t[k].ms ? t[k].ms + at / 256 : nullptr;
+      x.vs = t[k].vs ? t[k].vs + at / 256 : nullptr;
+      x.copy = t[k].copy ? static_cast<char*>(t[k].copy) + at * 2 : nullptr;
+      x.n = n;
+      const int mb = bits == 8 ? 8 : 16;
+      tab.vec[tab.count] = aligned(x.param, 16) && aligned(x.grad, 16) && aligned(x.m, mb) && aligned(x.v, mb) &&
+                           (!x.copy || aligned(x.copy, 16));
+      tab.first[tab.count] = (int32_t)grid;
+      grid += (n + kChunk - 1) / kChunk;
+      tab.first[++tab.count] = (int32_t)grid;
+    }
+  }
+  return flush();
+}
+
+hipError_t launch_adamw_decode(const void* codes, bool second, const float* scales, int64_t n, float* out,
+                               hipStream_t s) {
+  const int vec = aligned(codes, 8) && aligned(out, 16);
+  constexpr int64_t kPiece = ((int64_t)1 << 30) * kElems;  // elements of a launch, a multiple of the block
+  for (int64_t at = 0; at < n; at += kPiece) {
+    const int64_t k = n - at < kPiece ? n - at : kPiece;
+    const int grid = (int)((k + kThreads * kElems - 1) / (kThreads * kElems));
+    const void* c = static_cast<const char*>(codes) + at;
+    if (second)
+      adamw_decode_kernel<true><<<grid, kThreads, 0, s>>>(c, scales + at / 256, k, out + at, vec);
+    else
+      adamw_decode_kernel<false><<<grid, kThreads, 0, s>>>(c, scales + at / 256, k, out + at, vec);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace fmx

@@ -9,6 +9,7 @@
 #include "../../include/fmx.h"
 #include "fmx_device.h"
 #include "fmx_kernels.h"
+#include "fmx_layers.h"
 
 namespace {
 
@@ -60,6 +61,17 @@ int device_cus() {
   }
   return cache[dev];
 }
+
+}  // namespace
+
+namespace fmx {
+
+int report(int code, const char* message) { return message ? fail(code, "%s", message) : ok(); }
+int layer_cus() { return device_cus(); }
+
+}  // namespace fmx
+
+namespace {
 
 // Whether fmx_fwd takes the tiled (MFMA-bound) kernel for this call.
 bool use_tiled(int64_t Nq, int64_t Lq, int64_t Ld, int64_t d, int shared_docs) {

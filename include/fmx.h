@@ -378,6 +378,76 @@ int fmx_convert_rows(int src_dtype, const void* src, int64_t s_stride_b, int64_t
 /* Workspace of fmx_bwd_batched: as fmx_bwd_workspace_bytes with Nq*Lq entries per doc. */
 size_t fmx_bwd_batched_workspace_bytes(int64_t Nq, int64_t B, int64_t Lq, int64_t Ld, int64_t d);
 
+/*
+ * The trained layers around MaxSim (no counterpart in the reference, whose
+ * training starts at the token embeddings): layer norm, a linear layer with its
+ * epilogue, and the optimizer step.
+ */
+
+/*
+ * Layer norm of the rows of x: mu = mean x, s = 1 / sqrt(mean (x - mu)^2 + eps),
+ * y = (x - mu) s weight + bias, sums in fp32.
+ *
+ *   x       [M, d]  dtype (F16, BF16 or F32), row stride x_stride (any, also 0)
+ *   weight  [d]     w_dtype (dtype, or F32), or NULL (ones); bias likewise, or NULL (zeros)
+ *   y       [M, d]  dtype, contiguous
+ *   mean    [M]     fp32, rstd likewise: mu and s for the backward, both or neither NULL
+ * 1 <= d <= FMX_MAX_D. Pointers are aligned to their elements.
+ */
+int fmx_layer_norm(int dtype, const void* x, int64_t x_stride, int w_dtype, const void* weight, const void* bias,
+                   int64_t M, int64_t d, double eps, void* y, float* mean, float* rstd, void* stream);
+
+/*
+ * Its backward from the forward's mean and rstd, with xh = (x - mean) rstd and
+ * wdy = weight dy:
+ *   dx = rstd (wdy - mean(wdy) - xh mean(wdy xh))   [M, d] dtype, contiguous
+ *   dw = sum over rows of dy xh, db = sum of dy     [d] w_dtype
+ * each skipped when NULL. dw and db are fp32 sums in a fixed order (the same
+ * bits each time). Workspace, for dw or db: fmx_layer_norm_bwd_workspace_bytes.
+ */
+int fmx_layer_norm_bwd(int dtype, const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, int w_dtype,
+                       const void* weight, const float* mean, const float* rstd, int64_t M, int64_t d, void* dx,
+                       void* dw, void* db, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t fmx_layer_norm_bwd_workspace_bytes(int64_t M, int64_t d);
+
+/*
+ * One tensor of an AdamW step; n elements, all arrays contiguous and aligned to
+ * their elements. state_bits 32: exp_avg and exp_avg_sq are fp32 and the scales
+ * unused. state_bits 8: exp_avg holds int8 codes c (moment c |c| scale),
+ * exp_avg_sq uint8 codes c (root of the moment c^2 scale), one fp32 scale for
+ * each 256 consecutive elements (the last block may be shorter).
+ */
+typedef struct fmx_adamw_tensor {
+  void* param;            /* param_dtype, updated in place */
+  const void* grad;       /* grad_dtype */
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  void* copy;             /* copy_dtype: the new parameters rounded; or NULL */
+  int64_t n;
+} fmx_adamw_tensor;
+
+#define FMX_ADAMW_BLOCK 256
+
+/*
+ * AdamW over `count` tensors (a host array, read before the call returns):
+ *   g = grad * *grad_scale (a device scalar; NULL: 1)
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * in fp32, p rounded once to its type. The step uses the moments before they are
+ * rounded to 8 bits. grad_dtype: param_dtype, F32, or for F32 parameters with
+ * copies the copies' type; copies (copy_dtype F16 or BF16) need F32 parameters.
+ * step >= 1.
+ */
+int fmx_adamw(int param_dtype, int grad_dtype, int copy_dtype, int state_bits, const fmx_adamw_tensor* tensors,
+              int64_t count, int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay,
+              const float* grad_scale, void* stream);
+
+/* fp32 moments of n 8-bit codes: int8 (second = 0: c |c| scale) or uint8 (second = 1: the square of c^2 scale). */
+int fmx_adamw_decode(int second, const void* codes, const float* scales, int64_t n, float* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

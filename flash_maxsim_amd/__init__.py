@@ -11,7 +11,8 @@ top-k retrieval on the GPU (topk_scores, flash_maxsim_topk,
 flash_maxsim_batched_topk, flash_maxsim_int8_topk), and training with doc
 lengths (flash_maxsim_train's doc_lengths) or several queries
 (flash_maxsim_train_batched). The layers that such training moves: layer norm
-(layer_norm) and AdamW with moments in 32 or 8 bits (AdamW, adamw_step).
+(layer_norm), a linear layer with bias, activation and residual (linear), and
+AdamW with moments in 32 or 8 bits (AdamW, adamw_step).
 """
 
 __version__ = "0.1.0"
@@ -23,6 +24,7 @@ from .flash_maxsim_sparse import flash_maxsim_sparse, maxsim_sparse_naive
 from .flash_maxsim_packed import (PackedDocs, PackedInt8Docs, flash_maxsim_int8_packed, flash_maxsim_packed,
                                   pack_docs, quantize_int8_packed)
 from .flash_maxsim_topk import flash_maxsim_batched_topk, flash_maxsim_int8_topk, flash_maxsim_topk, topk_scores
+from .flash_maxsim_linear import linear
 from .flash_maxsim_norm import layer_norm
 from .flash_maxsim_optim import AdamW, AdamW8bitState, adamw_state, adamw_step, dequantize_adamw
 
@@ -47,6 +49,7 @@ __all__ = [
     "flash_maxsim_batched_topk",
     "flash_maxsim_int8_topk",
     "flash_maxsim_train_batched",
+    "linear",
     "layer_norm",
     "AdamW",
     "AdamW8bitState",

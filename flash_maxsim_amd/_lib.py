@@ -95,6 +95,16 @@ _SIGNATURES = {
     ),
     "fmx_convert_rows": (_int, [_int, _ptr, _i64, _i64, _i64, _i64, _i64, _ptr, _int, _ptr, _i64, _ptr]),
     "fmx_bwd_batched_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64]),
+    "fmx_linear": (
+        _int,
+        [_int, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _i64, _int, _i64, _i64, _i64, _ptr, _ptr, _ptr, _size, _ptr],
+    ),
+    "fmx_linear_workspace_bytes": (_size, [_i64, _i64, _i64]),
+    "fmx_linear_bwd": (
+        _int,
+        [_int, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _int, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _size, _ptr],
+    ),
+    "fmx_linear_bwd_workspace_bytes": (_size, [_i64, _i64, _i64]),
     "fmx_layer_norm": (
         _int,
         [_int, _ptr, _i64, _int, _ptr, _ptr, _i64, _i64, _f64, _ptr, _ptr, _ptr, _ptr],

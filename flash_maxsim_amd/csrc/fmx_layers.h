@@ -65,4 +65,52 @@ hipError_t launch_adamw(int pkind, int gkind, int ckind, int bits, const AdamWTe
                         const AdamWScalars& sc, hipStream_t s);
 hipError_t launch_adamw_decode(const void* codes, bool second, const float* scales, int64_t n, float* out, hipStream_t s);
 
+// ---- linear (fmx_linear.hip) ----
+
+enum LinearForm { kLinearForward, kLinearInput, kLinearWeight };  // y, dx, dw
+enum LinearTile { kTile64, kTile128, kTile128x256, kTile256 };
+
+// C[I, J] = sum over k < K of A(i, k) B(j, k); see fmx_linear.hip for the operands of each form.
+struct LinearArgs {
+  const void* A;
+  const void* B;
+  int64_t sa, sb;         // row strides in memory, multiples of 8
+  int64_t I, J, K;        // K: a multiple of 8 where it runs along rows
+  int64_t Jr;             // B's columns or rows that exist (set by launch_linear)
+  void* y;                // [I, J] 16-bit, contiguous
+  void* z;                // forward: act's argument, like y; or null
+  const void* bias;       // forward: [J], or null
+  const void* res;        // forward: [I, J], row stride sres, or null
+  int64_t sres;
+  float* part;            // splits > 1: [splits][I][Jp]
+  int64_t Jp;
+  int64_t ti, tj;         // tiles
+  int64_t split_k, band;
+  int splits;
+  int act;
+  int vec_out, vec_res, vec_bias;  // 16-byte accesses allowed
+};
+
+struct LinearPlan {
+  int tile;
+  int splits;
+  int64_t ti, tj, split_k, band;
+};
+LinearPlan linear_plan(int64_t I, int64_t J, int64_t K);
+size_t linear_part_bytes(const LinearPlan& p, int64_t I, int64_t J);
+hipError_t launch_linear(bool bf16, LinearForm form, LinearArgs a, const LinearPlan& p, hipStream_t s);
+
+struct DzArgs {
+  const void* dy;         // [M, N], row stride sdy
+  const void* z;          // [M, N] contiguous, or null (no activation)
+  void* dz;               // [M, Np] 16-bit, or null
+  float* part;            // [parts][N] column sums, or null
+  int64_t sdy, M, N, Np;  // Np: N rounded up to 8
+  int act;
+  int vec_dy, vec_z;
+};
+int linear_dz_parts(int64_t M, int64_t N);
+hipError_t launch_linear_dz(bool bf16, const DzArgs& a, int parts, hipStream_t s);
+hipError_t launch_linear_db(bool bf16, const float* part, int parts, int64_t N, void* db, hipStream_t s);
+
 }  // namespace fmx

@@ -39,9 +39,171 @@ int check_norm(int dtype, int w_dtype, int64_t x_stride, int64_t M, int64_t d) {
   return FMX_OK;
 }
 
+int check_linear(int dtype, int64_t x_stride, int64_t w_stride, int act, int64_t M, int64_t N, int64_t K) {
+  if (dtype != FMX_DTYPE_F16 && dtype != FMX_DTYPE_BF16) return fail(FMX_ERR_INVALID, "unknown dtype %d", dtype);
+  if (act < FMX_ACT_NONE || act > FMX_ACT_SILU) return fail(FMX_ERR_INVALID, "unknown activation %d", act);
+  if (M < 0 || N < 1 || K < 1)
+    return fail(FMX_ERR_INVALID, "invalid sizes M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+  if (M >= (int64_t)1 << 31 || N >= 1 << 24 || K >= 1 << 24)
+    return fail(FMX_ERR_UNSUPPORTED, "M=%lld N=%lld K=%lld too large", (long long)M, (long long)N, (long long)K);
+  const int64_t k8 = (K + 7) / 8 * 8;
+  if (x_stride < k8 || (x_stride & 7) || w_stride < k8 || (w_stride & 7))
+    return fail(FMX_ERR_INVALID, "row strides %lld and %lld must be >= K rounded up to 8 and multiples of 8",
+                (long long)x_stride, (long long)w_stride);
+  if (x_stride >= 1 << 22 || w_stride >= 1 << 22)
+    return fail(FMX_ERR_UNSUPPORTED, "row strides %lld and %lld must be < 2^22", (long long)x_stride,
+                (long long)w_stride);
+  return FMX_OK;
+}
+
+size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Backward workspace: dz, the column sums, the partial products of dx and of dw (used one after
+// the other).
+struct LinearBwdWs {
+  size_t dz, sums, part;
+  size_t total() const { return dz + sums + part; }
+};
+LinearBwdWs linear_bwd_ws(int64_t M, int64_t N, int64_t K) {
+  const int64_t n8 = (N + 7) / 8 * 8;
+  LinearBwdWs w;
+  w.dz = round256((size_t)M * (size_t)n8 * 2);
+  w.sums = round256((size_t)fmx::linear_dz_parts(M, N) * (size_t)N * sizeof(float));
+  const size_t px = fmx::linear_part_bytes(fmx::linear_plan(M, K, n8), M, K);
+  const size_t pw = fmx::linear_part_bytes(fmx::linear_plan(N, K, M), N, K);
+  w.part = round256(px > pw ? px : pw);
+  return w;
+}
+
 }  // namespace
 
 extern "C" {
+
+size_t fmx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  return fmx::linear_part_bytes(fmx::linear_plan(M, N, (K + 7) / 8 * 8), M, N);
+}
+
+int fmx_linear(int dtype, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
+               const void* residual, int64_t r_stride, int act, int64_t M, int64_t N, int64_t K, void* y, void* z,
+               void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_linear(dtype, x_stride, w_stride, act, M, N, K);
+  if (rc) return rc;
+  if (residual && r_stride < 0) return fail(FMX_ERR_INVALID, "residual stride must be >= 0");
+  if (M == 0) return ok();
+  if (!x || !w || !y) return fail(FMX_ERR_INVALID, "x, w and y must be non-null");
+  if (!aligned(x, 16) || !aligned(w, 16)) return fail(FMX_ERR_INVALID, "x and w must be 16-byte aligned");
+  if (!aligned(y, 2) || !aligned(z, 2) || !aligned(bias, 2) || !aligned(residual, 2))
+    return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");
+  fmx::LinearArgs a = {};
+  a.A = x;
+  a.B = w;
+  a.sa = x_stride;
+  a.sb = w_stride;
+  a.I = M;
+  a.J = N;
+  a.K = (K + 7) / 8 * 8;
+  a.y = y;
+  a.z = z;
+  a.bias = bias;
+  a.res = residual;
+  a.sres = r_stride;
+  a.act = act;
+  a.part = static_cast<float*>(workspace);
+  a.vec_out = N % 8 == 0 && aligned(y, 16) && aligned(z, 16);
+  a.vec_res = r_stride % 8 == 0 && aligned(residual, 16);
+  a.vec_bias = aligned(bias, 16);
+  const fmx::LinearPlan p = fmx::linear_plan(M, N, a.K);
+  const size_t need = fmx::linear_part_bytes(p, M, N);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(FMX_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace_bytes);
+  return hip_status(fmx::launch_linear(dtype == FMX_DTYPE_BF16, fmx::kLinearForward, a, p,
+                                       static_cast<hipStream_t>(stream)),
+                    "fmx_linear launch");
+}
+
+size_t fmx_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  return linear_bwd_ws(M, N, K).total();
+}
+
+int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* dy,
+                   int64_t dy_stride, const void* z, int act, int64_t M, int64_t N, int64_t K, void* dx, void* dw,
+                   void* db, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_linear(dtype, x_stride, w_stride, act, M, N, K);
+  if (rc) return rc;
+  if (dy_stride < 0) return fail(FMX_ERR_INVALID, "dy stride must be >= 0");
+  if (!dx && !dw && !db) return ok();
+  if (M > 0 && (!x || !w || !dy || (act != FMX_ACT_NONE && !z)))
+    return fail(FMX_ERR_INVALID, "x, w, dy and (with an activation) z must be non-null");
+  if (!aligned(x, 16) || !aligned(w, 16)) return fail(FMX_ERR_INVALID, "x and w must be 16-byte aligned");
+  if (!aligned(dy, 2) || !aligned(z, 2) || !aligned(dx, 2) || !aligned(dw, 2) || !aligned(db, 2))
+    return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");
+  const bool bf = dtype == FMX_DTYPE_BF16;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (M == 0) {  // no rows: zeros
+    hipError_t e = hipSuccess;
+    if (dw) e = fmx::launch_linear_db(bf, nullptr, 0, N * K, dw, s);
+    if (db && e == hipSuccess) e = fmx::launch_linear_db(bf, nullptr, 0, N, db, s);
+    return hip_status(e, "fmx_linear_bwd launch");
+  }
+  const LinearBwdWs ws = linear_bwd_ws(M, N, K);
+  if (!workspace || workspace_bytes < ws.total() || !aligned(workspace, 16))
+    return fail(FMX_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", ws.total(), workspace_bytes);
+  char* base = static_cast<char*>(workspace);
+  const int64_t n8 = (N + 7) / 8 * 8;
+  // dy serves as dz where it is one already and its rows can be read as an operand
+  const bool as_is = act == FMX_ACT_NONE && N % 8 == 0 && dy_stride % 8 == 0 && dy_stride >= N &&
+                     dy_stride < 1 << 22 && aligned(dy, 16);
+  const bool make = !as_is && (dx || dw);
+  hipError_t e = hipSuccess;
+  if (make || db) {
+    fmx::DzArgs a = {};
+    a.dy = dy;
+    a.z = act == FMX_ACT_NONE ? nullptr : z;
+    a.dz = make ? base : nullptr;
+    a.part = db ? reinterpret_cast<float*>(base + ws.dz) : nullptr;
+    a.sdy = dy_stride;
+    a.M = M;
+    a.N = N;
+    a.Np = n8;
+    a.act = act;
+    a.vec_dy = dy_stride % 8 == 0 && aligned(dy, 16);
+    a.vec_z = N % 8 == 0 && aligned(z, 16);
+    const int parts = fmx::linear_dz_parts(M, N);
+    e = fmx::launch_linear_dz(bf, a, parts, s);
+    if (db && e == hipSuccess) e = fmx::launch_linear_db(bf, a.part, parts, N, db, s);
+    if (e != hipSuccess) return hip_status(e, "fmx_linear_bwd launch");
+  }
+  fmx::LinearArgs a = {};
+  a.A = as_is ? dy : base;
+  a.sa = as_is ? dy_stride : n8;
+  a.part = reinterpret_cast<float*>(base + ws.dz + ws.sums);
+  a.vec_out = K % 8 == 0;
+  if (dx) {
+    a.B = w;
+    a.sb = w_stride;
+    a.I = M;
+    a.J = K;
+    a.K = N;
+    a.y = dx;
+    fmx::LinearArgs b = a;
+    b.vec_out = a.vec_out && aligned(dx, 16);
+    e = fmx::launch_linear(bf, fmx::kLinearInput, b, fmx::linear_plan(M, K, n8), s);
+    if (e != hipSuccess) return hip_status(e, "fmx_linear_bwd launch");
+  }
+  if (dw) {
+    a.B = x;
+    a.sb = x_stride;
+    a.I = N;
+    a.J = K;
+    a.K = M;
+    a.y = dw;
+    a.vec_out = a.vec_out && aligned(dw, 16);
+    e = fmx::launch_linear(bf, fmx::kLinearWeight, a, fmx::linear_plan(N, K, M), s);
+  }
+  return hip_status(e, "fmx_linear_bwd launch");
+}
 
 int fmx_layer_norm(int dtype, const void* x, int64_t x_stride, int w_dtype, const void* weight, const void* bias,
                    int64_t M, int64_t d, double eps, void* y, float* mean, float* rstd, void* stream) {

@@ -1,0 +1,582 @@
+// Linear layer on MFMA: y = act(x W^T + b) + r, and the products of its backward.
+//
+// One kernel computes C[i, j] = sum_k A(i, k) B(j, k) for all three:
+//   forward  i = row,  j = output,  k = input:  A = x [i, k],   B = W [j, k]
+//   dx       i = row,  j = input,   k = output: A = dz [i, k],  B = W [k, j]
+//   dw       i = out,  j = input,   k = row:    A = dz [k, i],  B = x [k, j]
+// An operand stored [i, k] ("K-major") is read from LDS with 16-byte reads of 8
+// k values; one stored [k, i] ("row-major") with transposing reads
+// (ds_read_b64_tr_b16: of the 16 lanes that read a 4 x 16 block, lane l gets
+// column l), so no operand is transposed in memory first.
+//
+// A workgroup computes a TI x TJ tile, its waves TI / WI x TJ / WJ each in
+// registers. Stages of BK k values stream global -> LDS by DMA (16 bytes a
+// lane) into NS buffers, the next stage in flight while one is multiplied.
+// Chunk positions in LDS are XOR-swizzled so that the lanes of a read fall in
+// distinct banks. C's j runs along the MFMA's result rows, so a lane holds 4
+// (K-major B: 8, W's rows being read in a permuted order) consecutive outputs
+// of one row and stores them together.
+//
+// A product whose tiles do not fill the GPU, or whose k is much longer than
+// its tiles are many, is split over k: float32 partial tiles go to the
+// workspace and a second kernel adds them in order (no atomics) and applies
+// the epilogue.
+#include <stdlib.h>
+
+#include <type_traits>
+
+#include "fmx_device.h"
+#include "fmx_layers.h"
+
+#include "../../include/fmx.h"
+
+namespace fmx {
+namespace {
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, bool bf) {
+  if (bf) {
+    const __bf16 x = (__bf16)a, y = (__bf16)b;
+    return (uint32_t)__builtin_bit_cast(uint16_t, x) | ((uint32_t)__builtin_bit_cast(uint16_t, y) << 16);
+  }
+  const _Float16 x = (_Float16)a, y = (_Float16)b;
+  return (uint32_t)__builtin_bit_cast(uint16_t, x) | ((uint32_t)__builtin_bit_cast(uint16_t, y) << 16);
+}
+__device__ __forceinline__ float unpack(uint32_t bits16, bool bf) {
+  return bf ? bf16_bits_to_float(bits16) : half_bits_to_float(bits16);
+}
+
+// ---- activations ----
+
+// Phi(z), the normal distribution function, and e = exp(-z^2 / 2): Abramowitz and
+// Stegun 7.1.26 (erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off
+// by 1.5e-7 at most) at x = |z| / sqrt 2; the lower tail has no cancellation.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  const float a = __builtin_fabsf(z);
+  e = __builtin_amdgcn_exp2f(z * z * -0.72134752044f);  // exp(-z^2 / 2)
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.2316418882f, a, 1.0f));  // p / sqrt 2
+  float q = fmaf(t, 0.5307027145f, -0.7265760135f);  // the halves of a5 .. a1
+  q = fmaf(t, q, 0.7107068705f);
+  q = fmaf(t, q, -0.142248368f);
+  q = fmaf(t, q, 0.1274147960f);
+  q = q * t * e;
+  return z < 0.0f ? q : 1.0f - q;
+}
+__device__ __forceinline__ float sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504089f));
+}
+
+__device__ __forceinline__ float act_value(float z, int act) {
+  switch (act) {
+    case FMX_ACT_RELU: return z > 0.0f ? z : z != z ? z : 0.0f;
+    case FMX_ACT_GELU: {
+      float e;
+      return z * normal_cdf(z, e);
+    }
+    // z (1 + tanh u) / 2 = z sigmoid(2 u)
+    case FMX_ACT_GELU_TANH: return z * sigmoid(1.5957691216f * z * fmaf(0.044715f, z * z, 1.0f));
+    case FMX_ACT_SILU: return z * sigmoid(z);
+    default: return z;
+  }
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+  switch (act) {
+    case FMX_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+    case FMX_ACT_GELU: {
+      float e;
+      const float p = normal_cdf(z, e);
+      return fmaf(z * 0.3989422804f, e, p);
+    }
+    case FMX_ACT_GELU_TANH: {
+      const float s = sigmoid(1.5957691216f * z * fmaf(0.044715f, z * z, 1.0f));
+      return s + z * s * (1.0f - s) * 1.5957691216f * fmaf(0.134145f, z * z, 1.0f);
+    }
+    case FMX_ACT_SILU: {
+      const float s = sigmoid(z);
+      return s + z * s * (1.0f - s);
+    }
+    default: return 1.0f;
+  }
+}
+
+// ---- epilogue: V consecutive outputs j .. j + V - 1 of row i ----
+
+template <int V>
+__device__ __forceinline__ void store16(void* base, int64_t at, int left, const float (&v)[V], bool bf, bool vec) {
+  uint16_t* p = static_cast<uint16_t*>(base) + at;
+  if (vec && left >= V) {
+    if constexpr (V == 8) {
+      *reinterpret_cast<u32x4_t*>(p) = u32x4_t{pack2(v[0], v[1], bf), pack2(v[2], v[3], bf), pack2(v[4], v[5], bf),
+                                               pack2(v[6], v[7], bf)};
+    } else {
+      *reinterpret_cast<u32x2_t*>(p) = u32x2_t{pack2(v[0], v[1], bf), pack2(v[2], v[3], bf)};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < left) p[i] = (uint16_t)pack2(v[i], 0.0f, bf);
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void load16(float (&v)[V], const void* base, int64_t at, int left, bool bf, bool vec) {
+  const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+  if (vec && left >= V) {
+    uint32_t w[V / 2];
+    if constexpr (V == 8) {
+      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = x[i];
+    } else {
+      const u32x2_t x = *reinterpret_cast<const u32x2_t*>(p);
+      w[0] = x[0];
+      w[1] = x[1];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = unpack((i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xffffu, bf);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = i < left ? unpack(p[i], bf) : 0.0f;
+  }
+}
+
+// Products in v (the bias added already) to their place: z, the activation, the residual, y.
+template <int V, bool EPI>
+__device__ __forceinline__ void finish(const LinearArgs& a, int64_t i, int64_t j, float (&v)[V], bool bf) {
+  const int left = (int)(a.J - j < V ? a.J - j : V);
+  if constexpr (EPI) {
+    if (a.z) store16<V>(a.z, i * a.J + j, left, v, bf, a.vec_out);
+    switch (a.act) {  // uniform: one test a group of V
+#define FMX_CASE(A) \
+  case A: \
+    _Pragma("unroll") for (int k = 0; k < V; ++k) v[k] = act_value(v[k], A); \
+    break
+      FMX_CASE(FMX_ACT_RELU);
+      FMX_CASE(FMX_ACT_GELU);
+      FMX_CASE(FMX_ACT_GELU_TANH);
+      FMX_CASE(FMX_ACT_SILU);
+#undef FMX_CASE
+      default: break;
+    }
+    if (a.res) {
+      float r[V];
+      load16<V>(r, a.res, i * a.sres + j, left, bf, a.vec_res);
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] += r[k];
+    }
+  }
+  store16<V>(a.y, i * a.J + j, left, v, bf, a.vec_out);
+}
+
+// ---- the product ----
+
+// One operand's side of a tile: T rows (of i or j), from row r0 on.
+template <bool MAJ, bool PAIR, int T, int BK, int NT>
+struct Side {
+  static constexpr int kChunks = T * BK / 8;            // 16-byte chunks of a stage
+  static constexpr int kLoads = kChunks / NT;           // of a thread
+  static constexpr int kRow = MAJ ? T / 8 : BK / 8;     // chunks of an LDS row
+  static_assert(kChunks % NT == 0, "a stage splits evenly over the threads");
+  const char* base;
+  int64_t step;        // bytes from one stage to the next
+  uint32_t off[kLoads];
+  int k[kLoads];       // the chunk's (first) k inside its stage
+
+  // position of chunk ch of LDS row r is ch ^ key(r)
+  static __device__ __forceinline__ int key(int r) {
+    if constexpr (MAJ) return (2 * (r & 3) | (kRow > 8 ? ((r >> 3) & 1) << 3 : 0)) & (kRow - 1);
+    // PAIR: the rows of one fragment are 0-3, 8-11, 16-19, 24-27 (and 4 more)
+    if constexpr (BK == 64) return PAIR ? (r & 3) | ((r >> 3) & 1) << 2 : r & 7;
+    return PAIR ? ((r >> 1) & 1) | ((r >> 3) & 1) << 1 : (r >> 1) & 3;
+  }
+
+  __device__ __forceinline__ Side(const void* p, int64_t stride, int64_t r0, int64_t rows, int64_t k0, int tid) {
+    base = static_cast<const char*>(p) + (MAJ ? k0 * stride + r0 : r0 * stride + k0) * 2;
+    step = (MAJ ? stride : 1) * (int64_t)BK * 2;
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const int at = n * NT + tid, r = at / kRow, ch = (at % kRow) ^ key(r);
+      k[n] = MAJ ? r : ch * 8;
+      const int row = MAJ ? ch * 8 : r;  // of i or j, inside the tile
+      off[n] = r0 + row < rows ? (uint32_t)(r * stride * 2 + ch * 16) : kOOB;
+    }
+  }
+  // Stage `it` to LDS; kleft: k values left from its start (those at or past it read as zeros)
+  __device__ __forceinline__ void issue(unsigned char* lds, int it, int64_t kleft, int wave) const {
+    const rsrc_t r = make_rsrc(base + it * step, kleft > 0 ? 0x7fffffffu : 0u);
+    if (kleft >= BK || kleft <= 0) {
+#pragma unroll
+      for (int n = 0; n < kLoads; ++n) dma16_lds<false>(r, lds + (n * NT + wave * 64) * 16, off[n]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < kLoads; ++n)
+        dma16_lds<false>(r, lds + (n * NT + wave * 64) * 16, k[n] < kleft ? off[n] : kOOB);
+    }
+  }
+};
+
+// Fragment reader of one operand: 16 rows x 32 k of fragment f, k-step kk.
+template <bool MAJ, bool PAIR, int T, int BK, int F>
+struct Frags {
+  uint32_t at[MAJ ? F : BK / 32];
+  __device__ __forceinline__ Frags(int row0, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    if constexpr (MAJ) {
+      const int q = c >> 2, s = c & 3, r = 8 * g + q;
+      const int key = Side<MAJ, PAIR, T, BK, 64>::key(r);
+#pragma unroll
+      for (int f = 0; f < F; ++f)
+        at[f] = (uint32_t)(r * T * 2 + (((row0 >> 3) + 2 * f + (s >> 1)) ^ key) * 16 + 8 * (s & 1));
+    } else {
+      const int row = row0 + (PAIR ? 8 * (c >> 2) + (c & 3) : c);
+      const int key = BK == 64 ? c & 7 : (c >> 1) & 3;
+#pragma unroll
+      for (int kk = 0; kk < BK / 32; ++kk) at[kk] = (uint32_t)(row * BK * 2 + ((kk * 4 + g) ^ key) * 16);
+    }
+  }
+  __device__ __forceinline__ u32x4_t read(const unsigned char* lds, int f, int kk) const {
+    if constexpr (MAJ) {
+      typedef __attribute__((address_space(3))) s16x4_t lds_t;
+      // k rows 32 kk + 8 g + 0..3, then + 4..7 (the key of row r + 4 is that of r)
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(lds + at[f] + (32 * kk) * T * 2));
+      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(lds + at[f] + (32 * kk + 4) * T * 2));
+      const u32x2_t l = __builtin_bit_cast(u32x2_t, lo), h = __builtin_bit_cast(u32x2_t, hi);
+      return u32x4_t{l[0], l[1], h[0], h[1]};
+    } else {
+      const int o = PAIR ? (f >> 1) * 32 + 4 * (f & 1) : f * 16;
+      return *reinterpret_cast<const u32x4_t*>(lds + at[kk] + o * BK * 2);
+    }
+  }
+};
+
+// LDS buffers are separate objects, named at compile time in the unrolled stage
+// loop: the compiler then knows that reads of one do not alias the DMA writes in
+// flight to another and puts no wait for those in front of them.
+__device__ __forceinline__ void stage_barrier() {
+  __asm__ volatile("" ::: "memory");
+  wait_lds();
+  __builtin_amdgcn_s_barrier();
+  __asm__ volatile("" ::: "memory");
+}
+
+template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int BK, int NS, bool EPI>
+__global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
+  constexpr int TI = WI * FI * 16, TJ = WJ * FJ * 16, NT = WI * WJ * 64;
+  constexpr int BYTES = (TI + TJ) * BK * 2;
+  using SideA = Side<AMAJ, false, TI, BK, NT>;
+  using SideB = Side<BMAJ, !BMAJ, TJ, BK, NT>;
+  constexpr int LOADS = SideA::kLoads + SideB::kLoads;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds0[BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds1[BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds2[NS > 2 ? BYTES : 16];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds3[NS > 3 ? BYTES : 16];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wi = wave % WI, wj = wave / WI;
+
+  // Workgroups go to the eight XCDs in turn; each XCD takes a run of consecutive tiles, which share
+  // operand rows in its L2. Runs of `band` tile rows are walked column by column.
+  const int64_t tiles = a.ti * a.tj;
+  int64_t id = blockIdx.x;
+  {
+    const int64_t total = tiles * a.splits, per = total / 8, x = id & 7, rest = total & 7;
+    id = (id >> 3) + x * per + (x < rest ? x : rest);
+  }
+  const int64_t split = id / tiles;
+  int64_t t = id - split * tiles;
+  const int64_t band = t / (a.band * a.tj);
+  const int64_t rows = a.ti - band * a.band < a.band ? a.ti - band * a.band : a.band;
+  t -= band * a.band * a.tj;
+  const int64_t i0 = (band * a.band + t % rows) * TI, j0 = t / rows * TJ;
+  const int64_t k0 = split * a.split_k;
+  const int64_t kn = a.K - k0 < a.split_k ? a.K - k0 : a.split_k;
+  const int nit = (int)((kn + BK - 1) / BK);
+
+  const SideA sa(a.A, a.sa, i0, a.I, k0, tid);
+  const SideB sb(a.B, a.sb, j0, a.Jr, k0, tid);
+  const Frags<AMAJ, false, TI, BK, FI> fa(wi * FI * 16, lane);
+  const Frags<BMAJ, !BMAJ, TJ, BK, FJ> fb(wj * FJ * 16, lane);
+
+  f32x4_t acc[FI][FJ];
+#pragma unroll
+  for (int x = 0; x < FI; ++x)
+#pragma unroll
+    for (int y = 0; y < FJ; ++y) acc[x][y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  auto buffer = [&](auto s) -> unsigned char* {
+    constexpr int S = decltype(s)::value % NS;
+    if constexpr (S == 0) return lds0;
+    if constexpr (S == 1) return lds1;
+    if constexpr (S == 2) return lds2;
+    return lds3;
+  };
+  auto issue = [&](unsigned char* lds, int it) __attribute__((always_inline)) {
+    const int64_t left = kn - (int64_t)it * BK;
+    sa.issue(lds, it, left, wave);
+    sb.issue(lds + TI * BK * 2, it, left, wave);
+  };
+  auto stage = [&](auto s, int it) __attribute__((always_inline)) {
+    constexpr int S = decltype(s)::value;
+    wait_vmem<(NS - 2) * LOADS>();
+    stage_barrier();
+    issue(buffer(std::integral_constant<int, S + NS - 1>{}), it + NS - 1);
+    const unsigned char* la = buffer(s);
+    const unsigned char* lb = la + TI * BK * 2;
+#pragma unroll
+    for (int kk = 0; kk < BK / 32; ++kk) {
+      u32x4_t va[FI], vb[FJ];
+#pragma unroll
+      for (int y = 0; y < FJ; ++y) vb[y] = fb.read(lb, y, kk);
+#pragma unroll
+      for (int x = 0; x < FI; ++x) va[x] = fa.read(la, x, kk);
+#pragma unroll
+      for (int x = 0; x < FI; ++x)
+#pragma unroll
+        for (int y = 0; y < FJ; ++y) acc[x][y] = mfma16x16x32<BF>(vb[y], va[x], acc[x][y]);
+    }
+  };
+
+  issue(lds0, 0);
+  if constexpr (NS > 2) issue(lds1, 1);
+  if constexpr (NS > 3) issue(lds2, 2);
+  for (int it = 0; it < nit; it += NS) {
+    stage(std::integral_constant<int, 0>{}, it);
+    if (it + 1 < nit) stage(std::integral_constant<int, 1>{}, it + 1);
+    if constexpr (NS > 2) {
+      if (it + 2 < nit) stage(std::integral_constant<int, 2>{}, it + 2);
+    }
+    if constexpr (NS > 3) {
+      if (it + 3 < nit) stage(std::integral_constant<int, 3>{}, it + 3);
+    }
+  }
+  wait_vmem<0>();  // the stages past the end: their (empty) DMA writes no longer reach LDS after this wave ends
+
+  const int c = lane & 15, g = lane >> 4;
+  constexpr int V = BMAJ ? 4 : 8, PER = V / 4;  // consecutive outputs of a lane
+#pragma unroll
+  for (int y = 0; y < FJ / PER; ++y) {
+    const int64_t j = j0 + wj * FJ * 16 + y * 16 * PER + V * g;
+    if (j >= a.J) continue;
+    float b[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) b[k] = 0.0f;
+    if (EPI && a.bias && a.splits == 1)
+      load16<V>(b, a.bias, j, (int)(a.J - j < V ? a.J - j : V), BF, a.vec_bias);
+#pragma unroll
+    for (int x = 0; x < FI; ++x) {
+      const int64_t i = i0 + wi * FI * 16 + x * 16 + c;
+      if (i >= a.I) continue;
+      if (a.splits > 1) {
+        float* p = a.part + (split * a.I + i) * a.Jp + j;  // Jp: J rounded up to 8
+#pragma unroll
+        for (int k = 0; k < PER; ++k) *reinterpret_cast<f32x4_t*>(p + 4 * k) = acc[x][y * PER + k];
+      } else {
+        float v[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = acc[x][y * PER + k / 4][k % 4] + b[k];
+        finish<V, EPI>(a, i, j, v, BF);
+      }
+    }
+  }
+}
+
+// Adds the partial products of a split in their order and finishes 8 outputs a lane.
+template <bool BF, bool EPI>
+__global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a) {
+  const int64_t per = a.Jp / 8, n = a.I * per;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
+    const int64_t i = t / per, j = (t - i * per) * 8;
+    const float* p = a.part + i * a.Jp + j;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+    const int left = (int)(a.J - j < 8 ? a.J - j : 8);
+    if (EPI && a.bias) load16<8>(v, a.bias, j, left, BF, a.vec_bias);
+    f32x4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+      s0 += *reinterpret_cast<const f32x4_t*>(p + s * a.I * a.Jp);
+      s1 += *reinterpret_cast<const f32x4_t*>(p + s * a.I * a.Jp + 4);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] += s0[k];
+      v[4 + k] += s1[k];
+    }
+    finish<8, EPI>(a, i, j, v, BF);
+  }
+}
+
+// dz = dy act'(z) in 16 bits (rows padded with zeros to Np), and the column sums of the
+// unrounded dz over each workgroup's rows. A lane holds 8 columns, a wave 512; the
+// four waves of a workgroup take rows in turn.
+template <bool BF>
+__global__ void __launch_bounds__(256) linear_dz_kernel(DzArgs a) {
+  __shared__ float sums[4][512];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t j = (int64_t)blockIdx.x * 512 + lane * 8;
+  const int left = (int)(a.N - j < 0 ? 0 : a.N - j < 8 ? a.N - j : 8);
+  float s[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s[k] = 0.0f;
+  if (j < a.Np) {
+    for (int64_t i = (int64_t)blockIdx.y * 4 + wave; i < a.M; i += (int64_t)gridDim.y * 4) {
+      float v[8];
+      load16<8>(v, a.dy, i * a.sdy + j, left, BF, a.vec_dy);
+      if (a.z) {
+        float z[8];
+        load16<8>(z, a.z, i * a.N + j, left, BF, a.vec_z);
+        switch (a.act) {
+#define FMX_CASE(A) \
+  case A: \
+    _Pragma("unroll") for (int k = 0; k < 8; ++k) v[k] *= act_slope(z[k], A); \
+    break
+          FMX_CASE(FMX_ACT_RELU);
+          FMX_CASE(FMX_ACT_GELU);
+          FMX_CASE(FMX_ACT_GELU_TANH);
+          FMX_CASE(FMX_ACT_SILU);
+#undef FMX_CASE
+          default: break;
+        }
+      }
+      if (a.dz) store16<8>(a.dz, i * a.Np + j, 8, v, BF, true);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[k] += v[k];
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sums[wave][lane * 8 + k] = s[k];
+  __syncthreads();
+  for (int c = threadIdx.x; c < 512; c += 256) {
+    const int64_t col = (int64_t)blockIdx.x * 512 + c;
+    if (col < a.N) a.part[(int64_t)blockIdx.y * a.N + col] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+  }
+}
+
+// db: the columns of the partial rows, 64 a workgroup, the rows over its 16 waves.
+template <typename O>
+__global__ void __launch_bounds__(1024) linear_db_kernel(const float* part, int parts, int64_t N, O* db) {
+  __shared__ float sums[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t j = (int64_t)blockIdx.x * 64 + lane;
+  float s = 0.0f;
+  if (j < N)
+    for (int p = wave; p < parts; p += 16) s += part[p * N + j];
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && j < N) {
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += sums[i][lane];
+    db[j] = (O)s;
+  }
+}
+
+template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int BK, int NS, bool EPI>
+void run(const LinearArgs& a, int64_t grid, hipStream_t s) {
+  linear_kernel<BF, AMAJ, BMAJ, WI, WJ, FI, FJ, BK, NS, EPI><<<(unsigned)grid, WI * WJ * 64, 0, s>>>(a);
+}
+
+template <bool BF, bool AMAJ, bool BMAJ, bool EPI>
+hipError_t launch(const LinearArgs& a, int tile, hipStream_t s) {
+  const int64_t grid = a.ti * a.tj * a.splits;
+  switch (tile) {
+    case kTile256: run<BF, AMAJ, BMAJ, 2, 4, 8, 4, 64, 2, EPI>(a, grid, s); break;
+    case kTile128x256: run<BF, AMAJ, BMAJ, 2, 2, 4, 8, 32, 3, EPI>(a, grid, s); break;
+    case kTile128: run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 64, 2, EPI>(a, grid, s); break;
+    default: run<BF, AMAJ, BMAJ, 2, 2, 2, 2, 64, 4, EPI>(a, grid, s); break;
+  }
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 1) return e;
+  const int64_t groups = (a.I * (a.Jp / 8) + 255) / 256;
+  linear_join_kernel<BF, EPI><<<(unsigned)(groups < 4096 ? groups : 4096), 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+LinearPlan linear_plan(int64_t I, int64_t J, int64_t K) {
+  LinearPlan p;
+  const int64_t cus = layer_cus();
+  auto count = [&](int64_t ti, int64_t tj) { return ((I + ti - 1) / ti) * ((J + tj - 1) / tj); };
+  if (count(256, 256) >= cus)
+    p.tile = kTile256;
+  else if (count(128, 128) >= cus / 2)
+    p.tile = kTile128;
+  else
+    p.tile = I > 64 && J > 64 && K >= 4096 ? kTile128 : kTile64;
+  static const char* force = getenv("FMX_TILE");
+  if (force) p.tile = force[0] - '0';
+  const int64_t ti = p.tile == kTile256 ? 256 : p.tile == kTile64 ? 64 : 128;
+  const int64_t tj = p.tile == kTile256 || p.tile == kTile128x256 ? 256 : p.tile == kTile64 ? 64 : 128;
+  p.ti = (I + ti - 1) / ti;
+  p.tj = (J + tj - 1) / tj;
+  // split k where the tiles leave compute units idle, at 512 k values a part at least
+  const int64_t tiles = p.ti * p.tj, want = p.tile == kTile256 ? cus : 2 * cus;
+  int64_t splits = tiles * 2 > want ? 1 : want / tiles;
+  const int64_t most = K / 512;
+  if (splits > most) splits = most;
+  if (splits > 64) splits = 64;
+  if (splits < 1) splits = 1;
+  int64_t per = (K + splits - 1) / splits;
+  per = (per + 63) / 64 * 64;
+  p.split_k = per;
+  p.splits = (int)((K + per - 1) / per);
+  if (p.splits < 1) p.splits = 1;
+  // operand rows that an XCD's L2 (4 MB) holds beside the other operand's: runs of 8 tile rows
+  p.band = 8;
+  return p;
+}
+
+size_t linear_part_bytes(const LinearPlan& p, int64_t I, int64_t J) {
+  return p.splits > 1 ? (size_t)p.splits * (size_t)I * (size_t)((J + 7) / 8 * 8) * sizeof(float) : 0;
+}
+
+hipError_t launch_linear(bool bf16, LinearForm form, LinearArgs a, const LinearPlan& p, hipStream_t s) {
+  a.ti = p.ti;
+  a.tj = p.tj;
+  a.splits = p.splits;
+  a.split_k = p.split_k;
+  a.band = p.band;
+  a.Jp = (a.J + 7) / 8 * 8;
+  a.Jr = form == kLinearForward ? a.J : a.Jp;  // row-major B: whole chunks of 8 columns
+  switch (form) {
+    case kLinearForward:
+      return bf16 ? launch<true, false, false, true>(a, p.tile, s) : launch<false, false, false, true>(a, p.tile, s);
+    case kLinearInput:
+      return bf16 ? launch<true, false, true, false>(a, p.tile, s) : launch<false, false, true, false>(a, p.tile, s);
+    default:
+      return bf16 ? launch<true, true, true, false>(a, p.tile, s) : launch<false, true, true, false>(a, p.tile, s);
+  }
+}
+
+int linear_dz_parts(int64_t M, int64_t N) {
+  const int64_t cols = (N + 511) / 512;
+  int64_t parts = (int64_t)layer_cus() * 8 / cols;  // about eight workgroups a CU
+  const int64_t rows = (M + 15) / 16;               // four rows a wave at least
+  if (parts > rows) parts = rows;
+  return (int)(parts < 1 ? 1 : parts > 65535 ? 65535 : parts);
+}
+
+hipError_t launch_linear_dz(bool bf16, const DzArgs& a, int parts, hipStream_t s) {
+  const dim3 grid((unsigned)((a.Np + 511) / 512), (unsigned)parts);
+  if (bf16)
+    linear_dz_kernel<true><<<grid, 256, 0, s>>>(a);
+  else
+    linear_dz_kernel<false><<<grid, 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t launch_linear_db(bool bf16, const float* part, int parts, int64_t N, void* db, hipStream_t s) {
+  const unsigned grid = (unsigned)((N + 63) / 64);
+  if (bf16)
+    linear_db_kernel<__bf16><<<grid, 1024, 0, s>>>(part, parts, N, static_cast<__bf16*>(db));
+  else
+    linear_db_kernel<_Float16><<<grid, 1024, 0, s>>>(part, parts, N, static_cast<_Float16*>(db));
+  return hipGetLastError();
+}
+
+}  // namespace fmx

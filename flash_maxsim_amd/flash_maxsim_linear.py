@@ -1,0 +1,119 @@
+"""Linear layer with bias, activation and residual in its epilogue, on MI355X.
+
+What turns an encoder's hidden states into the token embeddings that MaxSim
+scores: y = act(x W^T + bias) + residual in one pass, and its backward. Extension
+of the reference API (no counterpart in flash_maxsim 0.1.0, whose training starts
+at the token embeddings).
+
+Operands are all float16 or all bfloat16; products run on MFMA with float32 sums,
+and y is rounded once. The backward rounds dz = dy act'(z) to the operands' type,
+as MFMA takes it, and keeps z = x W^T + bias in that type between the passes (only
+with an activation); bias gradients sum the unrounded dz. Sums have a fixed order:
+the same inputs give the same bits.
+
+x and weight are read in place when their rows are 16-byte aligned and K is a
+multiple of 8; other layouts are copied once per call with K zero-padded to a
+multiple of 8.
+"""
+
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+
+from . import _lib
+from .flash_maxsim import _abi_ready, _check_devices, _device_guard
+from .flash_maxsim_norm import _rows
+
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def _operand(t: torch.Tensor) -> torch.Tensor:
+    """[rows, K] as the kernels read it: t itself, or a copy with K zero-padded to a multiple of 8."""
+    K = t.shape[1]
+    if K % 8 == 0 and _abi_ready(t, None) and t.stride(0) < 1 << 22:
+        return t
+    t = F.pad(t, (0, -K % 8)) if K % 8 else t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _check(x, weight, bias, activation, residual) -> None:
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation={activation!r} must be one of {list(ACTIVATIONS)}")
+    assert x.ndim >= 1 and weight.ndim == 2 and x.size(-1) == weight.size(1), "x must be [..., K] and weight [N, K]"
+    N, K = weight.shape
+    assert N >= 1 and K >= 1, "weight must have rows and columns"
+    assert bias is None or tuple(bias.shape) == (N,), f"bias must be [{N}]"
+    assert residual is None or tuple(residual.shape) == (*x.shape[:-1], N), "residual must be [..., N]"
+    types = {t.dtype for t in (x, weight, bias, residual) if t is not None}
+    if types not in ({torch.float16}, {torch.bfloat16}):
+        raise TypeError(f"x, weight, bias and residual must all be float16 or all bfloat16, got {sorted(map(str, types))}")
+
+
+def _forward(x, weight, bias, act, residual, save):
+    """y, the operands as the kernels read them, and with `save` and an activation z."""
+    N, K = weight.shape
+    dev = _check_devices(x, weight, bias, residual)
+    xk, wk = _operand(_rows(x, K)), _operand(weight)
+    res = None if residual is None else _rows(residual, N)
+    bias = None if bias is None else bias.contiguous()
+    M = xk.size(0)
+    y = torch.empty(*x.shape[:-1], N, device=dev, dtype=x.dtype)
+    z = torch.empty(M, N, device=dev, dtype=x.dtype) if save and act else None
+    lib = _lib.load()
+    with _device_guard(dev):
+        nbytes = lib.fmx_linear_workspace_bytes(M, N, K)
+        ws = _lib.workspace(nbytes, dev)
+        rc = lib.fmx_linear(
+            _lib.dtype_code(xk), xk.data_ptr(), xk.stride(0), wk.data_ptr(), wk.stride(0), _lib.ptr(bias),
+            _lib.ptr(res), 0 if res is None else res.stride(0), act, M, N, K, y.data_ptr(), _lib.ptr(z),
+            _lib.ptr(ws), nbytes, _lib.stream_of(x),
+        )
+    _lib.check(rc)
+    return y, xk, wk, z
+
+
+class _LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, act, residual):
+        y, xk, wk, z = _forward(x, weight, bias, act, residual, True)
+        ctx.save_for_backward(xk, wk, z)
+        ctx.act, ctx.shape, ctx.sizes = act, x.shape, tuple(weight.shape)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        xk, wk, z = ctx.saved_tensors
+        (N, K), M, dev = ctx.sizes, xk.size(0), xk.device
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = torch.empty(ctx.shape, device=dev, dtype=xk.dtype) if need_x else None
+        dw = torch.empty(N, K, device=dev, dtype=xk.dtype) if need_w else None
+        db = torch.empty(N, device=dev, dtype=xk.dtype) if need_b else None
+        if need_x or need_w or need_b:
+            dys = _rows(dy, N)
+            lib = _lib.load()
+            with _device_guard(dev):
+                nbytes = lib.fmx_linear_bwd_workspace_bytes(M, N, K)
+                ws = _lib.workspace(nbytes, dev)
+                rc = lib.fmx_linear_bwd(
+                    _lib.dtype_code(xk), xk.data_ptr(), xk.stride(0), wk.data_ptr(), wk.stride(0), dys.data_ptr(),
+                    dys.stride(0), _lib.ptr(z), ctx.act, M, N, K, _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db),
+                    _lib.ptr(ws), nbytes, _lib.stream_of(xk),
+                )
+            _lib.check(rc)
+        return dx, dw, db, None, dy if ctx.needs_input_grad[4] else None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+           residual: torch.Tensor | None = None) -> torch.Tensor:
+    """act(x W^T + bias) + residual: [..., N] in x's type.
+
+    x is [..., K], weight [N, K], bias [N], residual [..., N]; activation is
+    None, "relu", "gelu" (by the normal distribution function), "gelu_tanh" (its
+    tanh form) or "silu". Differentiable in x, weight, bias and residual.
+    """
+    _check(x, weight, bias, activation, residual)
+    act = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _LinearFn.apply(x, weight, bias, act, residual)
+    return _forward(x, weight, bias, act, residual, False)[0]

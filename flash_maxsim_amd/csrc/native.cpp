@@ -13,6 +13,9 @@
 // step's host time depends more on where autograd's thread runs: 85 or 150 us
 // before, 105 after, for 32 x 32 tokens over 256 docs of up to 180.)
 //
+// The trained layers (linear, layer_norm) have their autograd nodes here as well,
+// so that a backward pass takes neither the GIL nor Python.
+//
 // The library is reached through its C ABI alone.
 #include <Python.h>
 
@@ -21,9 +24,14 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <algorithm>
+#include <vector>
 
 #include "../../include/fmx.h"
 
@@ -462,10 +470,386 @@ PyObject* backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the trained layers ----
+
+// [..., d] as M rows: their stride in elements, where one describes them all and
+// a row's elements are adjacent.
+bool as_rows(const Tensor& t, int64_t* M, int64_t* stride) {
+  const int64_t n = t.dim();
+  if (n < 1 || t.size(n - 1) < 1 || (t.size(n - 1) > 1 && t.stride(n - 1) != 1)) return false;
+  *M = 1;
+  *stride = t.size(n - 1);
+  bool first = true;
+  for (int64_t i = n - 2; i >= 0; --i) {
+    const int64_t size = t.size(i);
+    if (size != 1) {
+      if (first)
+        *stride = t.stride(i);
+      else if (t.stride(i) != *stride * *M)
+        return false;
+      first = false;
+    }
+    *M *= size;
+  }
+  return true;
+}
+
+// A tensor argument that may be None: false if it is neither.
+bool take_optional(PyObject* o, const Tensor** out) {
+  *out = nullptr;
+  if (o == Py_None) return true;
+  *out = plain(o);
+  return *out != nullptr;
+}
+
+bool grad_wanted(std::initializer_list<const Tensor*> ts) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t && t->requires_grad()) return true;
+  return false;
+}
+
+// Tangents of forward-mode differentiation, which only the Python path refuses by name.
+bool has_tangent(const Tensor* t) { return t && t->_fw_grad(0).defined(); }
+
+bool is_vector(const Tensor* t, const Tensor& like, at::ScalarType type, int64_t n) {
+  return !t || (t->dim() == 1 && t->size(0) == n && t->scalar_type() == type && t->is_contiguous() &&
+                t->device() == like.device());
+}
+
+void must(int rc) { TORCH_CHECK(rc == 0, "flash_maxsim_amd: ", fmx_last_error(), " (code ", rc, ")"); }
+
+// Gradients that say so when they are differentiated again.
+torch::autograd::variable_list once(torch::autograd::variable_list grads) {
+  if (!c10::GradMode::is_enabled()) return grads;
+  bool any = false;
+  for (const Tensor& g : grads) any |= g.defined();
+  if (!any) return grads;
+  auto node = std::make_shared<torch::autograd::DelayedError>(
+      "the gradients of flash_maxsim_amd's layers cannot be differentiated again", (int)grads.size());
+  return (*node)(std::move(grads));
+}
+
+// dy as rows of n elements that the kernels read; `keep` holds a copy where it takes one.
+const Tensor& grad_rows(const Tensor& dy, Tensor* keep, int64_t* M, int64_t* stride) {
+  if (as_rows(dy, M, stride) && *stride >= 0) return dy;
+  *keep = dy.contiguous();
+  as_rows(*keep, M, stride);
+  return *keep;
+}
+
+struct LinearBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable x, w, z;  // x and w as the kernels read them
+  std::vector<int64_t> x_sizes;
+  int64_t M, N, K, x_stride, w_stride;
+  int dtype, act;
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    const Tensor dy0 = grads[0];
+    if (!dy0.defined()) return torch::autograd::variable_list(4);
+    const Tensor xk = x.unpack(), wk = w.unpack();
+    const Tensor zk = act ? z.unpack() : Tensor();
+    const bool again = c10::GradMode::is_enabled();
+    Tensor keep, dx, dw, db;
+    {
+      at::AutoGradMode off(false);
+      int64_t m, stride;
+      const Tensor& dy = grad_rows(dy0, &keep, &m, &stride);
+      const auto options = xk.options();
+      if (task_should_compute_output(0)) dx = at::empty(x_sizes, options);
+      if (task_should_compute_output(1)) dw = at::empty({N, K}, options);
+      if (task_should_compute_output(2)) db = at::empty({N}, options);
+      if (dx.defined() || dw.defined() || db.defined()) {
+        const size_t n = fmx_linear_bwd_workspace_bytes(M, N, K);
+        const Tensor ws = scratch(n, xk);
+        must(fmx_linear_bwd(dtype, xk.const_data_ptr(), x_stride, wk.const_data_ptr(), w_stride, dy.const_data_ptr(),
+                            stride, zk.defined() ? zk.const_data_ptr() : nullptr, act, M, N, K, ptr(dx), ptr(dw),
+                            ptr(db), ptr(ws), n, stream_of(xk)));
+      }
+    }
+    // the residual's gradient is dy itself
+    const Tensor dr = task_should_compute_output(3) ? dy0 : Tensor();
+    if (!again) return {dx, dw, db, dr};
+    auto grads3 = once({dx, dw, db});
+    return {grads3[0], grads3[1], grads3[2], dr};
+  }
+  void release_variables() override {
+    x.reset_data();
+    w.reset_data();
+    z.reset_data();
+  }
+  std::string name() const override { return "FlashMaxSimLinearBackward"; }
+};
+
+struct LayerNormBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable x, w, mean, rstd;
+  std::vector<int64_t> x_sizes;
+  int64_t M, d, x_stride;
+  int dtype, w_dtype;
+  at::ScalarType w_type;
+  bool has_w;
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    const Tensor dy0 = grads[0];
+    if (!dy0.defined()) return torch::autograd::variable_list(3);
+    const Tensor xk = x.unpack(), wk = has_w ? w.unpack() : Tensor(), mu = mean.unpack(), rs = rstd.unpack();
+    const bool again = c10::GradMode::is_enabled();
+    Tensor keep, dx, dw, db;
+    {
+      at::AutoGradMode off(false);
+      int64_t m, stride;
+      const Tensor& dy = grad_rows(dy0, &keep, &m, &stride);
+      const auto options = xk.options();
+      if (task_should_compute_output(0)) dx = at::empty(x_sizes, options);
+      if (task_should_compute_output(1)) dw = at::empty({d}, options.dtype(w_type));
+      if (task_should_compute_output(2)) db = at::empty({d}, options.dtype(w_type));
+      if (dx.defined() || dw.defined() || db.defined()) {
+        const size_t n = dw.defined() || db.defined() ? fmx_layer_norm_bwd_workspace_bytes(M, d) : 0;
+        const Tensor ws = scratch(n, xk);
+        must(fmx_layer_norm_bwd(dtype, xk.const_data_ptr(), x_stride, dy.const_data_ptr(), stride, w_dtype,
+                                wk.defined() ? wk.const_data_ptr() : nullptr, mu.const_data_ptr<float>(),
+                                rs.const_data_ptr<float>(), M, d, ptr(dx), ptr(dw), ptr(db), ptr(ws), n,
+                                stream_of(xk)));
+      }
+    }
+    return again ? once({dx, dw, db}) : torch::autograd::variable_list{dx, dw, db};
+  }
+  void release_variables() override {
+    x.reset_data();
+    w.reset_data();
+    mean.reset_data();
+    rstd.reset_data();
+  }
+  std::string name() const override { return "FlashMaxSimLayerNormBackward"; }
+};
+
+// linear(x [..., K], w [N, K], bias [N] or None, activation, residual [..., N] or None): y [..., N]
+PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  FMX_ARGS(5);
+  const Tensor *x = plain(args[0]), *w = plain(args[1]), *b, *r;
+  FMX_ORDINARY(x && w && take_optional(args[2], &b) && take_optional(args[4], &r) && PyLong_CheckExact(args[3]));
+  const long act = PyLong_AsLong(args[3]);
+  const at::ScalarType type = x->scalar_type();
+  FMX_ORDINARY((type == at::kHalf || type == at::kBFloat16) && act >= FMX_ACT_NONE && act <= FMX_ACT_SILU);
+  int64_t M, sx, sr = 0, Mr;
+  FMX_ORDINARY(w->dim() == 2 && w->scalar_type() == type && w->device() == x->device() && as_rows(*x, &M, &sx));
+  const int64_t N = w->size(0), K = w->size(1), K8 = (K + 7) / 8 * 8;
+  FMX_ORDINARY(N >= 1 && x->size(-1) == K && M > 0 && sx >= 0 && w->stride(0) >= 0 && (K == 1 || w->stride(1) == 1) &&
+               is_vector(b, *x, type, N) && here(*x));
+  auto sizes = x->sizes().vec();
+  sizes.back() = N;
+  FMX_ORDINARY(!r || (r->scalar_type() == type && r->device() == x->device() && r->sizes() == sizes &&
+                      as_rows(*r, &Mr, &sr) && sr >= 0));
+  FMX_ORDINARY(!has_tangent(x) && !has_tangent(w) && !has_tangent(b) && !has_tangent(r));
+  const int dtype = code_of(*x);
+  void* s = stream_of(*x);
+  // An operand as the kernels read it: itself, or a copy with its rows zero-padded to a multiple of 8.
+  int prc = 0;
+  bool fits = true;
+  auto operand = [&](const Tensor& t, int64_t rows, int64_t* stride) -> Tensor {
+    if (K == K8 && *stride >= K && (*stride & 7) == 0 && *stride < 1 << 22 &&
+        (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) == 0)
+      return t;
+    if (K8 >= 1 << 22 || rows > (INT32_MAX - 4096) / (K8 / 4)) {
+      fits = false;
+      return Tensor();
+    }
+    Tensor out = at::empty({rows, K8}, t.options());
+    prc = fmx_convert_rows(dtype, t.const_data_ptr(), 0, *stride, 1, rows, K, nullptr, dtype, out.data_ptr(), K8, s);
+    *stride = K8;
+    return out;
+  };
+  int64_t sw = w->stride(0);
+  const Tensor xk = operand(*x, M, &sx), wk = operand(*w, N, &sw);
+  FMX_ORDINARY(fits);
+  if (prc) return failed(prc);
+  const bool grad = grad_wanted({x, w, b, r});
+  Tensor y = at::empty(sizes, x->options());
+  Tensor z = grad && act ? at::empty({M, N}, x->options()) : Tensor();
+  const size_t n = fmx_linear_workspace_bytes(M, N, K);
+  const Tensor ws = scratch(n, *x);
+  const int rc = unlocked([&] {
+    return fmx_linear(dtype, xk.const_data_ptr(), sx, wk.const_data_ptr(), sw, b ? b->const_data_ptr() : nullptr,
+                      r ? r->const_data_ptr() : nullptr, sr, (int)act, M, N, K, y.data_ptr(), ptr(z), ptr(ws), n, s);
+  });
+  if (rc) return failed(rc);
+  if (grad) {
+    std::shared_ptr<LinearBackward> node(new LinearBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(*x, *w, b ? *b : Tensor(), r ? *r : Tensor()));
+    node->x = torch::autograd::SavedVariable(xk, false);
+    node->w = torch::autograd::SavedVariable(wk, false);
+    if (act) node->z = torch::autograd::SavedVariable(z, false);
+    node->x_sizes = x->sizes().vec();
+    node->M = M;
+    node->N = N;
+    node->K = K;
+    node->x_stride = sx;
+    node->w_stride = sw;
+    node->dtype = dtype;
+    node->act = (int)act;
+    torch::autograd::set_history(y, node);
+  }
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// layer_norm(x [..., d], weight [d] or None, bias [d] or None, eps): y [..., d]
+PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  FMX_ARGS(4);
+  const Tensor *x = plain(args[0]), *w, *b;
+  FMX_ORDINARY(x && take_optional(args[1], &w) && take_optional(args[2], &b) && PyFloat_CheckExact(args[3]));
+  const int dtype = code_of(*x);
+  int64_t M, sx;
+  FMX_ORDINARY(dtype >= 0 && as_rows(*x, &M, &sx) && M > 0 && sx >= 0 && here(*x));
+  const int64_t d = x->size(-1);
+  const at::ScalarType wt = w ? w->scalar_type() : b ? b->scalar_type() : x->scalar_type();
+  FMX_ORDINARY((wt == x->scalar_type() || wt == at::kFloat) && is_vector(w, *x, wt, d) && is_vector(b, *x, wt, d) &&
+               !has_tangent(x) && !has_tangent(w) && !has_tangent(b));
+  const int w_dtype = wt == at::kFloat ? FMX_DTYPE_F32 : dtype;
+  const bool grad = grad_wanted({x, w, b});
+  Tensor y = at::empty(x->sizes(), x->options()), mean, rstd;
+  if (grad) {
+    mean = at::empty({M}, x->options().dtype(at::kFloat));
+    rstd = at::empty({M}, x->options().dtype(at::kFloat));
+  }
+  void* s = stream_of(*x);
+  const double eps = PyFloat_AS_DOUBLE(args[3]);
+  const int rc = unlocked([&] {
+    return fmx_layer_norm(dtype, x->const_data_ptr(), sx, w_dtype, w ? w->const_data_ptr() : nullptr,
+                          b ? b->const_data_ptr() : nullptr, M, d, eps, y.data_ptr(), static_cast<float*>(ptr(mean)),
+                          static_cast<float*>(ptr(rstd)), s);
+  });
+  if (rc) return failed(rc);
+  if (grad) {
+    std::shared_ptr<LayerNormBackward> node(new LayerNormBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(*x, w ? *w : Tensor(), b ? *b : Tensor()));
+    node->x = torch::autograd::SavedVariable(*x, false);
+    node->has_w = w != nullptr;
+    if (w) node->w = torch::autograd::SavedVariable(*w, false);
+    node->mean = torch::autograd::SavedVariable(mean, false);
+    node->rstd = torch::autograd::SavedVariable(rstd, false);
+    node->x_sizes = x->sizes().vec();
+    node->M = M;
+    node->d = d;
+    node->x_stride = sx;
+    node->dtype = dtype;
+    node->w_dtype = w_dtype;
+    node->w_type = wt;
+    torch::autograd::set_history(y, node);
+  }
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay, grad_scale, copies): True
+// once done. Lists of contiguous tensors of one type each; a moment is a tensor or a pair.
+PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  FMX_ARGS(12);
+  PyObject *P = args[0], *G = args[1], *E = args[2], *S = args[3], *C = args[11];
+  FMX_ORDINARY(PyList_CheckExact(P) && PyList_CheckExact(G) && PyList_CheckExact(E) && PyList_CheckExact(S) &&
+               (C == Py_None || PyList_CheckExact(C)) && PyLong_CheckExact(args[4]));
+  const Py_ssize_t n = PyList_GET_SIZE(P);
+  FMX_ORDINARY(n > 0 && PyList_GET_SIZE(G) == n && PyList_GET_SIZE(E) == n && PyList_GET_SIZE(S) == n &&
+               (C == Py_None || PyList_GET_SIZE(C) == n));
+  const int64_t step = PyLong_AsLongLong(args[4]);
+  double h[5];
+  for (int i = 0; i < 5; ++i) {
+    FMX_ORDINARY(PyFloat_CheckExact(args[5 + i]));
+    h[i] = PyFloat_AS_DOUBLE(args[5 + i]);
+  }
+  if (step == -1 && PyErr_Occurred()) return nullptr;
+  const Tensor* scale;
+  FMX_ORDINARY(take_optional(args[10], &scale));
+  const bool eight = PyTuple_Check(PyList_GET_ITEM(E, 0));
+  auto state = [&](PyObject* o, const Tensor& p, at::ScalarType codes, void** data, float** scales) -> bool {
+    const Tensor *t, *q = nullptr;
+    if (eight) {
+      if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2) return false;
+      t = plain(PyTuple_GET_ITEM(o, 0));
+      q = plain(PyTuple_GET_ITEM(o, 1));
+      if (!q || q->scalar_type() != at::kFloat || q->numel() != (p.numel() + FMX_ADAMW_BLOCK - 1) / FMX_ADAMW_BLOCK ||
+          !q->is_contiguous() || q->device() != p.device())
+        return false;
+      *scales = static_cast<float*>(q->data_ptr());
+    } else {
+      t = plain(o);
+      *scales = nullptr;
+    }
+    if (!t || t->scalar_type() != (eight ? codes : at::kFloat) || t->numel() != p.numel() || !t->is_contiguous() ||
+        t->device() != p.device())
+      return false;
+    *data = t->data_ptr();
+    return true;
+  };
+  std::vector<fmx_adamw_tensor> table((size_t)n);
+  const Tensor* first = plain(PyList_GET_ITEM(P, 0));
+  const Tensor* first_g = plain(PyList_GET_ITEM(G, 0));
+  FMX_ORDINARY(first && first_g && here(*first));
+  const int pt = code_of(*first), gt = code_of(*first_g);
+  int ct = -1;
+  FMX_ORDINARY(pt >= 0 && gt >= 0 && (!scale || (scale->numel() == 1 && scale->scalar_type() == at::kFloat &&
+                                                 scale->device() == first->device())));
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const Tensor *p = plain(PyList_GET_ITEM(P, i)), *g = plain(PyList_GET_ITEM(G, i)), *c = nullptr;
+    FMX_ORDINARY(p && g && (C == Py_None || take_optional(PyList_GET_ITEM(C, i), &c)));
+    FMX_ORDINARY(code_of(*p) == pt && code_of(*g) == gt && p->is_contiguous() && g->is_contiguous() &&
+                 p->sizes() == g->sizes() && p->device() == first->device() && g->device() == first->device());
+    if (c) {
+      if (ct < 0) ct = code_of(*c);
+      FMX_ORDINARY(code_of(*c) == ct && (ct == FMX_DTYPE_F16 || ct == FMX_DTYPE_BF16) && pt == FMX_DTYPE_F32 &&
+                   c->is_contiguous() && c->sizes() == p->sizes() && c->device() == p->device());
+    }
+    fmx_adamw_tensor& t = table[(size_t)i];
+    t.param = p->data_ptr();
+    t.grad = g->const_data_ptr();
+    t.copy = c ? c->data_ptr() : nullptr;
+    t.n = p->numel();
+    FMX_ORDINARY(state(PyList_GET_ITEM(E, i), *p, at::kChar, &t.exp_avg, &t.exp_avg_scale) &&
+                 state(PyList_GET_ITEM(S, i), *p, at::kByte, &t.exp_avg_sq, &t.exp_avg_sq_scale));
+  }
+  FMX_ORDINARY(gt == pt || gt == FMX_DTYPE_F32 || (pt == FMX_DTYPE_F32 && (ct < 0 || ct == gt)));
+  void* s = stream_of(*first);
+  const int rc = unlocked([&] {
+    return fmx_adamw(pt, gt, ct < 0 ? FMX_DTYPE_BF16 : ct, eight ? 8 : 32, table.data(), n, step, h[0], h[1], h[2],
+                     h[3], h[4], scale ? scale->const_data_ptr<float>() : nullptr, s);
+  });
+  if (rc) return failed(rc);
+  for (Py_ssize_t i = 0; i < n; ++i) {  // written in place
+    plain(PyList_GET_ITEM(P, i))->unsafeGetTensorImpl()->bump_version();
+    if (C != Py_None && PyList_GET_ITEM(C, i) != Py_None)
+      plain(PyList_GET_ITEM(C, i))->unsafeGetTensorImpl()->bump_version();
+  }
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// adamw_decode(codes, scales): float32 values in the codes' shape
+PyObject* adamw_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  FMX_ARGS(2);
+  const Tensor *c = plain(args[0]), *q = plain(args[1]);
+  FMX_ORDINARY(c && q && (c->scalar_type() == at::kChar || c->scalar_type() == at::kByte) && c->is_contiguous() &&
+               q->scalar_type() == at::kFloat && q->is_contiguous() && q->device() == c->device() && here(*c) &&
+               q->numel() == (c->numel() + FMX_ADAMW_BLOCK - 1) / FMX_ADAMW_BLOCK);
+  Tensor out = at::empty(c->sizes(), q->options());
+  void* s = stream_of(*c);
+  const int rc = unlocked([&] {
+    return fmx_adamw_decode(c->scalar_type() == at::kByte, c->const_data_ptr(), q->const_data_ptr<float>(), c->numel(),
+                            out.data_ptr<float>(), s);
+  });
+  return rc ? failed(rc) : THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 #define FMX_METHOD(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FMX_METHOD(score),   FMX_METHOD(batched), FMX_METHOD(sparse),
                          FMX_METHOD(topk),    FMX_METHOD(int8),    FMX_METHOD(packed),
                          FMX_METHOD(int8_packed), FMX_METHOD(forward), FMX_METHOD(backward),
+                         FMX_METHOD(linear),  FMX_METHOD(layer_norm), FMX_METHOD(adamw),
+                         FMX_METHOD(adamw_decode),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .flash_maxsim import _abi_ready, _check_devices, _device_guard
@@ -82,6 +83,7 @@ class _LinearFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         xk, wk, z = ctx.saved_tensors
         (N, K), M, dev = ctx.sizes, xk.size(0), xk.device
@@ -112,6 +114,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     None, "relu", "gelu" (by the normal distribution function), "gelu_tanh" (its
     tanh form) or "silu". Differentiable in x, weight, bias and residual.
     """
+    out = _lib.native().linear(x, weight, bias, ACTIVATIONS.get(activation, -1), residual)
+    if out is not None:
+        return out
     _check(x, weight, bias, activation, residual)
     act = ACTIVATIONS[activation]
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):

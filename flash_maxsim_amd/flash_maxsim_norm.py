@@ -13,6 +13,7 @@ fixed order: the same inputs give the same bits.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .flash_maxsim import _check_devices, _device_guard
@@ -74,6 +75,7 @@ class _LayerNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         rows, weight, mean, rstd = ctx.saved_tensors
         M, d = rows.shape
@@ -104,6 +106,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     where None); the variance is the biased one. The result has x's shape and
     type; differentiable in x, weight and bias.
     """
+    out = _lib.native().layer_norm(x, weight, bias, eps)
+    if out is not None:
+        return out
     _check(x, weight, bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNormFn.apply(x, weight, bias, float(eps))

@@ -60,6 +60,9 @@ def dequantize_adamw(state: AdamW8bitState) -> torch.Tensor:
     """The float32 values of an 8-bit moment, in its codes' shape: the first
     moment of int8 codes, the second (the root's square) of uint8 codes."""
     codes, scales = state
+    out = _lib.native().adamw_decode(codes, scales)
+    if out is not None:
+        return out
     if codes.dtype not in (torch.int8, torch.uint8) or scales.dtype != torch.float32:
         raise TypeError(f"an 8-bit moment holds int8 or uint8 codes and float32 scales, got {codes.dtype}, {scales.dtype}")
     assert scales.numel() == -(-codes.numel() // BLOCK), "one scale per 256 codes"
@@ -150,10 +153,13 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step: int, lr: float = 1e-3
     copies, a list with a float16 or bfloat16 tensor (or None) for each
     parameter, receives the new float32 parameters rounded.
     """
+    step, betas = int(step), (float(betas[0]), float(betas[1]))
+    lr, eps, weight_decay = float(lr), float(eps), float(weight_decay)
+    if _lib.native().adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, *betas, eps, weight_decay, grad_scale, copies):
+        return
     params = list(params)
     copies = None if copies is None else list(copies)
-    _step_python(params, grads, exp_avgs, exp_avg_sqs, int(step), float(lr), (float(betas[0]), float(betas[1])),
-                 float(eps), float(weight_decay), grad_scale, copies)
+    _step_python(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, grad_scale, copies)
     torch.autograd.graph.increment_version(params if copies is None else params + [c for c in copies if c is not None])
 
 

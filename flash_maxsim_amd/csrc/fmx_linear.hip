@@ -177,11 +177,11 @@ struct Side {
   static constexpr int kChunks = T * BK / 8;            // 16-byte chunks of a stage
   static constexpr int kLoads = kChunks / NT;           // of a thread
   static constexpr int kRow = MAJ ? T / 8 : BK / 8;     // chunks of an LDS row
-  static_assert(kChunks % NT == 0, "a stage splits evenly over the threads");
+  static_assert(kChunks % NT == 0 && NT % (8 * kRow) == 0 || MAJ, "a stage splits evenly over the threads");
   const char* base;
   int64_t step;        // bytes from one stage to the next
   uint32_t off[kLoads];
-  int k[kLoads];       // the chunk's (first) k inside its stage
+  int kfirst;          // the first chunk's (first) k inside its stage
 
   // position of chunk ch of LDS row r is ch ^ key(r)
   static __device__ __forceinline__ int key(int r) {
@@ -197,12 +197,13 @@ struct Side {
 #pragma unroll
     for (int n = 0; n < kLoads; ++n) {
       const int at = n * NT + tid, r = at / kRow, ch = (at % kRow) ^ key(r);
-      k[n] = MAJ ? r : ch * 8;
+      if (n == 0) kfirst = MAJ ? r : ch * 8;
       const int row = MAJ ? ch * 8 : r;  // of i or j, inside the tile
       off[n] = r0 + row < rows ? (uint32_t)(r * stride * 2 + ch * 16) : kOOB;
     }
   }
-  // Stage `it` to LDS; kleft: k values left from its start (those at or past it read as zeros)
+  // Stage `it` to LDS; kleft: k values left from its start (those at or past it read as zeros).
+  // K-major: a thread's chunks lie 8 rows (or a multiple) apart, so they hold the same k.
   __device__ __forceinline__ void issue(unsigned char* lds, int it, int64_t kleft, int wave) const {
     const rsrc_t r = make_rsrc(base + it * step, kleft > 0 ? 0x7fffffffu : 0u);
     if (kleft >= BK || kleft <= 0) {
@@ -211,23 +212,21 @@ struct Side {
     } else {
 #pragma unroll
       for (int n = 0; n < kLoads; ++n)
-        dma16_lds<false>(r, lds + (n * NT + wave * 64) * 16, k[n] < kleft ? off[n] : kOOB);
+        dma16_lds<false>(r, lds + (n * NT + wave * 64) * 16,
+                         kfirst + (MAJ ? n * (NT / kRow) : 0) < kleft ? off[n] : kOOB);
     }
   }
 };
 
 // Fragment reader of one operand: 16 rows x 32 k of fragment f, k-step kk.
-template <bool MAJ, bool PAIR, int T, int BK, int F>
+template <bool MAJ, bool PAIR, int T, int BK>
 struct Frags {
-  uint32_t at[MAJ ? F : BK / 32];
+  uint32_t at[MAJ ? 1 : BK / 32];
   __device__ __forceinline__ Frags(int row0, int lane) {
     const int c = lane & 15, g = lane >> 4;
     if constexpr (MAJ) {
       const int q = c >> 2, s = c & 3, r = 8 * g + q;
-      const int key = Side<MAJ, PAIR, T, BK, 64>::key(r);
-#pragma unroll
-      for (int f = 0; f < F; ++f)
-        at[f] = (uint32_t)(r * T * 2 + (((row0 >> 3) + 2 * f + (s >> 1)) ^ key) * 16 + 8 * (s & 1));
+      at[0] = (uint32_t)(r * T * 2 + (((row0 >> 3) + (s >> 1)) ^ Side<MAJ, PAIR, T, BK, 64 * 8>::key(r)) * 16 + 8 * (s & 1));
     } else {
       const int row = row0 + (PAIR ? 8 * (c >> 2) + (c & 3) : c);
       const int key = BK == 64 ? c & 7 : (c >> 1) & 3;
@@ -238,9 +237,11 @@ struct Frags {
   __device__ __forceinline__ u32x4_t read(const unsigned char* lds, int f, int kk) const {
     if constexpr (MAJ) {
       typedef __attribute__((address_space(3))) s16x4_t lds_t;
-      // k rows 32 kk + 8 g + 0..3, then + 4..7 (the key of row r + 4 is that of r)
-      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(lds + at[f] + (32 * kk) * T * 2));
-      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(lds + at[f] + (32 * kk + 4) * T * 2));
+      // chunk 2 f further: row0 is a multiple of 8 chunks and rows are powers of two apart, so it is an
+      // exclusive or of the address; k rows 32 kk + 8 g + 0..3, then + 4..7 (the key of row r + 4 is that of r)
+      const unsigned char* p = lds + (at[0] ^ (uint32_t)(32 * f));
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(p + (32 * kk) * T * 2));
+      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(p + (32 * kk + 4) * T * 2));
       const u32x2_t l = __builtin_bit_cast(u32x2_t, lo), h = __builtin_bit_cast(u32x2_t, hi);
       return u32x4_t{l[0], l[1], h[0], h[1]};
     } else {
@@ -296,8 +297,8 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
 
   const SideA sa(a.A, a.sa, i0, a.I, k0, tid);
   const SideB sb(a.B, a.sb, j0, a.Jr, k0, tid);
-  const Frags<AMAJ, false, TI, BK, FI> fa(wi * FI * 16, lane);
-  const Frags<BMAJ, !BMAJ, TJ, BK, FJ> fb(wj * FJ * 16, lane);
+  const Frags<AMAJ, false, TI, BK> fa(wi * FI * 16, lane);
+  const Frags<BMAJ, !BMAJ, TJ, BK> fb(wj * FJ * 16, lane);
 
   f32x4_t acc[FI][FJ];
 #pragma unroll
@@ -317,30 +318,46 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
     sa.issue(lds, it, left, wave);
     sb.issue(lds + TI * BK * 2, it, left, wave);
   };
+  // Fragments of one k-step of 32: a set is multiplied while the next one is read. Before the first read of a new
+  // stage every wave waits for its own DMA of it and for its reads of the old one, then all meet; the
+  // old one's buffer takes the DMA of the stage NS ahead.
+  constexpr int KK = BK / 32;
+  static_assert(KK == 2 || NS % 2 == 0, "the two sets alternate over an unrolled round of stages");
+  u32x4_t va[2][FI], vb[2][FJ];
+  auto read = [&](auto set, const unsigned char* lds, int kk) __attribute__((always_inline)) {
+    constexpr int Z = decltype(set)::value % 2;
+#pragma unroll
+    for (int y = 0; y < FJ; ++y) vb[Z][y] = fb.read(lds + TI * BK * 2, y, kk);
+#pragma unroll
+    for (int x = 0; x < FI; ++x) va[Z][x] = fa.read(lds, x, kk);
+  };
+  auto multiply = [&](auto set) __attribute__((always_inline)) {
+    constexpr int Z = decltype(set)::value % 2;
+#pragma unroll
+    for (int x = 0; x < FI; ++x)
+#pragma unroll
+      for (int y = 0; y < FJ; ++y) acc[x][y] = mfma16x16x32<BF>(vb[Z][y], va[Z][x], acc[x][y]);
+  };
   auto stage = [&](auto s, int it) __attribute__((always_inline)) {
-    constexpr int S = decltype(s)::value;
+    constexpr int S = decltype(s)::value, H = S * KK;
+    if constexpr (KK == 2) {
+      read(std::integral_constant<int, H + 1>{}, buffer(s), 1);
+      multiply(std::integral_constant<int, H>{});
+    }
     wait_vmem<(NS - 2) * LOADS>();
     stage_barrier();
-    issue(buffer(std::integral_constant<int, S + NS - 1>{}), it + NS - 1);
-    const unsigned char* la = buffer(s);
-    const unsigned char* lb = la + TI * BK * 2;
-#pragma unroll
-    for (int kk = 0; kk < BK / 32; ++kk) {
-      u32x4_t va[FI], vb[FJ];
-#pragma unroll
-      for (int y = 0; y < FJ; ++y) vb[y] = fb.read(lb, y, kk);
-#pragma unroll
-      for (int x = 0; x < FI; ++x) va[x] = fa.read(la, x, kk);
-#pragma unroll
-      for (int x = 0; x < FI; ++x)
-#pragma unroll
-        for (int y = 0; y < FJ; ++y) acc[x][y] = mfma16x16x32<BF>(vb[y], va[x], acc[x][y]);
-    }
+    issue(buffer(s), it + NS);
+    read(std::integral_constant<int, H + KK>{}, buffer(std::integral_constant<int, S + 1>{}), 0);
+    multiply(std::integral_constant<int, H + KK - 1>{});
   };
 
   issue(lds0, 0);
-  if constexpr (NS > 2) issue(lds1, 1);
-  if constexpr (NS > 3) issue(lds2, 2);
+  issue(lds1, 1);
+  if constexpr (NS > 2) issue(lds2, 2);
+  if constexpr (NS > 3) issue(lds3, 3);
+  wait_vmem<(NS - 1) * LOADS>();
+  stage_barrier();
+  read(std::integral_constant<int, 0>{}, lds0, 0);
   for (int it = 0; it < nit; it += NS) {
     stage(std::integral_constant<int, 0>{}, it);
     if (it + 1 < nit) stage(std::integral_constant<int, 1>{}, it + 1);
@@ -485,7 +502,7 @@ hipError_t launch(const LinearArgs& a, int tile, hipStream_t s) {
   const int64_t grid = a.ti * a.tj * a.splits;
   switch (tile) {
     case kTile256: run<BF, AMAJ, BMAJ, 2, 4, 8, 4, 64, 2, EPI>(a, grid, s); break;
-    case kTile128x256: run<BF, AMAJ, BMAJ, 2, 2, 4, 8, 32, 3, EPI>(a, grid, s); break;
+    case kTile128x256: run<BF, AMAJ, BMAJ, 2, 4, 8, 4, 32, 4, EPI>(a, grid, s); break;
     case kTile128: run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 64, 2, EPI>(a, grid, s); break;
     default: run<BF, AMAJ, BMAJ, 2, 2, 2, 2, 64, 4, EPI>(a, grid, s); break;
   }
@@ -510,7 +527,7 @@ LinearPlan linear_plan(int64_t I, int64_t J, int64_t K) {
     p.tile = I > 64 && J > 64 && K >= 4096 ? kTile128 : kTile64;
   static const char* force = getenv("FMX_TILE");
   if (force) p.tile = force[0] - '0';
-  const int64_t ti = p.tile == kTile256 ? 256 : p.tile == kTile64 ? 64 : 128;
+  const int64_t ti = p.tile >= kTile128x256 ? 256 : p.tile == kTile64 ? 64 : 128;
   const int64_t tj = p.tile == kTile256 || p.tile == kTile128x256 ? 256 : p.tile == kTile64 ? 64 : 128;
   p.ti = (I + ti - 1) / ti;
   p.tj = (J + tj - 1) / tj;

@@ -68,7 +68,7 @@ hipError_t launch_adamw_decode(const void* codes, bool second, const float* scal
 // ---- linear (fmx_linear.hip) ----
 
 enum LinearForm { kLinearForward, kLinearInput, kLinearWeight };  // y, dx, dw
-enum LinearTile { kTile64, kTile128, kTile128x256, kTile256 };
+enum LinearTile { kTile64, kTile128, kTile256 };
 
 // C[I, J] = sum over k < K of A(i, k) B(j, k); see fmx_linear.hip for the operands of each form.
 struct LinearArgs {

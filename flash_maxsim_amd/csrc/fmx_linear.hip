@@ -171,13 +171,15 @@ __device__ __forceinline__ void finish(const LinearArgs& a, int64_t i, int64_t j
 
 // ---- the product ----
 
+constexpr int BK = 64;  // k values of a stage: 128-byte rows of a K-major operand, whole lines of memory
+
 // One operand's side of a tile: T rows (of i or j), from row r0 on.
-template <bool MAJ, bool PAIR, int T, int BK, int NT>
+template <bool MAJ, bool PAIR, int T, int NT>
 struct Side {
   static constexpr int kChunks = T * BK / 8;            // 16-byte chunks of a stage
   static constexpr int kLoads = kChunks / NT;           // of a thread
   static constexpr int kRow = MAJ ? T / 8 : BK / 8;     // chunks of an LDS row
-  static_assert(kChunks % NT == 0 && NT % (8 * kRow) == 0 || MAJ, "a stage splits evenly over the threads");
+  static_assert(kChunks % NT == 0 && (MAJ || NT % (8 * kRow) == 0), "a stage splits evenly over the threads");
   const char* base;
   int64_t step;        // bytes from one stage to the next
   uint32_t off[kLoads];
@@ -187,8 +189,7 @@ struct Side {
   static __device__ __forceinline__ int key(int r) {
     if constexpr (MAJ) return (2 * (r & 3) | (kRow > 8 ? ((r >> 3) & 1) << 3 : 0)) & (kRow - 1);
     // PAIR: the rows of one fragment are 0-3, 8-11, 16-19, 24-27 (and 4 more)
-    if constexpr (BK == 64) return PAIR ? (r & 3) | ((r >> 3) & 1) << 2 : r & 7;
-    return PAIR ? ((r >> 1) & 1) | ((r >> 3) & 1) << 1 : (r >> 1) & 3;
+    return PAIR ? (r & 3) | ((r >> 3) & 1) << 2 : r & 7;
   }
 
   __device__ __forceinline__ Side(const void* p, int64_t stride, int64_t r0, int64_t rows, int64_t k0, int tid) {
@@ -204,32 +205,26 @@ struct Side {
   }
   // Stage `it` to LDS; kleft: k values left from its start (those at or past it read as zeros).
   // K-major: a thread's chunks lie 8 rows (or a multiple) apart, so they hold the same k.
-  __device__ __forceinline__ void issue(unsigned char* lds, int it, int64_t kleft, int wave) const {
-    const rsrc_t r = make_rsrc(base + it * step, kleft > 0 ? 0x7fffffffu : 0u);
-    if (kleft >= BK || kleft <= 0) {
+  __device__ __forceinline__ void issue(unsigned char* lds, int it, int kleft, int wave) const {
+    const rsrc_t r = make_rsrc(base + it * step, 0x7fffffffu);
 #pragma unroll
-      for (int n = 0; n < kLoads; ++n) dma16_lds<false>(r, lds + (n * NT + wave * 64) * 16, off[n]);
-    } else {
-#pragma unroll
-      for (int n = 0; n < kLoads; ++n)
-        dma16_lds<false>(r, lds + (n * NT + wave * 64) * 16,
-                         kfirst + (MAJ ? n * (NT / kRow) : 0) < kleft ? off[n] : kOOB);
-    }
+    for (int n = 0; n < kLoads; ++n)
+      dma16_lds<false>(r, lds + (n * NT + wave * 64) * 16, kfirst + (MAJ ? n * (NT / kRow) : 0) < kleft ? off[n] : kOOB);
   }
 };
 
 // Fragment reader of one operand: 16 rows x 32 k of fragment f, k-step kk.
-template <bool MAJ, bool PAIR, int T, int BK>
+template <bool MAJ, bool PAIR, int T>
 struct Frags {
   uint32_t at[MAJ ? 1 : BK / 32];
   __device__ __forceinline__ Frags(int row0, int lane) {
     const int c = lane & 15, g = lane >> 4;
     if constexpr (MAJ) {
       const int q = c >> 2, s = c & 3, r = 8 * g + q;
-      at[0] = (uint32_t)(r * T * 2 + (((row0 >> 3) + (s >> 1)) ^ Side<MAJ, PAIR, T, BK, 64 * 8>::key(r)) * 16 + 8 * (s & 1));
+      at[0] = (uint32_t)(r * T * 2 + (((row0 >> 3) + (s >> 1)) ^ Side<MAJ, PAIR, T, 64 * 8>::key(r)) * 16 + 8 * (s & 1));
     } else {
       const int row = row0 + (PAIR ? 8 * (c >> 2) + (c & 3) : c);
-      const int key = BK == 64 ? c & 7 : (c >> 1) & 3;
+      const int key = c & 7;  // of the row, and of all others of the lane's fragments
 #pragma unroll
       for (int kk = 0; kk < BK / 32; ++kk) at[kk] = (uint32_t)(row * BK * 2 + ((kk * 4 + g) ^ key) * 16);
     }
@@ -261,17 +256,18 @@ __device__ __forceinline__ void stage_barrier() {
   __asm__ volatile("" ::: "memory");
 }
 
-template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int BK, int NS, bool EPI>
+template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int NS, bool EPI>
 __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
   constexpr int TI = WI * FI * 16, TJ = WJ * FJ * 16, NT = WI * WJ * 64;
   constexpr int BYTES = (TI + TJ) * BK * 2;
-  using SideA = Side<AMAJ, false, TI, BK, NT>;
-  using SideB = Side<BMAJ, !BMAJ, TJ, BK, NT>;
+  using SideA = Side<AMAJ, false, TI, NT>;
+  using SideB = Side<BMAJ, !BMAJ, TJ, NT>;
   constexpr int LOADS = SideA::kLoads + SideB::kLoads;
   __shared__ __attribute__((aligned(1024))) unsigned char lds0[BYTES];
   __shared__ __attribute__((aligned(1024))) unsigned char lds1[BYTES];
   __shared__ __attribute__((aligned(1024))) unsigned char lds2[NS > 2 ? BYTES : 16];
-  __shared__ __attribute__((aligned(1024))) unsigned char lds3[NS > 3 ? BYTES : 16];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds3[NS > 2 ? BYTES : 16];
+  static_assert(NS == 2 || NS == 4, "stage buffers");
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -297,8 +293,8 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
 
   const SideA sa(a.A, a.sa, i0, a.I, k0, tid);
   const SideB sb(a.B, a.sb, j0, a.Jr, k0, tid);
-  const Frags<AMAJ, false, TI, BK> fa(wi * FI * 16, lane);
-  const Frags<BMAJ, !BMAJ, TJ, BK> fb(wj * FJ * 16, lane);
+  const Frags<AMAJ, false, TI> fa(wi * FI * 16, lane);
+  const Frags<BMAJ, !BMAJ, TJ> fb(wj * FJ * 16, lane);
 
   f32x4_t acc[FI][FJ];
 #pragma unroll
@@ -314,57 +310,73 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
     return lds3;
   };
   auto issue = [&](unsigned char* lds, int it) __attribute__((always_inline)) {
-    const int64_t left = kn - (int64_t)it * BK;
+    const int left = (int)kn - it * BK;
     sa.issue(lds, it, left, wave);
     sb.issue(lds + TI * BK * 2, it, left, wave);
   };
   // Fragments of one k-step of 32: a set is multiplied while the next one is read. Before the first read of a new
   // stage every wave waits for its own DMA of it and for its reads of the old one, then all meet; the
   // old one's buffer takes the DMA of the stage NS ahead.
-  constexpr int KK = BK / 32;
-  static_assert(KK == 2 || NS % 2 == 0, "the two sets alternate over an unrolled round of stages");
+  constexpr std::integral_constant<int, 0> set0{};
+  constexpr std::integral_constant<int, 1> set1{};
   u32x4_t va[2][FI], vb[2][FJ];
   auto read = [&](auto set, const unsigned char* lds, int kk) __attribute__((always_inline)) {
-    constexpr int Z = decltype(set)::value % 2;
+    constexpr int Z = decltype(set)::value;
 #pragma unroll
     for (int y = 0; y < FJ; ++y) vb[Z][y] = fb.read(lds + TI * BK * 2, y, kk);
 #pragma unroll
     for (int x = 0; x < FI; ++x) va[Z][x] = fa.read(lds, x, kk);
   };
   auto multiply = [&](auto set) __attribute__((always_inline)) {
-    constexpr int Z = decltype(set)::value % 2;
+    constexpr int Z = decltype(set)::value;
 #pragma unroll
     for (int x = 0; x < FI; ++x)
 #pragma unroll
       for (int y = 0; y < FJ; ++y) acc[x][y] = mfma16x16x32<BF>(vb[Z][y], va[Z][x], acc[x][y]);
   };
-  auto stage = [&](auto s, int it) __attribute__((always_inline)) {
-    constexpr int S = decltype(s)::value, H = S * KK;
-    if constexpr (KK == 2) {
-      read(std::integral_constant<int, H + 1>{}, buffer(s), 1);
-      multiply(std::integral_constant<int, H>{});
+  // The order of the instructions after a barrier: the multiplication of the set at hand runs from the
+  // first one on, between the loads and reads.
+  auto interleave = [&]() __attribute__((always_inline)) {
+    constexpr int READS = FJ * (BMAJ ? 2 : 1) + FI * (AMAJ ? 2 : 1), M = FI * FJ, R = READS > 12 ? 2 : 1;
+#pragma unroll
+    for (int n = 0; n < LOADS; ++n) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
     }
+#pragma unroll
+    for (int n = 0; n < READS / R; ++n) {
+      __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+  };
+  auto stage = [&](auto s, int it) __attribute__((always_inline)) {
+    read(set1, buffer(s), 1);
+    multiply(set0);
     wait_vmem<(NS - 2) * LOADS>();
     stage_barrier();
+    __builtin_amdgcn_sched_barrier(0);
     issue(buffer(s), it + NS);
-    read(std::integral_constant<int, H + KK>{}, buffer(std::integral_constant<int, S + 1>{}), 0);
-    multiply(std::integral_constant<int, H + KK - 1>{});
+    read(set0, buffer(std::integral_constant<int, decltype(s)::value + 1>{}), 0);
+    multiply(set1);
+    interleave();
+    __builtin_amdgcn_sched_barrier(0);
   };
 
   issue(lds0, 0);
   issue(lds1, 1);
-  if constexpr (NS > 2) issue(lds2, 2);
-  if constexpr (NS > 3) issue(lds3, 3);
+  if constexpr (NS > 2) {
+    issue(lds2, 2);
+    issue(lds3, 3);
+  }
   wait_vmem<(NS - 1) * LOADS>();
   stage_barrier();
-  read(std::integral_constant<int, 0>{}, lds0, 0);
+  read(set0, lds0, 0);
   for (int it = 0; it < nit; it += NS) {
     stage(std::integral_constant<int, 0>{}, it);
     if (it + 1 < nit) stage(std::integral_constant<int, 1>{}, it + 1);
     if constexpr (NS > 2) {
       if (it + 2 < nit) stage(std::integral_constant<int, 2>{}, it + 2);
-    }
-    if constexpr (NS > 3) {
       if (it + 3 < nit) stage(std::integral_constant<int, 3>{}, it + 3);
     }
   }
@@ -492,19 +504,18 @@ __global__ void __launch_bounds__(1024) linear_db_kernel(const float* part, int 
   }
 }
 
-template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int BK, int NS, bool EPI>
+template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int NS, bool EPI>
 void run(const LinearArgs& a, int64_t grid, hipStream_t s) {
-  linear_kernel<BF, AMAJ, BMAJ, WI, WJ, FI, FJ, BK, NS, EPI><<<(unsigned)grid, WI * WJ * 64, 0, s>>>(a);
+  linear_kernel<BF, AMAJ, BMAJ, WI, WJ, FI, FJ, NS, EPI><<<(unsigned)grid, WI * WJ * 64, 0, s>>>(a);
 }
 
 template <bool BF, bool AMAJ, bool BMAJ, bool EPI>
 hipError_t launch(const LinearArgs& a, int tile, hipStream_t s) {
   const int64_t grid = a.ti * a.tj * a.splits;
   switch (tile) {
-    case kTile256: run<BF, AMAJ, BMAJ, 2, 4, 8, 4, 64, 2, EPI>(a, grid, s); break;
-    case kTile128x256: run<BF, AMAJ, BMAJ, 2, 4, 8, 4, 32, 4, EPI>(a, grid, s); break;
-    case kTile128: run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 64, 2, EPI>(a, grid, s); break;
-    default: run<BF, AMAJ, BMAJ, 2, 2, 2, 2, 64, 4, EPI>(a, grid, s); break;
+    case kTile256: run<BF, AMAJ, BMAJ, 2, 4, 8, 4, 2, EPI>(a, grid, s); break;
+    case kTile128: run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 2, EPI>(a, grid, s); break;
+    default: run<BF, AMAJ, BMAJ, 2, 2, 2, 2, 4, EPI>(a, grid, s); break;
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
@@ -527,8 +538,7 @@ LinearPlan linear_plan(int64_t I, int64_t J, int64_t K) {
     p.tile = I > 64 && J > 64 && K >= 4096 ? kTile128 : kTile64;
   static const char* force = getenv("FMX_TILE");
   if (force) p.tile = force[0] - '0';
-  const int64_t ti = p.tile >= kTile128x256 ? 256 : p.tile == kTile64 ? 64 : 128;
-  const int64_t tj = p.tile == kTile256 || p.tile == kTile128x256 ? 256 : p.tile == kTile64 ? 64 : 128;
+  const int64_t ti = p.tile == kTile256 ? 256 : p.tile == kTile64 ? 64 : 128, tj = ti;
   p.ti = (I + ti - 1) / ti;
   p.tj = (J + tj - 1) / tj;
   // split k where the tiles leave compute units idle, at 512 k values a part at least

@@ -36,8 +36,10 @@ struct NormArgs {
 int norm_parts(int64_t M, int d);  // rows of NormArgs::part
 hipError_t launch_norm_fwd(int kind, const NormArgs& a, bool vec, hipStream_t s);
 hipError_t launch_norm_bwd(int kind, const NormArgs& a, bool vec, hipStream_t s);
-// out0[c] = sum over parts of part[p][0][c], out1 likewise; either may be null.
-hipError_t launch_norm_join(int out_kind, const float* part, int parts, int d, void* out0, void* out1, hipStream_t s);
+// Sums over `parts` rows of n0 + n1 float32 values: the first n0 columns to out0, the others to out1, in
+// out_kind's type; either may be null. No rows: zeros.
+hipError_t launch_join(int out_kind, const float* part, int parts, int64_t n0, int64_t n1, void* out0, void* out1,
+                       hipStream_t s);
 
 // ---- AdamW (fmx_adamw.hip) ----
 
@@ -68,7 +70,7 @@ hipError_t launch_adamw_decode(const void* codes, bool second, const float* scal
 // ---- linear (fmx_linear.hip) ----
 
 enum LinearForm { kLinearForward, kLinearInput, kLinearWeight };  // y, dx, dw
-enum LinearTile { kTile64, kTile128, kTile256 };
+enum LinearTile { kTile64, kTile128, kTile128Deep, kTile256 };  // deep: four stages in LDS, not two
 
 // C[I, J] = sum over k < K of A(i, k) B(j, k); see fmx_linear.hip for the operands of each form.
 struct LinearArgs {
@@ -106,11 +108,11 @@ struct DzArgs {
   void* dz;               // [M, Np] 16-bit, or null
   float* part;            // [parts][N] column sums, or null
   int64_t sdy, M, N, Np;  // Np: N rounded up to 8
+  int lanes;              // of a row, a power of two; set by launch_linear_dz
   int act;
   int vec_dy, vec_z;
 };
 int linear_dz_parts(int64_t M, int64_t N);
-hipError_t launch_linear_dz(bool bf16, const DzArgs& a, int parts, hipStream_t s);
-hipError_t launch_linear_db(bool bf16, const float* part, int parts, int64_t N, void* db, hipStream_t s);
+hipError_t launch_linear_dz(bool bf16, DzArgs a, int parts, hipStream_t s);
 
 }  // namespace fmx

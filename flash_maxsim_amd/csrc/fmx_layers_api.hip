@@ -143,8 +143,8 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (M == 0) {  // no rows: zeros
     hipError_t e = hipSuccess;
-    if (dw) e = fmx::launch_linear_db(bf, nullptr, 0, N * K, dw, s);
-    if (db && e == hipSuccess) e = fmx::launch_linear_db(bf, nullptr, 0, N, db, s);
+    if (dw) e = fmx::launch_join(dtype, nullptr, 0, N * K, 0, dw, nullptr, s);
+    if (db && e == hipSuccess) e = fmx::launch_join(dtype, nullptr, 0, N, 0, db, nullptr, s);
     return hip_status(e, "fmx_linear_bwd launch");
   }
   const LinearBwdWs ws = linear_bwd_ws(M, N, K);
@@ -172,7 +172,7 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
     a.vec_z = N % 8 == 0 && aligned(z, 16);
     const int parts = fmx::linear_dz_parts(M, N);
     e = fmx::launch_linear_dz(bf, a, parts, s);
-    if (db && e == hipSuccess) e = fmx::launch_linear_db(bf, a.part, parts, N, db, s);
+    if (db && e == hipSuccess) e = fmx::launch_join(dtype, a.part, parts, N, 0, db, nullptr, s);
     if (e != hipSuccess) return hip_status(e, "fmx_linear_bwd launch");
   }
   fmx::LinearArgs a = {};
@@ -274,7 +274,7 @@ int fmx_layer_norm_bwd(int dtype, const void* x, int64_t x_stride, const void* d
   }
   if (sums) {
     const int parts = M > 0 ? fmx::norm_parts(M, (int)d) : 0;  // no rows: zeros
-    return hip_status(fmx::launch_norm_join(w_dtype, static_cast<const float*>(workspace), parts, (int)d, dw, db, s),
+    return hip_status(fmx::launch_join(w_dtype, static_cast<const float*>(workspace), parts, d, d, dw, db, s),
                       "fmx_layer_norm_bwd launch");
   }
   return ok();

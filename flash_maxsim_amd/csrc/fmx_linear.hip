@@ -21,8 +21,6 @@
 // its tiles are many, is split over k: float32 partial tiles go to the
 // workspace and a second kernel adds them in order (no atomics) and applies
 // the epilogue.
-#include <stdlib.h>
-
 #include <type_traits>
 
 #include "fmx_device.h"
@@ -100,57 +98,50 @@ __device__ __forceinline__ float act_slope(float z, int act) {
   }
 }
 
-// ---- epilogue: V consecutive outputs j .. j + V - 1 of row i ----
+// ---- epilogue: 8 consecutive outputs j .. j + 7 of row i, of which `left` exist ----
 
-template <int V>
-__device__ __forceinline__ void store16(void* base, int64_t at, int left, const float (&v)[V], bool bf, bool vec) {
+__device__ __forceinline__ void store16(void* base, int64_t at, int left, const float (&v)[8], bool bf, bool vec) {
   uint16_t* p = static_cast<uint16_t*>(base) + at;
-  if (vec && left >= V) {
-    if constexpr (V == 8) {
-      *reinterpret_cast<u32x4_t*>(p) = u32x4_t{pack2(v[0], v[1], bf), pack2(v[2], v[3], bf), pack2(v[4], v[5], bf),
-                                               pack2(v[6], v[7], bf)};
-    } else {
-      *reinterpret_cast<u32x2_t*>(p) = u32x2_t{pack2(v[0], v[1], bf), pack2(v[2], v[3], bf)};
-    }
+  if (vec && left >= 8) {
+    *reinterpret_cast<u32x4_t*>(p) = u32x4_t{pack2(v[0], v[1], bf), pack2(v[2], v[3], bf), pack2(v[4], v[5], bf),
+                                             pack2(v[6], v[7], bf)};
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i)
+    for (int i = 0; i < 8; ++i)
       if (i < left) p[i] = (uint16_t)pack2(v[i], 0.0f, bf);
   }
 }
 
-template <int V>
-__device__ __forceinline__ void load16(float (&v)[V], const void* base, int64_t at, int left, bool bf, bool vec) {
+__device__ __forceinline__ u32x4_t load_raw(const void* base, int64_t at, int left, bool vec) {
   const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-  if (vec && left >= V) {
-    uint32_t w[V / 2];
-    if constexpr (V == 8) {
-      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(p);
+  if (vec && left >= 8) return *reinterpret_cast<const u32x4_t*>(p);
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = x[i];
-    } else {
-      const u32x2_t x = *reinterpret_cast<const u32x2_t*>(p);
-      w[0] = x[0];
-      w[1] = x[1];
-    }
+  for (int i = 0; i < 8; ++i)
+    if (i < left) w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
+  return u32x4_t{w[0], w[1], w[2], w[3]};
+}
+__device__ __forceinline__ void unpack8(float (&v)[8], const u32x4_t& w, bool bf) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = unpack((i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xffffu, bf);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = i < left ? unpack(p[i], bf) : 0.0f;
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t x = w[i / 2];
+    v[i] = unpack((i & 1) ? x >> 16 : x & 0xffffu, bf);
   }
 }
+__device__ __forceinline__ void load16(float (&v)[8], const void* base, int64_t at, int left, bool bf, bool vec) {
+  unpack8(v, load_raw(base, at, left, vec), bf);
+}
 
-// Products in v (the bias added already) to their place: z, the activation, the residual, y.
-template <int V, bool EPI>
-__device__ __forceinline__ void finish(const LinearArgs& a, int64_t i, int64_t j, float (&v)[V], bool bf) {
-  const int left = (int)(a.J - j < V ? a.J - j : V);
+// Products in v (the bias added already) to their place: z, the activation, the residual in `res`, y.
+template <bool EPI>
+__device__ __forceinline__ void finish(const LinearArgs& a, int64_t i, int64_t j, int left, float (&v)[8],
+                                       const u32x4_t& res, bool bf) {
   if constexpr (EPI) {
-    if (a.z) store16<V>(a.z, i * a.J + j, left, v, bf, a.vec_out);
-    switch (a.act) {  // uniform: one test a group of V
+    if (a.z) store16(a.z, i * a.J + j, left, v, bf, a.vec_out);
+    switch (a.act) {  // uniform: one test a group of 8
 #define FMX_CASE(A) \
   case A: \
-    _Pragma("unroll") for (int k = 0; k < V; ++k) v[k] = act_value(v[k], A); \
+    _Pragma("unroll") for (int k = 0; k < 8; ++k) v[k] = act_value(v[k], A); \
     break
       FMX_CASE(FMX_ACT_RELU);
       FMX_CASE(FMX_ACT_GELU);
@@ -160,13 +151,13 @@ __device__ __forceinline__ void finish(const LinearArgs& a, int64_t i, int64_t j
       default: break;
     }
     if (a.res) {
-      float r[V];
-      load16<V>(r, a.res, i * a.sres + j, left, bf, a.vec_res);
+      float r[8];
+      unpack8(r, res, bf);
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[k] += r[k];
+      for (int k = 0; k < 8; ++k) v[k] += r[k];
     }
   }
-  store16<V>(a.y, i * a.J + j, left, v, bf, a.vec_out);
+  store16(a.y, i * a.J + j, left, v, bf, a.vec_out);
 }
 
 // ---- the product ----
@@ -382,30 +373,55 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
   }
   wait_vmem<0>();  // the stages past the end: their (empty) DMA writes no longer reach LDS after this wave ends
 
+  // A lane's results: row c of each i fragment, and of a pair of j fragments 8 columns. K-major B: its rows
+  // were read so that they are consecutive. Row-major B: fragments y and y + 1 hold columns 4 g .. + 3 each, of
+  // which an exchange between neighbouring 16-lane groups makes 8 of y (even g) or of y + 1 (odd g).
   const int c = lane & 15, g = lane >> 4;
-  constexpr int V = BMAJ ? 4 : 8, PER = V / 4;  // consecutive outputs of a lane
+  auto pair = [&](int x, int y, float (&v)[8]) __attribute__((always_inline)) {
 #pragma unroll
-  for (int y = 0; y < FJ / PER; ++y) {
-    const int64_t j = j0 + wj * FJ * 16 + y * 16 * PER + V * g;
-    if (j >= a.J) continue;
-    float b[V];
+    for (int k = 0; k < 4; ++k) {
+      v[k] = acc[x][y][k];
+      v[4 + k] = acc[x][y + 1][k];
+      if constexpr (BMAJ) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v[k]),
+                                                        __builtin_bit_cast(uint32_t, v[4 + k]), false, false);
+        const uint32_t r0 = r[0], r1 = r[1];
+        v[k] = __builtin_bit_cast(float, r0);
+        v[4 + k] = __builtin_bit_cast(float, r1);
+      }
+    }
+  };
 #pragma unroll
-    for (int k = 0; k < V; ++k) b[k] = 0.0f;
-    if (EPI && a.bias && a.splits == 1)
-      load16<V>(b, a.bias, j, (int)(a.J - j < V ? a.J - j : V), BF, a.vec_bias);
+  for (int y = 0; y < FJ; y += 2) {
+    const int64_t j = j0 + wj * FJ * 16 + y * 16 + (BMAJ ? (g & 1) * 16 + (g >> 1) * 8 : 8 * g);
+    const int left = (int)(a.J - j < 8 ? a.J - j : 8);  // columns inside; none: nothing is stored
+    float b[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) b[k] = 0.0f;
+    if (EPI && a.bias && a.splits == 1 && left > 0) load16(b, a.bias, j, left, BF, a.vec_bias);
+    // all of the residual before the first store: loads behind stores would wait for them
+    u32x4_t res[FI];
+    if (EPI && a.res && a.splits == 1) {
+#pragma unroll
+      for (int x = 0; x < FI; ++x) {
+        const int64_t i = i0 + wi * FI * 16 + x * 16 + c;
+        res[x] = i < a.I && left > 0 ? load_raw(a.res, i * a.sres + j, left, a.vec_res) : u32x4_t{0u, 0u, 0u, 0u};
+      }
+    }
 #pragma unroll
     for (int x = 0; x < FI; ++x) {
       const int64_t i = i0 + wi * FI * 16 + x * 16 + c;
-      if (i >= a.I) continue;
+      float v[8];
+      pair(x, y, v);  // by all lanes: the exchange reads its partners' registers
+      if (i >= a.I || left <= 0) continue;
       if (a.splits > 1) {
         float* p = a.part + (split * a.I + i) * a.Jp + j;  // Jp: J rounded up to 8
-#pragma unroll
-        for (int k = 0; k < PER; ++k) *reinterpret_cast<f32x4_t*>(p + 4 * k) = acc[x][y * PER + k];
+        *reinterpret_cast<f32x4_t*>(p) = f32x4_t{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4_t*>(p + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
       } else {
-        float v[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = acc[x][y * PER + k / 4][k % 4] + b[k];
-        finish<V, EPI>(a, i, j, v, BF);
+        for (int k = 0; k < 8; ++k) v[k] += b[k];
+        finish<EPI>(a, i, j, left, v, res[x], BF);
       }
     }
   }
@@ -422,7 +438,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = 0.0f;
     const int left = (int)(a.J - j < 8 ? a.J - j : 8);
-    if (EPI && a.bias) load16<8>(v, a.bias, j, left, BF, a.vec_bias);
+    if (EPI && a.bias) load16(v, a.bias, j, left, BF, a.vec_bias);
     f32x4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
@@ -434,29 +450,30 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a) {
       v[k] += s0[k];
       v[4 + k] += s1[k];
     }
-    finish<8, EPI>(a, i, j, v, BF);
+    const u32x4_t res = EPI && a.res ? load_raw(a.res, i * a.sres + j, left, a.vec_res) : u32x4_t{0u, 0u, 0u, 0u};
+    finish<EPI>(a, i, j, left, v, res, BF);
   }
 }
 
 // dz = dy act'(z) in 16 bits (rows padded with zeros to Np), and the column sums of the
-// unrounded dz over each workgroup's rows. A lane holds 8 columns, a wave 512; the
-// four waves of a workgroup take rows in turn.
+// unrounded dz over each workgroup's rows. A lane holds 8 columns; a row takes as few lanes as hold it (up to
+// 64), so a workgroup takes 256 / lanes rows at a time.
 template <bool BF>
 __global__ void __launch_bounds__(256) linear_dz_kernel(DzArgs a) {
-  __shared__ float sums[4][512];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t j = (int64_t)blockIdx.x * 512 + lane * 8;
+  __shared__ float sums[256 * 9];
+  const int lanes = a.lanes, rows = 256 / lanes, lane = threadIdx.x & (lanes - 1), row = threadIdx.x / lanes;
+  const int64_t j0 = (int64_t)blockIdx.x * lanes * 8, j = j0 + lane * 8;
   const int left = (int)(a.N - j < 0 ? 0 : a.N - j < 8 ? a.N - j : 8);
   float s[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) s[k] = 0.0f;
   if (j < a.Np) {
-    for (int64_t i = (int64_t)blockIdx.y * 4 + wave; i < a.M; i += (int64_t)gridDim.y * 4) {
+    for (int64_t i = (int64_t)blockIdx.y * rows + row; i < a.M; i += (int64_t)gridDim.y * rows) {
       float v[8];
-      load16<8>(v, a.dy, i * a.sdy + j, left, BF, a.vec_dy);
+      load16(v, a.dy, i * a.sdy + j, left, BF, a.vec_dy);
       if (a.z) {
         float z[8];
-        load16<8>(z, a.z, i * a.N + j, left, BF, a.vec_z);
+        load16(z, a.z, i * a.N + j, left, BF, a.vec_z);
         switch (a.act) {
 #define FMX_CASE(A) \
   case A: \
@@ -470,37 +487,20 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(DzArgs a) {
           default: break;
         }
       }
-      if (a.dz) store16<8>(a.dz, i * a.Np + j, 8, v, BF, true);
+      if (a.dz) store16(a.dz, i * a.Np + j, 8, v, BF, true);
 #pragma unroll
       for (int k = 0; k < 8; ++k) s[k] += v[k];
     }
   }
   if (!a.part) return;
+  // column k of a lane at a pitch of 9: the lanes' writes fall in different banks
 #pragma unroll
-  for (int k = 0; k < 8; ++k) sums[wave][lane * 8 + k] = s[k];
+  for (int k = 0; k < 8; ++k) sums[threadIdx.x * 9 + k] = s[k];
   __syncthreads();
-  for (int c = threadIdx.x; c < 512; c += 256) {
-    const int64_t col = (int64_t)blockIdx.x * 512 + c;
-    if (col < a.N) a.part[(int64_t)blockIdx.y * a.N + col] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
-  }
-}
-
-// db: the columns of the partial rows, 64 a workgroup, the rows over its 16 waves.
-template <typename O>
-__global__ void __launch_bounds__(1024) linear_db_kernel(const float* part, int parts, int64_t N, O* db) {
-  __shared__ float sums[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t j = (int64_t)blockIdx.x * 64 + lane;
-  float s = 0.0f;
-  if (j < N)
-    for (int p = wave; p < parts; p += 16) s += part[p * N + j];
-  sums[wave][lane] = s;
-  __syncthreads();
-  if (wave == 0 && j < N) {
-    s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s += sums[i][lane];
-    db[j] = (O)s;
+  for (int c = threadIdx.x; c < lanes * 8; c += 256) {
+    float t = 0.0f;
+    for (int r = 0; r < rows; ++r) t += sums[(r * lanes + c / 8) * 9 + c % 8];
+    if (j0 + c < a.N) a.part[(int64_t)blockIdx.y * a.N + j0 + c] = t;
   }
 }
 
@@ -515,6 +515,7 @@ hipError_t launch(const LinearArgs& a, int tile, hipStream_t s) {
   switch (tile) {
     case kTile256: run<BF, AMAJ, BMAJ, 2, 4, 8, 4, 2, EPI>(a, grid, s); break;
     case kTile128: run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 2, EPI>(a, grid, s); break;
+    case kTile128Deep: run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 4, EPI>(a, grid, s); break;
     default: run<BF, AMAJ, BMAJ, 2, 2, 2, 2, 4, EPI>(a, grid, s); break;
   }
   hipError_t e = hipGetLastError();
@@ -526,36 +527,49 @@ hipError_t launch(const LinearArgs& a, int tile, hipStream_t s) {
 
 }  // namespace
 
+// Time of a product by tile and split, in us, from times measured on one MI355X: a stage of 64 k with a compute unit's
+// workgroups alone and all there, and what a tile costs besides (first loads, epilogue). Sizes that take it
+// the other way, measured / by this rule (bf16):
+//   16384 x 4096, k 1024: 256 tiles 132 / 127, 128 tiles 158 / 158      8192 x 1024, k 4096: 128 tiles 62 / 69, 256 99 / 101
+//   24576 x 128, k 2048: 128 deep 34 / 23 (bound by HBM), 64 45 / 30    2048 x 1024, k 1024: 64 tiles 10 / 10, 128 16 / 16
+//   128 x 2048, k 24576: 128 deep in 16 parts 33 / 25, 128 in 32 36 / 27
+//   1024 x 4096, k 7777: 256 in 4 parts 69 / 73, 128 deep 84 / 75, 128 in 2 85 / 76
+struct TileCost {
+  int tile, size, per_cu;
+  double alone, full, rest;
+};
+constexpr TileCost kCosts[] = {{kTile256, 256, 1, 1.45, 1.45, 8.5},
+                               {kTile128, 128, 2, 0.75, 1.02, 3.4},
+                               {kTile128Deep, 128, 1, 0.58, 0.58, 4.0},
+                               {kTile64, 64, 2, 0.33, 0.43, 3.0}};
+
 LinearPlan linear_plan(int64_t I, int64_t J, int64_t K) {
-  LinearPlan p;
   const int64_t cus = layer_cus();
-  auto count = [&](int64_t ti, int64_t tj) { return ((I + ti - 1) / ti) * ((J + tj - 1) / tj); };
-  if (count(256, 256) >= cus)
-    p.tile = kTile256;
-  else if (count(128, 128) >= cus / 2)
-    p.tile = kTile128;
-  else
-    p.tile = I > 64 && J > 64 && K >= 4096 ? kTile128 : kTile64;
-  static const char* force = getenv("FMX_TILE");
-  if (force) p.tile = force[0] - '0';
-  const int64_t ti = p.tile == kTile256 ? 256 : p.tile == kTile64 ? 64 : 128, tj = ti;
-  p.ti = (I + ti - 1) / ti;
-  p.tj = (J + tj - 1) / tj;
-  // split k where the tiles leave compute units idle, at 512 k values a part at least
-  const int64_t tiles = p.ti * p.tj, want = p.tile == kTile256 ? cus : 2 * cus;
-  int64_t splits = tiles * 2 > want ? 1 : want / tiles;
-  const int64_t most = K / 512;
-  if (splits > most) splits = most;
-  if (splits > 64) splits = 64;
-  if (splits < 1) splits = 1;
-  int64_t per = (K + splits - 1) / splits;
-  per = (per + 63) / 64 * 64;
-  p.split_k = per;
-  p.splits = (int)((K + per - 1) / per);
-  if (p.splits < 1) p.splits = 1;
-  // operand rows that an XCD's L2 (4 MB) holds beside the other operand's: runs of 8 tile rows
-  p.band = 8;
-  return p;
+  LinearPlan best = {};
+  double least = 0;
+  for (const TileCost& c : kCosts) {
+    const int64_t ti = (I + c.size - 1) / c.size, tj = (J + c.size - 1) / c.size, slots = cus * c.per_cu;
+    for (int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+      int64_t per = ((K + want - 1) / want + BK - 1) / BK * BK;
+      if (want > 1 && per < 4 * BK) break;  // a part shorter than its loads' latency
+      const int64_t splits = (K + per - 1) / per, n = ti * tj * splits, whole = n / slots, left = n % slots;
+      const double stages = (double)((per + BK - 1) / BK);
+      double us = whole * (stages * c.full + c.rest);
+      if (left) us += stages * (left > cus ? c.full : c.alone) + c.rest;
+      // partial products written and read, mostly in the caches, and the second kernel
+      if (splits > 1) us += 2.5 + (double)splits * (double)I * (double)J * 8.0 / 8e6;
+      if (best.splits == 0 || us < least) {
+        least = us;
+        best.tile = c.tile;
+        best.splits = (int)splits;
+        best.ti = ti;
+        best.tj = tj;
+        best.split_k = per;
+      }
+    }
+  }
+  best.band = 8;  // tile rows walked together: with 8 columns or more of tiles, their operands fit an XCD's L2 (4 MB)
+  return best;
 }
 
 size_t linear_part_bytes(const LinearPlan& p, int64_t I, int64_t J) {
@@ -580,29 +594,33 @@ hipError_t launch_linear(bool bf16, LinearForm form, LinearArgs a, const LinearP
   }
 }
 
+namespace {
+int dz_lanes(int64_t N) {
+  int lanes = 1;
+  while (lanes < 64 && lanes * 8 < N) lanes *= 2;
+  return lanes;
+}
+}  // namespace
+
 int linear_dz_parts(int64_t M, int64_t N) {
-  const int64_t cols = (N + 511) / 512;
-  int64_t parts = (int64_t)layer_cus() * 8 / cols;  // about eight workgroups a CU
-  const int64_t rows = (M + 15) / 16;               // four rows a wave at least
-  if (parts > rows) parts = rows;
-  return (int)(parts < 1 ? 1 : parts > 65535 ? 65535 : parts);
+  const int64_t lanes = dz_lanes(N), rows = 256 / lanes, cols = (N + lanes * 8 - 1) / (lanes * 8);
+  int64_t parts = (int64_t)layer_cus() * 8 / cols;      // about eight workgroups a CU
+  if (parts > 256) parts = 256;                         // rows that the second kernel adds
+  const int64_t most = (M + rows * 4 - 1) / (rows * 4);  // four rows a thread at least
+  if (parts > most) parts = most;
+  return (int)(parts < 1 ? 1 : parts);
 }
 
-hipError_t launch_linear_dz(bool bf16, const DzArgs& a, int parts, hipStream_t s) {
-  const dim3 grid((unsigned)((a.Np + 511) / 512), (unsigned)parts);
+hipError_t launch_linear_dz(bool bf16, DzArgs a, int parts, hipStream_t s) {
+  a.lanes = dz_lanes(a.N);
+  // without the sums to hold them together, the rows go to as many workgroups as they fill
+  const int64_t rows = 4 * 256 / a.lanes, most = (a.M + rows - 1) / rows;
+  const int64_t y = a.part ? parts : most < 65535 ? most : 65535;
+  const dim3 grid((unsigned)((a.Np + a.lanes * 8 - 1) / (a.lanes * 8)), (unsigned)y);
   if (bf16)
     linear_dz_kernel<true><<<grid, 256, 0, s>>>(a);
   else
     linear_dz_kernel<false><<<grid, 256, 0, s>>>(a);
-  return hipGetLastError();
-}
-
-hipError_t launch_linear_db(bool bf16, const float* part, int parts, int64_t N, void* db, hipStream_t s) {
-  const unsigned grid = (unsigned)((N + 63) / 64);
-  if (bf16)
-    linear_db_kernel<__bf16><<<grid, 1024, 0, s>>>(part, parts, N, static_cast<__bf16*>(db));
-  else
-    linear_db_kernel<_Float16><<<grid, 1024, 0, s>>>(part, parts, N, static_cast<_Float16*>(db));
   return hipGetLastError();
 }
 

@@ -100,11 +100,14 @@ __device__ __forceinline__ float act_slope(float z, int act) {
 
 // ---- epilogue: 8 consecutive outputs j .. j + 7 of row i, of which `left` exist ----
 
+__device__ __forceinline__ u32x4_t pack8(const float (&v)[8], bool bf) {
+  return u32x4_t{pack2(v[0], v[1], bf), pack2(v[2], v[3], bf), pack2(v[4], v[5], bf), pack2(v[6], v[7], bf)};
+}
+
 __device__ __forceinline__ void store16(void* base, int64_t at, int left, const float (&v)[8], bool bf, bool vec) {
   uint16_t* p = static_cast<uint16_t*>(base) + at;
   if (vec && left >= 8) {
-    *reinterpret_cast<u32x4_t*>(p) = u32x4_t{pack2(v[0], v[1], bf), pack2(v[2], v[3], bf), pack2(v[4], v[5], bf),
-                                             pack2(v[6], v[7], bf)};
+    *reinterpret_cast<u32x4_t*>(p) = pack8(v, bf);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -132,24 +135,29 @@ __device__ __forceinline__ void load16(float (&v)[8], const void* base, int64_t 
   unpack8(v, load_raw(base, at, left, vec), bf);
 }
 
+// The activation of 8 values: one (uniform) test for all of them.
+__device__ __forceinline__ void activate(float (&v)[8], int act) {
+  switch (act) {
+#define FMX_CASE(A) \
+  case A: \
+    _Pragma("unroll") for (int k = 0; k < 8; ++k) v[k] = act_value(v[k], A); \
+    break
+    FMX_CASE(FMX_ACT_RELU);
+    FMX_CASE(FMX_ACT_GELU);
+    FMX_CASE(FMX_ACT_GELU_TANH);
+    FMX_CASE(FMX_ACT_SILU);
+#undef FMX_CASE
+    default: break;
+  }
+}
+
 // Products in v (the bias added already) to their place: z, the activation, the residual in `res`, y.
 template <bool EPI>
 __device__ __forceinline__ void finish(const LinearArgs& a, int64_t i, int64_t j, int left, float (&v)[8],
                                        const u32x4_t& res, bool bf) {
   if constexpr (EPI) {
     if (a.z) store16(a.z, i * a.J + j, left, v, bf, a.vec_out);
-    switch (a.act) {  // uniform: one test a group of 8
-#define FMX_CASE(A) \
-  case A: \
-    _Pragma("unroll") for (int k = 0; k < 8; ++k) v[k] = act_value(v[k], A); \
-    break
-      FMX_CASE(FMX_ACT_RELU);
-      FMX_CASE(FMX_ACT_GELU);
-      FMX_CASE(FMX_ACT_GELU_TANH);
-      FMX_CASE(FMX_ACT_SILU);
-#undef FMX_CASE
-      default: break;
-    }
+    activate(v, a.act);
     if (a.res) {
       float r[8];
       unpack8(r, res, bf);
@@ -391,6 +399,67 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
       }
     }
   };
+  if (FJ == 4 && a.splits == 1 && a.vec_out && i0 + TI <= a.I && j0 + TJ <= a.J) {
+    // A whole tile: a wave turns its 16 x 64 blocks into rows of 128 bytes, whole lines of memory, in LDS
+    // that nothing is read from or loaded into any more.
+    wait_vmem<0>();
+    stage_barrier();
+    unsigned char* mine = (wave < WI * WJ / 2 ? lds0 : lds1) + (wave % (WI * WJ / 2)) * (BYTES / (WI * WJ / 2));
+    const int64_t jw = j0 + wj * FJ * 16;
+    float b[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) b[h][k] = 0.0f;
+      if (EPI && a.bias) load16(b[h], a.bias, jw + 32 * h + (BMAJ ? (g & 1) * 16 + (g >> 1) * 8 : 8 * g), 8, BF, a.vec_bias);
+    }
+    const int row = lane >> 3, ch = lane & 7;
+    auto put = [&](int x, int h, const u32x4_t& w) __attribute__((always_inline)) {
+      const int at = 4 * h + (BMAJ ? (g & 1) * 2 + (g >> 1) : g);
+      *reinterpret_cast<u32x4_t*>(mine + x * 2048 + c * 128 + ((at ^ (c & 7)) << 4)) = w;
+    };
+    auto flush = [&](int x, void* out) __attribute__((always_inline)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(mine + x * 2048 + (row + 8 * h) * 128 + ((ch ^ row) << 4));
+        const int64_t i = i0 + wi * FI * 16 + x * 16 + row + 8 * h;
+        *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(out) + i * a.J + jw + ch * 8) = w;
+      }
+    };
+#pragma unroll
+    for (int x = 0; x < FI; ++x) {
+      float v[2][8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        pair(x, 2 * h, v[h]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[h][k] += b[h][k];
+      }
+      if constexpr (EPI) {
+        if (a.z) {
+          put(x, 0, pack8(v[0], BF));
+          put(x, 1, pack8(v[1], BF));
+          flush(x, a.z);
+        }
+        activate(v[0], a.act);
+        activate(v[1], a.act);
+        if (a.res) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int64_t i = i0 + wi * FI * 16 + x * 16 + c, j = jw + 32 * h + 8 * g;
+            float r[8];
+            load16(r, a.res, i * a.sres + j, 8, BF, a.vec_res);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[h][k] += r[k];
+          }
+        }
+      }
+      put(x, 0, pack8(v[0], BF));
+      put(x, 1, pack8(v[1], BF));
+      flush(x, a.y);
+    }
+    return;
+  }
 #pragma unroll
   for (int y = 0; y < FJ; y += 2) {
     const int64_t j = j0 + wj * FJ * 16 + y * 16 + (BMAJ ? (g & 1) * 16 + (g >> 1) * 8 : 8 * g);
@@ -568,7 +637,7 @@ LinearPlan linear_plan(int64_t I, int64_t J, int64_t K) {
       }
     }
   }
-  best.band = 8;  // tile rows walked together: with 8 columns or more of tiles, their operands fit an XCD's L2 (4 MB)
+  best.band = 4;  // tile rows walked together
   return best;
 }
 

@@ -33,9 +33,10 @@ struct NormArgs {
 };
 
 // kind: FMX_DTYPE_*
-int norm_parts(int64_t M, int d);  // rows of NormArgs::part
+int norm_parts(int64_t M, int d);  // rows of NormArgs::part at most
 hipError_t launch_norm_fwd(int kind, const NormArgs& a, bool vec, hipStream_t s);
-hipError_t launch_norm_bwd(int kind, const NormArgs& a, bool vec, hipStream_t s);
+// *parts: the rows of NormArgs::part written
+hipError_t launch_norm_bwd(int kind, const NormArgs& a, bool vec, int* parts, hipStream_t s);
 // Sums over `parts` rows of n0 + n1 float32 values: the first n0 columns to out0, the others to out1, in
 // out_kind's type; either may be null. No rows: zeros.
 hipError_t launch_join(int out_kind, const float* part, int parts, int64_t n0, int64_t n1, void* out0, void* out1,

@@ -228,7 +228,8 @@ int fmx_layer_norm(int dtype, const void* x, int64_t x_stride, int w_dtype, cons
   a.d = (int)d;
   a.w32 = w_dtype == FMX_DTYPE_F32;
   a.eps = (float)eps;
-  const bool vec = d % V == 0 && x_stride % V == 0 && aligned(x, 16) && aligned(y, 16);
+  const bool vec = d % V == 0 && x_stride % V == 0 && aligned(x, 16) && aligned(y, 16) &&
+                   aligned(weight, 16) && aligned(bias, 16);
   return hip_status(fmx::launch_norm_fwd(dtype, a, vec, static_cast<hipStream_t>(stream)), "fmx_layer_norm launch");
 }
 
@@ -253,6 +254,7 @@ int fmx_layer_norm_bwd(int dtype, const void* x, int64_t x_stride, const void* d
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(FMX_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace_bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);
+  int parts = 0;  // no rows: zeros
   if (M > 0 && (dx || sums)) {
     fmx::NormArgs a = {};
     a.x = x;
@@ -268,12 +270,11 @@ int fmx_layer_norm_bwd(int dtype, const void* x, int64_t x_stride, const void* d
     a.d = (int)d;
     a.w32 = w_dtype == FMX_DTYPE_F32;
     const bool vec = d % V == 0 && x_stride % V == 0 && dy_stride % V == 0 && aligned(x, 16) && aligned(dy, 16) &&
-                     aligned(dx, 16);
-    const hipError_t e = fmx::launch_norm_bwd(dtype, a, vec, s);
+                     aligned(dx, 16) && aligned(weight, 16);
+    const hipError_t e = fmx::launch_norm_bwd(dtype, a, vec, &parts, s);
     if (e != hipSuccess) return hip_status(e, "fmx_layer_norm_bwd launch");
   }
   if (sums) {
-    const int parts = M > 0 ? fmx::norm_parts(M, (int)d) : 0;  // no rows: zeros
     return hip_status(fmx::launch_join(w_dtype, static_cast<const float*>(workspace), parts, d, d, dw, db, s),
                       "fmx_layer_norm_bwd launch");
   }

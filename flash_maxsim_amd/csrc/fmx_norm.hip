@@ -27,7 +27,7 @@ namespace fmx {
 namespace {
 
 template <typename T, int V>
-struct __attribute__((aligned(sizeof(T) * V))) Pack {
+struct __attribute__((aligned(sizeof(T) * V > 16 ? 16 : sizeof(T) * V))) Pack {
   T v[V];
 };
 
@@ -94,13 +94,28 @@ struct Cols {
       }
     }
   }
-  // w or b as float32, `other` where there is none or past the row
+  // w or b as float32, `other` where there is none or past the row; 16-byte aligned where V > 1
+  template <typename W>
+  __device__ __forceinline__ void weights_of(float (&o)[NV][V], const W* w, float other) const {
+    Pack<W, V> p[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (in[j]) p[j] = *reinterpret_cast<const Pack<W, V>*>(w + col[j]);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[j][i] = in[j] ? (float)p[j].v[i] : other;
+  }
   __device__ __forceinline__ void weights(float (&o)[NV][V], const void* w, int w32, float other) const {
+    if (!w) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
+      for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        o[j][i] = !w || !in[j] ? other : w32 ? static_cast<const float*>(w)[col[j] + i] : (float)static_cast<const T*>(w)[col[j] + i];
+        for (int i = 0; i < V; ++i) o[j][i] = other;
+    } else if (w32) {
+      weights_of(o, static_cast<const float*>(w), other);
+    } else {
+      weights_of(o, static_cast<const T*>(w), other);
     }
   }
 };
@@ -112,9 +127,6 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_kernel(NormArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Cols<T, V, NV, NW> c(wave, lane, a.d);
-  float w[NV][V], b[NV][V];
-  c.weights(w, a.w, a.w32, 1.0f);
-  c.weights(b, a.b, a.w32, 0.0f);
   const float inv = 1.0f / (float)a.d;
   const int64_t step = (int64_t)gridDim.x * NG;
   const T* x0 = static_cast<const T*>(a.x);
@@ -122,6 +134,9 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_kernel(NormArgs a) {
   Pack<T, V> x[NV], next[NV];
   int64_t row = (int64_t)blockIdx.x * NG + wave / NW;
   c.load(x, x0 + row * a.sx, row < a.M);
+  float w[NV][V], b[NV][V];
+  c.weights(w, a.w, a.w32, 1.0f);
+  c.weights(b, a.b, a.w32, 0.0f);
   // base, and so the number of barriers, is the same for all rows of the workgroup
   for (int64_t base = (int64_t)blockIdx.x * NG; base < a.M; base += step, row += step) {
     c.load(next, x0 + (row + step) * a.sx, row + step < a.M);
@@ -372,89 +387,105 @@ int waves_of(int d, bool bwd) {
   return !bwd && d <= 64 * kWaves * 2 * kMaxE ? kWaves : 0;
 }
 
-int grid_of(int64_t M, int d, bool bwd) {
-  const int nw = waves_of(d, bwd), rows = nw ? kWaves / nw : 1;
-  const int64_t want = (M + rows - 1) / rows;
-  // forward: up to four workgroups a CU, each with a row or more for every wave; backward: two, whose
-  // partial sums are written once each
-  const int64_t most = (int64_t)layer_cus() * (bwd ? 2 : 4);
+// Workgroups for M rows, `group` at a time: as many as run at once (per_cu on each compute unit), so that
+// all of them share the rows evenly. 65536 x 1024 bf16 forward, of whose workgroups a unit holds three:
+// four a unit 66 us, three 56.
+int grid_of(int64_t M, int group, int per_cu) {
+  const int64_t want = (M + group - 1) / group, most = (int64_t)layer_cus() * per_cu;
   return (int)(want < most ? want : most);
 }
 
+// Workgroups of this kernel that a compute unit holds.
+int held(const void* kernel) {
+  int n = 0;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, 0) != hipSuccess || n < 1) n = 1;
+  return n;
+}
+
+// Backward workgroups write their partial sums once each: two a unit at most.
+constexpr int kBwdPerCu = 2;
+
 template <typename T, int V, int E, int NW>
-void run(const NormArgs& a, bool bwd, int grid, hipStream_t s) {
+int run(const NormArgs& a, bool bwd, hipStream_t s) {
+  constexpr int group = kWaves / NW;
   if constexpr (E <= kMaxE) {
     if (bwd) {
+      static const int n = held(reinterpret_cast<const void*>(norm_bwd_kernel<T, V, E / V, NW>));
+      const int grid = grid_of(a.M, group, n < kBwdPerCu ? n : kBwdPerCu);
       norm_bwd_kernel<T, V, E / V, NW><<<grid, kThreads, 0, s>>>(a);
-      return;
+      return grid;
     }
   }
+  static const int n = held(reinterpret_cast<const void*>(norm_fwd_kernel<T, V, E / V, NW>));
+  const int grid = grid_of(a.M, group, n);
   norm_fwd_kernel<T, V, E / V, NW><<<grid, kThreads, 0, s>>>(a);
+  return grid;
 }
 
 template <typename T, int V, int NW>
-void run_nw(const NormArgs& a, bool bwd, int grid, hipStream_t s) {
+int run_nw(const NormArgs& a, bool bwd, hipStream_t s) {
   const int e = (a.d + 64 * NW - 1) / (64 * NW);  // elements a lane
   if constexpr (NW == 1) {
-    if (e <= 4 && V <= 4) return run<T, V, V <= 4 ? 4 : 8, NW>(a, bwd, grid, s);
-    if (e <= 8) return run<T, V, 8, NW>(a, bwd, grid, s);
+    if (e <= 4 && V <= 4) return run<T, V, V <= 4 ? 4 : 8, NW>(a, bwd, s);
+    if (e <= 8) return run<T, V, 8, NW>(a, bwd, s);
   }
-  if (V <= 4 && e <= 12) return run<T, V, V <= 4 ? 12 : 16, NW>(a, bwd, grid, s);
+  if (V <= 4 && e <= 12) return run<T, V, V <= 4 ? 12 : 16, NW>(a, bwd, s);
   if constexpr (NW == kWaves) {
-    if (e > 16) return run<T, V, 32, NW>(a, false, grid, s);
+    if (e > 16) return run<T, V, 32, NW>(a, false, s);
   }
-  return run<T, V, 16, NW>(a, bwd, grid, s);
+  return run<T, V, 16, NW>(a, bwd, s);
 }
 
 template <typename T, int V>
-void run_v(const NormArgs& a, int nw, bool bwd, int grid, hipStream_t s) {
+int run_v(const NormArgs& a, int nw, bool bwd, hipStream_t s) {
   switch (nw) {
-    case 1: return run_nw<T, V, 1>(a, bwd, grid, s);
-    case 2: return run_nw<T, V, 2>(a, bwd, grid, s);
-    case 4: return run_nw<T, V, 4>(a, bwd, grid, s);
-    default: return run_nw<T, V, 8>(a, bwd, grid, s);
+    case 1: return run_nw<T, V, 1>(a, bwd, s);
+    case 2: return run_nw<T, V, 2>(a, bwd, s);
+    case 4: return run_nw<T, V, 4>(a, bwd, s);
+    default: return run_nw<T, V, 8>(a, bwd, s);
   }
 }
 
+constexpr int kWideParts = 64;  // stretches of rows whose weight gradients the wide kernel sums
+
+// *parts: the rows of partial sums written, of the backward
 template <typename T>
-hipError_t launch(const NormArgs& a, bool vec, bool bwd, hipStream_t s) {
+hipError_t launch(const NormArgs& a, bool vec, bool bwd, int* parts, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const int nw = waves_of(a.d, bwd);
-  const int grid = grid_of(a.M, a.d, bwd);
   if (nw) {
-    if (vec)
-      run_v<T, V>(a, nw, bwd, grid, s);
-    else
-      run_v<T, 1>(a, nw, bwd, grid, s);
+    *parts = vec ? run_v<T, V>(a, nw, bwd, s) : run_v<T, 1>(a, nw, bwd, s);
   } else if (!bwd) {
-    norm_fwd_wide_kernel<T><<<grid, kThreads, 0, s>>>(a);
+    norm_fwd_wide_kernel<T><<<grid_of(a.M, 1, 4), kThreads, 0, s>>>(a);
   } else {
-    if (a.y) norm_dx_wide_kernel<T><<<grid, kThreads, 0, s>>>(a);
+    if (a.y) norm_dx_wide_kernel<T><<<grid_of(a.M, 1, 4), kThreads, 0, s>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.part) norm_dw_wide_kernel<T><<<dim3((a.d + 255) / 256, grid < 64 ? grid : 64), 256, 0, s>>>(a);
+    *parts = a.M < kWideParts ? (int)a.M : kWideParts;
+    if (a.part) norm_dw_wide_kernel<T><<<dim3((a.d + 255) / 256, *parts), 256, 0, s>>>(a);
   }
   return hipGetLastError();
 }
 
-hipError_t launch_kind(int kind, const NormArgs& a, bool vec, bool bwd, hipStream_t s) {
-  if (kind == FMX_DTYPE_F32) return launch<float>(a, vec, bwd, s);
-  if (kind == FMX_DTYPE_BF16) return launch<__bf16>(a, vec, bwd, s);
-  return launch<_Float16>(a, vec, bwd, s);
+hipError_t launch_kind(int kind, const NormArgs& a, bool vec, bool bwd, int* parts, hipStream_t s) {
+  if (kind == FMX_DTYPE_F32) return launch<float>(a, vec, bwd, parts, s);
+  if (kind == FMX_DTYPE_BF16) return launch<__bf16>(a, vec, bwd, parts, s);
+  return launch<_Float16>(a, vec, bwd, parts, s);
 }
 
 }  // namespace
 
 int norm_parts(int64_t M, int d) {
-  const int g = grid_of(M, d, true);
-  return waves_of(d, true) == 0 && g > 64 ? 64 : g;
+  const int nw = waves_of(d, true);
+  return nw ? grid_of(M, kWaves / nw, kBwdPerCu) : (int)(M < kWideParts ? M : kWideParts);
 }
 
 hipError_t launch_norm_fwd(int kind, const NormArgs& a, bool vec, hipStream_t s) {
-  return launch_kind(kind, a, vec, false, s);
+  int parts;
+  return launch_kind(kind, a, vec, false, &parts, s);
 }
-hipError_t launch_norm_bwd(int kind, const NormArgs& a, bool vec, hipStream_t s) {
-  return launch_kind(kind, a, vec, true, s);
+hipError_t launch_norm_bwd(int kind, const NormArgs& a, bool vec, int* parts, hipStream_t s) {
+  return launch_kind(kind, a, vec, true, parts, s);
 }
 
 hipError_t launch_join(int out_kind, const float* part, int parts, int64_t n0, int64_t n1, void* out0, void* out1,

@@ -71,7 +71,7 @@ hipError_t launch_adamw_decode(const void* codes, bool second, const float* scal
 // ---- linear (fmx_linear.hip) ----
 
 enum LinearForm { kLinearForward, kLinearInput, kLinearWeight };  // y, dx, dw
-enum LinearTile { kTile64, kTile128, kTile128Deep, kTile256 };  // deep: four stages in LDS, not two
+enum LinearTile { kTile64, kTile128, kTile128Deep, kTile256, kFewRows };  // deep: four stages in LDS, not two
 
 // C[I, J] = sum over k < K of A(i, k) B(j, k); see fmx_linear.hip for the operands of each form.
 struct LinearArgs {
@@ -99,7 +99,7 @@ struct LinearPlan {
   int splits;
   int64_t ti, tj, split_k, band;
 };
-LinearPlan linear_plan(int64_t I, int64_t J, int64_t K);
+LinearPlan linear_plan(LinearForm form, int64_t I, int64_t J, int64_t K);
 size_t linear_part_bytes(const LinearPlan& p, int64_t I, int64_t J);
 hipError_t launch_linear(bool bf16, LinearForm form, LinearArgs a, const LinearPlan& p, hipStream_t s);
 

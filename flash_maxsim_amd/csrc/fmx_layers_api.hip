@@ -69,8 +69,8 @@ LinearBwdWs linear_bwd_ws(int64_t M, int64_t N, int64_t K) {
   LinearBwdWs w;
   w.dz = round256((size_t)M * (size_t)n8 * 2);
   w.sums = round256((size_t)fmx::linear_dz_parts(M, N) * (size_t)N * sizeof(float));
-  const size_t px = fmx::linear_part_bytes(fmx::linear_plan(M, K, n8), M, K);
-  const size_t pw = fmx::linear_part_bytes(fmx::linear_plan(N, K, M), N, K);
+  const size_t px = fmx::linear_part_bytes(fmx::linear_plan(fmx::kLinearInput, M, K, n8), M, K);
+  const size_t pw = fmx::linear_part_bytes(fmx::linear_plan(fmx::kLinearWeight, N, K, M), N, K);
   w.part = round256(px > pw ? px : pw);
   return w;
 }
@@ -81,7 +81,7 @@ extern "C" {
 
 size_t fmx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (M < 1 || N < 1 || K < 1) return 0;
-  return fmx::linear_part_bytes(fmx::linear_plan(M, N, (K + 7) / 8 * 8), M, N);
+  return fmx::linear_part_bytes(fmx::linear_plan(fmx::kLinearForward, M, N, (K + 7) / 8 * 8), M, N);
 }
 
 int fmx_linear(int dtype, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
@@ -113,7 +113,7 @@ int fmx_linear(int dtype, const void* x, int64_t x_stride, const void* w, int64_
   a.vec_out = N % 8 == 0 && aligned(y, 16) && aligned(z, 16);
   a.vec_res = r_stride % 8 == 0 && aligned(residual, 16);
   a.vec_bias = aligned(bias, 16);
-  const fmx::LinearPlan p = fmx::linear_plan(M, N, a.K);
+  const fmx::LinearPlan p = fmx::linear_plan(fmx::kLinearForward, M, N, a.K);
   const size_t need = fmx::linear_part_bytes(p, M, N);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(FMX_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace_bytes);
@@ -189,7 +189,7 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
     a.y = dx;
     fmx::LinearArgs b = a;
     b.vec_out = a.vec_out && aligned(dx, 16);
-    e = fmx::launch_linear(bf, fmx::kLinearInput, b, fmx::linear_plan(M, K, n8), s);
+    e = fmx::launch_linear(bf, fmx::kLinearInput, b, fmx::linear_plan(fmx::kLinearInput, M, K, n8), s);
     if (e != hipSuccess) return hip_status(e, "fmx_linear_bwd launch");
   }
   if (dw) {
@@ -200,7 +200,7 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
     a.K = M;
     a.y = dw;
     a.vec_out = a.vec_out && aligned(dw, 16);
-    e = fmx::launch_linear(bf, fmx::kLinearWeight, a, fmx::linear_plan(N, K, M), s);
+    e = fmx::launch_linear(bf, fmx::kLinearWeight, a, fmx::linear_plan(fmx::kLinearWeight, N, K, M), s);
   }
   return hip_status(e, "fmx_linear_bwd launch");
 }

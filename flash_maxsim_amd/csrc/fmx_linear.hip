@@ -524,6 +524,73 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a) {
   }
 }
 
+// Forward of few rows (up to 16 MF): a workgroup computes 16 outputs of all rows, its eight waves take every
+// eighth k-step of 32 each, straight from memory to registers: W is read once, by N / 16 workgroups,
+// with all loads of a wave in flight, where a tile would wait for its stages one by one. The waves' sums meet in
+// LDS in the waves' order.
+template <bool BF, int MF>
+__global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
+  __shared__ __attribute__((aligned(16))) float sums[8][MF][256];
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t j0 = (int64_t)blockIdx.x * 16;
+  // rows past the end read the last one again; what comes of them is not stored
+  const int last = (int)(a.J - 1 - j0), jr = c < last ? c : last;
+  const rsrc_t rw = make_rsrc(static_cast<const uint16_t*>(a.B) + j0 * a.sb, 0x7fffffffu);
+  const rsrc_t rx = make_rsrc(a.A, 0x7fffffffu);
+  const uint32_t ow = (uint32_t)(jr * a.sb * 2);
+  uint32_t ox[MF];
+#pragma unroll
+  for (int f = 0; f < MF; ++f) ox[f] = (uint32_t)((f * 16 + c < a.I ? f * 16 + c : a.I - 1) * a.sa * 2);
+  f32x4_t acc[MF];
+#pragma unroll
+  for (int f = 0; f < MF; ++f) acc[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  constexpr int U = 4;  // k-steps in flight
+  const int K = (int)a.K;
+  for (int k0 = wave * 32; k0 < K; k0 += U * 256) {
+    u32x4_t vw[U], vx[U][MF];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * 256 + g * 8;  // chunks past K read as zeros
+      vw[u] = ld16(rw, k < K ? ow + 2 * k : kOOB);
+#pragma unroll
+      for (int f = 0; f < MF; ++f) vx[u][f] = ld16(rx, k < K ? ox[f] + 2 * k : kOOB);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int f = 0; f < MF; ++f) acc[f] = mfma16x16x32<BF>(vw[u], vx[u][f], acc[f]);
+  }
+  // lane (c, g) holds outputs j0 + 4 g .. + 3 of row c
+#pragma unroll
+  for (int f = 0; f < MF; ++f) *reinterpret_cast<f32x4_t*>(&sums[wave][f][c * 16 + 4 * g]) = acc[f];
+  __syncthreads();
+  if (threadIdx.x < MF * 32) {
+    const int f = threadIdx.x >> 5, at = (threadIdx.x & 31) * 8;  // 8 outputs of a row
+    const int64_t i = f * 16 + at / 16, j = j0 + at % 16;
+    const int left = (int)(a.J - j < 8 ? a.J - j : 8);
+    if (i < a.I && left > 0) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+      if (a.bias) load16(v, a.bias, j, left, BF, a.vec_bias);
+      const u32x4_t res = a.res ? load_raw(a.res, i * a.sres + j, left, a.vec_res) : u32x4_t{0u, 0u, 0u, 0u};
+      f32x4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        s0 += *reinterpret_cast<const f32x4_t*>(&sums[u][f][at]);
+        s1 += *reinterpret_cast<const f32x4_t*>(&sums[u][f][at + 4]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[k] += s0[k];
+        v[4 + k] += s1[k];
+      }
+      finish<true>(a, i, j, left, v, res, BF);
+    }
+  }
+}
+
 // dz = dy act'(z) in 16 bits (rows padded with zeros to Np), and the column sums of the
 // unrounded dz over each workgroup's rows. A lane holds 8 columns; a row takes as few lanes as hold it (up to
 // 64), so a workgroup takes 256 / lanes rows at a time.
@@ -578,6 +645,18 @@ void run(const LinearArgs& a, int64_t grid, hipStream_t s) {
   linear_kernel<BF, AMAJ, BMAJ, WI, WJ, FI, FJ, NS, EPI><<<(unsigned)grid, WI * WJ * 64, 0, s>>>(a);
 }
 
+template <bool BF>
+hipError_t launch_few(const LinearArgs& a, hipStream_t s) {
+  const unsigned grid = (unsigned)((a.J + 15) / 16);
+  switch ((a.I + 15) / 16) {
+    case 1: linear_few_kernel<BF, 1><<<grid, 512, 0, s>>>(a); break;
+    case 2: linear_few_kernel<BF, 2><<<grid, 512, 0, s>>>(a); break;
+    case 3: linear_few_kernel<BF, 3><<<grid, 512, 0, s>>>(a); break;
+    default: linear_few_kernel<BF, 4><<<grid, 512, 0, s>>>(a); break;
+  }
+  return hipGetLastError();
+}
+
 template <bool BF, bool AMAJ, bool BMAJ, bool EPI>
 hipError_t launch(const LinearArgs& a, int tile, hipStream_t s) {
   const int64_t grid = a.ti * a.tj * a.splits;
@@ -612,9 +691,17 @@ constexpr TileCost kCosts[] = {{kTile256, 256, 1, 1.45, 1.45, 8.5},
                                {kTile128Deep, 128, 1, 0.58, 0.58, 4.0},
                                {kTile64, 64, 2, 0.33, 0.43, 3.0}};
 
-LinearPlan linear_plan(int64_t I, int64_t J, int64_t K) {
+LinearPlan linear_plan(LinearForm form, int64_t I, int64_t J, int64_t K) {
   const int64_t cus = layer_cus();
   LinearPlan best = {};
+  // Few rows straight from memory: every workgroup reads all of x, which costs more than the tiles' waits once
+  // x is large (us, few / tiles; 32 x 768 -> 128 4.4 / 7.0, 64 x 1024 -> 4096 7.4 / 9.6, 16 x 4096 -> 1024 9.6 / 9.1,
+  // 32 x 2048 -> 128 7.6 / 7.5, 64 x 4096 -> 1024 20 / 11).
+  if (form == kLinearForward && I <= 64 && (I + 15) / 16 * K <= 4096) {
+    best.tile = kFewRows;
+    best.splits = 1;
+    return best;
+  }
   double least = 0;
   for (const TileCost& c : kCosts) {
     const int64_t ti = (I + c.size - 1) / c.size, tj = (J + c.size - 1) / c.size, slots = cus * c.per_cu;
@@ -653,6 +740,7 @@ hipError_t launch_linear(bool bf16, LinearForm form, LinearArgs a, const LinearP
   a.band = p.band;
   a.Jp = (a.J + 7) / 8 * 8;
   a.Jr = form == kLinearForward ? a.J : a.Jp;  // row-major B: whole chunks of 8 columns
+  if (p.tile == kFewRows) return bf16 ? launch_few<true>(a, s) : launch_few<false>(a, s);
   switch (form) {
     case kLinearForward:
       return bf16 ? launch<true, false, false, true>(a, p.tile, s) : launch<false, false, false, true>(a, p.tile, s);

@@ -96,6 +96,7 @@ struct LinearArgs {
 
 struct LinearPlan {
   int tile;
+  int size;               // of the tile
   int splits;
   int64_t ti, tj, split_k, band;
 };

@@ -86,6 +86,10 @@ struct LinearArgs {
   const void* res;        // forward: [I, J], row stride sres, or null
   int64_t sres;
   float* part;            // splits > 1: [splits][I][Jp]
+  float* db_part;         // dw: sums over k of A's columns, [db_parts][I]
+  int db_beside;          // dw: this product writes them, [splits][I]
+  int db_parts;
+  void* db;               // dw, splits > 1: their totals, by the second kernel; or null
   int64_t Jp;
   int64_t ti, tj;         // tiles
   int64_t split_k, band;
@@ -102,6 +106,8 @@ struct LinearPlan {
 };
 LinearPlan linear_plan(LinearForm form, int64_t I, int64_t J, int64_t K);
 size_t linear_part_bytes(const LinearPlan& p, int64_t I, int64_t J);
+// Whether the dw product of this plan adds up its A's columns beside it (its registers hold no more at 256 x 256).
+inline bool linear_sums_columns(const LinearPlan& p) { return p.tile != kTile256; }
 hipError_t launch_linear(bool bf16, LinearForm form, LinearArgs a, const LinearPlan& p, hipStream_t s);
 
 struct DzArgs {

@@ -68,9 +68,11 @@ LinearBwdWs linear_bwd_ws(int64_t M, int64_t N, int64_t K) {
   const int64_t n8 = (N + 7) / 8 * 8;
   LinearBwdWs w;
   w.dz = round256((size_t)M * (size_t)n8 * 2);
-  w.sums = round256((size_t)fmx::linear_dz_parts(M, N) * (size_t)N * sizeof(float));
+  const fmx::LinearPlan plan_w = fmx::linear_plan(fmx::kLinearWeight, N, K, M);
+  const int parts = fmx::linear_dz_parts(M, N);
+  w.sums = round256((size_t)(parts > plan_w.splits ? parts : plan_w.splits) * (size_t)N * sizeof(float));
   const size_t px = fmx::linear_part_bytes(fmx::linear_plan(fmx::kLinearInput, M, K, n8), M, K);
-  const size_t pw = fmx::linear_part_bytes(fmx::linear_plan(fmx::kLinearWeight, N, K, M), N, K);
+  const size_t pw = fmx::linear_part_bytes(plan_w, N, K);
   w.part = round256(px > pw ? px : pw);
   return w;
 }
@@ -156,13 +158,19 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
   const bool as_is = act == FMX_ACT_NONE && N % 8 == 0 && dy_stride % 8 == 0 && dy_stride >= N &&
                      dy_stride < 1 << 22 && aligned(dy, 16);
   const bool make = !as_is && (dx || dw);
+  const fmx::LinearPlan plan_w = fmx::linear_plan(fmx::kLinearWeight, N, K, M);
+  // its columns' sums come with the dw product where dy needs no pass of its own
+  const bool beside = as_is && dw && db && fmx::linear_sums_columns(plan_w);
+  const bool later = dw && db && plan_w.splits > 1;  // added up by the launch that joins dw's parts
+  const int parts = beside ? plan_w.splits : fmx::linear_dz_parts(M, N);
+  float* sums = reinterpret_cast<float*>(base + ws.dz);
   hipError_t e = hipSuccess;
-  if (make || db) {
+  if (make || (db && !beside)) {
     fmx::DzArgs a = {};
     a.dy = dy;
     a.z = act == FMX_ACT_NONE ? nullptr : z;
     a.dz = make ? base : nullptr;
-    a.part = db ? reinterpret_cast<float*>(base + ws.dz) : nullptr;
+    a.part = db ? sums : nullptr;
     a.sdy = dy_stride;
     a.M = M;
     a.N = N;
@@ -170,9 +178,8 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
     a.act = act;
     a.vec_dy = dy_stride % 8 == 0 && aligned(dy, 16);
     a.vec_z = N % 8 == 0 && aligned(z, 16);
-    const int parts = fmx::linear_dz_parts(M, N);
     e = fmx::launch_linear_dz(bf, a, parts, s);
-    if (db && e == hipSuccess) e = fmx::launch_join(dtype, a.part, parts, N, 0, db, nullptr, s);
+    if (db && !later && e == hipSuccess) e = fmx::launch_join(dtype, sums, parts, N, 0, db, nullptr, s);
     if (e != hipSuccess) return hip_status(e, "fmx_linear_bwd launch");
   }
   fmx::LinearArgs a = {};
@@ -200,7 +207,12 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
     a.K = M;
     a.y = dw;
     a.vec_out = a.vec_out && aligned(dw, 16);
-    e = fmx::launch_linear(bf, fmx::kLinearWeight, a, fmx::linear_plan(fmx::kLinearWeight, N, K, M), s);
+    a.db_part = sums;
+    a.db_beside = beside;
+    a.db_parts = parts;
+    a.db = later ? db : nullptr;
+    e = fmx::launch_linear(bf, fmx::kLinearWeight, a, plan_w, s);
+    if (beside && !later && e == hipSuccess) e = fmx::launch_join(dtype, sums, parts, N, 0, db, nullptr, s);
   }
   return hip_status(e, "fmx_linear_bwd launch");
 }

@@ -349,9 +349,26 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
     }
     __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
   };
+  // dw: the sums of A's columns (db), by a product with ones in the waves that hold the tile's first columns of C
+  constexpr bool SUMS = AMAJ && BMAJ && FI <= 4;
+  const bool sums = SUMS && a.db_beside && j0 == 0 && wj == 0;
+  f32x4_t total[SUMS ? FI : 1];
+#pragma unroll
+  for (int x = 0; x < (SUMS ? FI : 1); ++x) total[x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  auto add_up = [&](auto set) __attribute__((always_inline)) {
+    if constexpr (SUMS) {
+      const uint32_t one = BF ? 0x3f803f80u : 0x3c003c00u;
+      if (sums) {
+#pragma unroll
+        for (int x = 0; x < FI; ++x)
+          total[x] = mfma16x16x32<BF>(u32x4_t{one, one, one, one}, va[decltype(set)::value][x], total[x]);
+      }
+    }
+  };
   auto stage = [&](auto s, int it) __attribute__((always_inline)) {
     read(set1, buffer(s), 1);
     multiply(set0);
+    add_up(set0);
     wait_vmem<(NS - 2) * LOADS>();
     stage_barrier();
     __builtin_amdgcn_sched_barrier(0);
@@ -360,6 +377,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
     multiply(set1);
     interleave();
     __builtin_amdgcn_sched_barrier(0);
+    add_up(set1);
   };
 
   issue(lds0, 0);
@@ -380,6 +398,16 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
     }
   }
   wait_vmem<0>();  // the stages past the end: their (empty) DMA writes no longer reach LDS after this wave ends
+
+  if constexpr (SUMS) {
+    if (sums && lane < 16) {  // every row of the product with ones is the sums
+#pragma unroll
+      for (int x = 0; x < FI; ++x) {
+        const int64_t i = i0 + wi * FI * 16 + x * 16 + lane;
+        if (i < a.I) a.db_part[split * a.I + i] = total[x][0];
+      }
+    }
+  }
 
   // A lane's results: row c of each i fragment, and of a pair of j fragments 8 columns. K-major B: its rows
   // were read so that they are consecutive. Row-major B: fragments y and y + 1 hold columns 4 g .. + 3 each, of
@@ -496,11 +524,32 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
   }
 }
 
-// Adds the partial products of a split in their order and finishes 8 outputs a lane.
+// Adds the partial products of a split in their order and finishes 8 outputs a lane, in `groups` workgroups.
+// The workgroups after those add up db's partial sums, 16 columns each, 16 rows at a time: one launch where
+// two would follow each other.
 template <bool BF, bool EPI>
-__global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a) {
+__global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a, int groups) {
+  if ((int)blockIdx.x >= groups) {
+    __shared__ float sums[16][17];
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+    const int64_t i = (int64_t)((int)blockIdx.x - groups) * 16 + c;
+    float s = 0.0f;
+    if (i < a.I) {
+#pragma unroll 4
+      for (int p = r; p < a.db_parts; p += 16) s += a.db_part[p * a.I + i];
+    }
+    sums[r][c] = s;
+    __syncthreads();
+    if (r == 0 && i < a.I) {
+      s = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) s += sums[k][c];
+      static_cast<uint16_t*>(a.db)[i] = (uint16_t)pack2(s, 0.0f, BF);
+    }
+    return;
+  }
   const int64_t per = a.Jp / 8, n = a.I * per;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)groups * 256) {
     const int64_t i = t / per, j = (t - i * per) * 8;
     const float* p = a.part + i * a.Jp + j;
     float v[8];
@@ -668,8 +717,9 @@ hipError_t launch(const LinearArgs& a, int tile, hipStream_t s) {
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  const int64_t groups = (a.I * (a.Jp / 8) + 255) / 256;
-  linear_join_kernel<BF, EPI><<<(unsigned)(groups < 4096 ? groups : 4096), 256, 0, s>>>(a);
+  const int64_t need = (a.I * (a.Jp / 8) + 255) / 256;
+  const int groups = (int)(need < 4096 ? need : 4096);
+  linear_join_kernel<BF, EPI><<<groups + (a.db ? (int)((a.I + 15) / 16) : 0), 256, 0, s>>>(a, groups);
   return hipGetLastError();
 }
 

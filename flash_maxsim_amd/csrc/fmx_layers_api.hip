@@ -44,7 +44,7 @@ int check_linear(int dtype, int64_t x_stride, int64_t w_stride, int act, int64_t
   if (act < FMX_ACT_NONE || act > FMX_ACT_SILU) return fail(FMX_ERR_INVALID, "unknown activation %d", act);
   if (M < 0 || N < 1 || K < 1)
     return fail(FMX_ERR_INVALID, "invalid sizes M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
-  if (M >= (int64_t)1 << 31 || N >= 1 << 24 || K >= 1 << 24)
+  if (M > FMX_LINEAR_MAX_ROWS || N >= 1 << 24 || K >= 1 << 24)
     return fail(FMX_ERR_UNSUPPORTED, "M=%lld N=%lld K=%lld too large", (long long)M, (long long)N, (long long)K);
   const int64_t k8 = (K + 7) / 8 * 8;
   if (x_stride < k8 || (x_stride & 7) || w_stride < k8 || (w_stride & 7))

@@ -78,21 +78,24 @@ __device__ __forceinline__ float act_value(float z, int act) {
     default: return z;
   }
 }
+// z comes rounded to 16 bits, so it may be infinite where the forward's was not; as a factor it is kept finite, or
+// its product with a tail that is zero would be NaN. (A NaN stays one through the other factors.)
 __device__ __forceinline__ float act_slope(float z, int act) {
+  const float f = __builtin_fminf(__builtin_fmaxf(z, -1e4f), 1e4f);
   switch (act) {
     case FMX_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
     case FMX_ACT_GELU: {
       float e;
       const float p = normal_cdf(z, e);
-      return fmaf(z * 0.3989422804f, e, p);
+      return fmaf(f * 0.3989422804f, e, p);
     }
     case FMX_ACT_GELU_TANH: {
       const float s = sigmoid(1.5957691216f * z * fmaf(0.044715f, z * z, 1.0f));
-      return s + z * s * (1.0f - s) * 1.5957691216f * fmaf(0.134145f, z * z, 1.0f);
+      return s + f * s * (1.0f - s) * 1.5957691216f * fmaf(0.134145f, f * f, 1.0f);
     }
     case FMX_ACT_SILU: {
       const float s = sigmoid(z);
-      return s + z * s * (1.0f - s);
+      return s + f * s * (1.0f - s);
     }
     default: return 1.0f;
   }
@@ -786,6 +789,23 @@ size_t linear_part_bytes(const LinearPlan& p, int64_t I, int64_t J) {
 }
 
 hipError_t launch_linear(bool bf16, LinearForm form, LinearArgs a, const LinearPlan& p, hipStream_t s) {
+  // a launch has fewer than 2^32 threads: more rows than this go in several (their tiles fill the GPU, so k is whole)
+  constexpr int64_t kRows = (int64_t)1 << 24;
+  if (form != kLinearWeight && a.I > kRows && p.splits == 1) {
+    for (int64_t at = 0; at < a.I; at += kRows) {
+      LinearArgs b = a;
+      b.I = a.I - at < kRows ? a.I - at : kRows;
+      b.A = static_cast<const uint16_t*>(a.A) + at * a.sa;
+      b.y = static_cast<uint16_t*>(a.y) + at * a.J;
+      if (a.z) b.z = static_cast<uint16_t*>(a.z) + at * a.J;
+      if (a.res) b.res = static_cast<const uint16_t*>(a.res) + at * a.sres;
+      LinearPlan q = p;
+      q.ti = (b.I + p.size - 1) / p.size;
+      const hipError_t e = launch_linear(bf16, form, b, q, s);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
   a.ti = p.ti;
   a.tj = p.tj;
   a.splits = p.splits;

@@ -384,6 +384,8 @@ size_t fmx_bwd_batched_workspace_bytes(int64_t Nq, int64_t B, int64_t Lq, int64_
  * epilogue, and the optimizer step.
  */
 
+#define FMX_LINEAR_MAX_ROWS (((int64_t)1 << 31) - 4096)
+
 #define FMX_ACT_NONE 0
 #define FMX_ACT_RELU 1
 #define FMX_ACT_GELU 2      /* z Phi(z) */
@@ -401,8 +403,8 @@ size_t fmx_bwd_batched_workspace_bytes(int64_t Nq, int64_t B, int64_t Lq, int64_
  *   y         [M, N]  dtype, contiguous
  *   z         [M, N]  dtype, contiguous: x W^T + bias for the backward; or NULL
  * x and w are 16-byte aligned, their strides multiples of 8 and at least K
- * rounded up to 8; elements from K up to there are zeros. M < 2^31, K and N
- * < 2^24, strides < 2^22.
+ * rounded up to 8; elements from K up to there are zeros. M <=
+ * FMX_LINEAR_MAX_ROWS, K and N < 2^24, strides < 2^22.
  */
 int fmx_linear(int dtype, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
                const void* residual, int64_t r_stride, int act, int64_t M, int64_t N, int64_t K, void* y, void* z,

@@ -199,12 +199,32 @@ def test_values_that_are_not_finite_stay_in_their_row():
             assert set(bad) <= {3, 60} and torch.isnan(y[3]).all()
 
 
+@pytest.mark.parametrize("dtype,far", [(torch.float16, 200.0), (torch.bfloat16, 1e37)])
 @pytest.mark.parametrize("name", ["gelu", "gelu_tanh", "silu"])
-def test_extreme_arguments(name):
+def test_extreme_arguments(name, dtype, far):
     """Activations far out: the identity above, zero below, finite slopes."""
-    x = torch.tensor([[-200.0], [-30.0], [-12.0], [-6.0], [0.0], [6.0], [12.0], [30.0], [200.0]], dtype=torch.float16)
-    s = {"x": x, "w": torch.ones(1, 1, dtype=torch.float16), "b": None, "r": None, "dy": torch.ones(9, 1, dtype=torch.float16)}
+    x = torch.tensor([[-far], [-30.0], [-12.0], [-6.0], [0.0], [6.0], [12.0], [30.0], [far]], dtype=dtype)
+    s = {"x": x, "w": torch.ones(1, 1, dtype=dtype), "b": None, "r": None, "dy": torch.ones(9, 1, dtype=dtype)}
     verify(s, name)
+
+
+@pytest.mark.parametrize("name", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_arguments_past_float16(name):
+    """z beyond 65504 is infinite once it is kept in float16; the slope there is still zero below and one above."""
+    x = torch.tensor([[-300.0], [300.0]], dtype=torch.float16).cuda().requires_grad_(True)
+    w = torch.full((1, 1), 300.0, dtype=torch.float16).cuda()
+    y = fm.linear(x, w, None, name)
+    (dx,) = torch.autograd.grad(y, x, torch.ones(2, 1, dtype=torch.float16).cuda())
+    assert y[0].item() == 0 and math.isinf(y[1].item()) and dx[:, 0].tolist() == [0.0, 300.0]
+
+
+def test_gradients_are_not_differentiable_again():
+    s = make(20, 16, 24, torch.float16, 3)
+    x, w = s["x"].cuda().requires_grad_(True), s["w"].cuda()
+    for y in (fm.linear(x, w, None, "gelu"), fm.linear(x.t().contiguous().t(), w, None, "gelu"), fm.layer_norm(x)):
+        (dx,) = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            dx.float().square().sum().backward()
 
 
 @pytest.mark.parametrize("name", [None, "gelu", "gelu_tanh", "silu"])

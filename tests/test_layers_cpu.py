@@ -44,6 +44,7 @@ def linear_bwd(lib, **kw):
     (dict(ws=56), INVALID, "strides"),
     (dict(xs=1 << 22), UNSUPPORTED, "strides"),
     (dict(K=1 << 24, xs=1 << 25, ws=1 << 25), UNSUPPORTED, "too large"),
+    (dict(M=(1 << 31) - 4095), UNSUPPORTED, "too large"),
     (dict(x=None), INVALID, "non-null"),
     (dict(x=FAKE + 8), INVALID, "16-byte"),
     (dict(y=FAKE + 1), INVALID, "aligned"),

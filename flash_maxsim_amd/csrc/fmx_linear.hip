@@ -277,19 +277,21 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
 
   // Workgroups go to the eight XCDs in turn; each XCD takes a run of consecutive tiles, which share
   // operand rows in its L2. Runs of `band` tile rows are walked column by column.
-  const int64_t tiles = a.ti * a.tj;
-  int64_t id = blockIdx.x;
+  // (32-bit divisions: a launch has fewer than 2^32 threads.)
+  const uint32_t tj = (uint32_t)a.tj, ti = (uint32_t)a.ti, tiles = ti * tj, bands = (uint32_t)a.band;
+  uint32_t id = blockIdx.x;
   {
-    const int64_t total = tiles * a.splits, per = total / 8, x = id & 7, rest = total & 7;
+    const uint32_t total = tiles * (uint32_t)a.splits, per = total / 8, x = id & 7, rest = total & 7;
     id = (id >> 3) + x * per + (x < rest ? x : rest);
   }
-  const int64_t split = id / tiles;
-  int64_t t = id - split * tiles;
-  const int64_t band = t / (a.band * a.tj);
-  const int64_t rows = a.ti - band * a.band < a.band ? a.ti - band * a.band : a.band;
-  t -= band * a.band * a.tj;
-  const int64_t i0 = (band * a.band + t % rows) * TI, j0 = t / rows * TJ;
-  const int64_t k0 = split * a.split_k;
+  const uint32_t split = a.splits > 1 ? id / tiles : 0;
+  uint32_t t = id - split * tiles;
+  const uint32_t band = t / (bands * tj);
+  const uint32_t rows = ti - band * bands < bands ? ti - band * bands : bands;
+  t -= band * bands * tj;
+  const uint32_t tcol = t / rows;
+  const int64_t i0 = (int64_t)(band * bands + (t - tcol * rows)) * TI, j0 = (int64_t)tcol * TJ;
+  const int64_t k0 = (int64_t)split * a.split_k;
   const int64_t kn = a.K - k0 < a.split_k ? a.K - k0 : a.split_k;
   const int nit = (int)((kn + BK - 1) / BK);
 
@@ -407,7 +409,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
 #pragma unroll
       for (int x = 0; x < FI; ++x) {
         const int64_t i = i0 + wi * FI * 16 + x * 16 + lane;
-        if (i < a.I) a.db_part[split * a.I + i] = total[x][0];
+        if (i < a.I) a.db_part[(int64_t)split * a.I + i] = total[x][0];
       }
     }
   }
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
       pair(x, y, v);  // by all lanes: the exchange reads its partners' registers
       if (i >= a.I || left <= 0) continue;
       if (a.splits > 1) {
-        float* p = a.part + (split * a.I + i) * a.Jp + j;  // Jp: J rounded up to 8
+        float* p = a.part + ((int64_t)split * a.I + i) * a.Jp + j;  // Jp: J rounded up to 8
         *reinterpret_cast<f32x4_t*>(p) = f32x4_t{v[0], v[1], v[2], v[3]};
         *reinterpret_cast<f32x4_t*>(p + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
       } else {

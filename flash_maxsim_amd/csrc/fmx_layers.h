@@ -81,7 +81,7 @@ struct LinearArgs {
   int64_t I, J, K;        // K: a multiple of 8 where it runs along rows
   int64_t Jr;             // B's columns or rows that exist (set by launch_linear)
   void* y;                // [I, J] 16-bit, contiguous
-  void* z;                // forward: act's argument, like y; or null
+  void* slope;            // forward: act's slopes, int16 steps of 2^-14, [I, J]; or null
   const void* bias;       // forward: [J], or null
   const void* res;        // forward: [I, J], row stride sres, or null
   int64_t sres;
@@ -112,13 +112,12 @@ hipError_t launch_linear(bool bf16, LinearForm form, LinearArgs a, const LinearP
 
 struct DzArgs {
   const void* dy;         // [M, N], row stride sdy
-  const void* z;          // [M, N] contiguous, or null (no activation)
+  const void* slope;      // [M, N] contiguous, or null (no activation)
   void* dz;               // [M, Np] 16-bit, or null
   float* part;            // [parts][N] column sums, or null
   int64_t sdy, M, N, Np;  // Np: N rounded up to 8
   int lanes;              // of a row, a power of two; set by launch_linear_dz
-  int act;
-  int vec_dy, vec_z;
+  int vec_dy, vec_slope;
 };
 int linear_dz_parts(int64_t M, int64_t N);
 hipError_t launch_linear_dz(bool bf16, DzArgs a, int parts, hipStream_t s);

@@ -87,7 +87,7 @@ size_t fmx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
 }
 
 int fmx_linear(int dtype, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
-               const void* residual, int64_t r_stride, int act, int64_t M, int64_t N, int64_t K, void* y, void* z,
+               const void* residual, int64_t r_stride, int act, int64_t M, int64_t N, int64_t K, void* y, int16_t* slope,
                void* workspace, size_t workspace_bytes, void* stream) {
   const int rc = check_linear(dtype, x_stride, w_stride, act, M, N, K);
   if (rc) return rc;
@@ -95,7 +95,7 @@ int fmx_linear(int dtype, const void* x, int64_t x_stride, const void* w, int64_
   if (M == 0) return ok();
   if (!x || !w || !y) return fail(FMX_ERR_INVALID, "x, w and y must be non-null");
   if (!aligned(x, 16) || !aligned(w, 16)) return fail(FMX_ERR_INVALID, "x and w must be 16-byte aligned");
-  if (!aligned(y, 2) || !aligned(z, 2) || !aligned(bias, 2) || !aligned(residual, 2))
+  if (!aligned(y, 2) || !aligned(slope, 2) || !aligned(bias, 2) || !aligned(residual, 2))
     return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");
   fmx::LinearArgs a = {};
   a.A = x;
@@ -106,13 +106,13 @@ int fmx_linear(int dtype, const void* x, int64_t x_stride, const void* w, int64_
   a.J = N;
   a.K = (K + 7) / 8 * 8;
   a.y = y;
-  a.z = z;
+  a.slope = act == FMX_ACT_NONE ? nullptr : slope;
   a.bias = bias;
   a.res = residual;
   a.sres = r_stride;
   a.act = act;
   a.part = static_cast<float*>(workspace);
-  a.vec_out = N % 8 == 0 && aligned(y, 16) && aligned(z, 16);
+  a.vec_out = N % 8 == 0 && aligned(y, 16) && aligned(slope, 16);
   a.vec_res = r_stride % 8 == 0 && aligned(residual, 16);
   a.vec_bias = aligned(bias, 16);
   const fmx::LinearPlan p = fmx::linear_plan(fmx::kLinearForward, M, N, a.K);
@@ -130,16 +130,16 @@ size_t fmx_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K) {
 }
 
 int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* dy,
-                   int64_t dy_stride, const void* z, int act, int64_t M, int64_t N, int64_t K, void* dx, void* dw,
+                   int64_t dy_stride, const int16_t* slope, int act, int64_t M, int64_t N, int64_t K, void* dx, void* dw,
                    void* db, void* workspace, size_t workspace_bytes, void* stream) {
   const int rc = check_linear(dtype, x_stride, w_stride, act, M, N, K);
   if (rc) return rc;
   if (dy_stride < 0) return fail(FMX_ERR_INVALID, "dy stride must be >= 0");
   if (!dx && !dw && !db) return ok();
-  if (M > 0 && (!x || !w || !dy || (act != FMX_ACT_NONE && !z)))
-    return fail(FMX_ERR_INVALID, "x, w, dy and (with an activation) z must be non-null");
+  if (M > 0 && (!x || !w || !dy || (act != FMX_ACT_NONE && !slope)))
+    return fail(FMX_ERR_INVALID, "x, w, dy and (with an activation) slope must be non-null");
   if (!aligned(x, 16) || !aligned(w, 16)) return fail(FMX_ERR_INVALID, "x and w must be 16-byte aligned");
-  if (!aligned(dy, 2) || !aligned(z, 2) || !aligned(dx, 2) || !aligned(dw, 2) || !aligned(db, 2))
+  if (!aligned(dy, 2) || !aligned(slope, 2) || !aligned(dx, 2) || !aligned(dw, 2) || !aligned(db, 2))
     return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");
   const bool bf = dtype == FMX_DTYPE_BF16;
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -168,16 +168,15 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
   if (make || (db && !beside)) {
     fmx::DzArgs a = {};
     a.dy = dy;
-    a.z = act == FMX_ACT_NONE ? nullptr : z;
+    a.slope = act == FMX_ACT_NONE ? nullptr : slope;
     a.dz = make ? base : nullptr;
     a.part = db ? sums : nullptr;
     a.sdy = dy_stride;
     a.M = M;
     a.N = N;
     a.Np = n8;
-    a.act = act;
     a.vec_dy = dy_stride % 8 == 0 && aligned(dy, 16);
-    a.vec_z = N % 8 == 0 && aligned(z, 16);
+    a.vec_slope = N % 8 == 0 && aligned(slope, 16);
     e = fmx::launch_linear_dz(bf, a, parts, s);
     if (db && !later && e == hipSuccess) e = fmx::launch_join(dtype, sums, parts, N, 0, db, nullptr, s);
     if (e != hipSuccess) return hip_status(e, "fmx_linear_bwd launch");

@@ -65,40 +65,49 @@ __device__ __forceinline__ float sigmoid(float z) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504089f));
 }
 
-__device__ __forceinline__ float act_value(float z, int act) {
+// act(z), and with SLOPE act'(z). As a factor of a tail that is zero z is kept finite: their product would be NaN.
+template <bool SLOPE>
+__device__ __forceinline__ float act_value(float z, int act, float& slope) {
+  const float f = SLOPE ? __builtin_fminf(__builtin_fmaxf(z, -1e4f), 1e4f) : z;
   switch (act) {
-    case FMX_ACT_RELU: return z > 0.0f ? z : z != z ? z : 0.0f;
-    case FMX_ACT_GELU: {
-      float e;
-      return z * normal_cdf(z, e);
-    }
-    // z (1 + tanh u) / 2 = z sigmoid(2 u)
-    case FMX_ACT_GELU_TANH: return z * sigmoid(1.5957691216f * z * fmaf(0.044715f, z * z, 1.0f));
-    case FMX_ACT_SILU: return z * sigmoid(z);
-    default: return z;
-  }
-}
-// z comes rounded to 16 bits, so it may be infinite where the forward's was not; as a factor it is kept finite, or
-// its product with a tail that is zero would be NaN. (A NaN stays one through the other factors.)
-__device__ __forceinline__ float act_slope(float z, int act) {
-  const float f = __builtin_fminf(__builtin_fmaxf(z, -1e4f), 1e4f);
-  switch (act) {
-    case FMX_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+    case FMX_ACT_RELU:
+      slope = z > 0.0f ? 1.0f : 0.0f;
+      return z > 0.0f ? z : z != z ? z : 0.0f;
     case FMX_ACT_GELU: {
       float e;
       const float p = normal_cdf(z, e);
-      return fmaf(f * 0.3989422804f, e, p);
+      slope = fmaf(f * 0.3989422804f, e, p);
+      return z * p;
     }
+    // z (1 + tanh u) / 2 = z sigmoid(2 u)
     case FMX_ACT_GELU_TANH: {
       const float s = sigmoid(1.5957691216f * z * fmaf(0.044715f, z * z, 1.0f));
-      return s + f * s * (1.0f - s) * 1.5957691216f * fmaf(0.134145f, f * f, 1.0f);
+      slope = s + f * s * (1.0f - s) * 1.5957691216f * fmaf(0.134145f, f * f, 1.0f);
+      return z * s;
     }
     case FMX_ACT_SILU: {
       const float s = sigmoid(z);
-      return s + f * s * (1.0f - s);
+      slope = s + f * s * (1.0f - s);
+      return z * s;
     }
-    default: return 1.0f;
+    default:
+      slope = 1.0f;
+      return z;
   }
+}
+
+// Slopes lie within -0.13 .. 1.13 and go from the forward to the backward in 16 bits, in steps of 2^-14, so they
+// are off by 2^-15 at most: a sixteenth of what rounding z itself to bf16 leaves of them (whose gradients then
+// were up to 1.57 times the error of ones rounded once; 1.41 is what the rounding of dz and of the result make),
+// and the backward has no exponentials. -2^15 stands for NaN.
+__device__ __forceinline__ uint32_t slopes2(float a, float b) {
+  const auto r = __builtin_amdgcn_cvt_pknorm_i16(a * (16384.0f / 32767.0f), b * (16384.0f / 32767.0f));
+  const uint32_t w = __builtin_bit_cast(uint32_t, r);
+  return (a == a ? w & 0xffffu : 0x8000u) | (b == b ? w & 0xffff0000u : 0x80000000u);
+}
+__device__ __forceinline__ float slope_of(uint32_t bits16) {
+  const int i = (int)(int16_t)bits16;
+  return i == -32768 ? __builtin_nanf("") : (float)i * 0x1p-14f;
 }
 
 // ---- epilogue: 8 consecutive outputs j .. j + 7 of row i, of which `left` exist ----
@@ -107,15 +116,20 @@ __device__ __forceinline__ u32x4_t pack8(const float (&v)[8], bool bf) {
   return u32x4_t{pack2(v[0], v[1], bf), pack2(v[2], v[3], bf), pack2(v[4], v[5], bf), pack2(v[6], v[7], bf)};
 }
 
-__device__ __forceinline__ void store16(void* base, int64_t at, int left, const float (&v)[8], bool bf, bool vec) {
+__device__ __forceinline__ void store_raw(void* base, int64_t at, int left, const u32x4_t& w, bool vec) {
   uint16_t* p = static_cast<uint16_t*>(base) + at;
   if (vec && left >= 8) {
-    *reinterpret_cast<u32x4_t*>(p) = pack8(v, bf);
+    *reinterpret_cast<u32x4_t*>(p) = w;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < left) p[i] = (uint16_t)pack2(v[i], 0.0f, bf);
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t x = w[i / 2];
+      if (i < left) p[i] = (uint16_t)((i & 1) ? x >> 16 : x);
+    }
   }
+}
+__device__ __forceinline__ void store16(void* base, int64_t at, int left, const float (&v)[8], bool bf, bool vec) {
+  store_raw(base, at, left, pack8(v, bf), vec);
 }
 
 __device__ __forceinline__ u32x4_t load_raw(const void* base, int64_t at, int left, bool vec) {
@@ -138,29 +152,46 @@ __device__ __forceinline__ void load16(float (&v)[8], const void* base, int64_t 
   unpack8(v, load_raw(base, at, left, vec), bf);
 }
 
-// The activation of 8 values: one (uniform) test for all of them.
-__device__ __forceinline__ void activate(float (&v)[8], int act) {
-  switch (act) {
+// What follows the sums: a form's own activation (FMX_ACT_*: the forward's tile kernels are compiled for each, their
+// unrolled epilogues hold the code many times over), one named at run time, or nothing (dx, dw).
+constexpr int kAnyAct = -1, kNoEpilogue = -2;
+
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void activate(float (&v)[8], float (&slope)[8], int act) {
+  if constexpr (ACT >= 0) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = act_value<SLOPE>(v[k], ACT, slope[k]);
+  } else {
+    switch (act) {  // uniform: one test for the eight
 #define FMX_CASE(A) \
-  case A: \
-    _Pragma("unroll") for (int k = 0; k < 8; ++k) v[k] = act_value(v[k], A); \
-    break
-    FMX_CASE(FMX_ACT_RELU);
-    FMX_CASE(FMX_ACT_GELU);
-    FMX_CASE(FMX_ACT_GELU_TANH);
-    FMX_CASE(FMX_ACT_SILU);
+  case A: activate<A, SLOPE>(v, slope, A); break
+      FMX_CASE(FMX_ACT_RELU);
+      FMX_CASE(FMX_ACT_GELU);
+      FMX_CASE(FMX_ACT_GELU_TANH);
+      FMX_CASE(FMX_ACT_SILU);
 #undef FMX_CASE
-    default: break;
+      default: break;
+    }
   }
 }
+__device__ __forceinline__ u32x4_t slopes8(const float (&s)[8]) {
+  return u32x4_t{slopes2(s[0], s[1]), slopes2(s[2], s[3]), slopes2(s[4], s[5]), slopes2(s[6], s[7])};
+}
 
-// Products in v (the bias added already) to their place: z, the activation, the residual in `res`, y.
-template <bool EPI>
+// Products in v (the bias added already) to their place: the activation, its slope, the residual in `res`, y.
+template <int EPI>
 __device__ __forceinline__ void finish(const LinearArgs& a, int64_t i, int64_t j, int left, float (&v)[8],
                                        const u32x4_t& res, bool bf) {
-  if constexpr (EPI) {
-    if (a.z) store16(a.z, i * a.J + j, left, v, bf, a.vec_out);
-    activate(v, a.act);
+  if constexpr (EPI != kNoEpilogue) {
+    if constexpr (EPI != FMX_ACT_NONE) {
+      float s[8];
+      if (a.slope) {
+        activate<EPI, true>(v, s, a.act);
+        store_raw(a.slope, i * a.J + j, left, slopes8(s), a.vec_out);
+      } else {
+        activate<EPI, false>(v, s, a.act);
+      }
+    }
     if (a.res) {
       float r[8];
       unpack8(r, res, bf);
@@ -258,7 +289,7 @@ __device__ __forceinline__ void stage_barrier() {
   __asm__ volatile("" ::: "memory");
 }
 
-template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int NS, bool EPI>
+template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int NS, int EPI>
 __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
   constexpr int TI = WI * FI * 16, TJ = WJ * FJ * 16, NT = WI * WJ * 64;
   constexpr int BYTES = (TI + TJ) * BK * 2;
@@ -444,7 +475,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) b[h][k] = 0.0f;
-      if (EPI && a.bias) load16(b[h], a.bias, jw + 32 * h + (BMAJ ? (g & 1) * 16 + (g >> 1) * 8 : 8 * g), 8, BF, a.vec_bias);
+      if (EPI != kNoEpilogue && a.bias) load16(b[h], a.bias, jw + 32 * h + (BMAJ ? (g & 1) * 16 + (g >> 1) * 8 : 8 * g), 8, BF, a.vec_bias);
     }
     const int row = lane >> 3, ch = lane & 7;
     auto put = [&](int x, int h, const u32x4_t& w) __attribute__((always_inline)) {
@@ -468,14 +499,21 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[h][k] += b[h][k];
       }
-      if constexpr (EPI) {
-        if (a.z) {
-          put(x, 0, pack8(v[0], BF));
-          put(x, 1, pack8(v[1], BF));
-          flush(x, a.z);
+      if constexpr (EPI != kNoEpilogue) {
+        if constexpr (EPI != FMX_ACT_NONE) {
+          float s[8];
+          if (a.slope) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              activate<EPI, true>(v[h], s, a.act);
+              put(x, h, slopes8(s));
+            }
+            flush(x, a.slope);
+          } else {
+            activate<EPI, false>(v[0], s, a.act);
+            activate<EPI, false>(v[1], s, a.act);
+          }
         }
-        activate(v[0], a.act);
-        activate(v[1], a.act);
         if (a.res) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -500,10 +538,10 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
     float b[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) b[k] = 0.0f;
-    if (EPI && a.bias && a.splits == 1 && left > 0) load16(b, a.bias, j, left, BF, a.vec_bias);
+    if (EPI != kNoEpilogue && a.bias && a.splits == 1 && left > 0) load16(b, a.bias, j, left, BF, a.vec_bias);
     // all of the residual before the first store: loads behind stores would wait for them
     u32x4_t res[FI];
-    if (EPI && a.res && a.splits == 1) {
+    if (EPI != kNoEpilogue && a.res && a.splits == 1) {
 #pragma unroll
       for (int x = 0; x < FI; ++x) {
         const int64_t i = i0 + wi * FI * 16 + x * 16 + c;
@@ -532,7 +570,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
 // Adds the partial products of a split in their order and finishes 8 outputs a lane, in `groups` workgroups.
 // The workgroups after those add up db's partial sums, 16 columns each, 16 rows at a time: one launch where
 // two would follow each other.
-template <bool BF, bool EPI>
+template <bool BF, int EPI>
 __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a, int groups) {
   if ((int)blockIdx.x >= groups) {
     __shared__ float sums[16][17];
@@ -561,7 +599,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a, int grou
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = 0.0f;
     const int left = (int)(a.J - j < 8 ? a.J - j : 8);
-    if (EPI && a.bias) load16(v, a.bias, j, left, BF, a.vec_bias);
+    if (EPI != kNoEpilogue && a.bias) load16(v, a.bias, j, left, BF, a.vec_bias);
     f32x4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
@@ -573,7 +611,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a, int grou
       v[k] += s0[k];
       v[4 + k] += s1[k];
     }
-    const u32x4_t res = EPI && a.res ? load_raw(a.res, i * a.sres + j, left, a.vec_res) : u32x4_t{0u, 0u, 0u, 0u};
+    const u32x4_t res = EPI != kNoEpilogue && a.res ? load_raw(a.res, i * a.sres + j, left, a.vec_res) : u32x4_t{0u, 0u, 0u, 0u};
     finish<EPI>(a, i, j, left, v, res, BF);
   }
 }
@@ -640,12 +678,12 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
         v[k] += s0[k];
         v[4 + k] += s1[k];
       }
-      finish<true>(a, i, j, left, v, res, BF);
+      finish<kAnyAct>(a, i, j, left, v, res, BF);
     }
   }
 }
 
-// dz = dy act'(z) in 16 bits (rows padded with zeros to Np), and the column sums of the
+// dz = dy act'(z) in 16 bits (rows padded with zeros to Np), from the forward's slopes, and the column sums of the
 // unrounded dz over each workgroup's rows. A lane holds 8 columns; a row takes as few lanes as hold it (up to
 // 64), so a workgroup takes 256 / lanes rows at a time.
 template <bool BF>
@@ -661,20 +699,12 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(DzArgs a) {
     for (int64_t i = (int64_t)blockIdx.y * rows + row; i < a.M; i += (int64_t)gridDim.y * rows) {
       float v[8];
       load16(v, a.dy, i * a.sdy + j, left, BF, a.vec_dy);
-      if (a.z) {
-        float z[8];
-        load16(z, a.z, i * a.N + j, left, BF, a.vec_z);
-        switch (a.act) {
-#define FMX_CASE(A) \
-  case A: \
-    _Pragma("unroll") for (int k = 0; k < 8; ++k) v[k] *= act_slope(z[k], A); \
-    break
-          FMX_CASE(FMX_ACT_RELU);
-          FMX_CASE(FMX_ACT_GELU);
-          FMX_CASE(FMX_ACT_GELU_TANH);
-          FMX_CASE(FMX_ACT_SILU);
-#undef FMX_CASE
-          default: break;
+      if (a.slope) {
+        const u32x4_t w = load_raw(a.slope, i * a.N + j, left, a.vec_slope);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t x = w[k / 2];
+          v[k] *= slope_of((k & 1) ? x >> 16 : x & 0xffffu);
         }
       }
       if (a.dz) store16(a.dz, i * a.Np + j, 8, v, BF, true);
@@ -694,7 +724,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(DzArgs a) {
   }
 }
 
-template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int NS, bool EPI>
+template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int NS, int EPI>
 void run(const LinearArgs& a, int64_t grid, hipStream_t s) {
   linear_kernel<BF, AMAJ, BMAJ, WI, WJ, FI, FJ, NS, EPI><<<(unsigned)grid, WI * WJ * 64, 0, s>>>(a);
 }
@@ -711,20 +741,36 @@ hipError_t launch_few(const LinearArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <bool BF, bool AMAJ, bool BMAJ, bool EPI>
+template <bool BF, bool AMAJ, bool BMAJ, int EPI>
+void run_tile(const LinearArgs& a, int tile, int64_t grid, hipStream_t s) {
+  switch (tile) {
+    case kTile256: return run<BF, AMAJ, BMAJ, 2, 4, 8, 4, 2, EPI>(a, grid, s);
+    case kTile128: return run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 2, EPI>(a, grid, s);
+    case kTile128Deep: return run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 4, EPI>(a, grid, s);
+    default: return run<BF, AMAJ, BMAJ, 2, 2, 2, 2, 4, EPI>(a, grid, s);
+  }
+}
+
+template <bool BF, bool AMAJ, bool BMAJ, bool FORWARD>
 hipError_t launch(const LinearArgs& a, int tile, hipStream_t s) {
   const int64_t grid = a.ti * a.tj * a.splits;
-  switch (tile) {
-    case kTile256: run<BF, AMAJ, BMAJ, 2, 4, 8, 4, 2, EPI>(a, grid, s); break;
-    case kTile128: run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 2, EPI>(a, grid, s); break;
-    case kTile128Deep: run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 4, EPI>(a, grid, s); break;
-    default: run<BF, AMAJ, BMAJ, 2, 2, 2, 2, 4, EPI>(a, grid, s); break;
+  constexpr int kJoin = FORWARD ? kAnyAct : kNoEpilogue;
+  if constexpr (!FORWARD) {
+    run_tile<BF, AMAJ, BMAJ, kNoEpilogue>(a, tile, grid, s);
+  } else {
+    switch (a.splits == 1 ? a.act : FMX_ACT_NONE) {  // parts of k: the second kernel has the epilogue
+      case FMX_ACT_RELU: run_tile<BF, AMAJ, BMAJ, FMX_ACT_RELU>(a, tile, grid, s); break;
+      case FMX_ACT_GELU: run_tile<BF, AMAJ, BMAJ, FMX_ACT_GELU>(a, tile, grid, s); break;
+      case FMX_ACT_GELU_TANH: run_tile<BF, AMAJ, BMAJ, FMX_ACT_GELU_TANH>(a, tile, grid, s); break;
+      case FMX_ACT_SILU: run_tile<BF, AMAJ, BMAJ, FMX_ACT_SILU>(a, tile, grid, s); break;
+      default: run_tile<BF, AMAJ, BMAJ, FMX_ACT_NONE>(a, tile, grid, s); break;
+    }
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   const int64_t need = (a.I * (a.Jp / 8) + 255) / 256;
   const int groups = (int)(need < 4096 ? need : 4096);
-  linear_join_kernel<BF, EPI><<<groups + (a.db ? (int)((a.I + 15) / 16) : 0), 256, 0, s>>>(a, groups);
+  linear_join_kernel<BF, kJoin><<<groups + (a.db ? (int)((a.I + 15) / 16) : 0), 256, 0, s>>>(a, groups);
   return hipGetLastError();
 }
 
@@ -799,7 +845,7 @@ hipError_t launch_linear(bool bf16, LinearForm form, LinearArgs a, const LinearP
       b.I = a.I - at < kRows ? a.I - at : kRows;
       b.A = static_cast<const uint16_t*>(a.A) + at * a.sa;
       b.y = static_cast<uint16_t*>(a.y) + at * a.J;
-      if (a.z) b.z = static_cast<uint16_t*>(a.z) + at * a.J;
+      if (a.slope) b.slope = static_cast<int16_t*>(a.slope) + at * a.J;
       if (a.res) b.res = static_cast<const uint16_t*>(a.res) + at * a.sres;
       LinearPlan q = p;
       q.ti = (b.I + p.size - 1) / p.size;

@@ -539,7 +539,7 @@ const Tensor& grad_rows(const Tensor& dy, Tensor* keep, int64_t* M, int64_t* str
 }
 
 struct LinearBackward : public torch::autograd::Node {
-  torch::autograd::SavedVariable x, w, z;  // x and w as the kernels read them
+  torch::autograd::SavedVariable x, w, slope;  // x and w as the kernels read them
   std::vector<int64_t> x_sizes;
   int64_t M, N, K, x_stride, w_stride;
   int dtype, act;
@@ -548,7 +548,7 @@ struct LinearBackward : public torch::autograd::Node {
     const Tensor dy0 = grads[0];
     if (!dy0.defined()) return torch::autograd::variable_list(4);
     const Tensor xk = x.unpack(), wk = w.unpack();
-    const Tensor zk = act ? z.unpack() : Tensor();
+    const Tensor sk = act ? slope.unpack() : Tensor();
     const bool again = c10::GradMode::is_enabled();
     Tensor keep, dx, dw, db;
     {
@@ -563,7 +563,7 @@ struct LinearBackward : public torch::autograd::Node {
         const size_t n = fmx_linear_bwd_workspace_bytes(M, N, K);
         const Tensor ws = scratch(n, xk);
         must(fmx_linear_bwd(dtype, xk.const_data_ptr(), x_stride, wk.const_data_ptr(), w_stride, dy.const_data_ptr(),
-                            stride, zk.defined() ? zk.const_data_ptr() : nullptr, act, M, N, K, ptr(dx), ptr(dw),
+                            stride, sk.defined() ? sk.const_data_ptr<int16_t>() : nullptr, act, M, N, K, ptr(dx), ptr(dw),
                             ptr(db), ptr(ws), n, stream_of(xk)));
       }
     }
@@ -576,7 +576,7 @@ struct LinearBackward : public torch::autograd::Node {
   void release_variables() override {
     x.reset_data();
     w.reset_data();
-    z.reset_data();
+    slope.reset_data();
   }
   std::string name() const override { return "FlashMaxSimLinearBackward"; }
 };
@@ -666,12 +666,12 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (prc) return failed(prc);
   const bool grad = grad_wanted({x, w, b, r});
   Tensor y = at::empty(sizes, x->options());
-  Tensor z = grad && act ? at::empty({M, N}, x->options()) : Tensor();
+  Tensor slope = grad && act ? at::empty({M, N}, x->options().dtype(at::kShort)) : Tensor();
   const size_t n = fmx_linear_workspace_bytes(M, N, K);
   const Tensor ws = scratch(n, *x);
   const int rc = unlocked([&] {
     return fmx_linear(dtype, xk.const_data_ptr(), sx, wk.const_data_ptr(), sw, b ? b->const_data_ptr() : nullptr,
-                      r ? r->const_data_ptr() : nullptr, sr, (int)act, M, N, K, y.data_ptr(), ptr(z), ptr(ws), n, s);
+                      r ? r->const_data_ptr() : nullptr, sr, (int)act, M, N, K, y.data_ptr(), static_cast<int16_t*>(ptr(slope)), ptr(ws), n, s);
   });
   if (rc) return failed(rc);
   if (grad) {
@@ -679,7 +679,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     node->set_next_edges(torch::autograd::collect_next_edges(*x, *w, b ? *b : Tensor(), r ? *r : Tensor()));
     node->x = torch::autograd::SavedVariable(xk, false);
     node->w = torch::autograd::SavedVariable(wk, false);
-    if (act) node->z = torch::autograd::SavedVariable(z, false);
+    if (act) node->slope = torch::autograd::SavedVariable(slope, false);
     node->x_sizes = x->sizes().vec();
     node->M = M;
     node->N = N;

@@ -7,8 +7,8 @@ at the token embeddings).
 
 Operands are all float16 or all bfloat16; products run on MFMA with float32 sums,
 and y is rounded once. The backward rounds dz = dy act'(z) to the operands' type,
-as MFMA takes it, and keeps z = x W^T + bias in that type between the passes (only
-with an activation); bias gradients sum the unrounded dz. Sums have a fixed order:
+as MFMA takes it; the slopes act'(z) are kept between the passes in 16 bits, in
+steps of 2^-14 (only with an activation). Bias gradients sum the unrounded dz. Sums have a fixed order:
 the same inputs give the same bits.
 
 x and weight are read in place when their rows are 16-byte aligned and K is a
@@ -52,7 +52,7 @@ def _check(x, weight, bias, activation, residual) -> None:
 
 
 def _forward(x, weight, bias, act, residual, save):
-    """y, the operands as the kernels read them, and with `save` and an activation z."""
+    """y, the operands as the kernels read them, and with `save` and an activation its slopes."""
     N, K = weight.shape
     dev = _check_devices(x, weight, bias, residual)
     xk, wk = _operand(_rows(x, K)), _operand(weight)
@@ -60,32 +60,32 @@ def _forward(x, weight, bias, act, residual, save):
     bias = None if bias is None else bias.contiguous()
     M = xk.size(0)
     y = torch.empty(*x.shape[:-1], N, device=dev, dtype=x.dtype)
-    z = torch.empty(M, N, device=dev, dtype=x.dtype) if save and act else None
+    slope = torch.empty(M, N, device=dev, dtype=torch.int16) if save and act else None
     lib = _lib.load()
     with _device_guard(dev):
         nbytes = lib.fmx_linear_workspace_bytes(M, N, K)
         ws = _lib.workspace(nbytes, dev)
         rc = lib.fmx_linear(
             _lib.dtype_code(xk), xk.data_ptr(), xk.stride(0), wk.data_ptr(), wk.stride(0), _lib.ptr(bias),
-            _lib.ptr(res), 0 if res is None else res.stride(0), act, M, N, K, y.data_ptr(), _lib.ptr(z),
+            _lib.ptr(res), 0 if res is None else res.stride(0), act, M, N, K, y.data_ptr(), _lib.ptr(slope),
             _lib.ptr(ws), nbytes, _lib.stream_of(x),
         )
     _lib.check(rc)
-    return y, xk, wk, z
+    return y, xk, wk, slope
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, act, residual):
-        y, xk, wk, z = _forward(x, weight, bias, act, residual, True)
-        ctx.save_for_backward(xk, wk, z)
+        y, xk, wk, slope = _forward(x, weight, bias, act, residual, True)
+        ctx.save_for_backward(xk, wk, slope)
         ctx.act, ctx.shape, ctx.sizes = act, x.shape, tuple(weight.shape)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        xk, wk, z = ctx.saved_tensors
+        xk, wk, slope = ctx.saved_tensors
         (N, K), M, dev = ctx.sizes, xk.size(0), xk.device
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dx = torch.empty(ctx.shape, device=dev, dtype=xk.dtype) if need_x else None
@@ -99,7 +99,7 @@ class _LinearFn(torch.autograd.Function):
                 ws = _lib.workspace(nbytes, dev)
                 rc = lib.fmx_linear_bwd(
                     _lib.dtype_code(xk), xk.data_ptr(), xk.stride(0), wk.data_ptr(), wk.stride(0), dys.data_ptr(),
-                    dys.stride(0), _lib.ptr(z), ctx.act, M, N, K, _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db),
+                    dys.stride(0), _lib.ptr(slope), ctx.act, M, N, K, _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db),
                     _lib.ptr(ws), nbytes, _lib.stream_of(xk),
                 )
             _lib.check(rc)

@@ -401,26 +401,27 @@ size_t fmx_bwd_batched_workspace_bytes(int64_t Nq, int64_t B, int64_t Lq, int64_
  *   bias      [N]     dtype, or NULL
  *   residual  [M, N]  dtype, row stride r_stride, or NULL
  *   y         [M, N]  dtype, contiguous
- *   z         [M, N]  dtype, contiguous: x W^T + bias for the backward; or NULL
+ *   slope     [M, N]  int16, contiguous: act'(x W^T + bias) in steps of 2^-14 (-2^15: NaN) for the
+ *                     backward; or NULL. Not written without an activation.
  * x and w are 16-byte aligned, their strides multiples of 8 and at least K
  * rounded up to 8; elements from K up to there are zeros. M <=
  * FMX_LINEAR_MAX_ROWS, K and N < 2^24, strides < 2^22.
  */
 int fmx_linear(int dtype, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
-               const void* residual, int64_t r_stride, int act, int64_t M, int64_t N, int64_t K, void* y, void* z,
+               const void* residual, int64_t r_stride, int act, int64_t M, int64_t N, int64_t K, void* y, int16_t* slope,
                void* workspace, size_t workspace_bytes, void* stream);
 
 size_t fmx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
 /*
- * Its backward: dz = dy act'(z) (rounded to dtype, the products' operand),
+ * Its backward: dz = dy slope (rounded to dtype, the products' operand),
  *   dx = dz W  [M, K],  dw = dz^T x  [N, K],  db = sum over rows of dz before rounding  [N]
  * contiguous in dtype, each skipped when NULL. x and w as in the forward; dy
- * [M, N] with row stride dy_stride; z as the forward wrote it (unused without
+ * [M, N] with row stride dy_stride; slope as the forward wrote it (unused without
  * an activation). The residual's gradient is dy itself. Deterministic.
  */
 int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* dy,
-                   int64_t dy_stride, const void* z, int act, int64_t M, int64_t N, int64_t K, void* dx, void* dw,
+                   int64_t dy_stride, const int16_t* slope, int act, int64_t M, int64_t N, int64_t K, void* dx, void* dw,
                    void* db, void* workspace, size_t workspace_bytes, void* stream);
 
 size_t fmx_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K);

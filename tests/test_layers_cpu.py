@@ -58,7 +58,7 @@ def test_linear_rejects(lib, kw, code, text):
 
 @pytest.mark.parametrize("kw,code,text", [
     (dict(dys=-1), INVALID, "dy stride"),
-    (dict(act=2), INVALID, "z"),
+    (dict(act=2), INVALID, "slope"),
     (dict(dy=None), INVALID, "non-null"),
     (dict(), WORKSPACE, "workspace"),
     (dict(w=FAKE + 2), INVALID, "16-byte"),

@@ -36,16 +36,27 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kElems = 8;                         // per lane: 32 lanes hold a block of 256
 constexpr int kChunk = kThreads * kElems;         // elements a workgroup takes
-constexpr int kMaxTensors = 48;                   // of one launch: the table travels in the kernel's arguments
+constexpr int kMaxTensors = 76;                   // of one launch: the table travels in the kernel's arguments
 constexpr float kTinyBlock = 0x1p-110f;           // a block below this is held as zeros (127^2 / it overflows soon after)
 
+// A tensor in 48 bytes (user-space addresses have 48 bits), so that 4 KB of arguments hold 76 of them: every launch
+// fills the GPU and drains it again, about 5 us that 150 tensors paid four times with 64 bytes each.
+struct Entry {
+  uint32_t lo[7];   // low halves of param, grad, m, v, ms, vs, copy
+  uint32_t hi[4];   // their bits 32 .. 47 in pairs; the last one's pair: all arrays allow 16-byte (codes: 8-byte) accesses
+  uint32_t n;
+};
 struct Table {
-  AdamWTensor t[kMaxTensors];
+  Entry t[kMaxTensors];
   int32_t first[kMaxTensors + 1];                 // first workgroup of each tensor
-  int32_t vec[kMaxTensors];                       // all of its arrays allow 16-byte (codes: 8-byte) accesses
   int32_t count;
 };
 static_assert(sizeof(Table) + sizeof(AdamWScalars) <= 4096, "kernel arguments");
+
+__device__ __forceinline__ void* address(const Entry& e, int k) {
+  const uint32_t hi = (k & 1) ? e.hi[k / 2] >> 16 : e.hi[k / 2] & 0xffffu;
+  return reinterpret_cast<void*>((uint64_t)hi << 32 | e.lo[k]);
+}
 
 template <typename T, int V>
 struct __attribute__((aligned(sizeof(T) * V >= 16 ? 16 : sizeof(T) * V))) Pack {
@@ -181,11 +192,19 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(Table tab, AdamWScalars
     else
       hi = mid;
   }
-  const AdamWTensor t = tab.t[lo];
+  const Entry e = tab.t[lo];
+  const AdamWTensor t = {address(e, 0),
+                         address(e, 1),
+                         address(e, 2),
+                         address(e, 3),
+                         static_cast<float*>(address(e, 4)),
+                         static_cast<float*>(address(e, 5)),
+                         address(e, 6),
+                         (int64_t)e.n};
   const int64_t start = (int64_t)((int)blockIdx.x - tab.first[lo]) * kChunk;
   const int64_t end = start + (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + 1) * (64 * kElems);
   const int64_t i0 = start + threadIdx.x * kElems;
-  if (tab.vec[lo] && end <= t.n)
+  if ((e.hi[3] >> 16) && end <= t.n)
     adamw_chunk<P, G, C, BITS, true>(t, sc, i0);
   else if (end - 64 * kElems < t.n)  // whole waves: the lanes of a block meet in its largest values
     adamw_chunk<P, G, C, BITS, false>(t, sc, i0);
@@ -268,18 +287,22 @@ hipError_t launch_adamw(int pkind, int gkind, int ckind, int bits, const AdamWTe
         if (e != hipSuccess) return e;
       }
       const int ps = pkind == FMX_DTYPE_F32 ? 4 : 2, gs = gkind == FMX_DTYPE_F32 ? 4 : 2, ms = bits == 8 ? 1 : 4;
-      AdamWTensor& x = tab.t[tab.count];
-      x.param = static_cast<char*>(t[k].param) + at * ps;
-      x.grad = static_cast<const char*>(t[k].grad) + at * gs;
-      x.m = static_cast<char*>(t[k].m) + at * ms;
-      x.v = static_cast<char*>(t[k].v) + at * ms;
-      x.ms = t[k].ms ? t[k].ms + at / 256 : nullptr;
-      x.vs = t[k].vs ? t[k].vs + at / 256 : nullptr;
-      x.copy = t[k].copy ? static_cast<char*>(t[k].copy) + at * 2 : nullptr;
-      x.n = n;
+      const void* p[7] = {static_cast<char*>(t[k].param) + at * ps, static_cast<const char*>(t[k].grad) + at * gs,
+                          static_cast<char*>(t[k].m) + at * ms,     static_cast<char*>(t[k].v) + at * ms,
+                          t[k].ms ? t[k].ms + at / 256 : nullptr,   t[k].vs ? t[k].vs + at / 256 : nullptr,
+                          t[k].copy ? static_cast<char*>(t[k].copy) + at * 2 : nullptr};
       const int mb = bits == 8 ? 8 : 16;
-      tab.vec[tab.count] = aligned(x.param, 16) && aligned(x.grad, 16) && aligned(x.m, mb) && aligned(x.v, mb) &&
-                           (!x.copy || aligned(x.copy, 16));
+      const bool vec = aligned(p[0], 16) && aligned(p[1], 16) && aligned(p[2], mb) && aligned(p[3], mb) && aligned(p[6], 16);
+      Entry& x = tab.t[tab.count];
+      x.hi[0] = x.hi[1] = x.hi[2] = 0;
+      x.hi[3] = vec ? 1u << 16 : 0u;
+      for (int i = 0; i < 7; ++i) {
+        const uint64_t v = reinterpret_cast<uint64_t>(p[i]);
+        if (v >> 48) return hipErrorInvalidValue;
+        x.lo[i] = (uint32_t)v;
+        x.hi[i / 2] |= (uint32_t)(v >> 32) << (16 * (i & 1));
+      }
+      x.n = (uint32_t)n;
       tab.first[tab.count] = (int32_t)grid;
       grid += (n + kChunk - 1) / kChunk;
       tab.first[++tab.count] = (int32_t)grid;

@@ -95,7 +95,6 @@ struct LinearArgs {
   int64_t split_k, band;
   int splits;
   int act;
-  int vec_out, vec_res, vec_bias;  // 16-byte accesses allowed
 };
 
 struct LinearPlan {
@@ -117,7 +116,6 @@ struct DzArgs {
   float* part;            // [parts][N] column sums, or null
   int64_t sdy, M, N, Np;  // Np: N rounded up to 8
   int lanes;              // of a row, a power of two; set by launch_linear_dz
-  int vec_dy, vec_slope;
 };
 int linear_dz_parts(int64_t M, int64_t N);
 hipError_t launch_linear_dz(bool bf16, DzArgs a, int parts, hipStream_t s);

@@ -112,9 +112,6 @@ int fmx_linear(int dtype, const void* x, int64_t x_stride, const void* w, int64_
   a.sres = r_stride;
   a.act = act;
   a.part = static_cast<float*>(workspace);
-  a.vec_out = N % 8 == 0 && aligned(y, 16) && aligned(slope, 16);
-  a.vec_res = r_stride % 8 == 0 && aligned(residual, 16);
-  a.vec_bias = aligned(bias, 16);
   const fmx::LinearPlan p = fmx::linear_plan(fmx::kLinearForward, M, N, a.K);
   const size_t need = fmx::linear_part_bytes(p, M, N);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
@@ -175,8 +172,6 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
     a.M = M;
     a.N = N;
     a.Np = n8;
-    a.vec_dy = dy_stride % 8 == 0 && aligned(dy, 16);
-    a.vec_slope = N % 8 == 0 && aligned(slope, 16);
     e = fmx::launch_linear_dz(bf, a, parts, s);
     if (db && !later && e == hipSuccess) e = fmx::launch_join(dtype, sums, parts, N, 0, db, nullptr, s);
     if (e != hipSuccess) return hip_status(e, "fmx_linear_bwd launch");
@@ -185,7 +180,6 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
   a.A = as_is ? dy : base;
   a.sa = as_is ? dy_stride : n8;
   a.part = reinterpret_cast<float*>(base + ws.dz + ws.sums);
-  a.vec_out = K % 8 == 0;
   if (dx) {
     a.B = w;
     a.sb = w_stride;
@@ -193,9 +187,7 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
     a.J = K;
     a.K = N;
     a.y = dx;
-    fmx::LinearArgs b = a;
-    b.vec_out = a.vec_out && aligned(dx, 16);
-    e = fmx::launch_linear(bf, fmx::kLinearInput, b, fmx::linear_plan(fmx::kLinearInput, M, K, n8), s);
+    e = fmx::launch_linear(bf, fmx::kLinearInput, a, fmx::linear_plan(fmx::kLinearInput, M, K, n8), s);
     if (e != hipSuccess) return hip_status(e, "fmx_linear_bwd launch");
   }
   if (dw) {
@@ -205,7 +197,6 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
     a.J = K;
     a.K = M;
     a.y = dw;
-    a.vec_out = a.vec_out && aligned(dw, 16);
     a.db_part = sums;
     a.db_beside = beside;
     a.db_parts = parts;

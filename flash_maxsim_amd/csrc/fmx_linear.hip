@@ -116,10 +116,12 @@ __device__ __forceinline__ u32x4_t pack8(const float (&v)[8], bool bf) {
   return u32x4_t{pack2(v[0], v[1], bf), pack2(v[2], v[3], bf), pack2(v[4], v[5], bf), pack2(v[6], v[7], bf)};
 }
 
-__device__ __forceinline__ void store_raw(void* base, int64_t at, int left, const u32x4_t& w, bool vec) {
+// Rows may begin at any element (odd widths): the 16-byte accesses need no more than 2-byte alignment here (gfx950
+// under the HSA runtime takes them as they come; 1003 x 77 with 2-byte ones: dz 10 us, the forward 7.6; so 6 and 6.1).
+__device__ __forceinline__ void store_raw(void* base, int64_t at, int left, const u32x4_t& w) {
   uint16_t* p = static_cast<uint16_t*>(base) + at;
-  if (vec && left >= 8) {
-    *reinterpret_cast<u32x4_t*>(p) = w;
+  if (left >= 8) {
+    __builtin_memcpy(p, &w, 16);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -128,17 +130,24 @@ __device__ __forceinline__ void store_raw(void* base, int64_t at, int left, cons
     }
   }
 }
-__device__ __forceinline__ void store16(void* base, int64_t at, int left, const float (&v)[8], bool bf, bool vec) {
-  store_raw(base, at, left, pack8(v, bf), vec);
+__device__ __forceinline__ void store16(void* base, int64_t at, int left, const float (&v)[8], bool bf) {
+  store_raw(base, at, left, pack8(v, bf));
 }
 
-__device__ __forceinline__ u32x4_t load_raw(const void* base, int64_t at, int left, bool vec) {
+__device__ __forceinline__ u32x4_t load_raw(const void* base, int64_t at, int left) {
   const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-  if (vec && left >= 8) return *reinterpret_cast<const u32x4_t*>(p);
+  u32x4_t v = {0u, 0u, 0u, 0u};
+  if (left >= 8) {
+    __builtin_memcpy(&v, p, 16);
+    return v;
+  }
   uint32_t w[4] = {0u, 0u, 0u, 0u};
+  // the last one again in place of those past it (left >= 1): no branches, all loads in flight
+  uint32_t e[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < left) w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
+  for (int i = 0; i < 8; ++i) e[i] = p[i < left ? i : left - 1];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i / 2] |= (i < left ? e[i] : 0u) << (16 * (i & 1));
   return u32x4_t{w[0], w[1], w[2], w[3]};
 }
 __device__ __forceinline__ void unpack8(float (&v)[8], const u32x4_t& w, bool bf) {
@@ -148,8 +157,8 @@ __device__ __forceinline__ void unpack8(float (&v)[8], const u32x4_t& w, bool bf
     v[i] = unpack((i & 1) ? x >> 16 : x & 0xffffu, bf);
   }
 }
-__device__ __forceinline__ void load16(float (&v)[8], const void* base, int64_t at, int left, bool bf, bool vec) {
-  unpack8(v, load_raw(base, at, left, vec), bf);
+__device__ __forceinline__ void load16(float (&v)[8], const void* base, int64_t at, int left, bool bf) {
+  unpack8(v, load_raw(base, at, left), bf);
 }
 
 // What follows the sums: a form's own activation (FMX_ACT_*: the forward's tile kernels are compiled for each, their
@@ -187,7 +196,7 @@ __device__ __forceinline__ void finish(const LinearArgs& a, int64_t i, int64_t j
       float s[8];
       if (a.slope) {
         activate<EPI, true>(v, s, a.act);
-        store_raw(a.slope, i * a.J + j, left, slopes8(s), a.vec_out);
+        store_raw(a.slope, i * a.J + j, left, slopes8(s));
       } else {
         activate<EPI, false>(v, s, a.act);
       }
@@ -199,7 +208,7 @@ __device__ __forceinline__ void finish(const LinearArgs& a, int64_t i, int64_t j
       for (int k = 0; k < 8; ++k) v[k] += r[k];
     }
   }
-  store16(a.y, i * a.J + j, left, v, bf, a.vec_out);
+  store16(a.y, i * a.J + j, left, v, bf);
 }
 
 // ---- the product ----
@@ -463,7 +472,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
       }
     }
   };
-  if (FJ == 4 && a.splits == 1 && a.vec_out && i0 + TI <= a.I && j0 + TJ <= a.J) {
+  if (FJ == 4 && a.splits == 1 && i0 + TI <= a.I && j0 + TJ <= a.J) {
     // A whole tile: a wave turns its 16 x 64 blocks into rows of 128 bytes, whole lines of memory, in LDS
     // that nothing is read from or loaded into any more.
     wait_vmem<0>();
@@ -475,7 +484,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) b[h][k] = 0.0f;
-      if (EPI != kNoEpilogue && a.bias) load16(b[h], a.bias, jw + 32 * h + (BMAJ ? (g & 1) * 16 + (g >> 1) * 8 : 8 * g), 8, BF, a.vec_bias);
+      if (EPI != kNoEpilogue && a.bias) load16(b[h], a.bias, jw + 32 * h + (BMAJ ? (g & 1) * 16 + (g >> 1) * 8 : 8 * g), 8, BF);
     }
     const int row = lane >> 3, ch = lane & 7;
     auto put = [&](int x, int h, const u32x4_t& w) __attribute__((always_inline)) {
@@ -487,7 +496,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
       for (int h = 0; h < 2; ++h) {
         const u32x4_t w = *reinterpret_cast<const u32x4_t*>(mine + x * 2048 + (row + 8 * h) * 128 + ((ch ^ row) << 4));
         const int64_t i = i0 + wi * FI * 16 + x * 16 + row + 8 * h;
-        *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(out) + i * a.J + jw + ch * 8) = w;
+        store_raw(out, i * a.J + jw + ch * 8, 8, w);
       }
     };
 #pragma unroll
@@ -519,7 +528,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
           for (int h = 0; h < 2; ++h) {
             const int64_t i = i0 + wi * FI * 16 + x * 16 + c, j = jw + 32 * h + 8 * g;
             float r[8];
-            load16(r, a.res, i * a.sres + j, 8, BF, a.vec_res);
+            load16(r, a.res, i * a.sres + j, 8, BF);
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[h][k] += r[k];
           }
@@ -538,14 +547,14 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
     float b[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) b[k] = 0.0f;
-    if (EPI != kNoEpilogue && a.bias && a.splits == 1 && left > 0) load16(b, a.bias, j, left, BF, a.vec_bias);
+    if (EPI != kNoEpilogue && a.bias && a.splits == 1 && left > 0) load16(b, a.bias, j, left, BF);
     // all of the residual before the first store: loads behind stores would wait for them
     u32x4_t res[FI];
     if (EPI != kNoEpilogue && a.res && a.splits == 1) {
 #pragma unroll
       for (int x = 0; x < FI; ++x) {
         const int64_t i = i0 + wi * FI * 16 + x * 16 + c;
-        res[x] = i < a.I && left > 0 ? load_raw(a.res, i * a.sres + j, left, a.vec_res) : u32x4_t{0u, 0u, 0u, 0u};
+        res[x] = i < a.I && left > 0 ? load_raw(a.res, i * a.sres + j, left) : u32x4_t{0u, 0u, 0u, 0u};
       }
     }
 #pragma unroll
@@ -599,7 +608,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a, int grou
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = 0.0f;
     const int left = (int)(a.J - j < 8 ? a.J - j : 8);
-    if (EPI != kNoEpilogue && a.bias) load16(v, a.bias, j, left, BF, a.vec_bias);
+    if (EPI != kNoEpilogue && a.bias) load16(v, a.bias, j, left, BF);
     f32x4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
@@ -611,7 +620,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a, int grou
       v[k] += s0[k];
       v[4 + k] += s1[k];
     }
-    const u32x4_t res = EPI != kNoEpilogue && a.res ? load_raw(a.res, i * a.sres + j, left, a.vec_res) : u32x4_t{0u, 0u, 0u, 0u};
+    const u32x4_t res = EPI != kNoEpilogue && a.res ? load_raw(a.res, i * a.sres + j, left) : u32x4_t{0u, 0u, 0u, 0u};
     finish<EPI>(a, i, j, left, v, res, BF);
   }
 }
@@ -665,8 +674,8 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
       float v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-      if (a.bias) load16(v, a.bias, j, left, BF, a.vec_bias);
-      const u32x4_t res = a.res ? load_raw(a.res, i * a.sres + j, left, a.vec_res) : u32x4_t{0u, 0u, 0u, 0u};
+      if (a.bias) load16(v, a.bias, j, left, BF);
+      const u32x4_t res = a.res ? load_raw(a.res, i * a.sres + j, left) : u32x4_t{0u, 0u, 0u, 0u};
       f32x4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
@@ -686,28 +695,29 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
 // dz = dy act'(z) in 16 bits (rows padded with zeros to Np), from the forward's slopes, and the column sums of the
 // unrounded dz over each workgroup's rows. A lane holds 8 columns; a row takes as few lanes as hold it (up to
 // 64), so a workgroup takes 256 / lanes rows at a time.
-template <bool BF>
+// WHOLE: N is a multiple of 8, no lane's columns end early (the code for those in the loop costs all rows 15 %).
+template <bool BF, bool WHOLE>
 __global__ void __launch_bounds__(256) linear_dz_kernel(DzArgs a) {
   __shared__ float sums[256 * 9];
   const int lanes = a.lanes, rows = 256 / lanes, lane = threadIdx.x & (lanes - 1), row = threadIdx.x / lanes;
   const int64_t j0 = (int64_t)blockIdx.x * lanes * 8, j = j0 + lane * 8;
-  const int left = (int)(a.N - j < 0 ? 0 : a.N - j < 8 ? a.N - j : 8);
+  const int left = WHOLE ? 8 : (int)(a.N - j < 0 ? 0 : a.N - j < 8 ? a.N - j : 8);
   float s[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) s[k] = 0.0f;
   if (j < a.Np) {
     for (int64_t i = (int64_t)blockIdx.y * rows + row; i < a.M; i += (int64_t)gridDim.y * rows) {
       float v[8];
-      load16(v, a.dy, i * a.sdy + j, left, BF, a.vec_dy);
+      load16(v, a.dy, i * a.sdy + j, left, BF);
       if (a.slope) {
-        const u32x4_t w = load_raw(a.slope, i * a.N + j, left, a.vec_slope);
+        const u32x4_t w = load_raw(a.slope, i * a.N + j, left);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const uint32_t x = w[k / 2];
           v[k] *= slope_of((k & 1) ? x >> 16 : x & 0xffffu);
         }
       }
-      if (a.dz) store16(a.dz, i * a.Np + j, 8, v, BF, true);
+      if (a.dz) store16(a.dz, i * a.Np + j, 8, v, BF);
 #pragma unroll
       for (int k = 0; k < 8; ++k) s[k] += v[k];
     }
@@ -884,7 +894,7 @@ int linear_dz_parts(int64_t M, int64_t N) {
   const int64_t lanes = dz_lanes(N), rows = 256 / lanes, cols = (N + lanes * 8 - 1) / (lanes * 8);
   int64_t parts = (int64_t)layer_cus() * 8 / cols;      // about eight workgroups a CU
   if (parts > 256) parts = 256;                         // rows that the second kernel adds
-  const int64_t most = (M + rows * 4 - 1) / (rows * 4);  // four rows a thread at least
+  const int64_t most = (M + rows * 2 - 1) / (rows * 2);  // two rows a thread at least
   if (parts > most) parts = most;
   return (int)(parts < 1 ? 1 : parts);
 }
@@ -895,10 +905,16 @@ hipError_t launch_linear_dz(bool bf16, DzArgs a, int parts, hipStream_t s) {
   const int64_t rows = 4 * 256 / a.lanes, most = (a.M + rows - 1) / rows;
   const int64_t y = a.part ? parts : most < 65535 ? most : 65535;
   const dim3 grid((unsigned)((a.Np + a.lanes * 8 - 1) / (a.lanes * 8)), (unsigned)y);
-  if (bf16)
-    linear_dz_kernel<true><<<grid, 256, 0, s>>>(a);
-  else
-    linear_dz_kernel<false><<<grid, 256, 0, s>>>(a);
+  if (a.N % 8 == 0) {
+    if (bf16)
+      linear_dz_kernel<true, true><<<grid, 256, 0, s>>>(a);
+    else
+      linear_dz_kernel<false, true><<<grid, 256, 0, s>>>(a);
+  } else if (bf16) {
+    linear_dz_kernel<true, false><<<grid, 256, 0, s>>>(a);
+  } else {
+    linear_dz_kernel<false, false><<<grid, 256, 0, s>>>(a);
+  }
   return hipGetLastError();
 }
 

@@ -538,22 +538,43 @@ const Tensor& grad_rows(const Tensor& dy, Tensor* keep, int64_t* M, int64_t* str
   return *keep;
 }
 
+// A saved tensor of `rows` x `width` elements. Hooks on saved tensors (offloading, compression) may give it back
+// in another layout than it had: its strides are those of now. With `stride` its rows are read by that one, of
+// an operand's multiples; without, it is contiguous.
+Tensor given_back(const torch::autograd::SavedVariable& saved, const Tensor& dy, at::ScalarType type, int64_t rows,
+                  int64_t width, int64_t* stride = nullptr, bool operand = false) {
+  const Tensor t = saved.unpack();
+  TORCH_CHECK(t.defined() && t.device() == dy.device() && t.scalar_type() == type && t.layout() == at::kStrided &&
+                  t.dim() >= 1 && t.size(-1) == width && t.numel() == rows * width,
+              "flash_maxsim_amd: a saved tensor came back with another shape, type or device");
+  if (!stride) return t.contiguous();
+  int64_t m;
+  if (as_rows(t, &m, stride) && *stride >= 0 &&
+      (!operand || (*stride >= width && (*stride & 7) == 0 && *stride < 1 << 22 &&
+                    (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) == 0)))
+    return t;
+  *stride = width;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+
 struct LinearBackward : public torch::autograd::Node {
   torch::autograd::SavedVariable x, w, slope;  // x and w as the kernels read them
   std::vector<int64_t> x_sizes;
-  int64_t M, N, K, x_stride, w_stride;
+  int64_t M, N, K;
   int dtype, act;
 
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     const Tensor dy0 = grads[0];
     if (!dy0.defined()) return torch::autograd::variable_list(4);
-    const Tensor xk = x.unpack(), wk = w.unpack();
-    const Tensor sk = act ? slope.unpack() : Tensor();
     const bool again = c10::GradMode::is_enabled();
     Tensor keep, dx, dw, db;
     {
       at::AutoGradMode off(false);
-      int64_t m, stride;
+      const at::ScalarType type = dy0.scalar_type();
+      const int64_t K8 = (K + 7) / 8 * 8;
+      int64_t m, stride, x_stride, w_stride;
+      const Tensor xk = given_back(x, dy0, type, M, K8, &x_stride, true), wk = given_back(w, dy0, type, N, K8, &w_stride, true);
+      const Tensor sk = act ? given_back(slope, dy0, at::kShort, M, N) : Tensor();
       const Tensor& dy = grad_rows(dy0, &keep, &m, &stride);
       const auto options = xk.options();
       if (task_should_compute_output(0)) dx = at::empty(x_sizes, options);
@@ -584,7 +605,7 @@ struct LinearBackward : public torch::autograd::Node {
 struct LayerNormBackward : public torch::autograd::Node {
   torch::autograd::SavedVariable x, w, mean, rstd;
   std::vector<int64_t> x_sizes;
-  int64_t M, d, x_stride;
+  int64_t M, d;
   int dtype, w_dtype;
   at::ScalarType w_type;
   bool has_w;
@@ -592,12 +613,14 @@ struct LayerNormBackward : public torch::autograd::Node {
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     const Tensor dy0 = grads[0];
     if (!dy0.defined()) return torch::autograd::variable_list(3);
-    const Tensor xk = x.unpack(), wk = has_w ? w.unpack() : Tensor(), mu = mean.unpack(), rs = rstd.unpack();
     const bool again = c10::GradMode::is_enabled();
     Tensor keep, dx, dw, db;
     {
       at::AutoGradMode off(false);
-      int64_t m, stride;
+      int64_t m, stride, x_stride;
+      const Tensor xk = given_back(x, dy0, dy0.scalar_type(), M, d, &x_stride);
+      const Tensor wk = has_w ? given_back(w, dy0, w_type, 1, d) : Tensor();
+      const Tensor mu = given_back(mean, dy0, at::kFloat, 1, M), rs = given_back(rstd, dy0, at::kFloat, 1, M);
       const Tensor& dy = grad_rows(dy0, &keep, &m, &stride);
       const auto options = xk.options();
       if (task_should_compute_output(0)) dx = at::empty(x_sizes, options);
@@ -684,8 +707,6 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     node->M = M;
     node->N = N;
     node->K = K;
-    node->x_stride = sx;
-    node->w_stride = sw;
     node->dtype = dtype;
     node->act = (int)act;
     torch::autograd::set_history(y, node);
@@ -733,7 +754,6 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     node->x_sizes = x->sizes().vec();
     node->M = M;
     node->d = d;
-    node->x_stride = sx;
     node->dtype = dtype;
     node->w_dtype = w_dtype;
     node->w_type = wt;

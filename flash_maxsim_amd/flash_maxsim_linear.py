@@ -86,6 +86,8 @@ class _LinearFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         xk, wk, slope = ctx.saved_tensors
+        # hooks on saved tensors may give them back in another layout
+        xk, wk, slope = _operand(xk), _operand(wk), None if slope is None else slope.contiguous()
         (N, K), M, dev = ctx.sizes, xk.size(0), xk.device
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dx = torch.empty(ctx.shape, device=dev, dtype=xk.dtype) if need_x else None

@@ -79,6 +79,9 @@ class _LayerNormFn(torch.autograd.Function):
     def backward(ctx, dy):
         rows, weight, mean, rstd = ctx.saved_tensors
         M, d = rows.shape
+        # hooks on saved tensors may give them back in another layout
+        rows, mean, rstd = _rows(rows, d), mean.contiguous(), rstd.contiguous()
+        weight = None if weight is None else weight.contiguous()
         dev = rows.device
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dys = _rows(dy, d)

@@ -17,6 +17,7 @@ import pytest
 import torch
 
 import flash_maxsim_amd as fm
+from flash_maxsim_amd.flash_maxsim_linear import ACTIVATIONS, _LinearFn
 
 pytestmark = pytest.mark.gpu
 
@@ -245,6 +246,33 @@ def test_gradient_against_differences(name):
         mine = got["d" + k].cpu().double() * d
         # dz, z and the gradient rounded to 11 bits: three errors of 2^-11 of each term at most
         assert abs(mine.sum() - (up - dn) / (2 * h)) <= 4 * 2.0 ** -11 * 3 * mine.abs().sum(), k
+
+
+def columns_first(t):
+    return t.t().contiguous().t() if t.dim() == 2 else t.clone()
+
+
+HOOKS = [(lambda t: t.cpu(), lambda t: t.cuda()), (lambda t: t, lambda t: t.contiguous().clone()), (lambda t: t, columns_first)]
+
+
+@pytest.mark.parametrize("name", [None, "silu"])
+@pytest.mark.parametrize("K", [96, 77])
+@pytest.mark.parametrize("pack,unpack", HOOKS)
+def test_saved_tensors_in_another_layout(pack, unpack, K, name):
+    M, N = 150, 72
+    s = {k: v.cuda() for k, v in make(M, N, K, torch.float16, 14, residual=True).items()}
+    x = torch.zeros(M, 128, device="cuda", dtype=torch.float16)[:, :K].copy_(s["x"]).requires_grad_(True)
+    w = torch.zeros(N, 256, device="cuda", dtype=torch.float16)[:, :K].copy_(s["w"]).requires_grad_(True)
+    for fn in (fm.linear, lambda x, w, b, a, r: _LinearFn.apply(x, w, b, ACTIVATIONS[a], r)):
+        want = torch.autograd.grad(fn(x, w, s["b"], name, s["r"]), (x, w), s["dy"])
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            y = fn(x, w, s["b"], name, s["r"])
+        got = torch.autograd.grad(y, (x, w), s["dy"])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:-1]):
+        y = fm.linear(x, w, s["b"], name, s["r"])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, (x, w), s["dy"])
 
 
 def test_repeats_bit_for_bit_and_on_another_stream():

@@ -13,6 +13,7 @@ import pytest
 import torch
 
 import flash_maxsim_amd as fm
+from flash_maxsim_amd.flash_maxsim_norm import _LayerNormFn
 
 pytestmark = pytest.mark.gpu
 
@@ -232,3 +233,19 @@ def test_refusals():
         fm.layer_norm(x, eps=-1.0)
     with pytest.raises(RuntimeError, match="FMX_MAX_D"):
         fm.layer_norm(torch.zeros(1, 65537, device="cuda"))
+
+
+@pytest.mark.parametrize("pack,unpack", [(lambda t: t.cpu(), lambda t: t.cuda()), (lambda t: t, lambda t: t.contiguous().clone()),
+                                         (lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t.clone())])
+def test_saved_tensors_in_another_layout(pack, unpack):
+    g = torch.Generator().manual_seed(3)
+    x = torch.zeros(70, 512, device="cuda")[:, :300].copy_(torch.randn(70, 300, generator=g)).requires_grad_(True)
+    w, b = (torch.randn(300, generator=g).cuda().requires_grad_(True) for _ in range(2))
+    dy = torch.randn(70, 300, generator=g).cuda()
+    for fn in (fm.layer_norm, lambda *a: _LayerNormFn.apply(*a, 1e-5)):
+        want = torch.autograd.grad(fn(x, w, b), (x, w, b), dy)
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            y = fn(x, w, b)
+        # the rows' alignment may differ, and with it the order of their sums: dw and db are sums of 70 rows
+        for a, e in zip(torch.autograd.grad(y, (x, w, b), dy), want):
+            assert (a - e).abs().max() <= 2.0 ** -24 * 300 * 8 * e.abs().max()

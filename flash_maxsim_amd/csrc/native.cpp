@@ -532,8 +532,8 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads) {
 
 // dy as rows of n elements that the kernels read; `keep` holds a copy where it takes one.
 const Tensor& grad_rows(const Tensor& dy, Tensor* keep, int64_t* M, int64_t* stride) {
-  if (as_rows(dy, M, stride) && *stride >= 0) return dy;
-  *keep = dy.contiguous();
+  if (!dy.is_neg() && as_rows(dy, M, stride) && *stride >= 0) return dy;
+  *keep = dy.resolve_neg().contiguous();
   as_rows(*keep, M, stride);
   return *keep;
 }
@@ -543,10 +543,11 @@ const Tensor& grad_rows(const Tensor& dy, Tensor* keep, int64_t* M, int64_t* str
 // an operand's multiples; without, it is contiguous.
 Tensor given_back(const torch::autograd::SavedVariable& saved, const Tensor& dy, at::ScalarType type, int64_t rows,
                   int64_t width, int64_t* stride = nullptr, bool operand = false) {
-  const Tensor t = saved.unpack();
+  Tensor t = saved.unpack();
   TORCH_CHECK(t.defined() && t.device() == dy.device() && t.scalar_type() == type && t.layout() == at::kStrided &&
                   t.dim() >= 1 && t.size(-1) == width && t.numel() == rows * width,
               "flash_maxsim_amd: a saved tensor came back with another shape, type or device");
+  t = t.resolve_neg();
   if (!stride) return t.contiguous();
   int64_t m;
   if (as_rows(t, &m, stride) && *stride >= 0 &&

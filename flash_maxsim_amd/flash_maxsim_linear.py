@@ -31,6 +31,7 @@ ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 def _operand(t: torch.Tensor) -> torch.Tensor:
     """[rows, K] as the kernels read it: t itself, or a copy with K zero-padded to a multiple of 8."""
+    t = t.resolve_neg()
     K = t.shape[1]
     if K % 8 == 0 and _abi_ready(t, None) and t.stride(0) < 1 << 22:
         return t
@@ -57,7 +58,7 @@ def _forward(x, weight, bias, act, residual, save):
     dev = _check_devices(x, weight, bias, residual)
     xk, wk = _operand(_rows(x, K)), _operand(weight)
     res = None if residual is None else _rows(residual, N)
-    bias = None if bias is None else bias.contiguous()
+    bias = None if bias is None else bias.resolve_neg().contiguous()
     M = xk.size(0)
     y = torch.empty(*x.shape[:-1], N, device=dev, dtype=x.dtype)
     slope = torch.empty(M, N, device=dev, dtype=torch.int16) if save and act else None

@@ -23,7 +23,7 @@ _CODES = {torch.float16: _lib.FMX_DTYPE_F16, torch.bfloat16: _lib.FMX_DTYPE_BF16
 
 def _rows(t: torch.Tensor, d: int) -> torch.Tensor:
     """t as [M, d] rows with adjacent elements, in place where its strides allow."""
-    t = t.reshape(-1, d)
+    t = t.resolve_neg().reshape(-1, d)
     return t if t.stride(1) == 1 or d == 1 else t.contiguous()
 
 
@@ -50,8 +50,8 @@ def _forward(x, weight, bias, eps, save):
     dev = _check_devices(x, weight, bias)
     wt = _weight_type(x, weight, bias)
     rows = _rows(x, d)
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
+    weight = None if weight is None else weight.resolve_neg().contiguous()
+    bias = None if bias is None else bias.resolve_neg().contiguous()
     M = rows.size(0)
     y = torch.empty(x.shape, device=dev, dtype=x.dtype)
     mean = torch.empty(M, device=dev, dtype=torch.float32) if save else None
@@ -81,7 +81,7 @@ class _LayerNormFn(torch.autograd.Function):
         M, d = rows.shape
         # hooks on saved tensors may give them back in another layout
         rows, mean, rstd = _rows(rows, d), mean.contiguous(), rstd.contiguous()
-        weight = None if weight is None else weight.contiguous()
+        weight = None if weight is None else weight.resolve_neg().contiguous()
         dev = rows.device
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dys = _rows(dy, d)

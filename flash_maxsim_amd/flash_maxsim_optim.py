@@ -119,13 +119,13 @@ def _step_python(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, wei
                                                             (c is None or c.dtype == g.dtype)):
             raise TypeError(f"gradients must be float32 or of their parameters' (or copies') type, got {g.dtype} for {p.dtype}")
         assert g.shape == p.shape and (c is None or c.shape == p.shape), "a gradient (copy) has its parameter's shape"
-        if not p.is_contiguous() or (c is not None and not c.is_contiguous()):
+        if any(t is not None and (t.is_neg() or not t.is_contiguous()) for t in (p, c)):
             raise ValueError("parameters and copies must be contiguous: they are written in place")
         m, ms = _moment(m, p, eight, torch.int8)
         v, vs = _moment(v, p, eight, torch.uint8)
         dev = _check_devices(p, g, m, v, ms, vs, c, grad_scale)
-        if not g.is_contiguous():
-            g = g.contiguous()
+        if g.is_neg() or not g.is_contiguous():
+            g = g.resolve_neg().contiguous()
             keep.append(g)
         row = _Tensor(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), _lib.ptr(ms), _lib.ptr(vs), _lib.ptr(c),
                       p.numel())

@@ -303,3 +303,14 @@ def test_refusals():
         fm.AdamW([torch.nn.Parameter(p)], copies=[None, None])
     with pytest.raises(TypeError):
         fm.dequantize_adamw((p, m8[1]))
+
+
+def test_gradients_read_with_their_sign():
+    p = [torch.ones(300, device="cuda"), torch.ones(300, device="cuda")]
+    g = torch.linspace(-1, 1, 300, device="cuda")
+    for q, h in zip(p, (torch._neg_view(g), -g)):
+        m, v = fm.adamw_state(q)
+        fm.adamw_step([q], [h], [m], [v], 1)
+    assert torch.equal(*p)
+    with pytest.raises(ValueError):
+        fm.adamw_step([torch._neg_view(p[0])], [g], [torch.zeros_like(g)], [torch.zeros_like(g)], 1)

@@ -320,3 +320,15 @@ def test_refusals():
         fm.linear(x.cpu(), w.cpu())
     with pytest.raises(RuntimeError):
         fm.linear(x, w.cpu())
+
+
+def test_views_read_with_their_sign():
+    s = {k: v.cuda() for k, v in make(30, 24, 40, torch.float16, 6, residual=True).items()}
+    got, want = [], []
+    for out, f in ((got, torch._neg_view), (want, lambda t: -t)):
+        leaves = [f(s[k]).detach().requires_grad_(True) for k in ("x", "w", "b", "r")]
+        y = fm.linear(leaves[0], leaves[1], leaves[2], "gelu", leaves[3])
+        out += [y, *torch.autograd.grad(y, leaves, f(s["dy"]))]
+        y = fm.linear(s["x"].requires_grad_(True), s["w"], None, "gelu")
+        out += torch.autograd.grad(y, s["x"], f(s["dy"]))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -249,3 +249,16 @@ def test_saved_tensors_in_another_layout(pack, unpack):
         # the rows' alignment may differ, and with it the order of their sums: dw and db are sums of 70 rows
         for a, e in zip(torch.autograd.grad(y, (x, w, b), dy), want):
             assert (a - e).abs().max() <= 2.0 ** -24 * 300 * 8 * e.abs().max()
+
+
+def test_views_read_with_their_sign():
+    """The imaginary part of a conjugate is a view whose elements are stored negated."""
+    g = torch.Generator().manual_seed(4)
+    z = torch.complex(torch.randn(20, 33, generator=g), torch.randn(20, 33, generator=g)).cuda()
+    w = torch._neg_view(torch.randn(33, generator=g).cuda())
+    x, dy = z.conj().imag, torch._neg_view(torch.randn(20, 33, generator=g).cuda())
+    assert x.is_neg() and w.is_neg() and dy.is_neg()
+    got, want = ([fm.layer_norm(a, b)] + list(torch.autograd.grad(fm.layer_norm(a, b), (a, b), e)) for a, b, e in (
+        [t.detach().requires_grad_(True) for t in (x, w)] + [dy],
+        [t.detach().resolve_neg().contiguous().requires_grad_(True) for t in (x, w)] + [dy.resolve_neg()]))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

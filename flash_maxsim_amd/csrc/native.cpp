@@ -532,6 +532,7 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads) {
 
 // dy as rows of n elements that the kernels read; `keep` holds a copy where it takes one.
 const Tensor& grad_rows(const Tensor& dy, Tensor* keep, int64_t* M, int64_t* stride) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(&dy), "flash_maxsim_amd: no forward-mode derivative of these gradients");
   if (!dy.is_neg() && as_rows(dy, M, stride) && *stride >= 0) return dy;
   *keep = dy.resolve_neg().contiguous();
   as_rows(*keep, M, stride);

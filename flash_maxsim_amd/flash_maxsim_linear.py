@@ -24,7 +24,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .flash_maxsim import _abi_ready, _check_devices, _device_guard
-from .flash_maxsim_norm import _rows
+from .flash_maxsim_norm import _differentiated, _rows
 
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
@@ -122,6 +122,6 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         return out
     _check(x, weight, bias, activation, residual)
     act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if _differentiated(x, weight, bias, residual):
         return _LinearFn.apply(x, weight, bias, act, residual)
     return _forward(x, weight, bias, act, residual, False)[0]

@@ -27,6 +27,12 @@ def _rows(t: torch.Tensor, d: int) -> torch.Tensor:
     return t if t.stride(1) == 1 or d == 1 else t.contiguous()
 
 
+def _differentiated(*tensors) -> bool:
+    """Whether autograd watches an operand (in forward mode too, which the Functions refuse)."""
+    return torch.autograd.forward_ad._current_level >= 0 or (
+        torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
+
+
 def _weight_type(x, weight, bias) -> torch.dtype:
     types = {t.dtype for t in (weight, bias) if t is not None}
     if not types:
@@ -113,6 +119,6 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if out is not None:
         return out
     _check(x, weight, bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _differentiated(x, weight, bias):
         return _LayerNormFn.apply(x, weight, bias, float(eps))
     return _forward(x, weight, bias, float(eps), False)[0]

@@ -332,3 +332,19 @@ def test_views_read_with_their_sign():
         y = fm.linear(s["x"].requires_grad_(True), s["w"], None, "gelu")
         out += torch.autograd.grad(y, s["x"], f(s["dy"]))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_tangents_refused():
+    x = torch.randn(4, 16, device="cuda", dtype=torch.float16)
+    w = torch.randn(8, 16, device="cuda", dtype=torch.float16)
+    with torch.autograd.forward_ad.dual_level():
+        t = torch.autograd.forward_ad.make_dual(x, x)
+        for f in (lambda: fm.linear(t, w), lambda: fm.linear(w, t), lambda: fm.layer_norm(t)):
+            with pytest.raises(NotImplementedError):
+                f()
+        inside = fm.linear(x, w), fm.layer_norm(x)
+        leaf = x.clone().requires_grad_(True)
+        dy = torch.ones(4, 8, device="cuda", dtype=torch.float16)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(fm.linear(leaf, w), leaf, torch.autograd.forward_ad.make_dual(dy, dy))
+    assert torch.equal(inside[0], fm.linear(x, w)) and torch.equal(inside[1], fm.layer_norm(x))

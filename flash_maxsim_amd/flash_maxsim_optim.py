@@ -225,11 +225,17 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """torch's, with each state tensor in its own type again (torch casts
-        float state to its parameter's type, which would round the moments)."""
+        float state to its parameter's type, which would round the moments).
+        A state of torch.optim.AdamW continues as one of 32 bits."""
+        if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
+            raise ValueError("this AdamW has neither amsgrad nor maximize")
         saved = state_dict["state"]
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         super().load_state_dict(state_dict)
         mine = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, mine):
             for k, v in saved.get(i, {}).items():
-                self.state[p][k] = v.detach().to(p.device, copy=True).contiguous() if torch.is_tensor(v) else v
+                if k == "step":  # a tensor in states of torch's optimizers
+                    self.state[p][k] = int(v)
+                else:
+                    self.state[p][k] = v.detach().to(p.device, copy=True).contiguous() if torch.is_tensor(v) else v

@@ -314,3 +314,24 @@ def test_gradients_read_with_their_sign():
     assert torch.equal(*p)
     with pytest.raises(ValueError):
         fm.adamw_step([torch._neg_view(p[0])], [g], [torch.zeros_like(g)], [torch.zeros_like(g)], 1)
+
+
+def test_optimizer_continues_torchs_state():
+    g = torch.Generator().manual_seed(9)
+    init, grads = torch.randn(50, 7, generator=g), [torch.randn(50, 7, generator=g) for _ in range(3)]
+    a, b = (torch.nn.Parameter(init.cuda()) for _ in range(2))
+    theirs = torch.optim.AdamW([a], **HP)
+    for k in range(2):
+        a.grad = grads[k].cuda()
+        theirs.step()
+    mine = fm.AdamW([b])
+    mine.load_state_dict(copy.deepcopy(theirs.state_dict()))
+    b.data.copy_(a.data)
+    want = exact(a.detach().cpu().double().flatten(), grads[2].flatten(), theirs.state[a]["exp_avg"].cpu().flatten(),
+                 theirs.state[a]["exp_avg_sq"].cpu().flatten(), 3, **HP)[0]
+    b.grad = grads[2].cuda()
+    mine.step()
+    assert type(mine.state[b]["step"]) is int and mine.state[b]["step"] == 3
+    assert (b.detach().cpu().double().flatten() - want).abs().max() <= 20 * F32 * want.abs().max()
+    with pytest.raises(ValueError):
+        mine.load_state_dict(torch.optim.AdamW([a], amsgrad=True).state_dict())

@@ -815,6 +815,9 @@ LinearPlan linear_plan(LinearForm form, int64_t I, int64_t J, int64_t K) {
   }
   double least = 0;
   for (const TileCost& c : kCosts) {
+    // The rows of a K-major tile are reached by 32-bit offsets below 2^31 from its first one. x and W have strides
+    // below 2^22, which all tiles hold; dz has N's, below 2^24: tiles of 256 rows to N = 4.2 million, of 128 to 8.4.
+    if (form != kLinearWeight && (c.size - 1) * K * 2 + BK * 2 > 0x7fffffff) continue;
     const int64_t ti = (I + c.size - 1) / c.size, tj = (J + c.size - 1) / c.size, slots = cus * c.per_cu;
     for (int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
       int64_t per = ((K + want - 1) / want + BK - 1) / BK * BK;

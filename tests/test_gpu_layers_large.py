@@ -99,3 +99,29 @@ def test_adamw():
     del md
     vd = fm.dequantize_adamw(v)
     assert ((vd[at].double() - 0.00025).abs() <= 0.00025 * 2.0 ** -20).all() and int((vd != 0).sum()) == len(at)
+
+
+@pytest.mark.parametrize("M,N,K", [(512, 4_300_004, 512), (128, 9_000_004, 512), (256, (1 << 24) - 1, 512)])
+@pytest.mark.parametrize("name", [None, "relu"])
+def test_linear_of_many_outputs(M, N, K, name):
+    """dz's rows are N wide: the last row of a tile of 256 (128) lies past 2^31 bytes of its first from N = 4.2 (8.4)
+    million on. Few columns of dy are not zero, so dx is a small product."""
+    g = torch.Generator(device=DEV).manual_seed(N)
+    w = torch.randn(1031, K, generator=g, device=DEV).bfloat16().repeat(-(-N // 1031), 1)[:N].requires_grad_(True)
+    x = torch.randn(M, K, generator=g, device=DEV).bfloat16().requires_grad_(True)
+    pick = torch.tensor([0, 7, 8, 63, 64, N // 3, N // 2, (1 << 22) - 1, 1 << 22, N - 9, N - 1], device=DEV)
+    y = fm.linear(x, w, None, name)
+    z = x.detach().double() @ w.detach()[pick].double().t()
+    dy = torch.zeros(M, N, dtype=torch.bfloat16, device=DEV)
+    dy[:, pick] = torch.randn(M, len(pick), generator=g, device=DEV).bfloat16()
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    far = z.abs() > F32 * (K + 4) * (x.detach().double().abs() @ w.detach()[pick].double().abs().t())  # relu's slope jumps at zero
+    dz = dy[:, pick].double() * (1.0 if name is None else (z > 0).double())
+    loose = torch.zeros_like(dz) if name is None else dy[:, pick].double().abs() * ~far
+    wp, xd = w.detach()[pick].double(), x.detach().double()
+    want, mag = dz @ wp, dz.abs() @ wp.abs()
+    # products and sums of eleven terms in float32, one rounding to 8 bits
+    assert ((dx.double() - want).abs() <= 2.0 ** -8 * want.abs() + 16 * F32 * mag + loose @ wp.abs() + 1e-30).all()
+    want, mag = dz.t() @ xd, dz.abs().t() @ xd.abs()
+    assert ((dw[pick].double() - want).abs() <= 2.0 ** -8 * want.abs() + (M + 4) * F32 * mag + loose.t() @ xd.abs() + 1e-30).all()
+    assert not dw[5000].any() and not dw[N - 2].any()

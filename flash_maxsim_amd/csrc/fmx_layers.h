@@ -38,7 +38,7 @@ hipError_t launch_norm_fwd(int kind, const NormArgs& a, bool vec, hipStream_t s)
 // *parts: the rows of NormArgs::part written
 hipError_t launch_norm_bwd(int kind, const NormArgs& a, bool vec, int* parts, hipStream_t s);
 // Sums over `parts` rows of n0 + n1 float32 values: the first n0 columns to out0, the others to out1, in
-// out_kind's type; either may be null. No rows: zeros.
+// out_kind's type; either may be null. No rows: zeros. 64 threads a column: fewer than 2^26 columns.
 hipError_t launch_join(int out_kind, const float* part, int parts, int64_t n0, int64_t n1, void* out0, void* out1,
                        hipStream_t s);
 
@@ -119,5 +119,6 @@ struct DzArgs {
 };
 int linear_dz_parts(int64_t M, int64_t N);
 hipError_t launch_linear_dz(bool bf16, DzArgs a, int parts, hipStream_t s);
+hipError_t launch_linear_zero(void* out, int64_t n, hipStream_t s);  // n > 0 zeros of 16 bits
 
 }  // namespace fmx

@@ -142,8 +142,8 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (M == 0) {  // no rows: zeros
     hipError_t e = hipSuccess;
-    if (dw) e = fmx::launch_join(dtype, nullptr, 0, N * K, 0, dw, nullptr, s);
-    if (db && e == hipSuccess) e = fmx::launch_join(dtype, nullptr, 0, N, 0, db, nullptr, s);
+    if (dw) e = fmx::launch_linear_zero(dw, N * K, s);
+    if (db && e == hipSuccess) e = fmx::launch_linear_zero(db, N, s);
     return hip_status(e, "fmx_linear_bwd launch");
   }
   const LinearBwdWs ws = linear_bwd_ws(M, N, K);

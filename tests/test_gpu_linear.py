@@ -190,6 +190,18 @@ def test_no_rows():
     assert y.shape == (0, 8) and dx.shape == (0, 16) and not dw.any() and not db.any()
 
 
+@pytest.mark.parametrize("N,K", [(8192, 8192), (8200, 16379), (3, 5)])
+def test_no_rows_of_a_large_weight(N, K):
+    """64 threads an element would pass a launch's 2^32 from 2^26 elements on."""
+    w = torch.ones(N, K, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    b = torch.ones(N, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    x = torch.empty(2, 0, K, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    torch.full((N * K + N,), float("nan"), device="cuda", dtype=torch.bfloat16)  # freed: what dw and db may get holds no zeros
+    y = fm.linear(x, w, b, "silu")
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty(2, 0, N, device="cuda", dtype=torch.bfloat16))
+    assert y.shape == (2, 0, N) and dx.shape == x.shape and dw.shape == (N, K) and not dw.any() and not db.any()
+
+
 def test_values_that_are_not_finite_stay_in_their_row():
     for M, N, K in ((70, 40, 48), (300, 200, 1000)):
         s = make(M, N, K, torch.float16, 2)

@@ -81,7 +81,7 @@ struct LinearArgs {
   int64_t I, J, K;        // K: a multiple of 8 where it runs along rows
   int64_t Jr;             // B's columns or rows that exist (set by launch_linear)
   void* y;                // [I, J] 16-bit, contiguous
-  void* slope;            // forward: act's slopes, int16 steps of 2^-14, [I, J]; or null
+  void* slope;            // forward: act's slopes in their 16-bit code, [I, J]; or null
   const void* bias;       // forward: [J], or null
   const void* res;        // forward: [I, J], row stride sres, or null
   int64_t sres;

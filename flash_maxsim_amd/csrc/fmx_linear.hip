@@ -96,18 +96,41 @@ __device__ __forceinline__ float act_value(float z, int act, float& slope) {
   }
 }
 
-// Slopes lie within -0.13 .. 1.13 and go from the forward to the backward in 16 bits, in steps of 2^-14, so they
-// are off by 2^-15 at most: a sixteenth of what rounding z itself to bf16 leaves of them (whose gradients then
-// were up to 1.57 times the error of ones rounded once; 1.41 is what the rounding of dz and of the result make),
-// and the backward has no exponentials. -2^15 stands for NaN.
-__device__ __forceinline__ uint32_t slopes2(float a, float b) {
-  const auto r = __builtin_amdgcn_cvt_pknorm_i16(a * (16384.0f / 32767.0f), b * (16384.0f / 32767.0f));
-  const uint32_t w = __builtin_bit_cast(uint32_t, r);
-  return (a == a ? w & 0xffffu : 0x8000u) | (b == b ? w & 0xffff0000u : 0x80000000u);
+// Slopes lie within -0.13 .. 1.13 and go from the forward to the backward in 16 bits, which get finer towards zero:
+// GELU's slope at -5 is -7e-6, and a unit whose arguments all lie there learns by it (steps of 2^-14 made it zero). The
+// bits of |slope| as float32, a measure of its logarithm, are shifted right by S, which divides the exponent by 2^S: a
+// root drawn with straight lines from power to power of two. The code is that root in steps of 1 / 32767; it is kOne
+// for a slope of 1, and the largest slope is below 32766. What a slope is off by, half a step, is
+//   fp16, S = 1  2^-15 for 1/2 to 1 (twice that above), at most 2^-14 of it down to 0.28, twice that for each
+//                two powers of two further down; 2^-30 is the smallest that is not zero (fp16's own: 2^-24)
+//   bf16, S = 2  2^-14 for 1/2 to 1, at most 2^-13 of it down to 0.07, twice that for each four powers of two;
+//                2^-60, where squares of gradients leave float32
+// 0 and 1 are exact. Beside dz's rounding to the operands' type (2^-11, 2^-8) that adds a hundredth to the gradients'
+// error; rounding z itself made them up to 1.57 times as far from 64 bits as ones rounded once (1.41 is what the
+// rounding of dz and of the result make). The backward needs no exponentials. NaN's bits give the code 32767 at
+// either sign.
+template <bool BF>
+struct SlopeCode {
+  static constexpr int S = BF ? 2 : 1;
+  static constexpr float kStep = 1.0f / 32767.0f, kOne = BF ? 32230.0f : 31700.0f;
+  static constexpr uint32_t kBias = __builtin_bit_cast(uint32_t, kOne * kStep) - (0x3f800000u >> S);
+};
+template <bool BF>
+__device__ __forceinline__ float slope_root(float a) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, a) & 0x7fffffffu;
+  return __builtin_copysignf(__builtin_bit_cast(float, (u >> SlopeCode<BF>::S) + SlopeCode<BF>::kBias), a);
 }
+template <bool BF>
+__device__ __forceinline__ uint32_t slopes2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(slope_root<BF>(a), slope_root<BF>(b)));
+}
+template <bool BF>
 __device__ __forceinline__ float slope_of(uint32_t bits16) {
-  const int i = (int)(int16_t)bits16;
-  return i == -32768 ? __builtin_nanf("") : (float)i * 0x1p-14f;
+  using C = SlopeCode<BF>;
+  const float root = (float)(int16_t)bits16 * C::kStep;
+  const uint32_t u = __builtin_bit_cast(uint32_t, root) & 0x7fffffffu;
+  const float v = __builtin_bit_cast(float, ((u > C::kBias ? u : C::kBias) - C::kBias) << C::S);
+  return u < 0x3f800000u ? __builtin_copysignf(v, root) : __builtin_nanf("");
 }
 
 // ---- epilogue: 8 consecutive outputs j .. j + 7 of row i, of which `left` exist ----
@@ -183,32 +206,33 @@ __device__ __forceinline__ void activate(float (&v)[8], float (&slope)[8], int a
     }
   }
 }
+template <bool BF>
 __device__ __forceinline__ u32x4_t slopes8(const float (&s)[8]) {
-  return u32x4_t{slopes2(s[0], s[1]), slopes2(s[2], s[3]), slopes2(s[4], s[5]), slopes2(s[6], s[7])};
+  return u32x4_t{slopes2<BF>(s[0], s[1]), slopes2<BF>(s[2], s[3]), slopes2<BF>(s[4], s[5]), slopes2<BF>(s[6], s[7])};
 }
 
 // Products in v (the bias added already) to their place: the activation, its slope, the residual in `res`, y.
-template <int EPI>
+template <bool BF, int EPI>
 __device__ __forceinline__ void finish(const LinearArgs& a, int64_t i, int64_t j, int left, float (&v)[8],
-                                       const u32x4_t& res, bool bf) {
+                                       const u32x4_t& res) {
   if constexpr (EPI != kNoEpilogue) {
     if constexpr (EPI != FMX_ACT_NONE) {
       float s[8];
       if (a.slope) {
         activate<EPI, true>(v, s, a.act);
-        store_raw(a.slope, i * a.J + j, left, slopes8(s));
+        store_raw(a.slope, i * a.J + j, left, slopes8<BF>(s));
       } else {
         activate<EPI, false>(v, s, a.act);
       }
     }
     if (a.res) {
       float r[8];
-      unpack8(r, res, bf);
+      unpack8(r, res, BF);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] += r[k];
     }
   }
-  store16(a.y, i * a.J + j, left, v, bf);
+  store16(a.y, i * a.J + j, left, v, BF);
 }
 
 // ---- the product ----
@@ -515,7 +539,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               activate<EPI, true>(v[h], s, a.act);
-              put(x, h, slopes8(s));
+              put(x, h, slopes8<BF>(s));
             }
             flush(x, a.slope);
           } else {
@@ -570,7 +594,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] += b[k];
-        finish<EPI>(a, i, j, left, v, res[x], BF);
+        finish<BF, EPI>(a, i, j, left, v, res[x]);
       }
     }
   }
@@ -621,7 +645,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a, int grou
       v[4 + k] += s1[k];
     }
     const u32x4_t res = EPI != kNoEpilogue && a.res ? load_raw(a.res, i * a.sres + j, left) : u32x4_t{0u, 0u, 0u, 0u};
-    finish<EPI>(a, i, j, left, v, res, BF);
+    finish<BF, EPI>(a, i, j, left, v, res);
   }
 }
 
@@ -687,7 +711,7 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
         v[k] += s0[k];
         v[4 + k] += s1[k];
       }
-      finish<kAnyAct>(a, i, j, left, v, res, BF);
+      finish<BF, kAnyAct>(a, i, j, left, v, res);
     }
   }
 }
@@ -714,7 +738,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(DzArgs a) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const uint32_t x = w[k / 2];
-          v[k] *= slope_of((k & 1) ? x >> 16 : x & 0xffffu);
+          v[k] *= slope_of<BF>((k & 1) ? x >> 16 : x & 0xffffu);
         }
       }
       if (a.dz) store16(a.dz, i * a.Np + j, 8, v, BF);

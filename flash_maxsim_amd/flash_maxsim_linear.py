@@ -7,9 +7,11 @@ at the token embeddings).
 
 Operands are all float16 or all bfloat16; products run on MFMA with float32 sums,
 and y is rounded once. The backward rounds dz = dy act'(z) to the operands' type,
-as MFMA takes it; the slopes act'(z) are kept between the passes in 16 bits, in
-steps of 2^-14 (only with an activation). Bias gradients sum the unrounded dz. Sums have a fixed order:
-the same inputs give the same bits.
+as MFMA takes it; the slopes act'(z) are kept between the passes in 16 bits (only
+with an activation), whose steps get finer towards zero: at most 2^-14 (bfloat16:
+2^-13) of the slope down to 0.28 (0.07), and slopes down to 2^-30 (2^-60) are not
+lost. Bias gradients sum the unrounded dz. Sums have a fixed order: the same
+inputs give the same bits.
 
 x and weight are read in place when their rows are 16-byte aligned and K is a
 multiple of 8; other layouts are copied once per call with K zero-padded to a

@@ -401,8 +401,9 @@ size_t fmx_bwd_batched_workspace_bytes(int64_t Nq, int64_t B, int64_t Lq, int64_
  *   bias      [N]     dtype, or NULL
  *   residual  [M, N]  dtype, row stride r_stride, or NULL
  *   y         [M, N]  dtype, contiguous
- *   slope     [M, N]  int16, contiguous: act'(x W^T + bias) in steps of 2^-14 (-2^15: NaN) for the
- *                     backward; or NULL. Not written without an activation.
+ *   slope     [M, N]  int16, contiguous: act'(x W^T + bias) for the backward of the same dtype, in a code of its
+ *                     own whose steps get finer towards zero (at 1/2 to 1 half a step is 2^-15, BF16 2^-14, and
+ *                     below a small part of the slope itself); or NULL. Not written without an activation.
  * x and w are 16-byte aligned, their strides multiples of 8 and at least K
  * rounded up to 8; elements from K up to there are zeros. M <=
  * FMX_LINEAR_MAX_ROWS, K and N < 2^24, strides < 2^22.

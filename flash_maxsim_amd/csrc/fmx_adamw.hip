@@ -19,7 +19,9 @@
 // is compared with c^2 + c + 1/4, which float32 holds exactly. A root that is
 // not zero keeps at least code 1, so no element's step grows because its second
 // moment was rounded to nothing. A block with a value that is not finite
-// decodes to NaN.
+// decodes to NaN: of the first moment zeros times an infinite scale, of the
+// second, whose codes of at least 1 would make that infinite (steps of zero for
+// all of the block from then on), by a scale that is NaN.
 //
 // Bound by HBM: 28 bytes a parameter in float32, 10 with bf16 parameters and
 // 8-bit moments, against about 40 (80) vector operations.
@@ -161,7 +163,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamWTensor& t, const AdamWSca
     const float im = zm ? 0.0f : 16129.0f / bm, iv = zv ? 0.0f : 65025.0f / bv;
     if ((threadIdx.x & 31) == 0 && (WHOLE || i0 < n)) {
       t.ms[block] = zm ? 0.0f : bm / 16129.0f;
-      t.vs[block] = zv ? 0.0f : bv / 65025.0f;
+      t.vs[block] = zv ? 0.0f : bv < __builtin_inff() ? bv / 65025.0f : __builtin_nanf("");
     }
     store8<WHOLE>(static_cast<int8_t*>(t.m), i0, n, [&](int i) {
       const int c = code_of(__builtin_fabsf(m[i]) * im);

@@ -187,6 +187,19 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"{len(copies)} copies for {len(mine)} parameters")
         self._copies = {id(p): c for p, c in zip(mine, copies) if c is not None}
 
+    def __getstate__(self):
+        """torch's, with the bits and the copies (deep copies and pickles)."""
+        params = [p for g in self.param_groups for p in g["params"]]
+        return super().__getstate__() | {"_bits": self._bits, "_copies": [self._copies.get(id(p)) for p in params]}
+
+    def __setstate__(self, state) -> None:
+        """torch calls this too when it loads a state_dict, whose state has neither."""
+        copies = state.get("_copies")
+        super().__setstate__({k: v for k, v in state.items() if k != "_copies"})
+        if copies is not None:
+            params = [p for g in self.param_groups for p in g["params"]]
+            self._copies = {id(p): c for p, c in zip(params, copies) if c is not None}
+
     @torch.no_grad()
     def step(self, closure=None, grad_scale: torch.Tensor | None = None):
         loss = None

@@ -169,7 +169,7 @@ class AdamW(torch.optim.Optimizer):
     state_bits is 32 or 8. copies, in the order of the parameters, are 16-bit
     tensors (or None) that receive the new float32 parameters. Learning-rate
     schedulers, parameter groups and state_dict work as with torch's optimizers;
-    loaded state keeps its types. `step(grad_scale=...)` passes a float32 GPU
+    loaded moments stay in the bits they have. `step(grad_scale=...)` passes a float32 GPU
     scalar that multiplies the gradients.
     """
 
@@ -237,9 +237,9 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict) -> None:
-        """torch's, with each state tensor in its own type again (torch casts
-        float state to its parameter's type, which would round the moments).
-        A state of torch.optim.AdamW continues as one of 32 bits."""
+        """torch's, with moments and scales in float32 and codes in their type again (torch casts
+        float state to its parameter's type, which would round the moments). A state of
+        torch.optim.AdamW, whose moments of 16-bit parameters are 16-bit, continues as one of 32 bits."""
         if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
             raise ValueError("this AdamW has neither amsgrad nor maximize")
         saved = state_dict["state"]
@@ -250,5 +250,8 @@ class AdamW(torch.optim.Optimizer):
             for k, v in saved.get(i, {}).items():
                 if k == "step":  # a tensor in states of torch's optimizers
                     self.state[p][k] = int(v)
+                elif torch.is_tensor(v):  # codes keep their type; torch's moments are of the parameters'
+                    dtype = torch.float32 if v.is_floating_point() else v.dtype
+                    self.state[p][k] = v.detach().to(p.device, dtype, copy=True).contiguous()
                 else:
-                    self.state[p][k] = v.detach().to(p.device, copy=True).contiguous() if torch.is_tensor(v) else v
+                    self.state[p][k] = v

@@ -221,17 +221,18 @@ class AdamW(torch.optim.Optimizer):
                     else:
                         s["exp_avg"], s["exp_avg_sq"] = m, v
                 s["step"] += 1
-                row = batches.setdefault(s["step"], ([], [], [], [], []))
+                eight = "exp_avg_scale" in s  # loaded 32-bit moments may stand beside new 8-bit ones
+                row = batches.setdefault((s["step"], eight), ([], [], [], [], []))
                 row[0].append(p)
                 row[1].append(p.grad)
-                if "exp_avg_scale" in s:
+                if eight:
                     row[2].append(AdamW8bitState(s["exp_avg"], s["exp_avg_scale"]))
                     row[3].append(AdamW8bitState(s["exp_avg_sq"], s["exp_avg_sq_scale"]))
                 else:
                     row[2].append(s["exp_avg"])
                     row[3].append(s["exp_avg_sq"])
                 row[4].append(self._copies.get(id(p)))
-            for step, (p, g, m, v, c) in batches.items():
+            for (step, _), (p, g, m, v, c) in batches.items():
                 adamw_step(p, g, m, v, step, group["lr"], group["betas"], group["eps"], group["weight_decay"],
                            grad_scale, c if any(x is not None for x in c) else None)
         return loss

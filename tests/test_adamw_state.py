@@ -84,3 +84,28 @@ def test_copied_optimizers_step_alike(again, bits):
     for p, q, c, e in zip(params(opt), params(other), copies_of(opt), copies_of(other)):
         assert p is not q and torch.equal(p, q)
         assert c is None or (torch.equal(e, q.detach().bfloat16()) and torch.equal(c, e) and c is not e)
+
+
+@pytest.mark.gpu
+def test_moments_of_both_kinds_at_one_step():
+    """A loaded 32-bit state beside parameters whose moments begin in 8 bits."""
+    g = torch.Generator().manual_seed(11)
+    init = [torch.randn(40, generator=g).cuda() for _ in range(2)]
+    grads = [torch.randn(40, generator=g).cuda() for _ in range(2)]
+
+    def step(opt, ps, which):
+        for i, p in enumerate(ps):
+            p.grad = grads[i].clone() if i in which else None
+        opt.step()
+
+    old = [torch.nn.Parameter(t.clone()) for t in init]
+    saved = fm.AdamW(old, state_bits=32)
+    step(saved, old, {0})
+    ps = [torch.nn.Parameter(t.detach().clone()) for t in old]
+    opt = fm.AdamW(ps, state_bits=8)
+    opt.load_state_dict(saved.state_dict())
+    step(opt, ps, {1})  # now both stand at one step, of 32 and of 8 bits
+    step(opt, ps, {0, 1})
+    assert opt.state[ps[0]]["exp_avg"].dtype == torch.float32 and opt.state[ps[1]]["exp_avg"].dtype == torch.int8
+    step(saved, old, {0})
+    assert torch.equal(old[0], ps[0]) and opt.state[ps[1]]["step"] == 2

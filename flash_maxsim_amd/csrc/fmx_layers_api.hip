@@ -129,12 +129,14 @@ size_t fmx_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K) {
 int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* dy,
                    int64_t dy_stride, const int16_t* slope, int act, int64_t M, int64_t N, int64_t K, void* dx, void* dw,
                    void* db, void* workspace, size_t workspace_bytes, void* stream) {
-  const int rc = check_linear(dtype, x_stride, w_stride, act, M, N, K);
+  // x is read for dw alone and w for dx; one that is missing has no stride
+  const int64_t k8 = (K + 7) / 8 * 8;
+  const int rc = check_linear(dtype, x ? x_stride : k8, w ? w_stride : k8, act, M, N, K);
   if (rc) return rc;
   if (dy_stride < 0) return fail(FMX_ERR_INVALID, "dy stride must be >= 0");
   if (!dx && !dw && !db) return ok();
-  if (M > 0 && (!x || !w || !dy || (act != FMX_ACT_NONE && !slope)))
-    return fail(FMX_ERR_INVALID, "x, w, dy and (with an activation) slope must be non-null");
+  if (M > 0 && ((dw && !x) || (dx && !w) || !dy || (act != FMX_ACT_NONE && !slope)))
+    return fail(FMX_ERR_INVALID, "x (for dw), w (for dx), dy and (with an activation) slope must be non-null");
   if (!aligned(x, 16) || !aligned(w, 16)) return fail(FMX_ERR_INVALID, "x and w must be 16-byte aligned");
   if (!aligned(dy, 2) || !aligned(slope, 2) || !aligned(dx, 2) || !aligned(dw, 2) || !aligned(db, 2))
     return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");

@@ -161,6 +161,7 @@ Tensor scratch(size_t n, const Tensor& like) {
   return n ? at::empty({(int64_t)((n + 3) / 4)}, like.options().dtype(at::kFloat)) : Tensor();
 }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+const void* const_ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
 PyObject* failed(int rc) {
   PyErr_Format(PyExc_RuntimeError, "flash_maxsim_amd: %s (code %d)", fmx_last_error(), rc);
@@ -560,7 +561,8 @@ Tensor given_back(const torch::autograd::SavedVariable& saved, const Tensor& dy,
 }
 
 struct LinearBackward : public torch::autograd::Node {
-  torch::autograd::SavedVariable x, w, slope;  // x and w as the kernels read them
+  // x and w as the kernels read them; each is there where a wanted gradient needs it: x for dw, w for dx
+  torch::autograd::SavedVariable x, w, slope;
   std::vector<int64_t> x_sizes;
   int64_t M, N, K;
   int dtype, act;
@@ -574,20 +576,23 @@ struct LinearBackward : public torch::autograd::Node {
       at::AutoGradMode off(false);
       const at::ScalarType type = dy0.scalar_type();
       const int64_t K8 = (K + 7) / 8 * 8;
-      int64_t m, stride, x_stride, w_stride;
-      const Tensor xk = given_back(x, dy0, type, M, K8, &x_stride, true), wk = given_back(w, dy0, type, N, K8, &w_stride, true);
-      const Tensor sk = act ? given_back(slope, dy0, at::kShort, M, N) : Tensor();
-      const Tensor& dy = grad_rows(dy0, &keep, &m, &stride);
-      const auto options = xk.options();
-      if (task_should_compute_output(0)) dx = at::empty(x_sizes, options);
-      if (task_should_compute_output(1)) dw = at::empty({N, K}, options);
-      if (task_should_compute_output(2)) db = at::empty({N}, options);
-      if (dx.defined() || dw.defined() || db.defined()) {
+      const bool want_x = task_should_compute_output(0), want_w = task_should_compute_output(1),
+                 want_b = task_should_compute_output(2);
+      if (want_x || want_w || want_b) {
+        int64_t m, stride, x_stride = 0, w_stride = 0;
+        const Tensor xk = want_w ? given_back(x, dy0, type, M, K8, &x_stride, true) : Tensor();
+        const Tensor wk = want_x ? given_back(w, dy0, type, N, K8, &w_stride, true) : Tensor();
+        const Tensor sk = act ? given_back(slope, dy0, at::kShort, M, N) : Tensor();
+        const Tensor& dy = grad_rows(dy0, &keep, &m, &stride);
+        const auto options = dy.options();
+        if (want_x) dx = at::empty(x_sizes, options);
+        if (want_w) dw = at::empty({N, K}, options);
+        if (want_b) db = at::empty({N}, options);
         const size_t n = fmx_linear_bwd_workspace_bytes(M, N, K);
-        const Tensor ws = scratch(n, xk);
-        must(fmx_linear_bwd(dtype, xk.const_data_ptr(), x_stride, wk.const_data_ptr(), w_stride, dy.const_data_ptr(),
-                            stride, sk.defined() ? sk.const_data_ptr<int16_t>() : nullptr, act, M, N, K, ptr(dx), ptr(dw),
-                            ptr(db), ptr(ws), n, stream_of(xk)));
+        const Tensor ws = scratch(n, dy);
+        must(fmx_linear_bwd(dtype, const_ptr(xk), x_stride, const_ptr(wk), w_stride, dy.const_data_ptr(), stride,
+                            static_cast<const int16_t*>(const_ptr(sk)), act, M, N, K, ptr(dx), ptr(dw), ptr(db), ptr(ws), n,
+                            stream_of(dy)));
       }
     }
     // the residual's gradient is dy itself
@@ -691,7 +696,8 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (prc) return failed(prc);
   const bool grad = grad_wanted({x, w, b, r});
   Tensor y = at::empty(sizes, x->options());
-  Tensor slope = grad && act ? at::empty({M, N}, x->options().dtype(at::kShort)) : Tensor();
+  const bool sloped = act && grad_wanted({x, w, b});  // the residual's gradient needs none
+  Tensor slope = sloped ? at::empty({M, N}, x->options().dtype(at::kShort)) : Tensor();
   const size_t n = fmx_linear_workspace_bytes(M, N, K);
   const Tensor ws = scratch(n, *x);
   const int rc = unlocked([&] {
@@ -702,9 +708,9 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (grad) {
     std::shared_ptr<LinearBackward> node(new LinearBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(*x, *w, b ? *b : Tensor(), r ? *r : Tensor()));
-    node->x = torch::autograd::SavedVariable(xk, false);
-    node->w = torch::autograd::SavedVariable(wk, false);
-    if (act) node->slope = torch::autograd::SavedVariable(slope, false);
+    if (w->requires_grad()) node->x = torch::autograd::SavedVariable(xk, false);
+    if (x->requires_grad()) node->w = torch::autograd::SavedVariable(wk, false);
+    if (sloped) node->slope = torch::autograd::SavedVariable(slope, false);
     node->x_sizes = x->sizes().vec();
     node->M = M;
     node->N = N;

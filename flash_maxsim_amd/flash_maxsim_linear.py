@@ -80,9 +80,11 @@ def _forward(x, weight, bias, act, residual, save):
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, act, residual):
-        y, xk, wk, slope = _forward(x, weight, bias, act, residual, True)
-        ctx.save_for_backward(xk, wk, slope)
-        ctx.act, ctx.shape, ctx.sizes = act, x.shape, tuple(weight.shape)
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        y, xk, wk, slope = _forward(x, weight, bias, act, residual, need_x or need_w or need_b)
+        # dx reads w, dw reads x: an operand that no wanted gradient needs is free to go or to change
+        ctx.save_for_backward(xk if need_w else None, wk if need_x else None, slope)
+        ctx.act, ctx.shape, ctx.sizes = act, x.shape, (xk.size(0), *weight.shape)
         return y
 
     @staticmethod
@@ -90,12 +92,13 @@ class _LinearFn(torch.autograd.Function):
     def backward(ctx, dy):
         xk, wk, slope = ctx.saved_tensors
         # hooks on saved tensors may give them back in another layout
-        xk, wk, slope = _operand(xk), _operand(wk), None if slope is None else slope.contiguous()
-        (N, K), M, dev = ctx.sizes, xk.size(0), xk.device
+        xk, wk = (None if t is None else _operand(t) for t in (xk, wk))
+        slope = None if slope is None else slope.contiguous()
+        (M, N, K), dev = ctx.sizes, dy.device
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(ctx.shape, device=dev, dtype=xk.dtype) if need_x else None
-        dw = torch.empty(N, K, device=dev, dtype=xk.dtype) if need_w else None
-        db = torch.empty(N, device=dev, dtype=xk.dtype) if need_b else None
+        dx = torch.empty(ctx.shape, device=dev, dtype=dy.dtype) if need_x else None
+        dw = torch.empty(N, K, device=dev, dtype=dy.dtype) if need_w else None
+        db = torch.empty(N, device=dev, dtype=dy.dtype) if need_b else None
         if need_x or need_w or need_b:
             dys = _rows(dy, N)
             lib = _lib.load()
@@ -103,9 +106,9 @@ class _LinearFn(torch.autograd.Function):
                 nbytes = lib.fmx_linear_bwd_workspace_bytes(M, N, K)
                 ws = _lib.workspace(nbytes, dev)
                 rc = lib.fmx_linear_bwd(
-                    _lib.dtype_code(xk), xk.data_ptr(), xk.stride(0), wk.data_ptr(), wk.stride(0), dys.data_ptr(),
-                    dys.stride(0), _lib.ptr(slope), ctx.act, M, N, K, _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db),
-                    _lib.ptr(ws), nbytes, _lib.stream_of(xk),
+                    _lib.dtype_code(dy), _lib.ptr(xk), 0 if xk is None else xk.stride(0), _lib.ptr(wk),
+                    0 if wk is None else wk.stride(0), dys.data_ptr(), dys.stride(0), _lib.ptr(slope), ctx.act, M, N, K,
+                    _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws), nbytes, _lib.stream_of(dys),
                 )
             _lib.check(rc)
         return dx, dw, db, None, dy if ctx.needs_input_grad[4] else None

@@ -417,9 +417,9 @@ size_t fmx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 /*
  * Its backward: dz = dy slope (rounded to dtype, the products' operand),
  *   dx = dz W  [M, K],  dw = dz^T x  [N, K],  db = sum over rows of dz before rounding  [N]
- * contiguous in dtype, each skipped when NULL. x and w as in the forward; dy
- * [M, N] with row stride dy_stride; slope as the forward wrote it (unused without
- * an activation). The residual's gradient is dy itself. Deterministic.
+ * contiguous in dtype, each skipped when NULL. x and w as in the forward, x only
+ * read for dw and w for dx (else they may be NULL); dy [M, N] with row stride
+ * dy_stride; slope as the forward wrote it (unused without an activation). The residual's gradient is dy itself. Deterministic.
  */
 int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* dy,
                    int64_t dy_stride, const int16_t* slope, int act, int64_t M, int64_t N, int64_t K, void* dx, void* dw,

@@ -136,3 +136,15 @@ def test_python_functions_refuse_cpu_tensors_and_bad_types():
     assert m.codes.dtype == torch.int8 and v.codes.dtype == torch.uint8 and m.scales.shape == (2,)
     with pytest.raises(ValueError):
         fm.adamw_state(p, 4)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(x=None, dw=None), WORKSPACE), (dict(w=None, dx=None), WORKSPACE),
+    (dict(x=None, xs=0, w=None, ws=0, dx=None, dw=None), WORKSPACE),  # db alone
+    (dict(x=None), INVALID), (dict(w=None), INVALID), (dict(x=None, dx=None), INVALID), (dict(w=None, dw=None), INVALID),
+    (dict(x=None, w=None, dy=None, dx=None, dw=None), INVALID),
+    (dict(x=None, w=None, act=2, dx=None, dw=None), INVALID),
+    (dict(x=None, dw=None, ws=60), INVALID), (dict(w=None, dx=None, xs=60), INVALID),
+])
+def test_linear_bwd_takes_the_operands_that_it_reads(lib, kw, code):
+    assert linear_bwd(lib, **kw) == code

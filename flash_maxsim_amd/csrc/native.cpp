@@ -691,9 +691,11 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return out;
   };
   int64_t sw = w->stride(0);
-  const Tensor xk = operand(*x, M, &sx), wk = operand(*w, N, &sw);
-  FMX_ORDINARY(fits);
+  const Tensor xk = operand(*x, M, &sx);
   if (prc) return failed(prc);
+  const Tensor wk = fits ? operand(*w, N, &sw) : Tensor();
+  if (prc) return failed(prc);
+  FMX_ORDINARY(fits);
   const bool grad = grad_wanted({x, w, b, r});
   Tensor y = at::empty(sizes, x->options());
   const bool sloped = act && grad_wanted({x, w, b});  // the residual's gradient needs none

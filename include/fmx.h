@@ -404,9 +404,9 @@ size_t fmx_bwd_batched_workspace_bytes(int64_t Nq, int64_t B, int64_t Lq, int64_
  *   slope     [M, N]  int16, contiguous: act'(x W^T + bias) for the backward of the same dtype, in a code of its
  *                     own whose steps get finer towards zero (at 1/2 to 1 half a step is 2^-15, BF16 2^-14, and
  *                     below a small part of the slope itself); or NULL. Not written without an activation.
- * x and w are 16-byte aligned, their strides multiples of 8 and at least K
- * rounded up to 8; elements from K up to there are zeros. M <=
- * FMX_LINEAR_MAX_ROWS, K and N < 2^24, strides < 2^22.
+ * x and w are 16-byte aligned, their strides multiples of 8, at least K rounded
+ * up to 8 (so that is their limit of K) and < 2^22; elements from K up to there
+ * are zeros. M <= FMX_LINEAR_MAX_ROWS, N < 2^24.
  */
 int fmx_linear(int dtype, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
                const void* residual, int64_t r_stride, int act, int64_t M, int64_t N, int64_t K, void* y, int16_t* slope,

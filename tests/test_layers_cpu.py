@@ -148,3 +148,11 @@ def test_python_functions_refuse_cpu_tensors_and_bad_types():
 ])
 def test_linear_bwd_takes_the_operands_that_it_reads(lib, kw, code):
     assert linear_bwd(lib, **kw) == code
+
+
+def test_linear_limit_of_k(lib):
+    """Rows hold K rounded up to 8 elements, and their strides are below 2^22."""
+    top = (1 << 22) - 8
+    assert linear(lib, K=top, xs=top, ws=top) == WORKSPACE and linear_bwd(lib, K=top, xs=top, ws=top) == WORKSPACE
+    for call in (linear, linear_bwd):
+        assert call(lib, K=top + 1, xs=top + 8, ws=top + 8) == UNSUPPORTED and "strides" in lib.fmx_last_error().decode()

@@ -172,3 +172,35 @@ def test_gradients_of_arguments_far_out(M, N, K, name, mean, dtype, size):
         assert off.max() <= 1.01, off.max().item()
         # and by their own size: roundings are not all of one sign
         assert (got - want).norm() <= (0.1 if dtype == torch.float16 else 0.02) * want.norm()
+
+
+@pytest.mark.parametrize("name", ["gelu", "silu"])
+def test_more_than_2_32_slopes(name):
+    """Gradients of a few rows of 4.3e9 outputs, the last ones among them."""
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GB of free GPU memory")
+    dtype, (M, N, K) = torch.float16, ((1 << 20) + 5, 4104, 16)
+    g = torch.Generator().manual_seed(5)
+    pick = torch.tensor([0, 1, 1023, 1 << 19, 1046527, 1046528, 1 << 20, M - 2, M - 1])  # 1046528 * 4104 passes 2^32
+    part = torch.randn(4099, K, generator=g).to(dtype)
+    w, b = torch.randn(N, K, generator=g).to(dtype), torch.full((N,), -4.0).to(dtype)
+    dyp = (64 * torch.randn(len(pick), N, generator=g)).to(dtype)
+    x = part.cuda().repeat(-(-M // 4099), 1)[:M].requires_grad_(True)
+    leaves = [x, w.cuda().requires_grad_(True), b.cuda().requires_grad_(True)]
+    dy = torch.zeros(M, N, dtype=dtype, device="cuda")
+    dy[pick.cuda()] = dyp.cuda()
+    dx, dw, db = torch.autograd.grad(fm.linear(*leaves, name), leaves, dy)
+    assert not dx[5000].any() and not dx[M - 3].any()
+    u, tiny = UNIT[dtype], TINY[dtype]
+    xd, wd, bd, dyd = part[pick % 4099].double(), w.double(), b.double(), dyp.double()
+    z = xd @ wd.t() + bd
+    ze = F32 * (K + 4) * (xd.abs() @ wd.abs().t() + bd.abs())
+    s, least, most = bound(z, name, dtype)
+    _, _, ds = slope(z, name)
+    dz, dze = dyd * s, dyd.abs() * (torch.maximum((most - s).abs(), (least - s).abs()) + ze * (1.1 * ds.abs() + 4 * ze))
+    dzr = dze + u * (dz.abs() + dze) + tiny
+    for got, want, tol in ((dx[pick.cuda()], dz @ wd, dzr @ wd.abs() + F32 * (N + 4) * (dz.abs() @ wd.abs())),
+                           (dw, dz.t() @ xd, dzr.t() @ xd.abs() + F32 * (len(pick) + 4) * (dz.abs().t() @ xd.abs())),
+                           (db, dz.sum(0), dze.sum(0) + F32 * (len(pick) + 4) * dz.abs().sum(0))):
+        off = (got.cpu().double() - want).abs() / (tol + u * want.abs() + tiny)
+        assert off.max() <= 1.01, off.max().item()

@@ -63,6 +63,12 @@ def _abi_ready(t: torch.Tensor, dtype: torch.dtype | None) -> bool:
     return all(s % 8 == 0 for s in t.stride()[:-1])
 
 
+def _own_strides(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous t with the strides that its sizes give: torch calls a tensor contiguous whatever the stride of
+    a dimension of one is, or of any where it is empty, and the kernels' checks look at strides."""
+    return t.flatten().view(t.shape)
+
+
 def _prep(t: torch.Tensor, dtype: torch.dtype | None) -> torch.Tensor:
     """t itself when the kernels can read it in place, else a contiguous cast
     copy with d zero-padded to a multiple of 8, 16-byte aligned."""

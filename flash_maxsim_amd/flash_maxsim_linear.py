@@ -25,7 +25,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .flash_maxsim import _abi_ready, _check_devices, _device_guard
+from .flash_maxsim import _abi_ready, _check_devices, _device_guard, _own_strides
 from .flash_maxsim_norm import _differentiated, _rows
 
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
@@ -37,7 +37,7 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
     K = t.shape[1]
     if K % 8 == 0 and _abi_ready(t, None) and t.stride(0) < 1 << 22:
         return t
-    t = F.pad(t, (0, -K % 8)) if K % 8 else t.contiguous()
+    t = F.pad(t, (0, -K % 8)) if K % 8 else _own_strides(t.contiguous())
     return t.clone() if t.data_ptr() % 16 else t
 
 

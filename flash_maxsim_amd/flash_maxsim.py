@@ -82,7 +82,7 @@ def _prep(t: torch.Tensor, dtype: torch.dtype | None) -> torch.Tensor:
         t = F.pad(t, (0, pad))
     if t.data_ptr() % 16:
         t = t.clone()
-    return t
+    return _own_strides(t)
 
 
 def _lengths(total: int, device: torch.device, doc_lengths) -> torch.Tensor | None:

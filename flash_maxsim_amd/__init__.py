@@ -25,6 +25,7 @@ from .flash_maxsim_packed import (PackedDocs, PackedInt8Docs, flash_maxsim_int8_
                                   pack_docs, quantize_int8_packed)
 from .flash_maxsim_topk import flash_maxsim_batched_topk, flash_maxsim_int8_topk, flash_maxsim_topk, topk_scores
 from .flash_maxsim_linear import linear
+from .flash_maxsim_gated import gated_linear
 from .flash_maxsim_norm import layer_norm
 from .flash_maxsim_optim import AdamW, AdamW8bitState, adamw_state, adamw_step, dequantize_adamw
 
@@ -50,6 +51,7 @@ __all__ = [
     "flash_maxsim_int8_topk",
     "flash_maxsim_train_batched",
     "linear",
+    "gated_linear",
     "layer_norm",
     "AdamW",
     "AdamW8bitState",

@@ -105,6 +105,17 @@ _SIGNATURES = {
         [_int, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _int, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _size, _ptr],
     ),
     "fmx_linear_bwd_workspace_bytes": (_size, [_i64, _i64, _i64]),
+    "fmx_gated": (
+        _int,
+        [_int, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _int, _i64, _i64, _i64, _ptr, _ptr, _ptr, _size, _ptr],
+    ),
+    "fmx_gated_workspace_bytes": (_size, [_i64, _i64, _i64]),
+    "fmx_gated_bwd": (
+        _int,
+        [_int, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr,
+         _ptr, _size, _ptr],
+    ),
+    "fmx_gated_bwd_workspace_bytes": (_size, [_i64, _i64, _i64]),
     "fmx_layer_norm": (
         _int,
         [_int, _ptr, _i64, _int, _ptr, _ptr, _i64, _i64, _f64, _ptr, _ptr, _ptr, _ptr],

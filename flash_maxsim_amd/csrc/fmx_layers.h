@@ -95,6 +95,9 @@ struct LinearArgs {
   int64_t split_k, band;
   int splits;
   int act;
+  const void* B2;         // dx of a gated layer: rows of B for the first `half` stages of k, then those of B2, kb of each
+  int64_t sb2;
+  int half, kb;
 };
 
 struct LinearPlan {
@@ -120,5 +123,43 @@ struct DzArgs {
 int linear_dz_parts(int64_t M, int64_t N);
 hipError_t launch_linear_dz(bool bf16, DzArgs a, int parts, hipStream_t s);
 hipError_t launch_linear_zero(void* out, int64_t n, hipStream_t s);  // n > 0 zeros of 16 bits
+
+// ---- gated linear (fmx_gated.hip) ----
+
+struct GatedArgs {
+  const void* x;          // [I, K], row stride sx; the weights [J, K]
+  const void* wg;
+  const void* wu;
+  int64_t sx, swg, swu;   // multiples of 8
+  int64_t I, J, K;
+  int64_t I0;             // rows of the whole call (set by launch_gated)
+  const void* bg;         // [J] each, or null
+  const void* bu;
+  void* y;                // [I, J] 16-bit, contiguous
+  void* keep;             // the backward's factors: planes of [I0, J] 16-bit words, of dg's, of du's and (fp16) of their
+                          // low bytes; or null
+  float* part;            // splits > 1: [splits][2][I][Jp]
+  int64_t Jp, ti, tj, split_k, band;
+  int splits, act;
+};
+
+struct GatedPlan {
+  int tile, rows, splits;
+  int64_t ti, tj, split_k, band;
+};
+GatedPlan gated_plan(int64_t I, int64_t J, int64_t K);
+size_t gated_part_bytes(const GatedPlan& p, int64_t I, int64_t J);
+hipError_t launch_gated(bool bf16, GatedArgs a, const GatedPlan& p, hipStream_t s);
+
+struct GatedDzArgs {
+  const void* dy;         // [M, N], row stride sdy
+  const void* keep;       // as GatedArgs
+  void* dz;               // [M, 2 Np] 16-bit, or null
+  float* part;            // [parts][2][N] column sums, or null
+  int64_t sdy, M, N, Np;  // Np: N rounded up to a stage of 64
+  int lanes;              // of a row, a power of two; set by launch_gated_dz
+};
+int gated_dz_parts(int64_t M, int64_t N);
+hipError_t launch_gated_dz(bool bf16, GatedDzArgs a, int parts, hipStream_t s);
 
 }  // namespace fmx

@@ -77,6 +77,31 @@ LinearBwdWs linear_bwd_ws(int64_t M, int64_t N, int64_t K) {
   return w;
 }
 
+int check_gated(int dtype, int64_t x_stride, int64_t wg_stride, int64_t wu_stride, int act, int64_t M, int64_t N, int64_t K) {
+  const int rc = check_linear(dtype, x_stride, wg_stride, act, M, N, K);
+  if (rc) return rc;
+  if (N >= 1 << 20) return fail(FMX_ERR_UNSUPPORTED, "N=%lld too large", (long long)N);
+  return check_linear(dtype, x_stride, wu_stride, act, M, N, K);
+}
+
+// Backward workspace: dg and du beside each other, their column sums, the partial products of dx and of one weight's
+// gradient (used one after the other).
+struct GatedBwdWs {
+  size_t dz, sums, part;
+  size_t total() const { return dz + sums + part; }
+};
+int64_t gated_np(int64_t N) { return (N + 63) / 64 * 64; }
+GatedBwdWs gated_bwd_ws(int64_t M, int64_t N, int64_t K) {
+  const int64_t np = gated_np(N);
+  GatedBwdWs w;
+  w.dz = round256((size_t)M * (size_t)np * 4);
+  w.sums = round256((size_t)fmx::gated_dz_parts(M, N) * 2 * (size_t)N * sizeof(float));
+  const size_t px = fmx::linear_part_bytes(fmx::linear_plan(fmx::kLinearInput, M, K, 2 * np), M, K);
+  const size_t pw = fmx::linear_part_bytes(fmx::linear_plan(fmx::kLinearWeight, N, K, M), N, K);
+  w.part = round256(px > pw ? px : pw);
+  return w;
+}
+
 }  // namespace
 
 extern "C" {
@@ -207,6 +232,133 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
     if (beside && !later && e == hipSuccess) e = fmx::launch_join(dtype, sums, parts, N, 0, db, nullptr, s);
   }
   return hip_status(e, "fmx_linear_bwd launch");
+}
+
+size_t fmx_gated_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  return fmx::gated_part_bytes(fmx::gated_plan(M, N, (K + 7) / 8 * 8), M, N);
+}
+
+int fmx_gated(int dtype, const void* x, int64_t x_stride, const void* wg, int64_t wg_stride, const void* wu,
+              int64_t wu_stride, const void* bg, const void* bu, int act, int64_t M, int64_t N, int64_t K, void* y,
+              int16_t* factors, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_gated(dtype, x_stride, wg_stride, wu_stride, act, M, N, K);
+  if (rc) return rc;
+  if (M == 0) return ok();
+  if (!x || !wg || !wu || !y) return fail(FMX_ERR_INVALID, "x, wg, wu and y must be non-null");
+  if (!aligned(x, 16) || !aligned(wg, 16) || !aligned(wu, 16))
+    return fail(FMX_ERR_INVALID, "x, wg and wu must be 16-byte aligned");
+  if (!aligned(y, 2) || !aligned(factors, 2) || !aligned(bg, 2) || !aligned(bu, 2))
+    return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");
+  fmx::GatedArgs a = {};
+  a.x = x;
+  a.wg = wg;
+  a.wu = wu;
+  a.sx = x_stride;
+  a.swg = wg_stride;
+  a.swu = wu_stride;
+  a.I = M;
+  a.J = N;
+  a.K = (K + 7) / 8 * 8;
+  a.bg = bg;
+  a.bu = bu;
+  a.y = y;
+  a.keep = factors;
+  a.act = act;
+  a.part = static_cast<float*>(workspace);
+  const fmx::GatedPlan p = fmx::gated_plan(M, N, a.K);
+  const size_t need = fmx::gated_part_bytes(p, M, N);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(FMX_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace_bytes);
+  return hip_status(fmx::launch_gated(dtype == FMX_DTYPE_BF16, a, p, static_cast<hipStream_t>(stream)), "fmx_gated launch");
+}
+
+size_t fmx_gated_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  return gated_bwd_ws(M, N, K).total();
+}
+
+int fmx_gated_bwd(int dtype, const void* x, int64_t x_stride, const void* wg, int64_t wg_stride, const void* wu,
+                  int64_t wu_stride, const void* dy, int64_t dy_stride, const int16_t* factors, int64_t M, int64_t N,
+                  int64_t K, void* dx, void* dwg, void* dwu, void* dbg, void* dbu, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+  // x is read for the weights' gradients alone and the weights for dx; one that is missing has no stride
+  const int64_t k8 = (K + 7) / 8 * 8;
+  const int rc = check_gated(dtype, x ? x_stride : k8, wg ? wg_stride : k8, wu ? wu_stride : k8, FMX_ACT_NONE, M, N, K);
+  if (rc) return rc;
+  if (dy_stride < 0) return fail(FMX_ERR_INVALID, "dy stride must be >= 0");
+  const bool weights = dwg || dwu, sums = dbg || dbu;
+  if (!dx && !weights && !sums) return ok();
+  if (M > 0 && ((weights && !x) || (dx && (!wg || !wu)) || !dy || !factors))
+    return fail(FMX_ERR_INVALID, "x (for dwg and dwu), wg and wu (for dx), dy and factors must be non-null");
+  if (!aligned(x, 16) || !aligned(wg, 16) || !aligned(wu, 16))
+    return fail(FMX_ERR_INVALID, "x, wg and wu must be 16-byte aligned");
+  if (!aligned(dy, 2) || !aligned(factors, 2) || !aligned(dx, 2) || !aligned(dwg, 2) || !aligned(dwu, 2) ||
+      !aligned(dbg, 2) || !aligned(dbu, 2))
+    return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");
+  const bool bf = dtype == FMX_DTYPE_BF16;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipError_t e = hipSuccess;
+  if (M == 0) {  // no rows: zeros
+    for (void* w : {dwg, dwu})
+      if (w && e == hipSuccess) e = fmx::launch_linear_zero(w, N * K, s);
+    for (void* b : {dbg, dbu})
+      if (b && e == hipSuccess) e = fmx::launch_linear_zero(b, N, s);
+    return hip_status(e, "fmx_gated_bwd launch");
+  }
+  const GatedBwdWs ws = gated_bwd_ws(M, N, K);
+  if (!workspace || workspace_bytes < ws.total() || !aligned(workspace, 16))
+    return fail(FMX_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", ws.total(), workspace_bytes);
+  char* base = static_cast<char*>(workspace);
+  const int64_t np = gated_np(N);
+  const int parts = fmx::gated_dz_parts(M, N);
+  float* column_sums = reinterpret_cast<float*>(base + ws.dz);
+  fmx::GatedDzArgs z = {};
+  z.dy = dy;
+  z.keep = factors;
+  z.dz = dx || weights ? base : nullptr;
+  z.part = sums ? column_sums : nullptr;
+  z.sdy = dy_stride;
+  z.M = M;
+  z.N = N;
+  z.Np = np;
+  e = fmx::launch_gated_dz(bf, z, parts, s);
+  if (sums && e == hipSuccess) e = fmx::launch_join(dtype, column_sums, parts, N, N, dbg, dbu, s);
+  if (e != hipSuccess) return hip_status(e, "fmx_gated_bwd launch");
+  fmx::LinearArgs a = {};
+  a.sa = 2 * np;
+  a.part = reinterpret_cast<float*>(base + ws.dz + ws.sums);
+  if (dx) {
+    a.A = base;
+    a.B = wg;
+    a.sb = wg_stride;
+    a.B2 = wu;
+    a.sb2 = wu_stride;
+    a.half = (int)(np / 64);
+    a.kb = (int)N;
+    a.I = M;
+    a.J = K;
+    a.K = 2 * np;
+    a.y = dx;
+    e = fmx::launch_linear(bf, fmx::kLinearInput, a, fmx::linear_plan(fmx::kLinearInput, M, K, 2 * np), s);
+    if (e != hipSuccess) return hip_status(e, "fmx_gated_bwd launch");
+    a.B2 = nullptr;
+  }
+  const fmx::LinearPlan plan_w = fmx::linear_plan(fmx::kLinearWeight, N, K, M);
+  for (int up = 0; up < 2; ++up) {
+    void* dw = up ? dwu : dwg;
+    if (!dw) continue;
+    a.A = base + (up ? np * 2 : 0);
+    a.B = x;
+    a.sb = x_stride;
+    a.I = N;
+    a.J = K;
+    a.K = M;
+    a.y = dw;
+    e = fmx::launch_linear(bf, fmx::kLinearWeight, a, plan_w, s);
+    if (e != hipSuccess) return hip_status(e, "fmx_gated_bwd launch");
+  }
+  return hip_status(e, "fmx_gated_bwd launch");
 }
 
 int fmx_layer_norm(int dtype, const void* x, int64_t x_stride, int w_dtype, const void* weight, const void* bias,

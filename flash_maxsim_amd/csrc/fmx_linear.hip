@@ -21,80 +21,14 @@
 // its tiles are many, is split over k: float32 partial tiles go to the
 // workspace and a second kernel adds them in order (no atomics) and applies
 // the epilogue.
-#include <type_traits>
-
 #include "fmx_device.h"
 #include "fmx_layers.h"
+#include "fmx_product.h"
 
 #include "../../include/fmx.h"
 
 namespace fmx {
 namespace {
-
-typedef short s16x4_t __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ uint32_t pack2(float a, float b, bool bf) {
-  if (bf) {
-    const __bf16 x = (__bf16)a, y = (__bf16)b;
-    return (uint32_t)__builtin_bit_cast(uint16_t, x) | ((uint32_t)__builtin_bit_cast(uint16_t, y) << 16);
-  }
-  const _Float16 x = (_Float16)a, y = (_Float16)b;
-  return (uint32_t)__builtin_bit_cast(uint16_t, x) | ((uint32_t)__builtin_bit_cast(uint16_t, y) << 16);
-}
-__device__ __forceinline__ float unpack(uint32_t bits16, bool bf) {
-  return bf ? bf16_bits_to_float(bits16) : half_bits_to_float(bits16);
-}
-
-// ---- activations ----
-
-// Phi(z), the normal distribution function, and e = exp(-z^2 / 2): Abramowitz and
-// Stegun 7.1.26 (erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off
-// by 1.5e-7 at most) at x = |z| / sqrt 2; the lower tail has no cancellation.
-__device__ __forceinline__ float normal_cdf(float z, float& e) {
-  const float a = __builtin_fabsf(z);
-  e = __builtin_amdgcn_exp2f(z * z * -0.72134752044f);  // exp(-z^2 / 2)
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.2316418882f, a, 1.0f));  // p / sqrt 2
-  float q = fmaf(t, 0.5307027145f, -0.7265760135f);  // the halves of a5 .. a1
-  q = fmaf(t, q, 0.7107068705f);
-  q = fmaf(t, q, -0.142248368f);
-  q = fmaf(t, q, 0.1274147960f);
-  q = q * t * e;
-  return z < 0.0f ? q : 1.0f - q;
-}
-__device__ __forceinline__ float sigmoid(float z) {
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504089f));
-}
-
-// act(z), and with SLOPE act'(z). As a factor of a tail that is zero z is kept finite: their product would be NaN.
-template <bool SLOPE>
-__device__ __forceinline__ float act_value(float z, int act, float& slope) {
-  const float f = SLOPE ? __builtin_fminf(__builtin_fmaxf(z, -1e4f), 1e4f) : z;
-  switch (act) {
-    case FMX_ACT_RELU:
-      slope = z > 0.0f ? 1.0f : 0.0f;
-      return z > 0.0f ? z : z != z ? z : 0.0f;
-    case FMX_ACT_GELU: {
-      float e;
-      const float p = normal_cdf(z, e);
-      slope = fmaf(f * 0.3989422804f, e, p);
-      return z * p;
-    }
-    // z (1 + tanh u) / 2 = z sigmoid(2 u)
-    case FMX_ACT_GELU_TANH: {
-      const float s = sigmoid(1.5957691216f * z * fmaf(0.044715f, z * z, 1.0f));
-      slope = s + f * s * (1.0f - s) * 1.5957691216f * fmaf(0.134145f, f * f, 1.0f);
-      return z * s;
-    }
-    case FMX_ACT_SILU: {
-      const float s = sigmoid(z);
-      slope = s + f * s * (1.0f - s);
-      return z * s;
-    }
-    default:
-      slope = 1.0f;
-      return z;
-  }
-}
 
 // Slopes lie within -0.13 .. 1.13 and go from the forward to the backward in 16 bits, which get finer towards zero:
 // GELU's slope at -5 is -7e-6, and a unit whose arguments all lie there learns by it (steps of 2^-14 made it zero). The
@@ -133,79 +67,6 @@ __device__ __forceinline__ float slope_of(uint32_t bits16) {
   return u < 0x3f800000u ? __builtin_copysignf(v, root) : __builtin_nanf("");
 }
 
-// ---- epilogue: 8 consecutive outputs j .. j + 7 of row i, of which `left` exist ----
-
-__device__ __forceinline__ u32x4_t pack8(const float (&v)[8], bool bf) {
-  return u32x4_t{pack2(v[0], v[1], bf), pack2(v[2], v[3], bf), pack2(v[4], v[5], bf), pack2(v[6], v[7], bf)};
-}
-
-// Rows may begin at any element (odd widths): the 16-byte accesses need no more than 2-byte alignment here (gfx950
-// under the HSA runtime takes them as they come; 1003 x 77 with 2-byte ones: dz 10 us, the forward 7.6; so 6 and 6.1).
-__device__ __forceinline__ void store_raw(void* base, int64_t at, int left, const u32x4_t& w) {
-  uint16_t* p = static_cast<uint16_t*>(base) + at;
-  if (left >= 8) {
-    __builtin_memcpy(p, &w, 16);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t x = w[i / 2];
-      if (i < left) p[i] = (uint16_t)((i & 1) ? x >> 16 : x);
-    }
-  }
-}
-__device__ __forceinline__ void store16(void* base, int64_t at, int left, const float (&v)[8], bool bf) {
-  store_raw(base, at, left, pack8(v, bf));
-}
-
-__device__ __forceinline__ u32x4_t load_raw(const void* base, int64_t at, int left) {
-  const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-  u32x4_t v = {0u, 0u, 0u, 0u};
-  if (left >= 8) {
-    __builtin_memcpy(&v, p, 16);
-    return v;
-  }
-  uint32_t w[4] = {0u, 0u, 0u, 0u};
-  // the last one again in place of those past it (left >= 1): no branches, all loads in flight
-  uint32_t e[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = p[i < left ? i : left - 1];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i / 2] |= (i < left ? e[i] : 0u) << (16 * (i & 1));
-  return u32x4_t{w[0], w[1], w[2], w[3]};
-}
-__device__ __forceinline__ void unpack8(float (&v)[8], const u32x4_t& w, bool bf) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t x = w[i / 2];
-    v[i] = unpack((i & 1) ? x >> 16 : x & 0xffffu, bf);
-  }
-}
-__device__ __forceinline__ void load16(float (&v)[8], const void* base, int64_t at, int left, bool bf) {
-  unpack8(v, load_raw(base, at, left), bf);
-}
-
-// What follows the sums: a form's own activation (FMX_ACT_*: the forward's tile kernels are compiled for each, their
-// unrolled epilogues hold the code many times over), one named at run time, or nothing (dx, dw).
-constexpr int kAnyAct = -1, kNoEpilogue = -2;
-
-template <int ACT, bool SLOPE>
-__device__ __forceinline__ void activate(float (&v)[8], float (&slope)[8], int act) {
-  if constexpr (ACT >= 0) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = act_value<SLOPE>(v[k], ACT, slope[k]);
-  } else {
-    switch (act) {  // uniform: one test for the eight
-#define FMX_CASE(A) \
-  case A: activate<A, SLOPE>(v, slope, A); break
-      FMX_CASE(FMX_ACT_RELU);
-      FMX_CASE(FMX_ACT_GELU);
-      FMX_CASE(FMX_ACT_GELU_TANH);
-      FMX_CASE(FMX_ACT_SILU);
-#undef FMX_CASE
-      default: break;
-    }
-  }
-}
 template <bool BF>
 __device__ __forceinline__ u32x4_t slopes8(const float (&s)[8]) {
   return u32x4_t{slopes2<BF>(s[0], s[1]), slopes2<BF>(s[2], s[3]), slopes2<BF>(s[4], s[5]), slopes2<BF>(s[6], s[7])};
@@ -237,92 +98,9 @@ __device__ __forceinline__ void finish(const LinearArgs& a, int64_t i, int64_t j
 
 // ---- the product ----
 
-constexpr int BK = 64;  // k values of a stage: 128-byte rows of a K-major operand, whole lines of memory
-
-// One operand's side of a tile: T rows (of i or j), from row r0 on.
-template <bool MAJ, bool PAIR, int T, int NT>
-struct Side {
-  static constexpr int kChunks = T * BK / 8;            // 16-byte chunks of a stage
-  static constexpr int kLoads = kChunks / NT;           // of a thread
-  static constexpr int kRow = MAJ ? T / 8 : BK / 8;     // chunks of an LDS row
-  static_assert(kChunks % NT == 0 && (MAJ || NT % (8 * kRow) == 0), "a stage splits evenly over the threads");
-  const char* base;
-  int64_t step;        // bytes from one stage to the next
-  uint32_t off[kLoads];
-  int kfirst;          // the first chunk's (first) k inside its stage
-
-  // position of chunk ch of LDS row r is ch ^ key(r)
-  static __device__ __forceinline__ int key(int r) {
-    if constexpr (MAJ) return (2 * (r & 3) | (kRow > 8 ? ((r >> 3) & 1) << 3 : 0)) & (kRow - 1);
-    // PAIR: the rows of one fragment are 0-3, 8-11, 16-19, 24-27 (and 4 more)
-    return PAIR ? (r & 3) | ((r >> 3) & 1) << 2 : r & 7;
-  }
-
-  __device__ __forceinline__ Side(const void* p, int64_t stride, int64_t r0, int64_t rows, int64_t k0, int tid) {
-    base = static_cast<const char*>(p) + (MAJ ? k0 * stride + r0 : r0 * stride + k0) * 2;
-    step = (MAJ ? stride : 1) * (int64_t)BK * 2;
-#pragma unroll
-    for (int n = 0; n < kLoads; ++n) {
-      const int at = n * NT + tid, r = at / kRow, ch = (at % kRow) ^ key(r);
-      if (n == 0) kfirst = MAJ ? r : ch * 8;
-      const int row = MAJ ? ch * 8 : r;  // of i or j, inside the tile
-      off[n] = r0 + row < rows ? (uint32_t)(r * stride * 2 + ch * 16) : kOOB;
-    }
-  }
-  // Stage `it` to LDS; kleft: k values left from its start (those at or past it read as zeros).
-  // K-major: a thread's chunks lie 8 rows (or a multiple) apart, so they hold the same k.
-  __device__ __forceinline__ void issue(unsigned char* lds, int it, int kleft, int wave) const {
-    const rsrc_t r = make_rsrc(base + it * step, 0x7fffffffu);
-#pragma unroll
-    for (int n = 0; n < kLoads; ++n)
-      dma16_lds<false>(r, lds + (n * NT + wave * 64) * 16, kfirst + (MAJ ? n * (NT / kRow) : 0) < kleft ? off[n] : kOOB);
-  }
-};
-
-// Fragment reader of one operand: 16 rows x 32 k of fragment f, k-step kk.
-template <bool MAJ, bool PAIR, int T>
-struct Frags {
-  uint32_t at[MAJ ? 1 : BK / 32];
-  __device__ __forceinline__ Frags(int row0, int lane) {
-    const int c = lane & 15, g = lane >> 4;
-    if constexpr (MAJ) {
-      const int q = c >> 2, s = c & 3, r = 8 * g + q;
-      at[0] = (uint32_t)(r * T * 2 + (((row0 >> 3) + (s >> 1)) ^ Side<MAJ, PAIR, T, 64 * 8>::key(r)) * 16 + 8 * (s & 1));
-    } else {
-      const int row = row0 + (PAIR ? 8 * (c >> 2) + (c & 3) : c);
-      const int key = c & 7;  // of the row, and of all others of the lane's fragments
-#pragma unroll
-      for (int kk = 0; kk < BK / 32; ++kk) at[kk] = (uint32_t)(row * BK * 2 + ((kk * 4 + g) ^ key) * 16);
-    }
-  }
-  __device__ __forceinline__ u32x4_t read(const unsigned char* lds, int f, int kk) const {
-    if constexpr (MAJ) {
-      typedef __attribute__((address_space(3))) s16x4_t lds_t;
-      // chunk 2 f further: row0 is a multiple of 8 chunks and rows are powers of two apart, so it is an
-      // exclusive or of the address; k rows 32 kk + 8 g + 0..3, then + 4..7 (the key of row r + 4 is that of r)
-      const unsigned char* p = lds + (at[0] ^ (uint32_t)(32 * f));
-      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(p + (32 * kk) * T * 2));
-      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(p + (32 * kk + 4) * T * 2));
-      const u32x2_t l = __builtin_bit_cast(u32x2_t, lo), h = __builtin_bit_cast(u32x2_t, hi);
-      return u32x4_t{l[0], l[1], h[0], h[1]};
-    } else {
-      const int o = PAIR ? (f >> 1) * 32 + 4 * (f & 1) : f * 16;
-      return *reinterpret_cast<const u32x4_t*>(lds + at[kk] + o * BK * 2);
-    }
-  }
-};
-
-// LDS buffers are separate objects, named at compile time in the unrolled stage
-// loop: the compiler then knows that reads of one do not alias the DMA writes in
-// flight to another and puts no wait for those in front of them.
-__device__ __forceinline__ void stage_barrier() {
-  __asm__ volatile("" ::: "memory");
-  wait_lds();
-  __builtin_amdgcn_s_barrier();
-  __asm__ volatile("" ::: "memory");
-}
-
-template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int NS, int EPI>
+// PAIRED (dx of a gated layer): k runs over the rows of B and then over those of B2, which A's columns meet after
+// `half` stages.
+template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int NS, int EPI, bool PAIRED>
 __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
   constexpr int TI = WI * FI * 16, TJ = WJ * FJ * 16, NT = WI * WJ * 64;
   constexpr int BYTES = (TI + TJ) * BK * 2;
@@ -333,34 +111,21 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds1[BYTES];
   __shared__ __attribute__((aligned(1024))) unsigned char lds2[NS > 2 ? BYTES : 16];
   __shared__ __attribute__((aligned(1024))) unsigned char lds3[NS > 2 ? BYTES : 16];
-  static_assert(NS == 2 || NS == 4, "stage buffers");
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wi = wave % WI, wj = wave / WI;
 
-  // Workgroups go to the eight XCDs in turn; each XCD takes a run of consecutive tiles, which share
-  // operand rows in its L2. Runs of `band` tile rows are walked column by column.
-  // (32-bit divisions: a launch has fewer than 2^32 threads.)
-  const uint32_t tj = (uint32_t)a.tj, ti = (uint32_t)a.ti, tiles = ti * tj, bands = (uint32_t)a.band;
-  uint32_t id = blockIdx.x;
-  {
-    const uint32_t total = tiles * (uint32_t)a.splits, per = total / 8, x = id & 7, rest = total & 7;
-    id = (id >> 3) + x * per + (x < rest ? x : rest);
-  }
-  const uint32_t split = a.splits > 1 ? id / tiles : 0;
-  uint32_t t = id - split * tiles;
-  const uint32_t band = t / (bands * tj);
-  const uint32_t rows = ti - band * bands < bands ? ti - band * bands : bands;
-  t -= band * bands * tj;
-  const uint32_t tcol = t / rows;
-  const int64_t i0 = (int64_t)(band * bands + (t - tcol * rows)) * TI, j0 = (int64_t)tcol * TJ;
+  const Place at(blockIdx.x, (uint32_t)a.ti, (uint32_t)a.tj, (uint32_t)a.splits, (uint32_t)a.band);
+  const uint32_t split = at.split;
+  const int64_t i0 = (int64_t)at.row * TI, j0 = (int64_t)at.col * TJ;
   const int64_t k0 = (int64_t)split * a.split_k;
   const int64_t kn = a.K - k0 < a.split_k ? a.K - k0 : a.split_k;
   const int nit = (int)((kn + BK - 1) / BK);
 
   const SideA sa(a.A, a.sa, i0, a.I, k0, tid);
-  const SideB sb(a.B, a.sb, j0, a.Jr, k0, tid);
+  const SideB sb(a.B, a.sb, j0, a.Jr, PAIRED ? 0 : k0, tid);
+  const SideB sb2(PAIRED ? a.B2 : a.B, PAIRED ? a.sb2 : a.sb, j0, a.Jr, PAIRED ? 0 : k0, tid);
   const Frags<AMAJ, false, TI> fa(wi * FI * 16, lane);
   const Frags<BMAJ, !BMAJ, TJ> fb(wj * FJ * 16, lane);
 
@@ -380,13 +145,16 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
   auto issue = [&](unsigned char* lds, int it) __attribute__((always_inline)) {
     const int left = (int)kn - it * BK;
     sa.issue(lds, it, left, wave);
-    sb.issue(lds + TI * BK * 2, it, left, wave);
+    if constexpr (PAIRED) {
+      const int stage = (int)(k0 / BK) + it, own = stage < a.half ? stage : stage - a.half;
+      if (stage < a.half)
+        sb.issue(lds + TI * BK * 2, own, a.kb - own * BK, wave);
+      else
+        sb2.issue(lds + TI * BK * 2, own, a.kb - own * BK, wave);
+    } else {
+      sb.issue(lds + TI * BK * 2, it, left, wave);
+    }
   };
-  // Fragments of one k-step of 32: a set is multiplied while the next one is read. Before the first read of a new
-  // stage every wave waits for its own DMA of it and for its reads of the old one, then all meet; the
-  // old one's buffer takes the DMA of the stage NS ahead.
-  constexpr std::integral_constant<int, 0> set0{};
-  constexpr std::integral_constant<int, 1> set1{};
   u32x4_t va[2][FI], vb[2][FJ];
   auto read = [&](auto set, const unsigned char* lds, int kk) __attribute__((always_inline)) {
     constexpr int Z = decltype(set)::value;
@@ -401,22 +169,6 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
     for (int x = 0; x < FI; ++x)
 #pragma unroll
       for (int y = 0; y < FJ; ++y) acc[x][y] = mfma16x16x32<BF>(vb[Z][y], va[Z][x], acc[x][y]);
-  };
-  // The order of the instructions after a barrier: the multiplication of the set at hand runs from the
-  // first one on, between the loads and reads.
-  auto interleave = [&]() __attribute__((always_inline)) {
-    constexpr int READS = FJ * (BMAJ ? 2 : 1) + FI * (AMAJ ? 2 : 1), M = FI * FJ, R = READS > 12 ? 2 : 1;
-#pragma unroll
-    for (int n = 0; n < LOADS; ++n) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-    }
-#pragma unroll
-    for (int n = 0; n < READS / R; ++n) {
-      __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
   };
   // dw: the sums of A's columns (db), by a product with ones in the waves that hold the tile's first columns of C
   constexpr bool SUMS = AMAJ && BMAJ && FI <= 4;
@@ -434,39 +186,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
       }
     }
   };
-  auto stage = [&](auto s, int it) __attribute__((always_inline)) {
-    read(set1, buffer(s), 1);
-    multiply(set0);
-    add_up(set0);
-    wait_vmem<(NS - 2) * LOADS>();
-    stage_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    issue(buffer(s), it + NS);
-    read(set0, buffer(std::integral_constant<int, decltype(s)::value + 1>{}), 0);
-    multiply(set1);
-    interleave();
-    __builtin_amdgcn_sched_barrier(0);
-    add_up(set1);
-  };
-
-  issue(lds0, 0);
-  issue(lds1, 1);
-  if constexpr (NS > 2) {
-    issue(lds2, 2);
-    issue(lds3, 3);
-  }
-  wait_vmem<(NS - 1) * LOADS>();
-  stage_barrier();
-  read(set0, lds0, 0);
-  for (int it = 0; it < nit; it += NS) {
-    stage(std::integral_constant<int, 0>{}, it);
-    if (it + 1 < nit) stage(std::integral_constant<int, 1>{}, it + 1);
-    if constexpr (NS > 2) {
-      if (it + 2 < nit) stage(std::integral_constant<int, 2>{}, it + 2);
-      if (it + 3 < nit) stage(std::integral_constant<int, 3>{}, it + 3);
-    }
-  }
-  wait_vmem<0>();  // the stages past the end: their (empty) DMA writes no longer reach LDS after this wave ends
+  run_stages<NS, LOADS, FJ*(BMAJ ? 2 : 1) + FI*(AMAJ ? 2 : 1), FI * FJ>(nit, buffer, issue, read, multiply, add_up);
 
   if constexpr (SUMS) {
     if (sums && lane < 16) {  // every row of the product with ones is the sums
@@ -764,9 +484,9 @@ __global__ void __launch_bounds__(256) linear_zero_kernel(void* out, int64_t n) 
     store_raw(out, at, (int)(n - at < 8 ? n - at : 8), u32x4_t{0u, 0u, 0u, 0u});
 }
 
-template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int NS, int EPI>
+template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int NS, int EPI, bool PAIRED>
 void run(const LinearArgs& a, int64_t grid, hipStream_t s) {
-  linear_kernel<BF, AMAJ, BMAJ, WI, WJ, FI, FJ, NS, EPI><<<(unsigned)grid, WI * WJ * 64, 0, s>>>(a);
+  linear_kernel<BF, AMAJ, BMAJ, WI, WJ, FI, FJ, NS, EPI, PAIRED><<<(unsigned)grid, WI * WJ * 64, 0, s>>>(a);
 }
 
 template <bool BF>
@@ -781,13 +501,13 @@ hipError_t launch_few(const LinearArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <bool BF, bool AMAJ, bool BMAJ, int EPI>
+template <bool BF, bool AMAJ, bool BMAJ, int EPI, bool PAIRED = false>
 void run_tile(const LinearArgs& a, int tile, int64_t grid, hipStream_t s) {
   switch (tile) {
-    case kTile256: return run<BF, AMAJ, BMAJ, 2, 4, 8, 4, 2, EPI>(a, grid, s);
-    case kTile128: return run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 2, EPI>(a, grid, s);
-    case kTile128Deep: return run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 4, EPI>(a, grid, s);
-    default: return run<BF, AMAJ, BMAJ, 2, 2, 2, 2, 4, EPI>(a, grid, s);
+    case kTile256: return run<BF, AMAJ, BMAJ, 2, 4, 8, 4, 2, EPI, PAIRED>(a, grid, s);
+    case kTile128: return run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 2, EPI, PAIRED>(a, grid, s);
+    case kTile128Deep: return run<BF, AMAJ, BMAJ, 2, 2, 4, 4, 4, EPI, PAIRED>(a, grid, s);
+    default: return run<BF, AMAJ, BMAJ, 2, 2, 2, 2, 4, EPI, PAIRED>(a, grid, s);
   }
 }
 
@@ -796,7 +516,14 @@ hipError_t launch(const LinearArgs& a, int tile, hipStream_t s) {
   const int64_t grid = a.ti * a.tj * a.splits;
   constexpr int kJoin = FORWARD ? kAnyAct : kNoEpilogue;
   if constexpr (!FORWARD) {
-    run_tile<BF, AMAJ, BMAJ, kNoEpilogue>(a, tile, grid, s);
+    bool done = false;
+    if constexpr (!AMAJ && BMAJ) {
+      if (a.B2) {
+        run_tile<BF, AMAJ, BMAJ, kNoEpilogue, true>(a, tile, grid, s);
+        done = true;
+      }
+    }
+    if (!done) run_tile<BF, AMAJ, BMAJ, kNoEpilogue>(a, tile, grid, s);
   } else {
     switch (a.splits == 1 ? a.act : FMX_ACT_NONE) {  // parts of k: the second kernel has the epilogue
       case FMX_ACT_RELU: run_tile<BF, AMAJ, BMAJ, FMX_ACT_RELU>(a, tile, grid, s); break;

@@ -428,6 +428,42 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
 size_t fmx_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
 /*
+ * Gated linear layer: y = act(x Wg^T + bg) * (x Wu^T + bu) on MFMA with fp32 sums, rounded once.
+ *
+ *   x        [M, K]  dtype (F16 or BF16), row stride x_stride
+ *   wg, wu   [N, K]  dtype, row strides wg_stride and wu_stride
+ *   bg, bu   [N]     dtype, or NULL
+ *   y        [M, N]  dtype, contiguous
+ *   factors  the backward's factors (x Wu^T + bu) act'(..) and act(..), in codes of their own:
+ *            FMX_GATED_PLANES(dtype) planes of [M, N] int16, contiguous; or NULL
+ * x and the weights are 16-byte aligned, their strides multiples of 8, at least K
+ * rounded up to 8 and < 2^22; elements from K up to there are zeros.
+ * M <= FMX_LINEAR_MAX_ROWS, N < 2^20.
+ */
+#define FMX_GATED_PLANES(dtype) ((dtype) == FMX_DTYPE_BF16 ? 2 : 3)
+
+int fmx_gated(int dtype, const void* x, int64_t x_stride, const void* wg, int64_t wg_stride, const void* wu,
+              int64_t wu_stride, const void* bg, const void* bu, int act, int64_t M, int64_t N, int64_t K, void* y,
+              int16_t* factors, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t fmx_gated_workspace_bytes(int64_t M, int64_t N, int64_t K);
+
+/*
+ * Its backward: with g = x Wg^T + bg and u = x Wu^T + bu, dg = dy u act'(g) and du = dy act(g) (rounded to dtype,
+ * the products' operands),
+ *   dx = dg Wg + du Wu  [M, K],  dwg = dg^T x,  dwu = du^T x  [N, K],  dbg, dbu: sums over rows before rounding  [N]
+ * contiguous in dtype, each skipped when NULL. x and the weights as in the forward, x only read for dwg and dwu and
+ * the weights for dx (else they may be NULL); dy [M, N] with row stride dy_stride; factors as the forward wrote
+ * them. Deterministic.
+ */
+int fmx_gated_bwd(int dtype, const void* x, int64_t x_stride, const void* wg, int64_t wg_stride, const void* wu,
+                  int64_t wu_stride, const void* dy, int64_t dy_stride, const int16_t* factors, int64_t M, int64_t N,
+                  int64_t K, void* dx, void* dwg, void* dwu, void* dbg, void* dbu, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
+size_t fmx_gated_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K);
+
+/*
  * Layer norm of the rows of x: mu = mean x, s = 1 / sqrt(mean (x - mu)^2 + eps),
  * y = (x - mu) s weight + bias, sums in fp32.
  *

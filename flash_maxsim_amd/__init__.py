@@ -28,6 +28,7 @@ from .flash_maxsim_linear import linear
 from .flash_maxsim_gated import gated_linear
 from .flash_maxsim_norm import layer_norm
 from .flash_maxsim_optim import AdamW, AdamW8bitState, adamw_state, adamw_step, dequantize_adamw
+from .flash_maxsim_muon import Muon, muon_step, orthogonalize
 
 __all__ = [
     "flash_maxsim",
@@ -58,4 +59,7 @@ __all__ = [
     "adamw_state",
     "adamw_step",
     "dequantize_adamw",
+    "Muon",
+    "muon_step",
+    "orthogonalize",
 ]

@@ -130,6 +130,16 @@ _SIGNATURES = {
         [_int, _int, _int, _int, _ptr, _i64, _i64, _f64, _f64, _f64, _f64, _f64, _ptr, _ptr],
     ),
     "fmx_adamw_decode": (_int, [_int, _ptr, _ptr, _i64, _ptr, _ptr]),
+    "fmx_muon": (
+        _int,
+        [_int, _int, _int, _ptr, _i64, _f64, _f64, _int, _f64, _int, _f64, _f64, _f64, _f64, _int, _ptr, _ptr, _size,
+         _ptr],
+    ),
+    "fmx_orthogonalize": (
+        _int,
+        [_int, _int, _ptr, _i64, _int, _f64, _f64, _f64, _f64, _ptr, _size, _ptr],
+    ),
+    "fmx_muon_workspace_bytes": (_size, [_ptr, _i64]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -162,4 +162,26 @@ struct GatedDzArgs {
 int gated_dz_parts(int64_t M, int64_t N);
 hipError_t launch_gated_dz(bool bf16, GatedDzArgs a, int parts, hipStream_t s);
 
+// ---- orthogonalised updates (fmx_muon.hip) ----
+
+struct MuonMatrix {
+  void* param;       // moved in place, or the orthogonalised result
+  const void* grad;
+  float* momentum;   // or null: the gradient itself is orthogonalised
+  void* copy;        // 16-bit copy of the new parameters, or null
+  int64_t rows, cols;
+};
+
+struct MuonScalars {
+  double lr;
+  float mu, omu, eps, keep;  // omu: 1 - mu; keep: 1 - lr * weight decay
+  float a, b, c;
+  int steps, nesterov, by_rms, apply;
+  const float* grad_scale;   // one value, or null
+};
+
+size_t muon_workspace_bytes(const MuonMatrix* x, int64_t count);
+hipError_t launch_muon(int pkind, int gkind, int ckind, const MuonMatrix* x, int64_t count, const MuonScalars& sc, void* ws,
+                       hipStream_t s);
+
 }  // namespace fmx

@@ -102,6 +102,51 @@ GatedBwdWs gated_bwd_ws(int64_t M, int64_t N, int64_t K) {
   return w;
 }
 
+static_assert(sizeof(fmx_muon_matrix) == sizeof(fmx::MuonMatrix), "the same fields in the same order");
+
+bool muon_sides(const fmx_muon_matrix& x) {
+  const int64_t n = x.rows < x.cols ? x.rows : x.cols, m = x.rows < x.cols ? x.cols : x.rows;
+  return n >= 0 && n <= FMX_MUON_MAX_SHORT && m <= FMX_MUON_MAX_LONG;
+}
+
+int check_muon(int dtype, int grad_dtype, const fmx_muon_matrix* matrices, int64_t count, int steps, double a, double b,
+               double c, double eps, bool step, bool* copies) {
+  if (count < 0) return fail(FMX_ERR_INVALID, "invalid count=%lld", (long long)count);
+  if (steps < 1 || steps > 100) return fail(FMX_ERR_INVALID, "steps=%d must be in 1 .. 100", steps);
+  if (!(eps > 0) || !isfinite(eps) || !isfinite(a) || !isfinite(b) || !isfinite(c))
+    return fail(FMX_ERR_INVALID, "eps must be > 0 and finite, the coefficients finite");
+  if (count > 0 && !matrices) return fail(FMX_ERR_INVALID, "matrices must be non-null");
+  for (int64_t i = 0; i < count; ++i) {
+    const fmx_muon_matrix& x = matrices[i];
+    if (x.rows < 0 || x.cols < 0)
+      return fail(FMX_ERR_INVALID, "matrix %lld has %lld x %lld elements", (long long)i, (long long)x.rows, (long long)x.cols);
+    if (!muon_sides(x))
+      return fail(FMX_ERR_UNSUPPORTED, "matrix %lld of %lld x %lld: sides of up to %d and %d", (long long)i,
+                  (long long)x.rows, (long long)x.cols, FMX_MUON_MAX_SHORT, FMX_MUON_MAX_LONG);
+    if (x.rows == 0 || x.cols == 0) continue;
+    if (!x.param || !x.grad || (step && !x.momentum)) return fail(FMX_ERR_INVALID, "matrix %lld: null pointer", (long long)i);
+    if (!aligned(x.param, size_of(dtype)) || !aligned(x.grad, size_of(grad_dtype)) || !aligned(x.momentum, 4) ||
+        !aligned(x.copy, 2))
+      return fail(FMX_ERR_INVALID, "matrix %lld: pointers must be aligned to their elements", (long long)i);
+    *copies |= x.copy != nullptr;
+  }
+  return FMX_OK;
+}
+
+int run_muon(int pd, int gd, int cd, const fmx_muon_matrix* matrices, int64_t count, fmx::MuonScalars sc, int steps, double a,
+             double b, double c, double eps, void* workspace, size_t bytes, void* stream, const char* what) {
+  sc.steps = steps;
+  sc.a = (float)a;
+  sc.b = (float)b;
+  sc.c = (float)c;
+  sc.eps = (float)eps;
+  const fmx::MuonMatrix* list = reinterpret_cast<const fmx::MuonMatrix*>(matrices);
+  const size_t need = fmx::muon_workspace_bytes(list, count);
+  if (need > 0 && (!workspace || bytes < need || !aligned(workspace, 256)))
+    return fail(FMX_ERR_WORKSPACE, "workspace of %zu bytes required, 256-byte aligned, %zu given", need, bytes);
+  return hip_status(fmx::launch_muon(pd, gd, cd, list, count, sc, workspace, static_cast<hipStream_t>(stream)), what);
+}
+
 }  // namespace
 
 extern "C" {
@@ -492,6 +537,53 @@ int fmx_adamw_decode(int second, const void* codes, const float* scales, int64_t
   if (!aligned(scales, 4) || !aligned(out, 4)) return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");
   return hip_status(fmx::launch_adamw_decode(codes, second != 0, scales, n, out, static_cast<hipStream_t>(stream)),
                     "fmx_adamw_decode launch");
+}
+
+size_t fmx_muon_workspace_bytes(const fmx_muon_matrix* matrices, int64_t count) {
+  if (!matrices || count < 1) return 0;
+  for (int64_t i = 0; i < count; ++i)
+    if (!muon_sides(matrices[i])) return 0;
+  return fmx::muon_workspace_bytes(reinterpret_cast<const fmx::MuonMatrix*>(matrices), count);
+}
+
+int fmx_muon(int param_dtype, int grad_dtype, int copy_dtype, const fmx_muon_matrix* matrices, int64_t count, double lr,
+             double momentum, int nesterov, double weight_decay, int steps, double a, double b, double c, double eps,
+             int match_rms, const float* grad_scale, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!known(param_dtype) || !known(grad_dtype))
+    return fail(FMX_ERR_INVALID, "unknown dtype %d or %d", param_dtype, grad_dtype);
+  if (!(lr >= 0) || !(weight_decay >= 0) || !(momentum >= 0 && momentum < 1))
+    return fail(FMX_ERR_INVALID, "lr and weight_decay must be >= 0, momentum in [0, 1)");
+  bool copies = false;
+  const int rc = check_muon(param_dtype, grad_dtype, matrices, count, steps, a, b, c, eps, true, &copies);
+  if (rc) return rc;
+  if (copies && (param_dtype != FMX_DTYPE_F32 || (copy_dtype != FMX_DTYPE_F16 && copy_dtype != FMX_DTYPE_BF16)))
+    return fail(FMX_ERR_INVALID, "copies are fp16 or bf16, of fp32 parameters");
+  if (!copies) copy_dtype = grad_dtype != FMX_DTYPE_F32 ? grad_dtype : FMX_DTYPE_BF16;
+  if (grad_dtype != FMX_DTYPE_F32 && grad_dtype != param_dtype &&
+      !(param_dtype == FMX_DTYPE_F32 && grad_dtype == copy_dtype))
+    return fail(FMX_ERR_INVALID, "gradients must be fp32 or of the parameters' (or their copies') dtype");
+  fmx::MuonScalars sc = {};
+  sc.lr = lr;
+  sc.mu = (float)momentum;
+  sc.omu = (float)(1.0 - momentum);
+  sc.keep = (float)(1.0 - lr * weight_decay);
+  sc.nesterov = nesterov != 0;
+  sc.by_rms = match_rms != 0;
+  sc.apply = 1;
+  sc.grad_scale = grad_scale;
+  return run_muon(param_dtype, grad_dtype, copy_dtype, matrices, count, sc, steps, a, b, c, eps, workspace, workspace_bytes,
+                  stream, "fmx_muon launch");
+}
+
+int fmx_orthogonalize(int out_dtype, int dtype, const fmx_muon_matrix* matrices, int64_t count, int steps, double a, double b,
+                      double c, double eps, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!known(out_dtype) || !known(dtype)) return fail(FMX_ERR_INVALID, "unknown dtype %d or %d", out_dtype, dtype);
+  bool copies = false;
+  const int rc = check_muon(out_dtype, dtype, matrices, count, steps, a, b, c, eps, false, &copies);
+  if (rc) return rc;
+  fmx::MuonScalars sc = {};
+  return run_muon(out_dtype, dtype, FMX_DTYPE_BF16, matrices, count, sc, steps, a, b, c, eps, workspace, workspace_bytes,
+                  stream, "fmx_orthogonalize launch");
 }
 
 }  // extern "C"

@@ -527,6 +527,42 @@ int fmx_adamw(int param_dtype, int grad_dtype, int copy_dtype, int state_bits, c
 /* fp32 moments of n 8-bit codes: int8 (second = 0: c |c| scale) or uint8 (second = 1: the square of c^2 scale). */
 int fmx_adamw_decode(int second, const void* codes, const float* scales, int64_t n, float* out, void* stream);
 
+/*
+ * One matrix of an orthogonalised step (as the Muon optimiser makes it): rows x cols elements, all arrays contiguous
+ * and aligned to their elements.
+ */
+typedef struct fmx_muon_matrix {
+  void* param;       /* param_dtype, updated in place */
+  const void* grad;  /* grad_dtype */
+  float* momentum;   /* updated in place */
+  void* copy;        /* copy_dtype: the new parameters rounded; or NULL */
+  int64_t rows, cols;
+} fmx_muon_matrix;
+
+/* the most of a matrix's shorter and of its longer side */
+#define FMX_MUON_MAX_SHORT (1 << 14)
+#define FMX_MUON_MAX_LONG (1 << 20)
+
+/*
+ * An orthogonalised step over `count` matrices (a host array, read before the call returns):
+ *   g = grad * *grad_scale (a device scalar; NULL: 1),  m = momentum m + (1 - momentum) g
+ *   u = (1 - momentum) g + momentum m with nesterov, else m;  X = u / max(|u|, eps), |u| the root of its squares' sum
+ *   `steps` times, X's shorter side first:  X = a X + (b X X^T + c (X X^T)^2) X
+ *   p = p (1 - lr weight_decay) - lr f X,  f = sqrt(max(1, rows / cols)), with match_rms 0.2 sqrt(max(rows, cols))
+ * Products on fp16 MFMA with fp32 sums, X held as a pair of fp16 values (the result is within about 2e-3 of the
+ * formula's, by the root of the squares), everything else in fp32 (|u| in 64 bits); p is rounded once. Types as
+ * fmx_adamw's. Deterministic. Workspace: fmx_muon_workspace_bytes, 256-byte aligned.
+ */
+int fmx_muon(int param_dtype, int grad_dtype, int copy_dtype, const fmx_muon_matrix* matrices, int64_t count, double lr,
+             double momentum, int nesterov, double weight_decay, int steps, double a, double b, double c, double eps,
+             int match_rms, const float* grad_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* X of that iteration alone: `param` (out_dtype) receives it for u = `grad` (dtype); the other pointers are unused. */
+int fmx_orthogonalize(int out_dtype, int dtype, const fmx_muon_matrix* matrices, int64_t count, int steps, double a, double b,
+                      double c, double eps, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t fmx_muon_workspace_bytes(const fmx_muon_matrix* matrices, int64_t count);
+
 #ifdef __cplusplus
 }
 #endif

@@ -27,6 +27,7 @@ from .flash_maxsim_topk import flash_maxsim_batched_topk, flash_maxsim_int8_topk
 from .flash_maxsim_linear import linear
 from .flash_maxsim_gated import gated_linear
 from .flash_maxsim_norm import layer_norm
+from .flash_maxsim_residual_norm import residual_norm
 from .flash_maxsim_optim import AdamW, AdamW8bitState, adamw_state, adamw_step, dequantize_adamw
 from .flash_maxsim_muon import Muon, muon_step, orthogonalize
 
@@ -54,6 +55,7 @@ __all__ = [
     "linear",
     "gated_linear",
     "layer_norm",
+    "residual_norm",
     "AdamW",
     "AdamW8bitState",
     "adamw_state",

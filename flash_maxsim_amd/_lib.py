@@ -130,6 +130,17 @@ _SIGNATURES = {
         [_int, _int, _int, _int, _ptr, _i64, _i64, _f64, _f64, _f64, _f64, _f64, _ptr, _ptr],
     ),
     "fmx_adamw_decode": (_int, [_int, _ptr, _ptr, _i64, _ptr, _ptr]),
+    "fmx_residual_norm": (
+        _int,
+        [_int, _ptr, _i64, _ptr, _i64, _ptr, _i64, _int, _ptr, _ptr, _int, _ptr, _ptr, _ptr, _f64, _int, _f64, _i64,
+         _i64, _ptr, _ptr, _ptr, _ptr],
+    ),
+    "fmx_residual_norm_bwd": (
+        _int,
+        [_int, _ptr, _i64, _ptr, _i64, _ptr, _i64, _int, _ptr, _int, _ptr, _ptr, _ptr, _f64, _int, _ptr, _ptr, _i64,
+         _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _size, _ptr],
+    ),
+    "fmx_residual_norm_bwd_workspace_bytes": (_size, [_i64, _i64]),
     "fmx_muon": (
         _int,
         [_int, _int, _int, _ptr, _i64, _f64, _f64, _int, _f64, _int, _f64, _f64, _f64, _f64, _int, _ptr, _ptr, _size,

@@ -184,4 +184,28 @@ size_t muon_workspace_bytes(const MuonMatrix* x, int64_t count);
 hipError_t launch_muon(int pkind, int gkind, int ckind, const MuonMatrix* x, int64_t count, const MuonScalars& sc, void* ws,
                        hipStream_t s);
 
+// ---- residual norm (fmx_residual_norm.hip) ----
+
+struct ResidualNormArgs {
+  const void *x, *r, *gate;      // [M, d] each with a row stride of its own; the gate may be null
+  const void *w, *b, *pw, *pb, *scale;  // [d] or null
+  void *h, *y;                   // forward: [M, d] contiguous
+  float* stats;                  // [M][4]: both norms' mean and inverse deviation; forward: may be null
+  const void *dh, *dy;           // backward: [M, d] with row strides, or null
+  void *dx, *dr, *dgate;         // [M, d] contiguous, or null
+  float* part;                   // [parts][wanted][d], or null
+  void* sums[5];                 // dw, db, dscale, dpw, dpb: [d] each, or null
+  int64_t sx, sr, sg, sdh, sdy;
+  int64_t M;
+  int d;
+  int wanted;                    // of the sums
+  int w32;                       // the vectors are float32, else of x's type
+  int rms, post;
+  float alpha, eps;
+};
+
+int residual_norm_parts(int64_t M, int d);  // rows of ResidualNormArgs::part at most
+hipError_t launch_residual_norm_fwd(int kind, const ResidualNormArgs& a, hipStream_t s);
+hipError_t launch_residual_norm_bwd(int kind, const ResidualNormArgs& a, hipStream_t s);
+
 }  // namespace fmx

@@ -102,6 +102,19 @@ GatedBwdWs gated_bwd_ws(int64_t M, int64_t N, int64_t K) {
   return w;
 }
 
+int check_residual_norm(int dtype, int w_dtype, int64_t x_stride, int64_t r_stride, int64_t g_stride, double alpha, int64_t M,
+                        int64_t d) {
+  if (!known(dtype)) return fail(FMX_ERR_INVALID, "unknown dtype %d", dtype);
+  if (w_dtype != dtype && w_dtype != FMX_DTYPE_F32)
+    return fail(FMX_ERR_INVALID, "weights must be of the rows' dtype or fp32, got dtype %d", w_dtype);
+  if (M < 0 || d < 1 || x_stride < 0 || r_stride < 0 || g_stride < 0)
+    return fail(FMX_ERR_INVALID, "invalid sizes M=%lld d=%lld or strides", (long long)M, (long long)d);
+  if (d > FMX_RESIDUAL_NORM_MAX_D)
+    return fail(FMX_ERR_UNSUPPORTED, "d=%lld exceeds FMX_RESIDUAL_NORM_MAX_D=%d", (long long)d, FMX_RESIDUAL_NORM_MAX_D);
+  if (!isfinite(alpha)) return fail(FMX_ERR_INVALID, "alpha must be finite");
+  return FMX_OK;
+}
+
 static_assert(sizeof(fmx_muon_matrix) == sizeof(fmx::MuonMatrix), "the same fields in the same order");
 
 bool muon_sides(const fmx_muon_matrix& x) {
@@ -537,6 +550,114 @@ int fmx_adamw_decode(int second, const void* codes, const float* scales, int64_t
   if (!aligned(scales, 4) || !aligned(out, 4)) return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");
   return hip_status(fmx::launch_adamw_decode(codes, second != 0, scales, n, out, static_cast<hipStream_t>(stream)),
                     "fmx_adamw_decode launch");
+}
+
+int fmx_residual_norm(int dtype, const void* x, int64_t x_stride, const void* residual, int64_t r_stride, const void* gate,
+                      int64_t g_stride, int w_dtype, const void* weight, const void* bias, int post, const void* post_weight,
+                      const void* post_bias, const void* scale, double alpha, int rms, double eps, int64_t M, int64_t d,
+                      void* h, void* y, float* stats, void* stream) {
+  const int rc = check_residual_norm(dtype, w_dtype, x_stride, r_stride, gate ? g_stride : 0, alpha, M, d);
+  if (rc) return rc;
+  if (!(eps >= 0)) return fail(FMX_ERR_INVALID, "eps must be >= 0");
+  if (!post && (post_weight || post_bias)) return fail(FMX_ERR_INVALID, "weights of a norm of x that is not wanted");
+  if (M == 0) return ok();
+  if (!x || !residual || !h || !y) return fail(FMX_ERR_INVALID, "x, residual, h and y must be non-null");
+  const int es = size_of(dtype), ws = size_of(w_dtype);
+  if (!aligned(x, es) || !aligned(residual, es) || !aligned(gate, es) || !aligned(h, es) || !aligned(y, es) ||
+      !aligned(weight, ws) || !aligned(bias, ws) || !aligned(post_weight, ws) || !aligned(post_bias, ws) ||
+      !aligned(scale, ws))
+    return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");
+  if (!aligned(stats, 16)) return fail(FMX_ERR_INVALID, "stats must be 16-byte aligned");
+  fmx::ResidualNormArgs a = {};
+  a.x = x;
+  a.r = residual;
+  a.gate = gate;
+  a.w = weight;
+  a.b = bias;
+  a.pw = post_weight;
+  a.pb = post_bias;
+  a.scale = scale;
+  a.h = h;
+  a.y = y;
+  a.stats = stats;
+  a.sx = x_stride;
+  a.sr = r_stride;
+  a.sg = g_stride;
+  a.M = M;
+  a.d = (int)d;
+  a.w32 = w_dtype == FMX_DTYPE_F32;
+  a.rms = rms != 0;
+  a.post = post != 0;
+  a.alpha = (float)alpha;
+  a.eps = (float)eps;
+  return hip_status(fmx::launch_residual_norm_fwd(dtype, a, static_cast<hipStream_t>(stream)), "fmx_residual_norm launch");
+}
+
+size_t fmx_residual_norm_bwd_workspace_bytes(int64_t M, int64_t d) {
+  if (M < 1 || d < 1 || d > FMX_RESIDUAL_NORM_MAX_D) return 0;
+  return (size_t)fmx::residual_norm_parts(M, (int)d) * 5 * (size_t)d * sizeof(float);
+}
+
+int fmx_residual_norm_bwd(int dtype, const void* x, int64_t x_stride, const void* residual, int64_t r_stride,
+                          const void* gate, int64_t g_stride, int w_dtype, const void* weight, int post,
+                          const void* post_weight, const void* post_bias, const void* scale, double alpha, int rms,
+                          const float* stats, const void* dh, int64_t dh_stride, const void* dy, int64_t dy_stride, int64_t M,
+                          int64_t d, void* dx, void* dr, void* dgate, void* dw, void* db, void* dscale, void* dpw, void* dpb,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_residual_norm(dtype, w_dtype, x_stride, r_stride, gate ? g_stride : 0, alpha, M, d);
+  if (rc) return rc;
+  if ((dh && dh_stride < 0) || (dy && dy_stride < 0)) return fail(FMX_ERR_INVALID, "strides must be >= 0");
+  if (!post && (dpw || dpb)) return fail(FMX_ERR_INVALID, "gradients of a norm of x that is not there");
+  if (dgate && !gate) return fail(FMX_ERR_INVALID, "a gradient of a gate that is not there");
+  const bool any = dx || dr || dgate || dw || db || dscale || dpw || dpb;
+  if (!any) return ok();
+  if (M > 0 && (!x || !residual || !stats || (!dh && !dy)))
+    return fail(FMX_ERR_INVALID, "x, residual, stats and one of dh and dy must be non-null");
+  if ((dw || db) && M > 0 && !dy) return fail(FMX_ERR_INVALID, "dw and db come of dy");
+  const int es = size_of(dtype), ws = size_of(w_dtype);
+  for (const void* p : {x, residual, gate, dh, dy, (const void*)dx, (const void*)dr, (const void*)dgate})
+    if (!aligned(p, es)) return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");
+  for (const void* p : {weight, post_weight, post_bias, scale, (const void*)dw, (const void*)db, (const void*)dscale,
+                        (const void*)dpw, (const void*)dpb})
+    if (!aligned(p, ws)) return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");
+  if (!aligned(stats, 16)) return fail(FMX_ERR_INVALID, "stats must be 16-byte aligned");
+  fmx::ResidualNormArgs a = {};
+  a.sums[0] = dw;
+  a.sums[1] = db;
+  a.sums[2] = dscale;
+  a.sums[3] = dpw;
+  a.sums[4] = dpb;
+  for (void* s : a.sums) a.wanted += s != nullptr;
+  const size_t need = a.wanted ? fmx_residual_norm_bwd_workspace_bytes(M, d) : 0;
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 4)))
+    return fail(FMX_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace_bytes);
+  a.x = x;
+  a.r = residual;
+  a.gate = gate;
+  a.w = weight;
+  a.pw = post_weight;
+  a.pb = post_bias;
+  a.scale = scale;
+  a.stats = const_cast<float*>(stats);
+  a.dh = dh;
+  a.dy = dy;
+  a.dx = dx;
+  a.dr = dr;
+  a.dgate = dgate;
+  a.part = a.wanted ? static_cast<float*>(workspace) : nullptr;
+  a.sx = x_stride;
+  a.sr = r_stride;
+  a.sg = g_stride;
+  a.sdh = dh_stride;
+  a.sdy = dy_stride;
+  a.M = M;
+  a.d = (int)d;
+  a.w32 = w_dtype == FMX_DTYPE_F32;
+  a.rms = rms != 0;
+  a.post = post != 0;
+  a.alpha = (float)alpha;
+  return hip_status(fmx::launch_residual_norm_bwd(dtype, a, static_cast<hipStream_t>(stream)),
+                    "fmx_residual_norm_bwd launch");
 }
 
 size_t fmx_muon_workspace_bytes(const fmx_muon_matrix* matrices, int64_t count) {

@@ -1,0 +1,537 @@
+// The step from one block of an encoder to the next over rows of d elements: the block's output, normalised, gated and
+// scaled, is added to the hidden states, and their norm is what the next block reads. Forward and backward.
+//
+//   norm(v) = (v - mu) s,  s = 1 / sqrt(mean (v - mu)^2 + eps),  mu = mean v (layer) or 0 (rms)
+//   t = norm(x) pw + pb   (or x),   h = alpha r + scale gate t,   y = norm(h) w + b
+// and with g = dh + s2 (wdy - mean(wdy) - hh mean(wdy hh)), wdy = w dy, hh = norm(h) (rms: without the first mean):
+//   dr = alpha g,  dgate = g scale t,  q = g scale gate,  dx = s1 (q pw - mean(q pw) - xh mean(q pw xh)) (or q)
+//   dw = sum dy hh,  db = sum dy,  dscale = sum g gate t,  dpw = sum q xh,  dpb = sum q   over the rows
+//
+// Bound by HBM: the forward reads x, r (and the gate) and writes h and y, once each; the backward reads x, r, the gate,
+// dh and dy and writes dx, dr and dgate. y is the norm of h before its rounding, and the backward makes h anew from x
+// and r rather than read the rounded one: the same bytes, and no gradient sees that rounding. Both norms' mu and s are
+// kept, 16 bytes a row.
+//
+// A row lives in the registers of one to eight waves between its sums and its outputs, 8 elements a lane in the backward
+// (its five column sums, four vectors of weights and two rows of five arrays spill at 16, which only rows of more than
+// 4096 elements take) and up to 16 in the forward; a workgroup's eight waves walk the rows in strides of the launch, the next row loaded while
+// this one is summed. Variances are those of centred values, from registers. Rows may begin at any element: accesses of
+// 16 bytes need no more than an element's alignment here, and the last piece of an odd row is taken element by element.
+//
+// Weight gradients: a workgroup adds its waves' sums in LDS in the waves' order and writes one row of partial sums; a
+// second kernel adds those rows in a fixed order. No atomics.
+#include "fmx_device.h"
+#include "fmx_layers.h"
+
+#include "../../include/fmx.h"
+
+namespace fmx {
+namespace {
+
+constexpr int kWaves = 8;  // of a workgroup
+constexpr int kThreads = kWaves * 64;
+
+// Sums of a and of b over the NW waves that share a row, in every lane.
+template <int NW>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int wave) {
+  a = wave_sum(a);
+  b = wave_sum(b);
+  if constexpr (NW > 1) {
+    if ((threadIdx.x & 63) == 0) {
+      red[2 * wave] = a;
+      red[2 * wave + 1] = b;
+    }
+    __syncthreads();
+    const float* mine = red + 2 * (wave & -NW);
+    a = 0.0f;
+    b = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      a += mine[2 * i];
+      b += mine[2 * i + 1];
+    }
+  }
+}
+
+// V consecutive elements of type T as they lie in memory.
+template <typename T, int V>
+struct Piece {
+  T v[V];
+  // `left` of them are there, the others are zeros
+  template <bool WHOLE>
+  __device__ __forceinline__ void load(const T* p, int left) {
+    if (WHOLE ? left > 0 : left >= V) {
+      __builtin_memcpy(v, p, sizeof(v));
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = T(0.0f);
+      if constexpr (!WHOLE) {
+#pragma unroll
+        for (int i = 0; i < V - 1; ++i)
+          if (i < left) v[i] = p[i];
+      }
+    }
+  }
+  template <bool WHOLE>
+  __device__ __forceinline__ void store(T* p, int left) const {
+    if (WHOLE ? left > 0 : left >= V) {
+      __builtin_memcpy(p, v, sizeof(v));
+    } else if constexpr (!WHOLE) {
+#pragma unroll
+      for (int i = 0; i < V - 1; ++i)
+        if (i < left) p[i] = v[i];
+    }
+  }
+};
+
+// Where a lane's elements lie: piece j of V elements at column ((j * NW + sub) * 64 + lane) * V, sub the wave's place
+// among the NW of its row. WHOLE: d is a multiple of V, no piece ends early.
+template <typename T, int NV, int NW, bool WHOLE>
+struct Cols {
+  static constexpr int V = 16 / sizeof(T);
+  using Row = Piece<T, V>[NV];
+  int col[NV], left[NV];
+  __device__ __forceinline__ Cols(int wave, int lane, int d) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      col[j] = ((j * NW + wave % NW) * 64 + lane) * V;
+      left[j] = d - col[j];
+    }
+  }
+  __device__ __forceinline__ bool in(int j, int i) const { return WHOLE ? left[j] > 0 : i < left[j]; }
+  // a row's elements; zeros past it, and everywhere without a row
+  __device__ __forceinline__ void load(Row& x, const void* base, int64_t at, bool have) const {
+    const T* row = static_cast<const T*>(base) + at;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) x[j].template load<WHOLE>(row + col[j], have ? left[j] : 0);
+  }
+  __device__ __forceinline__ void store(void* base, int64_t at, const float (&v)[NV][V]) const {
+    T* row = static_cast<T*>(base) + at;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      Piece<T, V> o;
+#pragma unroll
+      for (int i = 0; i < V; ++i) o.v[i] = (T)v[j][i];
+      o.template store<WHOLE>(row + col[j], left[j]);
+    }
+  }
+  // a vector of weights as float32, `other` where there is none or past the row
+  template <typename W>
+  __device__ __forceinline__ void weights_of(float (&o)[NV][V], const W* w, float other) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      Piece<W, V> p;
+      p.template load<WHOLE>(w + col[j], left[j]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[j][i] = in(j, i) ? (float)p.v[i] : other;
+    }
+  }
+  __device__ __forceinline__ void weights(float (&o)[NV][V], const void* w, int w32, float other) const {
+    if (!w) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[j][i] = other;
+    } else if (w32) {
+      weights_of(o, static_cast<const float*>(w), other);
+    } else {
+      weights_of(o, static_cast<const T*>(w), other);
+    }
+  }
+};
+
+template <typename T, int NV, int NW, bool POST, bool WHOLE>
+__global__ void __launch_bounds__(kThreads) residual_norm_fwd_kernel(ResidualNormArgs a) {
+  using C = Cols<T, NV, NW, WHOLE>;
+  constexpr int V = C::V, NG = kWaves / NW;  // rows of a workgroup at a time
+  __shared__ float red[2][2 * kWaves];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const C c(wave, lane, a.d);
+  const float inv = 1.0f / (float)a.d;
+  const int64_t step = (int64_t)gridDim.x * NG;
+  typename C::Row x, r, g, nx, nr, ng;
+  int64_t row = (int64_t)blockIdx.x * NG + wave / NW;
+  c.load(x, a.x, row * a.sx, row < a.M);
+  c.load(r, a.r, row * a.sr, row < a.M);
+  if (a.gate) c.load(g, a.gate, row * a.sg, row < a.M);
+  float w[NV][V], b[NV][V], pw[NV][V], pb[NV][V], k[NV][V];
+  c.weights(w, a.w, a.w32, 1.0f);
+  c.weights(b, a.b, a.w32, 0.0f);
+  c.weights(k, a.scale, a.w32, 1.0f);
+  if constexpr (POST) {
+    c.weights(pw, a.pw, a.w32, 1.0f);
+    c.weights(pb, a.pb, a.w32, 0.0f);
+  }
+  int par = 0;
+  auto sum = [&](float s) {
+    float none = 0.0f;
+    row_sum2<NW>(s, none, red[par], wave);
+    par ^= 1;
+    return s;
+  };
+  float h[NV][V];
+  // mu and s of the values in h
+  auto moments = [&](float& mu, float& rs) {
+    mu = 0.0f;
+    if (!a.rms) {
+      float s = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s += h[j][i];
+      mu = sum(s) * inv;
+    }
+    float sq = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float e = h[j][i] - mu;
+        sq += c.in(j, i) ? e * e : 0.0f;
+      }
+    rs = 1.0f / sqrtf(sum(sq) * inv + a.eps);
+  };
+  // base, and so the number of barriers, is the same for all rows of the workgroup
+  for (int64_t base = (int64_t)blockIdx.x * NG; base < a.M; base += step, row += step) {
+    const bool more = row + step < a.M;
+    c.load(nx, a.x, (row + step) * a.sx, more);
+    c.load(nr, a.r, (row + step) * a.sr, more);
+    if (a.gate) c.load(ng, a.gate, (row + step) * a.sg, more);
+    float mu1 = 0.0f, rs1 = 1.0f, mu2, rs2;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) h[j][i] = (float)x[j].v[i];
+    if constexpr (POST) {
+      moments(mu1, rs1);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[j][i] = (h[j][i] - mu1) * rs1 * pw[j][i] + pb[j][i];
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float q = a.gate ? k[j][i] * (float)g[j].v[i] : k[j][i];
+        h[j][i] = c.in(j, i) ? a.alpha * (float)r[j].v[i] + q * h[j][i] : 0.0f;
+      }
+    moments(mu2, rs2);
+    if (row < a.M) {
+      c.store(a.h, row * a.d, h);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[j][i] = (h[j][i] - mu2) * rs2 * w[j][i] + b[j][i];
+      c.store(a.y, row * a.d, h);
+      if (a.stats && lane == 0 && wave % NW == 0)
+        reinterpret_cast<f32x4_t*>(a.stats)[row] = f32x4_t{mu1, rs1, mu2, rs2};
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      x[j] = nx[j];
+      r[j] = nr[j];
+      if (a.gate) g[j] = ng[j];
+    }
+  }
+}
+
+// Column sums in the order of the partial rows' slots.
+enum Sum { kDw, kDb, kDscale, kDpw, kDpb, kSums };
+
+template <typename T, int NV, int NW, bool POST, bool WHOLE>
+__global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNormArgs a) {
+  using C = Cols<T, NV, NW, WHOLE>;
+  constexpr int V = C::V, NG = kWaves / NW;
+  constexpr int W = 64 * V * NV * NW;  // columns that the registers of a row hold
+  constexpr int S = POST ? kSums : kDscale + 1;
+  __shared__ float red[2][2 * kWaves];
+  __shared__ float fold[NG > 1 ? W : 1];  // the workgroup's rows' sums meet here, one after the other
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const C c(wave, lane, a.d);
+  const float inv = 1.0f / (float)a.d;
+  const int64_t step = (int64_t)gridDim.x * NG;
+  float w[NV][V], pw[NV][V], pb[NV][V], k[NV][V], total[S][NV][V];
+  c.weights(w, a.w, a.w32, 1.0f);
+  c.weights(k, a.scale, a.w32, 1.0f);
+  if constexpr (POST) {
+    c.weights(pw, a.pw, a.w32, 1.0f);
+    c.weights(pb, a.pb, a.w32, 0.0f);
+  }
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) total[s][j][i] = 0.0f;
+  typename C::Row x, r, g, dh, dy, nx, nr, ng, ndh, ndy;
+  f32x4_t st, nst;
+  int64_t row = (int64_t)blockIdx.x * NG + wave / NW;
+  auto load = [&](typename C::Row& x, typename C::Row& r, typename C::Row& g, typename C::Row& dh, typename C::Row& dy,
+                  f32x4_t& st, int64_t at) __attribute__((always_inline)) {
+    const bool have = at < a.M;
+    c.load(x, a.x, at * a.sx, have);
+    c.load(r, a.r, at * a.sr, have);
+    if (a.gate) c.load(g, a.gate, at * a.sg, have);
+    if (a.dh) c.load(dh, a.dh, at * a.sdh, have);
+    if (a.dy) c.load(dy, a.dy, at * a.sdy, have);
+    st = have ? reinterpret_cast<const f32x4_t*>(a.stats)[at] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+  };
+  load(x, r, g, dh, dy, st, row);
+  int par = 0;
+  for (int64_t base = (int64_t)blockIdx.x * NG; base < a.M; base += step, row += step) {
+    load(nx, nr, ng, ndh, ndy, nst, row + step);
+    const float mu1 = st[0], rs1 = st[1], mu2 = st[2], rs2 = st[3];
+    const bool have = row < a.M;
+    float hh[NV][V], t[NV][V];  // hh: norm(h), then g
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float v = (float)x[j].v[i];
+        if constexpr (POST) v = (v - mu1) * rs1 * pw[j][i] + pb[j][i];
+        t[j][i] = v;
+        const float q = a.gate ? k[j][i] * (float)g[j].v[i] : k[j][i];
+        const float h = a.alpha * (float)r[j].v[i] + q * v;
+        // past the row, and without one, nothing is added: what is there may be made of a row that is not finite
+        const bool in = c.in(j, i) && have;
+        const float n = in ? (h - mu2) * rs2 : 0.0f;
+        hh[j][i] = n;
+        if (a.dy) {
+          const float d = (float)dy[j].v[i], wdy = d * w[j][i];
+          s1 += wdy;
+          s2 += in ? wdy * n : 0.0f;
+          total[kDw][j][i] += in ? d * n : 0.0f;
+          total[kDb][j][i] += d;
+        }
+      }
+    if (a.dy) {
+      row_sum2<NW>(s1, s2, red[par], wave);
+      par ^= 1;
+    }
+    const float c1 = a.rms ? 0.0f : s1 * inv, c2 = s2 * inv;
+    float o[NV][V];
+    s1 = s2 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float e = a.dh ? (float)dh[j].v[i] : 0.0f;
+        if (a.dy) e += rs2 * ((float)dy[j].v[i] * w[j][i] - c1 - hh[j][i] * c2);
+        const bool in = c.in(j, i) && have;
+        e = in ? e : 0.0f;
+        hh[j][i] = e;
+        const float gate = a.gate ? (float)g[j].v[i] : 1.0f, f = e * gate, q = f * k[j][i];
+        total[kDscale][j][i] += in ? f * t[j][i] : 0.0f;
+        if constexpr (POST) {
+          const float xh = in ? ((float)x[j].v[i] - mu1) * rs1 : 0.0f;
+          total[kDpw][j][i] += q * xh;
+          total[kDpb][j][i] += q;
+          s1 += q * pw[j][i];
+          s2 += q * pw[j][i] * xh;
+        }
+        o[j][i] = q;
+      }
+    if (POST && a.dx) {
+      row_sum2<NW>(s1, s2, red[par], wave);
+      par ^= 1;
+      const float e1 = a.rms ? 0.0f : s1 * inv, e2 = s2 * inv;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float xh = ((float)x[j].v[i] - mu1) * rs1;
+          o[j][i] = rs1 * (o[j][i] * pw[j][i] - e1 - xh * e2);
+        }
+    }
+    if (have) {
+      if (a.dx) c.store(a.dx, row * a.d, o);
+      if (a.dgate) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < V; ++i) o[j][i] = hh[j][i] * k[j][i] * t[j][i];
+        c.store(a.dgate, row * a.d, o);
+      }
+      if (a.dr) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < V; ++i) o[j][i] = a.alpha * hh[j][i];
+        c.store(a.dr, row * a.d, o);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      x[j] = nx[j];
+      r[j] = nr[j];
+      if (a.gate) g[j] = ng[j];
+      if (a.dh) dh[j] = ndh[j];
+      if (a.dy) dy[j] = ndy[j];
+    }
+    st = nst;
+  }
+  if (!a.part) return;
+  // wanted sums one behind the other, [parts][wanted][d]
+  float* part = a.part + (int64_t)blockIdx.x * a.wanted * a.d;
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    if (!a.sums[s]) continue;
+    if constexpr (NG > 1) {
+      for (int q = 0; q < NG; ++q) {
+        if (wave / NW == q) {
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const int at = c.col[j] + i;
+              fold[at] = q ? fold[at] + total[s][j][i] : total[s][j][i];
+            }
+        }
+        __syncthreads();
+      }
+      for (int at = threadIdx.x; at < a.d; at += kThreads) part[at] = fold[at];
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (c.in(j, i)) part[c.col[j] + i] = total[s][j][i];
+    }
+    part += a.d;
+  }
+}
+
+// The wanted sums: the columns of `parts` rows, 16 a workgroup, its threads 64 rows at a time.
+template <typename O>
+__global__ void __launch_bounds__(1024) residual_norm_join_kernel(ResidualNormArgs a, int parts) {
+  __shared__ float sums[64][17];
+  const int c = threadIdx.x & 15, group = threadIdx.x >> 4;
+  const int64_t n = (int64_t)a.wanted * a.d, at = (int64_t)blockIdx.x * 16 + c;
+  float s = 0.0f;
+  if (at < n) {
+#pragma unroll 4
+    for (int p = group; p < parts; p += 64) s += a.part[p * n + at];
+  }
+  sums[group][c] = s;
+  __syncthreads();
+#pragma unroll
+  for (int half = 32; half >= 4; half /= 2) {  // to four sums a column
+    if (group < half) sums[group][c] += sums[group + half][c];
+    __syncthreads();
+  }
+  if (group == 0 && at < n) {
+    s = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+    int slot = (int)(at / a.d);
+    const int k = (int)(at - (int64_t)slot * a.d);
+    for (int q = 0; q < kSums; ++q) {
+      if (!a.sums[q]) continue;
+      if (slot-- == 0) static_cast<O*>(a.sums[q])[k] = (O)s;
+    }
+  }
+}
+
+// Workgroups for M rows, `group` at a time: as many as run at once (per_cu on each compute unit).
+int grid_of(int64_t M, int group, int per_cu) {
+  const int64_t want = (M + group - 1) / group, most = (int64_t)layer_cus() * per_cu;
+  return (int)(want < most ? want : most);
+}
+
+// Workgroups of this kernel that a compute unit holds.
+int held(const void* kernel) {
+  int n = 0;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, 0) != hipSuccess || n < 1) n = 1;
+  return n;
+}
+
+// Backward workgroups write their partial sums once each: two a unit at most.
+constexpr int kBwdPerCu = 2;
+
+// Waves of a row, with 16 elements a lane in the forward and 8 in the backward (16 in the widest rows).
+int waves_of(int d, bool bwd) {
+  int nw = 1;
+  while (nw < kWaves && d > 64 * nw * (bwd ? 8 : 16)) nw *= 2;
+  return nw;
+}
+
+template <typename T, int E, int NW, bool POST, bool WHOLE, bool BWD>
+int run(const ResidualNormArgs& a, hipStream_t s) {
+  constexpr int NV = E * (int)sizeof(T) / 16;
+  if constexpr (BWD) {
+    static const int n = held(reinterpret_cast<const void*>(residual_norm_bwd_kernel<T, NV, NW, POST, WHOLE>));
+    const int grid = grid_of(a.M, kWaves / NW, n < kBwdPerCu ? n : kBwdPerCu);
+    residual_norm_bwd_kernel<T, NV, NW, POST, WHOLE><<<grid, kThreads, 0, s>>>(a);
+    return grid;
+  } else {
+    static const int n = held(reinterpret_cast<const void*>(residual_norm_fwd_kernel<T, NV, NW, POST, WHOLE>));
+    const int grid = grid_of(a.M, kWaves / NW, n);
+    residual_norm_fwd_kernel<T, NV, NW, POST, WHOLE><<<grid, kThreads, 0, s>>>(a);
+    return grid;
+  }
+}
+
+template <typename T, bool POST, bool WHOLE>
+int run_row(const ResidualNormArgs& a, bool bwd, hipStream_t s) {
+  const int nw = waves_of(a.d, bwd);
+  const bool eight = a.d <= 64 * nw * 8;
+  if (bwd) {
+    switch (nw) {
+      case 1: return run<T, 8, 1, POST, WHOLE, true>(a, s);
+      case 2: return run<T, 8, 2, POST, WHOLE, true>(a, s);
+      case 4: return run<T, 8, 4, POST, WHOLE, true>(a, s);
+      default: return eight ? run<T, 8, 8, POST, WHOLE, true>(a, s) : run<T, 16, 8, POST, WHOLE, true>(a, s);
+    }
+  }
+  switch (nw) {
+    case 1: return eight ? run<T, 8, 1, POST, WHOLE, false>(a, s) : run<T, 16, 1, POST, WHOLE, false>(a, s);
+    case 2: return run<T, 16, 2, POST, WHOLE, false>(a, s);
+    case 4: return run<T, 16, 4, POST, WHOLE, false>(a, s);
+    default: return run<T, 16, 8, POST, WHOLE, false>(a, s);
+  }
+}
+
+template <typename T>
+int launch(const ResidualNormArgs& a, bool bwd, hipStream_t s) {
+  const bool whole = a.d % (16 / sizeof(T)) == 0;
+  if (a.post) return whole ? run_row<T, true, true>(a, bwd, s) : run_row<T, true, false>(a, bwd, s);
+  return whole ? run_row<T, false, true>(a, bwd, s) : run_row<T, false, false>(a, bwd, s);
+}
+
+int launch_kind(int kind, const ResidualNormArgs& a, bool bwd, hipStream_t s) {
+  if (kind == FMX_DTYPE_F32) return launch<float>(a, bwd, s);
+  if (kind == FMX_DTYPE_BF16) return launch<__bf16>(a, bwd, s);
+  return launch<_Float16>(a, bwd, s);
+}
+
+}  // namespace
+
+int residual_norm_parts(int64_t M, int d) { return grid_of(M, kWaves / waves_of(d, true), kBwdPerCu); }
+
+hipError_t launch_residual_norm_fwd(int kind, const ResidualNormArgs& a, hipStream_t s) {
+  launch_kind(kind, a, false, s);
+  return hipGetLastError();
+}
+
+hipError_t launch_residual_norm_bwd(int kind, const ResidualNormArgs& a, hipStream_t s) {
+  int parts = 0;  // no rows: the sums of nothing
+  if (a.M > 0) {
+    parts = launch_kind(kind, a, true, s);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (!a.wanted) return hipSuccess;
+  const unsigned grid = (unsigned)(((int64_t)a.wanted * a.d + 15) / 16);
+  if (a.w32 || kind == FMX_DTYPE_F32)
+    residual_norm_join_kernel<float><<<grid, 1024, 0, s>>>(a, parts);
+  else if (kind == FMX_DTYPE_BF16)
+    residual_norm_join_kernel<__bf16><<<grid, 1024, 0, s>>>(a, parts);
+  else
+    residual_norm_join_kernel<_Float16><<<grid, 1024, 0, s>>>(a, parts);
+  return hipGetLastError();
+}
+
+}  // namespace fmx

@@ -491,6 +491,40 @@ int fmx_layer_norm_bwd(int dtype, const void* x, int64_t x_stride, const void* d
 size_t fmx_layer_norm_bwd_workspace_bytes(int64_t M, int64_t d);
 
 /*
+ * The step between two blocks, over rows of d elements, sums in fp32:
+ *   norm(v) = (v - mu) s,  s = 1 / sqrt(mean (v - mu)^2 + eps),  mu = mean v, with rms 0
+ *   t = norm(x) post_weight + post_bias with post, else x
+ *   h = alpha residual + scale gate t,   y = norm(h) weight + bias   (of h before it is rounded)
+ *
+ *   x, residual, gate  [M, d]  dtype (F16, BF16 or F32), each with a row stride (any, also 0); gate: or NULL (ones)
+ *   weight, bias, post_weight, post_bias, scale  [d]  w_dtype (dtype, or F32), or NULL (ones; biases: zeros)
+ *   h, y   [M, d]  dtype, contiguous
+ *   stats  [M, 4]  fp32, 16-byte aligned: both norms' mu and s for the backward; or NULL
+ * 1 <= d <= FMX_RESIDUAL_NORM_MAX_D. Pointers are aligned to their elements.
+ */
+#define FMX_RESIDUAL_NORM_MAX_D 8192
+
+int fmx_residual_norm(int dtype, const void* x, int64_t x_stride, const void* residual, int64_t r_stride, const void* gate,
+                      int64_t g_stride, int w_dtype, const void* weight, const void* bias, int post, const void* post_weight,
+                      const void* post_bias, const void* scale, double alpha, int rms, double eps, int64_t M, int64_t d,
+                      void* h, void* y, float* stats, void* stream);
+
+/*
+ * Its backward from the same inputs, the forward's stats and the gradients dh and dy of h and y (rows with strides; one of
+ * them may be NULL: zeros): dx, dr, dgate [M, d] in dtype, contiguous, and the weights' gradients [d] in w_dtype,
+ * sums in fp32 in a fixed order, each skipped when NULL (dw and db need dy).
+ * Workspace, for a weight's gradient: fmx_residual_norm_bwd_workspace_bytes.
+ */
+int fmx_residual_norm_bwd(int dtype, const void* x, int64_t x_stride, const void* residual, int64_t r_stride,
+                          const void* gate, int64_t g_stride, int w_dtype, const void* weight, int post,
+                          const void* post_weight, const void* post_bias, const void* scale, double alpha, int rms,
+                          const float* stats, const void* dh, int64_t dh_stride, const void* dy, int64_t dy_stride, int64_t M,
+                          int64_t d, void* dx, void* dr, void* dgate, void* dw, void* db, void* dscale, void* dpw, void* dpb,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+size_t fmx_residual_norm_bwd_workspace_bytes(int64_t M, int64_t d);
+
+/*
  * One tensor of an AdamW step; n elements, all arrays contiguous and aligned to
  * their elements. state_bits 32: exp_avg and exp_avg_sq are fp32 and the scales
  * unused. state_bits 8: exp_avg holds int8 codes c (moment c |c| scale),

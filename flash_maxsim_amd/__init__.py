@@ -28,6 +28,7 @@ from .flash_maxsim_linear import linear
 from .flash_maxsim_gated import gated_linear
 from .flash_maxsim_norm import layer_norm
 from .flash_maxsim_residual_norm import residual_norm
+from .flash_maxsim_embedding import embedding
 from .flash_maxsim_optim import AdamW, AdamW8bitState, adamw_state, adamw_step, dequantize_adamw
 from .flash_maxsim_muon import Muon, muon_step, orthogonalize
 
@@ -56,6 +57,7 @@ __all__ = [
     "gated_linear",
     "layer_norm",
     "residual_norm",
+    "embedding",
     "AdamW",
     "AdamW8bitState",
     "adamw_state",

@@ -141,6 +141,12 @@ _SIGNATURES = {
          _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _size, _ptr],
     ),
     "fmx_residual_norm_bwd_workspace_bytes": (_size, [_i64, _i64]),
+    "fmx_embedding": (_int, [_int, _ptr, _int, _ptr, _i64, _f64, _i64, _i64, _i64, _ptr, _ptr]),
+    "fmx_embedding_bwd": (
+        _int,
+        [_int, _ptr, _int, _ptr, _i64, _f64, _i64, _i64, _i64, _i64, _ptr, _ptr, _size, _ptr],
+    ),
+    "fmx_embedding_bwd_workspace_bytes": (_size, [_int, _i64, _i64, _i64]),
     "fmx_muon": (
         _int,
         [_int, _int, _int, _ptr, _i64, _f64, _f64, _int, _f64, _int, _f64, _f64, _f64, _f64, _int, _ptr, _ptr, _size,

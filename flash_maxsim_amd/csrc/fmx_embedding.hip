@@ -1,0 +1,391 @@
+// Embedding lookup y[t] = scale W[ids[t]], and its gradient dW[v] = scale sum of dy[t] over the t with ids[t] = v.
+//
+// Bound by HBM: the lookup reads and writes T rows, the gradient reads T rows of dy and writes all V rows of dW.
+//
+// The gradient has no atomics on values: tokens are sorted by id (stable), so that the rows of an id lie in a fixed
+// order, and the sorted list is cut into stretches of kStretch tokens whatever their ids: a wave sums a stretch's
+// rows in registers and writes the ids that begin and end in it to dW; of an id that goes on past the
+// stretch's end it writes a float32 partial sum, and a second kernel adds an id's partial sums in order. So an id that
+// makes up half of the tokens costs no more than others. Rows of ids that do not occur get zeros from other workgroups of
+// the first kernel, which look for their ids in the sorted list.
+//
+// Sorting: up to kRankMost tokens each counts the tokens before it (T^2 comparisons, one launch: 1024 tokens 3, 16384 16 us);
+// more go through passes of a radix sort, of 2 launches each, by digits of up to 10 bits.
+#include "fmx_device.h"
+#include "fmx_layers.h"
+#include "fmx_rows.h"
+
+#include "../../include/fmx.h"
+
+namespace fmx {
+namespace {
+
+constexpr int kStretch = 32;         // sorted tokens that a wave sums
+constexpr int64_t kRankMost = 16384;
+constexpr int kBits = 10;            // of a digit, at most
+constexpr int kTile = 4096;          // tokens of a workgroup of the radix sort
+
+// The id of token t as a key of the sort: V for tokens without a gradient (outside 0 .. V - 1, or the padding id).
+__device__ __forceinline__ int32_t key_of(const EmbeddingArgs& a, int64_t t) {
+  const int64_t id = a.ids64 ? static_cast<const int64_t*>(a.ids)[t] : (int64_t)static_cast<const int32_t*>(a.ids)[t];
+  return id >= 0 && id < a.V && id != a.padding ? (int32_t)id : (int32_t)a.V;
+}
+
+// ---- lookup ----
+
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(256) embedding_kernel(EmbeddingArgs a, int lanes) {
+  constexpr int V = 16 / sizeof(T);
+  const int lane = threadIdx.x & (lanes - 1), rows = 256 / lanes;
+  for (int64_t t = (int64_t)blockIdx.x * rows + threadIdx.x / lanes; t < a.T; t += (int64_t)gridDim.x * rows) {
+    const int64_t id = a.ids64 ? static_cast<const int64_t*>(a.ids)[t] : (int64_t)static_cast<const int32_t*>(a.ids)[t];
+    const bool there = id >= 0 && id < a.V;
+    const T* w = static_cast<const T*>(a.w) + (there ? id : 0) * a.sw;
+    T* y = static_cast<T*>(a.out) + t * a.d;
+    for (int col = lane * V; col < a.d; col += lanes * V) {
+      Piece<T, V> p;
+      p.template load<WHOLE>(w + col, a.d - col);
+#pragma unroll
+      for (int i = 0; i < V; ++i) p.v[i] = (T)(there ? (float)p.v[i] * a.scale : __builtin_nanf(""));
+      p.template store<WHOLE>(y + col, a.d - col);
+    }
+  }
+}
+
+// ---- sorting ----
+
+// Each token's place: how many come before it. A workgroup ranks 64 tokens, each of its 16 waves against a sixteenth.
+__global__ void __launch_bounds__(1024) embedding_rank_kernel(EmbeddingArgs a) {
+  __shared__ int counts[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int T = (int)a.T, t = blockIdx.x * 64 + lane;
+  const int32_t mine = t < T ? key_of(a, t) : 0;
+  const int per = (T + 15) / 16, from = wave * per, end = from + per < T ? from + per : T;
+  int before = 0;
+  for (int base = from; base < end; base += 64) {
+    const int32_t theirs = base + lane < end ? key_of(a, base + lane) : 0;
+    const int n = end - base < 64 ? end - base : 64;
+    for (int k = 0; k < n; ++k) {
+      const int32_t other = __builtin_amdgcn_readlane(theirs, k);
+      before += other < mine || (other == mine && base + k < t) ? 1 : 0;
+    }
+  }
+  counts[wave][lane] = before;
+  __syncthreads();
+  if (wave == 0 && t < T) {
+    int place = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) place += counts[w][lane];
+    a.keys[place] = mine;
+    a.order[place] = t;
+  }
+}
+
+// One pass of the radix sort: the key's bits `shift` .. shift + bits - 1. FIRST: keys come from the ids.
+template <bool FIRST>
+__global__ void __launch_bounds__(1024) embedding_count_kernel(EmbeddingArgs a, int shift, int bits, const int32_t* keys,
+                                                              int32_t* counts) {
+  __shared__ int32_t hist[1 << kBits];
+  const int digits = 1 << bits;
+  if ((int)threadIdx.x < digits) hist[threadIdx.x] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kTile / 1024; ++k) {
+    const int64_t t = (int64_t)blockIdx.x * kTile + k * 1024 + threadIdx.x;
+    if (t < a.T) atomicAdd(&hist[((FIRST ? key_of(a, t) : keys[t]) >> shift) & (digits - 1)], 1);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < digits) counts[(int64_t)blockIdx.x * digits + threadIdx.x] = hist[threadIdx.x];
+}
+
+// Tokens to their places of this pass, in their order before it: digits before, workgroups before, waves before (a
+// wave has kTile / 16 neighbouring tokens), tokens of the wave before.
+template <bool FIRST>
+__global__ void __launch_bounds__(1024) embedding_place_kernel(EmbeddingArgs a, int shift, int bits, const int32_t* keys,
+                                                              const int32_t* order, const int32_t* counts, int groups,
+                                                              int32_t* keys_out, int32_t* order_out) {
+  __shared__ int32_t mine[16][1 << kBits];
+  __shared__ int32_t sums[16];
+  const int digits = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // how many tokens lie before this workgroup's of digit threadIdx.x
+  int total = 0, before = 0;
+  if ((int)threadIdx.x < digits) {
+#pragma unroll 8
+    for (int g = 0; g < groups; ++g) {
+      const int n = counts[(int64_t)g * digits + threadIdx.x];
+      total += n;
+      before += g < (int)blockIdx.x ? n : 0;
+    }
+  }
+  int scan = total;  // up to and with this digit
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) {
+    const int other = __shfl_up(scan, k);
+    scan += lane >= k ? other : 0;
+  }
+  if (lane == 63) sums[wave] = scan;
+  for (int k = threadIdx.x; k < 16 * digits; k += 1024) mine[k / digits][k & (digits - 1)] = 0;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) before += sums[w];
+  before += scan - total;
+
+  constexpr int kRounds = kTile / 1024;
+  int32_t key[kRounds], from[kRounds];
+  int place[kRounds];
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int64_t t = (int64_t)blockIdx.x * kTile + wave * (kTile / 16) + k * 64 + lane;
+    const bool there = t < a.T;
+    key[k] = there ? (FIRST ? key_of(a, t) : keys[t]) : 0;
+    from[k] = there ? (FIRST ? (int32_t)t : order[t]) : 0;
+    const int digit = (key[k] >> shift) & (digits - 1);
+    uint64_t same = __ballot(there);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t set = __ballot((digit >> b) & 1);
+      same &= (digit >> b) & 1 ? set : ~set;
+    }
+    const int ahead = __popcll(same & (((uint64_t)1 << lane) - 1));
+    place[k] = there ? mine[wave][digit] + ahead : -1;
+    // the wave's lanes have read the count; the last of each digit moves it on
+    __builtin_amdgcn_wave_barrier();
+    if (there && (same >> lane) == 1) mine[wave][digit] = place[k] + 1;
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < digits) {
+    int at = before;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      const int n = mine[w][threadIdx.x];
+      mine[w][threadIdx.x] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    if (place[k] < 0) continue;
+    const int to = mine[wave][(key[k] >> shift) & (digits - 1)] + place[k];
+    keys_out[to] = key[k];
+    order_out[to] = from[k];
+  }
+}
+
+// ---- sums ----
+
+// Workgroups before `sums` add up stretches, a wave a stretch of one block of 64 pieces of columns; the others write
+// the rows of ids that do not occur, 256 ids each.
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(256) embedding_sum_kernel(EmbeddingArgs a, uint32_t sums, int blocks) {
+  constexpr int V = 16 / sizeof(T);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  T* out = static_cast<T*>(a.out);
+  if (blockIdx.x >= sums) {
+    __shared__ uint8_t absent[256];
+    const int64_t v0 = (int64_t)(blockIdx.x - sums) * 256, v = v0 + threadIdx.x;
+    int64_t lo = 0, hi = a.T;  // the first token whose key is v or more
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (a.keys[mid] < v) lo = mid + 1; else hi = mid;
+    }
+    absent[threadIdx.x] = v < a.V && (lo == a.T || a.keys[lo] != v);
+    __syncthreads();
+    Piece<T, V> zero;
+#pragma unroll
+    for (int i = 0; i < V; ++i) zero.v[i] = T(0.0f);
+    for (int r = wave; r < 256; r += 4) {
+      if (!absent[r]) continue;
+      for (int col = lane * V; col < a.d; col += 64 * V) zero.template store<WHOLE>(out + (v0 + r) * a.d + col, a.d - col);
+    }
+    return;
+  }
+  const int64_t id = (int64_t)blockIdx.x * 4 + wave, stretch = id / blocks;
+  const int col = (int)(id - stretch * blocks) * 64 * V + lane * V;
+  const int64_t from = stretch * kStretch;
+  if (from >= a.T) return;
+  const int n = a.T - from < kStretch ? (int)(a.T - from) : kStretch;
+  const int32_t k = lane < n ? a.keys[from + lane] : (int32_t)a.V, t = lane < n ? a.order[from + lane] : 0;
+  const int32_t last = from > 0 ? a.keys[from - 1] : -1, next = from + n < a.T ? a.keys[from + n] : -1;
+  float s[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) s[i] = 0.0f;
+  const T* dy = static_cast<const T*>(a.dy);
+  constexpr int U = 8;  // rows in flight
+  Piece<T, V> p[U];
+  auto load = [&](int at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = __builtin_amdgcn_readlane(t, at + u < n ? at + u : n - 1);
+      p[u].template load<WHOLE>(dy + row * a.sdy + col, a.d - col);
+    }
+  };
+  for (int at = 0; at < n; at += U) {
+    load(at);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (at + u >= n) break;
+      const int32_t key = __builtin_amdgcn_readlane(k, at + u);
+      if (key >= a.V) return;  // tokens without a gradient come last
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] += (float)p[u].v[i];
+      const int32_t after = at + u + 1 < n ? __builtin_amdgcn_readlane(k, at + u + 1) : next;
+      if (after == key && at + u + 1 < n) continue;
+      const bool begins = __builtin_amdgcn_readlane(k, 0) != key || last != key, ends = after != key;
+      if (col < a.d) {
+        if (begins && ends) {
+          Piece<T, V> o;
+#pragma unroll
+          for (int i = 0; i < V; ++i) o.v[i] = (T)(s[i] * a.scale);
+          o.template store<WHOLE>(out + (int64_t)key * a.d + col, a.d - col);
+        } else {
+          // an id that goes on: its first stretch's sum in slot 1, the later ones' in slot 0
+          float* part = a.part + ((stretch * 2 + (begins ? 1 : 0)) * blocks) * 64 * V + col;
+#pragma unroll
+          for (int i = 0; i < V; i += 4) *reinterpret_cast<f32x4_t*>(part + i) = f32x4_t{s[i], s[i + 1], s[i + 2], s[i + 3]};
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] = 0.0f;
+    }
+  }
+}
+
+// Ids that go past a stretch's end: a workgroup for each stretch that such an id begins in (the others leave), and
+// 256 columns; the waves add every sixteenth partial sum, and then the waves' sums.
+template <typename T>
+__global__ void __launch_bounds__(1024) embedding_join_kernel(EmbeddingArgs a, int pitch) {
+  __shared__ __attribute__((aligned(16))) f32x4_t sums[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t stretch = blockIdx.x, end = (stretch + 1) * kStretch;
+  if (end >= a.T) return;
+  const int32_t key = a.keys[end - 1];
+  if (key >= a.V || a.keys[end] != key) return;
+  if (a.keys[stretch * kStretch] == key && stretch > 0 && a.keys[stretch * kStretch - 1] == key) return;  // began before
+  // the stretches after this one that begin with the id
+  int64_t more = 0;
+  for (;;) {
+    const int64_t at = (stretch + 1 + more + lane) * kStretch;
+    const uint64_t same = __ballot(at < a.T && a.keys[at < a.T ? at : 0] == key);
+    const int n = same == ~(uint64_t)0 ? 64 : __builtin_ctzll(~same);
+    more += n;
+    if (n < 64) break;
+  }
+  const int col = blockIdx.y * 256 + lane * 4;
+  f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+  if (col < pitch) {
+    const float* part = a.part + col;
+#pragma unroll 4
+    for (int64_t q = wave; q <= more; q += 16)
+      s += *reinterpret_cast<const f32x4_t*>(part + ((stretch + q) * 2 + (q == 0 ? 1 : 0)) * pitch);
+  }
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int w = 1; w < 16; ++w) s += sums[w][lane];
+  T* out = static_cast<T*>(a.out) + (int64_t)key * a.d;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (col + i < a.d) out[col + i] = (T)(s[i] * a.scale);
+}
+
+template <typename T>
+hipError_t lookup(const EmbeddingArgs& a, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  int lanes = 1;
+  while (lanes < 256 && lanes * V < a.d) lanes *= 2;
+  const int64_t rows = 256 / lanes, want = (a.T + rows - 1) / rows, most = (int64_t)layer_cus() * 16;
+  const unsigned grid = (unsigned)(want < most ? want : most);
+  if (a.d % V == 0)
+    embedding_kernel<T, true><<<grid, 256, 0, s>>>(a, lanes);
+  else
+    embedding_kernel<T, false><<<grid, 256, 0, s>>>(a, lanes);
+  return hipGetLastError();
+}
+
+int bits_of(int64_t V) {  // of the keys 0 .. V
+  int bits = 1;
+  while (V >> bits) ++bits;
+  return bits;
+}
+
+int64_t stretches_of(int64_t T) { return (T + kStretch - 1) / kStretch; }
+
+struct Layout {
+  int64_t keys, counts, part, total;  // bytes: two lists of keys and of tokens; digits' counts; partial sums
+};
+Layout layout(int kind, int64_t T, int64_t V, int64_t d) {
+  const int64_t per = 64 * (kind == FMX_DTYPE_F32 ? 4 : 8), pitch = (d + per - 1) / per * per;
+  const bool radix = T > kRankMost;
+  Layout l;
+  l.keys = (T * 4 + 255) / 256 * 256;
+  l.counts = radix ? (T + kTile - 1) / kTile * (4 << kBits) : 0;
+  l.part = stretches_of(T) * 2 * pitch * 4;
+  l.total = (radix ? 4 : 2) * l.keys + l.counts + l.part;
+  return l;
+}
+
+template <typename T>
+hipError_t gradient(int kind, EmbeddingArgs a, char* ws, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const Layout l = layout(kind, a.T, a.V, a.d);
+  int32_t* lists[4];
+  for (int i = 0; i < 4; ++i) lists[i] = reinterpret_cast<int32_t*>(ws + (i < 2 || a.T > kRankMost ? i * l.keys : 0));
+  a.keys = lists[0];
+  a.order = lists[1];
+  if (a.T > kRankMost) {
+    int32_t* counts = reinterpret_cast<int32_t*>(ws + 4 * l.keys);
+    const int bits = bits_of(a.V), passes = (bits + kBits - 1) / kBits, groups = (int)((a.T + kTile - 1) / kTile);
+    int shift = 0;
+    for (int p = 0; p < passes; ++p) {  // the bits left over the passes left
+      const int b = (bits - shift + passes - p - 1) / (passes - p), to = (p & 1) * 2, from = 2 - to;
+      if (p == 0) {
+        embedding_count_kernel<true><<<groups, 1024, 0, s>>>(a, shift, b, nullptr, counts);
+        embedding_place_kernel<true>
+            <<<groups, 1024, 0, s>>>(a, shift, b, nullptr, nullptr, counts, groups, lists[to], lists[to + 1]);
+      } else {
+        embedding_count_kernel<false><<<groups, 1024, 0, s>>>(a, shift, b, lists[from], counts);
+        embedding_place_kernel<false>
+            <<<groups, 1024, 0, s>>>(a, shift, b, lists[from], lists[from + 1], counts, groups, lists[to], lists[to + 1]);
+      }
+      a.keys = lists[to];
+      a.order = lists[to + 1];
+      shift += b;
+    }
+  } else if (a.T > 0) {
+    embedding_rank_kernel<<<(unsigned)((a.T + 63) / 64), 1024, 0, s>>>(a);
+  }
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  a.part = reinterpret_cast<float*>(ws + l.total - l.part);
+  const int blocks = (int)((a.d + 64 * V - 1) / (64 * V));
+  const uint32_t sums = (uint32_t)((stretches_of(a.T) * blocks + 3) / 4), rows = (uint32_t)((a.V + 255) / 256);
+  if (a.d % V == 0)
+    embedding_sum_kernel<T, true><<<sums + rows, 256, 0, s>>>(a, sums, blocks);
+  else
+    embedding_sum_kernel<T, false><<<sums + rows, 256, 0, s>>>(a, sums, blocks);
+  e = hipGetLastError();
+  if (e != hipSuccess || a.T <= kStretch) return e;
+  embedding_join_kernel<T><<<dim3((unsigned)(stretches_of(a.T) - 1), (unsigned)((a.d + 255) / 256)), 1024, 0, s>>>(
+      a, blocks * 64 * V);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+size_t embedding_workspace_bytes(int kind, int64_t T, int64_t V, int64_t d) { return (size_t)layout(kind, T, V, d).total; }
+
+hipError_t launch_embedding(int kind, const EmbeddingArgs& a, hipStream_t s) {
+  if (kind == FMX_DTYPE_F32) return lookup<float>(a, s);
+  if (kind == FMX_DTYPE_BF16) return lookup<__bf16>(a, s);
+  return lookup<_Float16>(a, s);
+}
+
+hipError_t launch_embedding_bwd(int kind, const EmbeddingArgs& a, void* ws, hipStream_t s) {
+  if (kind == FMX_DTYPE_F32) return gradient<float>(kind, a, static_cast<char*>(ws), s);
+  if (kind == FMX_DTYPE_BF16) return gradient<__bf16>(kind, a, static_cast<char*>(ws), s);
+  return gradient<_Float16>(kind, a, static_cast<char*>(ws), s);
+}
+
+}  // namespace fmx

@@ -208,4 +208,25 @@ int residual_norm_parts(int64_t M, int d);  // rows of ResidualNormArgs::part at
 hipError_t launch_residual_norm_fwd(int kind, const ResidualNormArgs& a, hipStream_t s);
 hipError_t launch_residual_norm_bwd(int kind, const ResidualNormArgs& a, hipStream_t s);
 
+// ---- embedding (fmx_embedding.hip) ----
+
+struct EmbeddingArgs {
+  const void* ids;       // [T], int64 or int32
+  const void* w;         // forward: [V, d], row stride sw
+  const void* dy;        // backward: [T, d], row stride sdy
+  void* out;             // forward: [T, d], backward: dw [V, d]; contiguous
+  int32_t* keys;         // backward, in the workspace: the ids sorted, and the tokens in their order
+  int32_t* order;
+  float* part;           // backward: [stretches][2][columns] sums of ids that go on
+  int64_t T, V, sw, sdy;
+  int64_t padding;       // the id without a gradient, or -1
+  int d;
+  int ids64;
+  float scale;
+};
+
+size_t embedding_workspace_bytes(int kind, int64_t T, int64_t V, int64_t d);
+hipError_t launch_embedding(int kind, const EmbeddingArgs& a, hipStream_t s);
+hipError_t launch_embedding_bwd(int kind, const EmbeddingArgs& a, void* ws, hipStream_t s);
+
 }  // namespace fmx

@@ -115,6 +115,18 @@ int check_residual_norm(int dtype, int w_dtype, int64_t x_stride, int64_t r_stri
   return FMX_OK;
 }
 
+int check_embedding(int dtype, int ids_bits, int64_t stride, double scale, int64_t T, int64_t V, int64_t d) {
+  if (!known(dtype)) return fail(FMX_ERR_INVALID, "unknown dtype %d", dtype);
+  if (ids_bits != 32 && ids_bits != 64) return fail(FMX_ERR_INVALID, "ids of %d bits, must be 32 or 64", ids_bits);
+  if (T < 0 || V < 1 || d < 1 || stride < 0)
+    return fail(FMX_ERR_INVALID, "invalid sizes T=%lld V=%lld d=%lld stride=%lld", (long long)T, (long long)V, (long long)d,
+                (long long)stride);
+  if (T > FMX_EMBEDDING_MAX_TOKENS || V > FMX_EMBEDDING_MAX_ROWS || d > FMX_MAX_D)
+    return fail(FMX_ERR_UNSUPPORTED, "T=%lld V=%lld d=%lld too large", (long long)T, (long long)V, (long long)d);
+  if (!isfinite(scale)) return fail(FMX_ERR_INVALID, "scale must be finite");
+  return FMX_OK;
+}
+
 static_assert(sizeof(fmx_muon_matrix) == sizeof(fmx::MuonMatrix), "the same fields in the same order");
 
 bool muon_sides(const fmx_muon_matrix& x) {
@@ -658,6 +670,59 @@ int fmx_residual_norm_bwd(int dtype, const void* x, int64_t x_stride, const void
   a.alpha = (float)alpha;
   return hip_status(fmx::launch_residual_norm_bwd(dtype, a, static_cast<hipStream_t>(stream)),
                     "fmx_residual_norm_bwd launch");
+}
+
+int fmx_embedding(int dtype, const void* ids, int ids_bits, const void* w, int64_t w_stride, double scale, int64_t T, int64_t V,
+                  int64_t d, void* y, void* stream) {
+  const int rc = check_embedding(dtype, ids_bits, w_stride, scale, T, V, d);
+  if (rc) return rc;
+  if (T == 0) return ok();
+  if (!ids || !w || !y) return fail(FMX_ERR_INVALID, "ids, w and y must be non-null");
+  if (!aligned(ids, ids_bits / 8) || !aligned(w, size_of(dtype)) || !aligned(y, size_of(dtype)))
+    return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");
+  fmx::EmbeddingArgs a = {};
+  a.ids = ids;
+  a.ids64 = ids_bits == 64;
+  a.w = w;
+  a.sw = w_stride;
+  a.out = y;
+  a.T = T;
+  a.V = V;
+  a.d = (int)d;
+  a.scale = (float)scale;
+  return hip_status(fmx::launch_embedding(dtype, a, static_cast<hipStream_t>(stream)), "fmx_embedding launch");
+}
+
+size_t fmx_embedding_bwd_workspace_bytes(int dtype, int64_t T, int64_t V, int64_t d) {
+  if (!known(dtype) || T < 0 || V < 1 || d < 1 || T > FMX_EMBEDDING_MAX_TOKENS || V > FMX_EMBEDDING_MAX_ROWS || d > FMX_MAX_D)
+    return 0;
+  return fmx::embedding_workspace_bytes(dtype, T, V, d);
+}
+
+int fmx_embedding_bwd(int dtype, const void* ids, int ids_bits, const void* dy, int64_t dy_stride, double scale,
+                      int64_t padding_id, int64_t T, int64_t V, int64_t d, void* dw, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  const int rc = check_embedding(dtype, ids_bits, dy_stride, scale, T, V, d);
+  if (rc) return rc;
+  if ((T > 0 && (!ids || !dy)) || !dw) return fail(FMX_ERR_INVALID, "ids, dy and dw must be non-null");
+  if (!aligned(ids, ids_bits / 8) || !aligned(dy, size_of(dtype)) || !aligned(dw, size_of(dtype)))
+    return fail(FMX_ERR_INVALID, "pointers must be aligned to their elements");
+  const size_t need = fmx_embedding_bwd_workspace_bytes(dtype, T, V, d);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
+    return fail(FMX_ERR_WORKSPACE, "workspace of %zu bytes required, 256-byte aligned, %zu given", need, workspace_bytes);
+  fmx::EmbeddingArgs a = {};
+  a.ids = ids;
+  a.ids64 = ids_bits == 64;
+  a.dy = dy;
+  a.sdy = dy_stride;
+  a.out = dw;
+  a.T = T;
+  a.V = V;
+  a.d = (int)d;
+  a.padding = padding_id;
+  a.scale = (float)scale;
+  return hip_status(fmx::launch_embedding_bwd(dtype, a, workspace, static_cast<hipStream_t>(stream)),
+                    "fmx_embedding_bwd launch");
 }
 
 size_t fmx_muon_workspace_bytes(const fmx_muon_matrix* matrices, int64_t count) {

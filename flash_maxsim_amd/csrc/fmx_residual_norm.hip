@@ -22,6 +22,7 @@
 // second kernel adds those rows in a fixed order. No atomics.
 #include "fmx_device.h"
 #include "fmx_layers.h"
+#include "fmx_rows.h"
 
 #include "../../include/fmx.h"
 
@@ -52,37 +53,6 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int wav
     }
   }
 }
-
-// V consecutive elements of type T as they lie in memory.
-template <typename T, int V>
-struct Piece {
-  T v[V];
-  // `left` of them are there, the others are zeros
-  template <bool WHOLE>
-  __device__ __forceinline__ void load(const T* p, int left) {
-    if (WHOLE ? left > 0 : left >= V) {
-      __builtin_memcpy(v, p, sizeof(v));
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = T(0.0f);
-      if constexpr (!WHOLE) {
-#pragma unroll
-        for (int i = 0; i < V - 1; ++i)
-          if (i < left) v[i] = p[i];
-      }
-    }
-  }
-  template <bool WHOLE>
-  __device__ __forceinline__ void store(T* p, int left) const {
-    if (WHOLE ? left > 0 : left >= V) {
-      __builtin_memcpy(p, v, sizeof(v));
-    } else if constexpr (!WHOLE) {
-#pragma unroll
-      for (int i = 0; i < V - 1; ++i)
-        if (i < left) p[i] = v[i];
-    }
-  }
-};
 
 // Where a lane's elements lie: piece j of V elements at column ((j * NW + sub) * 64 + lane) * V, sub the wave's place
 // among the NW of its row. WHOLE: d is a multiple of V, no piece ends early.

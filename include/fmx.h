@@ -525,6 +525,31 @@ int fmx_residual_norm_bwd(int dtype, const void* x, int64_t x_stride, const void
 size_t fmx_residual_norm_bwd_workspace_bytes(int64_t M, int64_t d);
 
 /*
+ * Embedding lookup: y[t] = scale w[ids[t]], rounded once.
+ *
+ *   ids  [T]     int64 or int32 (ids_bits); ids outside 0 .. V - 1 give rows of NaN
+ *   w    [V, d]  dtype (F16, BF16 or F32), row stride w_stride
+ *   y    [T, d]  dtype, contiguous
+ * T <= FMX_EMBEDDING_MAX_TOKENS, V <= FMX_EMBEDDING_MAX_ROWS, 1 <= d <= FMX_MAX_D. Pointers are aligned to their elements.
+ */
+#define FMX_EMBEDDING_MAX_TOKENS (1 << 26)
+#define FMX_EMBEDDING_MAX_ROWS (1 << 28)
+
+int fmx_embedding(int dtype, const void* ids, int ids_bits, const void* w, int64_t w_stride, double scale, int64_t T, int64_t V,
+                  int64_t d, void* y, void* stream);
+
+/*
+ * Its gradient: dw[v] = scale (sum of dy[t] over the t with ids[t] = v) [V, d] in dtype, contiguous, sums in fp32 in a
+ * fixed order, all rows written. Ids outside 0 .. V - 1 and padding_id (-1: none) add nothing. dy [T, d] with
+ * row stride dy_stride. Workspace: fmx_embedding_bwd_workspace_bytes, 256-byte aligned.
+ */
+int fmx_embedding_bwd(int dtype, const void* ids, int ids_bits, const void* dy, int64_t dy_stride, double scale,
+                      int64_t padding_id, int64_t T, int64_t V, int64_t d, void* dw, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+size_t fmx_embedding_bwd_workspace_bytes(int dtype, int64_t T, int64_t V, int64_t d);
+
+/*
  * One tensor of an AdamW step; n elements, all arrays contiguous and aligned to
  * their elements. state_bits 32: exp_avg and exp_avg_sq are fp32 and the scales
  * unused. state_bits 8: exp_avg holds int8 codes c (moment c |c| scale),

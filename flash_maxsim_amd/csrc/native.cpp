@@ -13,7 +13,7 @@
 // step's host time depends more on where autograd's thread runs: 85 or 150 us
 // before, 105 after, for 32 x 32 tokens over 256 docs of up to 180.)
 //
-// The trained layers (linear, layer_norm) have their autograd nodes here as well,
+// The trained layers (linear, gated_linear, layer_norm, residual_norm, embedding) have their autograd nodes here as well,
 // so that a backward pass takes neither the GIL nor Python.
 //
 // The library is reached through its C ABI alone.
@@ -653,6 +653,21 @@ struct LayerNormBackward : public torch::autograd::Node {
   std::string name() const override { return "FlashMaxSimLayerNormBackward"; }
 };
 
+// An operand of a product as the kernels read it: itself, or a copy with its rows zero-padded to a multiple of 8.
+// Undefined where only the Python path makes one (*rc says whether a launch failed).
+Tensor product_operand(const Tensor& t, int64_t rows, int64_t K, int64_t* stride, int* rc) {
+  const int64_t K8 = (K + 7) / 8 * 8;
+  if (K == K8 && *stride >= K && (*stride & 7) == 0 && *stride < 1 << 22 &&
+      (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) == 0)
+    return t;
+  if (K8 >= 1 << 22 || rows > (INT32_MAX - 4096) / (K8 / 4)) return Tensor();
+  Tensor out = at::empty({rows, K8}, t.options());
+  const int dtype = code_of(t);
+  *rc = fmx_convert_rows(dtype, t.const_data_ptr(), 0, *stride, 1, rows, K, nullptr, dtype, out.data_ptr(), K8, stream_of(t));
+  *stride = K8;
+  return out;
+}
+
 // linear(x [..., K], w [N, K], bias [N] or None, activation, residual [..., N] or None): y [..., N]
 PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -664,7 +679,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   FMX_ORDINARY((type == at::kHalf || type == at::kBFloat16) && act >= FMX_ACT_NONE && act <= FMX_ACT_SILU);
   int64_t M, sx, sr = 0, Mr;
   FMX_ORDINARY(w->dim() == 2 && w->scalar_type() == type && w->device() == x->device() && as_rows(*x, &M, &sx));
-  const int64_t N = w->size(0), K = w->size(1), K8 = (K + 7) / 8 * 8;
+  const int64_t N = w->size(0), K = w->size(1);
   FMX_ORDINARY(N >= 1 && x->size(-1) == K && M > 0 && sx >= 0 && w->stride(0) >= 0 && (K == 1 || w->stride(1) == 1) &&
                is_vector(b, *x, type, N) && here(*x));
   auto sizes = x->sizes().vec();
@@ -674,28 +689,13 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   FMX_ORDINARY(!has_tangent(x) && !has_tangent(w) && !has_tangent(b) && !has_tangent(r));
   const int dtype = code_of(*x);
   void* s = stream_of(*x);
-  // An operand as the kernels read it: itself, or a copy with its rows zero-padded to a multiple of 8.
   int prc = 0;
-  bool fits = true;
-  auto operand = [&](const Tensor& t, int64_t rows, int64_t* stride) -> Tensor {
-    if (K == K8 && *stride >= K && (*stride & 7) == 0 && *stride < 1 << 22 &&
-        (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) == 0)
-      return t;
-    if (K8 >= 1 << 22 || rows > (INT32_MAX - 4096) / (K8 / 4)) {
-      fits = false;
-      return Tensor();
-    }
-    Tensor out = at::empty({rows, K8}, t.options());
-    prc = fmx_convert_rows(dtype, t.const_data_ptr(), 0, *stride, 1, rows, K, nullptr, dtype, out.data_ptr(), K8, s);
-    *stride = K8;
-    return out;
-  };
   int64_t sw = w->stride(0);
-  const Tensor xk = operand(*x, M, &sx);
+  const Tensor xk = product_operand(*x, M, K, &sx, &prc);
   if (prc) return failed(prc);
-  const Tensor wk = fits ? operand(*w, N, &sw) : Tensor();
+  const Tensor wk = xk.defined() ? product_operand(*w, N, K, &sw, &prc) : Tensor();
   if (prc) return failed(prc);
-  FMX_ORDINARY(fits);
+  FMX_ORDINARY(wk.defined());
   const bool grad = grad_wanted({x, w, b, r});
   Tensor y = at::empty(sizes, x->options());
   const bool sloped = act && grad_wanted({x, w, b});  // the residual's gradient needs none
@@ -767,6 +767,316 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     node->dtype = dtype;
     node->w_dtype = w_dtype;
     node->w_type = wt;
+    torch::autograd::set_history(y, node);
+  }
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+struct GatedLinearBackward : public torch::autograd::Node {
+  // x and the weights as the kernels read them; each is there where a wanted gradient needs it
+  torch::autograd::SavedVariable x, wg, wu, factors;
+  std::vector<int64_t> x_sizes;
+  int64_t M, N, K;
+  int dtype;
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    const Tensor dy0 = grads[0];
+    if (!dy0.defined()) return torch::autograd::variable_list(5);
+    const bool again = c10::GradMode::is_enabled();
+    Tensor keep, d[5];
+    {
+      at::AutoGradMode off(false);
+      const at::ScalarType type = dy0.scalar_type();
+      const int64_t K8 = (K + 7) / 8 * 8;
+      bool want[5], any = false;
+      for (int i = 0; i < 5; ++i) any |= want[i] = task_should_compute_output(i);
+      if (any) {
+        int64_t m, stride, sx = 0, sg = 0, su = 0;
+        const Tensor xk = want[1] || want[2] ? given_back(x, dy0, type, M, K8, &sx, true) : Tensor();
+        const Tensor gk = want[0] ? given_back(wg, dy0, type, N, K8, &sg, true) : Tensor();
+        const Tensor uk = want[0] ? given_back(wu, dy0, type, N, K8, &su, true) : Tensor();
+        const Tensor fk = given_back(factors, dy0, at::kShort, FMX_GATED_PLANES(dtype) * M, N);
+        const Tensor& dy = grad_rows(dy0, &keep, &m, &stride);
+        const auto options = dy.options();
+        if (want[0]) d[0] = at::empty(x_sizes, options);
+        for (int i = 1; i < 3; ++i)
+          if (want[i]) d[i] = at::empty({N, K}, options);
+        for (int i = 3; i < 5; ++i)
+          if (want[i]) d[i] = at::empty({N}, options);
+        const size_t n = fmx_gated_bwd_workspace_bytes(M, N, K);
+        const Tensor ws = scratch(n, dy);
+        must(fmx_gated_bwd(dtype, const_ptr(xk), sx, const_ptr(gk), sg, const_ptr(uk), su, dy.const_data_ptr(), stride,
+                           static_cast<const int16_t*>(const_ptr(fk)), M, N, K, ptr(d[0]), ptr(d[1]), ptr(d[2]), ptr(d[3]),
+                           ptr(d[4]), ptr(ws), n, stream_of(dy)));
+      }
+    }
+    torch::autograd::variable_list out{d[0], d[1], d[2], d[3], d[4]};
+    return again ? once(std::move(out)) : out;
+  }
+  void release_variables() override {
+    x.reset_data();
+    wg.reset_data();
+    wu.reset_data();
+    factors.reset_data();
+  }
+  std::string name() const override { return "FlashMaxSimGatedLinearBackward"; }
+};
+
+struct ResidualNormBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable rows[3], vectors[4], stats;  // x, residual, gate; weight, post weight, post bias, scale
+  bool has[7];
+  std::vector<int64_t> sizes;
+  int64_t M, d;
+  int dtype, w_dtype, post, rms;
+  double alpha;
+  at::ScalarType type, w_type;
+
+  // gradients of x, residual, gate, weight, bias, post weight, post bias, scale
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    const Tensor dh0 = grads[0], dy0 = grads[1];
+    if (!dh0.defined() && !dy0.defined()) return torch::autograd::variable_list(8);
+    const Tensor& like = dh0.defined() ? dh0 : dy0;
+    const bool again = c10::GradMode::is_enabled();
+    Tensor keep[2], out[8];
+    {
+      at::AutoGradMode off(false);
+      int64_t m, stride[3] = {0, 0, 0}, sdh = 0, sdy = 0;
+      Tensor r[3], v[4];
+      for (int i = 0; i < 3; ++i)
+        if (has[i]) r[i] = given_back(rows[i], like, type, M, d, &stride[i]);
+      for (int i = 0; i < 4; ++i)
+        if (has[3 + i]) v[i] = given_back(vectors[i], like, w_type, 1, d);
+      const Tensor st = given_back(stats, like, at::kFloat, M, 4);
+      const Tensor dh = dh0.defined() ? grad_rows(dh0, &keep[0], &m, &sdh) : Tensor();
+      const Tensor dy = dy0.defined() ? grad_rows(dy0, &keep[1], &m, &sdy) : Tensor();
+      const auto options = r[0].options();
+      bool any = false, sums = false;
+      for (int i = 0; i < 8; ++i) {
+        // weight and bias have no part in h
+        if (!task_should_compute_output(i) || ((i == 3 || i == 4) && !dy.defined())) continue;
+        out[i] = i < 3 ? at::empty(sizes, options) : at::empty({d}, options.dtype(w_type));
+        any = true;
+        sums |= i >= 3;
+      }
+      if (any) {
+        const size_t n = sums ? fmx_residual_norm_bwd_workspace_bytes(M, d) : 0;
+        const Tensor ws = scratch(n, r[0]);
+        must(fmx_residual_norm_bwd(dtype, r[0].const_data_ptr(), stride[0], r[1].const_data_ptr(), stride[1], const_ptr(r[2]),
+                                   stride[2], w_dtype, const_ptr(v[0]), post, const_ptr(v[1]), const_ptr(v[2]), const_ptr(v[3]),
+                                   alpha, rms, st.const_data_ptr<float>(), const_ptr(dh), sdh, const_ptr(dy), sdy, M, d,
+                                   ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(out[3]), ptr(out[4]), ptr(out[7]), ptr(out[5]),
+                                   ptr(out[6]), ptr(ws), n, stream_of(r[0])));
+      }
+    }
+    torch::autograd::variable_list list(out, out + 8);
+    return again ? once(std::move(list)) : list;
+  }
+  void release_variables() override {
+    for (auto& t : rows) t.reset_data();
+    for (auto& t : vectors) t.reset_data();
+    stats.reset_data();
+  }
+  std::string name() const override { return "FlashMaxSimResidualNormBackward"; }
+};
+
+struct EmbeddingBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable ids;
+  at::ScalarType ids_type;
+  int64_t T, V, d, padding;
+  int dtype;
+  double scale;
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    const Tensor dy0 = grads[0];
+    if (!dy0.defined() || !task_should_compute_output(0)) return torch::autograd::variable_list(1);
+    const bool again = c10::GradMode::is_enabled();
+    Tensor keep, dw;
+    {
+      at::AutoGradMode off(false);
+      int64_t m, stride;
+      Tensor t = ids.unpack();
+      TORCH_CHECK(t.defined() && t.device() == dy0.device() && t.scalar_type() == ids_type && t.numel() == T,
+                  "flash_maxsim_amd: a saved tensor came back with another shape, type or device");
+      t = t.resolve_neg().contiguous();
+      const Tensor& dy = grad_rows(dy0, &keep, &m, &stride);
+      dw = at::empty({V, d}, dy.options());
+      const size_t n = fmx_embedding_bwd_workspace_bytes(dtype, T, V, d);
+      const Tensor ws = scratch(n, dy);
+      must(fmx_embedding_bwd(dtype, t.const_data_ptr(), ids_type == at::kLong ? 64 : 32, dy.const_data_ptr(), stride, scale,
+                             padding, T, V, d, dw.data_ptr(), ptr(ws), n, stream_of(dy)));
+    }
+    return again ? once({dw}) : torch::autograd::variable_list{dw};
+  }
+  void release_variables() override { ids.reset_data(); }
+  std::string name() const override { return "FlashMaxSimEmbeddingBackward"; }
+};
+
+// gated_linear(x [..., K], wg [N, K], wu [N, K], bg [N] or None, bu [N] or None, activation): y [..., N]
+PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  FMX_ARGS(6);
+  const Tensor *x = plain(args[0]), *wg = plain(args[1]), *wu = plain(args[2]), *bg, *bu;
+  FMX_ORDINARY(x && wg && wu && take_optional(args[3], &bg) && take_optional(args[4], &bu) && PyLong_CheckExact(args[5]));
+  const long act = PyLong_AsLong(args[5]);
+  const at::ScalarType type = x->scalar_type();
+  FMX_ORDINARY((type == at::kHalf || type == at::kBFloat16) && act >= FMX_ACT_NONE && act <= FMX_ACT_SILU);
+  int64_t M, sx;
+  FMX_ORDINARY(wg->dim() == 2 && as_rows(*x, &M, &sx));
+  const int64_t N = wg->size(0), K = wg->size(1);
+  for (const Tensor* w : {wg, wu})
+    FMX_ORDINARY(w->scalar_type() == type && w->device() == x->device() && w->sizes() == wg->sizes() && w->stride(0) >= 0 &&
+                 (K == 1 || w->stride(1) == 1));
+  FMX_ORDINARY(N >= 1 && K >= 1 && x->size(-1) == K && M > 0 && sx >= 0 && is_vector(bg, *x, type, N) &&
+               is_vector(bu, *x, type, N) && here(*x));
+  FMX_ORDINARY(!has_tangent(x) && !has_tangent(wg) && !has_tangent(wu) && !has_tangent(bg) && !has_tangent(bu));
+  const int dtype = code_of(*x);
+  void* s = stream_of(*x);
+  int prc = 0;
+  int64_t sg = wg->stride(0), su = wu->stride(0);
+  const Tensor xk = product_operand(*x, M, K, &sx, &prc);
+  if (prc) return failed(prc);
+  const Tensor gk = xk.defined() ? product_operand(*wg, N, K, &sg, &prc) : Tensor();
+  if (prc) return failed(prc);
+  const Tensor uk = gk.defined() ? product_operand(*wu, N, K, &su, &prc) : Tensor();
+  if (prc) return failed(prc);
+  FMX_ORDINARY(uk.defined());
+  const bool grad = grad_wanted({x, wg, wu, bg, bu});
+  auto sizes = x->sizes().vec();
+  sizes.back() = N;
+  Tensor y = at::empty(sizes, x->options());
+  Tensor factors = grad ? at::empty({FMX_GATED_PLANES(dtype), M, N}, x->options().dtype(at::kShort)) : Tensor();
+  const size_t n = fmx_gated_workspace_bytes(M, N, K);
+  const Tensor ws = scratch(n, *x);
+  const int rc = unlocked([&] {
+    return fmx_gated(dtype, xk.const_data_ptr(), sx, gk.const_data_ptr(), sg, uk.const_data_ptr(), su,
+                     bg ? bg->const_data_ptr() : nullptr, bu ? bu->const_data_ptr() : nullptr, (int)act, M, N, K, y.data_ptr(),
+                     static_cast<int16_t*>(ptr(factors)), ptr(ws), n, s);
+  });
+  if (rc) return failed(rc);
+  if (grad) {
+    std::shared_ptr<GatedLinearBackward> node(new GatedLinearBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(*x, *wg, *wu, bg ? *bg : Tensor(), bu ? *bu : Tensor()));
+    if (wg->requires_grad() || wu->requires_grad()) node->x = torch::autograd::SavedVariable(xk, false);
+    if (x->requires_grad()) {
+      node->wg = torch::autograd::SavedVariable(gk, false);
+      node->wu = torch::autograd::SavedVariable(uk, false);
+    }
+    node->factors = torch::autograd::SavedVariable(factors, false);
+    node->x_sizes = x->sizes().vec();
+    node->M = M;
+    node->N = N;
+    node->K = K;
+    node->dtype = dtype;
+    torch::autograd::set_history(y, node);
+  }
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// residual_norm(x, residual, gate, weight, bias, post_weight, post_bias, scale, post, alpha, rms, eps): (h, y). Rows [..., d],
+// vectors [d]; all but x and residual may be None.
+PyObject* residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  FMX_ARGS(12);
+  const Tensor *r[3] = {plain(args[0]), plain(args[1]), nullptr}, *v[5];
+  FMX_ORDINARY(r[0] && r[1] && take_optional(args[2], &r[2]));
+  for (int i = 0; i < 5; ++i) FMX_ORDINARY(take_optional(args[3 + i], &v[i]));
+  FMX_ORDINARY(PyBool_Check(args[8]) && PyFloat_CheckExact(args[9]) && PyLong_CheckExact(args[10]) && PyFloat_CheckExact(args[11]));
+  const int post = args[8] == Py_True, rms = PyLong_AsLong(args[10]) != 0;
+  const double alpha = PyFloat_AS_DOUBLE(args[9]), eps = PyFloat_AS_DOUBLE(args[11]);
+  const Tensor& x = *r[0];
+  const int dtype = code_of(x);
+  const at::ScalarType type = x.scalar_type();
+  int64_t M, m, stride[3] = {0, 0, 0};
+  FMX_ORDINARY(dtype >= 0 && as_rows(x, &M, &stride[0]) && M > 0 && here(x) && (post || (!v[2] && !v[3])));
+  const int64_t d = x.size(-1);
+  for (int i = 0; i < 3; ++i)
+    FMX_ORDINARY(!r[i] || (r[i]->scalar_type() == type && r[i]->device() == x.device() && r[i]->sizes() == x.sizes() &&
+                           as_rows(*r[i], &m, &stride[i]) && stride[i] >= 0 && !has_tangent(r[i])));
+  at::ScalarType wt = type;
+  for (int i = 4; i >= 0; --i)
+    if (v[i]) wt = v[i]->scalar_type();
+  FMX_ORDINARY(wt == type || wt == at::kFloat);
+  for (const Tensor* t : v) FMX_ORDINARY(is_vector(t, x, wt, d) && !has_tangent(t));
+  const int w_dtype = wt == at::kFloat ? FMX_DTYPE_F32 : dtype;
+  const bool grad = grad_wanted({r[0], r[1], r[2], v[0], v[1], v[2], v[3], v[4]});
+  Tensor h = at::empty(x.sizes(), x.options()), y = at::empty(x.sizes(), x.options());
+  Tensor stats = grad ? at::empty({M, 4}, x.options().dtype(at::kFloat)) : Tensor();
+  auto data = [](const Tensor* t) -> const void* { return t ? t->const_data_ptr() : nullptr; };
+  void* s = stream_of(x);
+  const int rc = unlocked([&] {
+    return fmx_residual_norm(dtype, data(r[0]), stride[0], data(r[1]), stride[1], data(r[2]), stride[2], w_dtype, data(v[0]),
+                             data(v[1]), post, data(v[2]), data(v[3]), data(v[4]), alpha, rms, eps, M, d, h.data_ptr(),
+                             y.data_ptr(), static_cast<float*>(ptr(stats)), s);
+  });
+  if (rc) return failed(rc);
+  if (grad) {
+    std::shared_ptr<ResidualNormBackward> node(new ResidualNormBackward(), torch::autograd::deleteNode);
+    auto some = [](const Tensor* t) { return t ? *t : Tensor(); };
+    node->set_next_edges(torch::autograd::collect_next_edges(*r[0], *r[1], some(r[2]), some(v[0]), some(v[1]), some(v[2]),
+                                                             some(v[3]), some(v[4])));
+    for (int i = 0; i < 3; ++i) {
+      node->has[i] = r[i] != nullptr;
+      if (r[i]) node->rows[i] = torch::autograd::SavedVariable(*r[i], false);
+    }
+    const Tensor* kept[4] = {v[0], v[2], v[3], v[4]};
+    for (int i = 0; i < 4; ++i) {
+      node->has[3 + i] = kept[i] != nullptr;
+      if (kept[i]) node->vectors[i] = torch::autograd::SavedVariable(*kept[i], false);
+    }
+    node->stats = torch::autograd::SavedVariable(stats, false);
+    node->sizes = x.sizes().vec();
+    node->M = M;
+    node->d = d;
+    node->dtype = dtype;
+    node->w_dtype = w_dtype;
+    node->post = post;
+    node->rms = rms;
+    node->alpha = alpha;
+    node->type = type;
+    node->w_type = wt;
+    torch::autograd::set_history(h, node);
+    torch::autograd::set_history(y, node);
+  }
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(h)), THPVariable_Wrap(std::move(y)));
+  END_HANDLE_TH_ERRORS
+}
+
+// embedding(ids [...], weight [V, d], scale, padding): y [..., d]
+PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  FMX_ARGS(4);
+  const Tensor *t = plain(args[0]), *w = plain(args[1]);
+  FMX_ORDINARY(t && w && PyFloat_CheckExact(args[2]) && PyLong_CheckExact(args[3]));
+  const int dtype = code_of(*w);
+  const double scale = PyFloat_AS_DOUBLE(args[2]);
+  const int64_t padding = PyLong_AsLongLong(args[3]), T = t->numel();
+  FMX_ORDINARY(dtype >= 0 && (t->scalar_type() == at::kLong || t->scalar_type() == at::kInt) && T > 0 && t->is_contiguous() &&
+               w->dim() == 2 && w->size(0) >= 1 && w->size(1) >= 1 && (w->size(1) == 1 || w->stride(1) == 1) &&
+               w->stride(0) >= 0 && t->device() == w->device() && here(*w) && !has_tangent(w));
+  const int64_t V = w->size(0), d = w->size(1);
+  const bool grad = grad_wanted({w});
+  auto sizes = t->sizes().vec();
+  sizes.push_back(d);
+  Tensor y = at::empty(sizes, w->options());
+  void* s = stream_of(*w);
+  const int rc = unlocked([&] {
+    return fmx_embedding(dtype, t->const_data_ptr(), t->scalar_type() == at::kLong ? 64 : 32, w->const_data_ptr(), w->stride(0),
+                         scale, T, V, d, y.data_ptr(), s);
+  });
+  if (rc) return failed(rc);
+  if (grad) {
+    std::shared_ptr<EmbeddingBackward> node(new EmbeddingBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(*w));
+    node->ids = torch::autograd::SavedVariable(*t, false);
+    node->ids_type = t->scalar_type();
+    node->T = T;
+    node->V = V;
+    node->d = d;
+    node->padding = padding;
+    node->dtype = dtype;
+    node->scale = scale;
     torch::autograd::set_history(y, node);
   }
   return THPVariable_Wrap(std::move(y));
@@ -879,7 +1189,8 @@ PyMethodDef methods[] = {FMX_METHOD(score),   FMX_METHOD(batched), FMX_METHOD(sp
                          FMX_METHOD(topk),    FMX_METHOD(int8),    FMX_METHOD(packed),
                          FMX_METHOD(int8_packed), FMX_METHOD(forward), FMX_METHOD(backward),
                          FMX_METHOD(linear),  FMX_METHOD(layer_norm), FMX_METHOD(adamw),
-                         FMX_METHOD(adamw_decode),
+                         FMX_METHOD(adamw_decode), FMX_METHOD(gated_linear), FMX_METHOD(residual_norm),
+                         FMX_METHOD(embedding),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

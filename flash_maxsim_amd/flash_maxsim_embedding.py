@@ -88,6 +88,10 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
     rows of NaN (a launch cannot raise) and no gradient. Differentiable in
     weight, with a dense gradient; tokens of padding_idx add nothing to it.
     """
+    if padding_idx is None and math.isfinite(scale):
+        out = _lib.native().embedding(ids, weight, float(scale), -1)
+        if out is not None:
+            return out
     _check(ids, weight, scale, padding_idx)
     scale, padding = float(scale), -1 if padding_idx is None else int(padding_idx)
     if _differentiated(weight):

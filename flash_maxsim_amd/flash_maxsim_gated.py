@@ -114,6 +114,9 @@ def gated_linear(x: torch.Tensor, weight_gate: torch.Tensor, weight_up: torch.Te
     "gelu" (by the normal distribution function), "gelu_tanh" (its tanh form) or
     "silu". Differentiable in x, the weights and the biases.
     """
+    out = _lib.native().gated_linear(x, weight_gate, weight_up, bias_gate, bias_up, ACTIVATIONS.get(activation, -1))
+    if out is not None:
+        return out
     _check(x, weight_gate, weight_up, bias_gate, bias_up, activation)
     act = ACTIVATIONS[activation]
     if _differentiated(x, weight_gate, weight_up, bias_gate, bias_up):

@@ -137,6 +137,10 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor 
     have x's shape and type; differentiable in all tensors.
     """
     vectors = weight, bias, post_weight, post_bias, scale
+    if norm in NORMS and math.isfinite(residual_scale):
+        out = _lib.native().residual_norm(x, residual, gate, *vectors, post_norm, float(residual_scale), NORMS[norm], eps)
+        if out is not None:
+            return out
     _check(x, residual, gate, vectors, norm, post_norm, post_weight, post_bias, residual_scale)
     args = (x, residual, gate, *vectors, bool(post_norm), float(residual_scale), NORMS[norm], float(eps))
     if _differentiated(x, residual, gate, *vectors):

@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kStretch = 32;         // sorted tokens that a wave sums
 constexpr int64_t kRankMost = 16384;
+constexpr int kRows = 32;            // ids of a workgroup that writes zeros
 constexpr int kBits = 10;            // of a digit, at most
 constexpr int kTile = 4096;          // tokens of a workgroup of the radix sort
 
@@ -33,49 +34,77 @@ __device__ __forceinline__ int32_t key_of(const EmbeddingArgs& a, int64_t t) {
 
 // ---- lookup ----
 
+// U rows of a thread at a time: their ids, then their rows, then the stores, each in flight together.
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(256) embedding_kernel(EmbeddingArgs a, int lanes) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), U = 4;
   const int lane = threadIdx.x & (lanes - 1), rows = 256 / lanes;
-  for (int64_t t = (int64_t)blockIdx.x * rows + threadIdx.x / lanes; t < a.T; t += (int64_t)gridDim.x * rows) {
-    const int64_t id = a.ids64 ? static_cast<const int64_t*>(a.ids)[t] : (int64_t)static_cast<const int32_t*>(a.ids)[t];
-    const bool there = id >= 0 && id < a.V;
-    const T* w = static_cast<const T*>(a.w) + (there ? id : 0) * a.sw;
-    T* y = static_cast<T*>(a.out) + t * a.d;
-    for (int col = lane * V; col < a.d; col += lanes * V) {
-      Piece<T, V> p;
-      p.template load<WHOLE>(w + col, a.d - col);
+  const int64_t step = (int64_t)gridDim.x * rows;
+  for (int64_t t = (int64_t)blockIdx.x * rows + threadIdx.x / lanes; t < a.T; t += U * step) {
+    int64_t id[U];
 #pragma unroll
-      for (int i = 0; i < V; ++i) p.v[i] = (T)(there ? (float)p.v[i] * a.scale : __builtin_nanf(""));
-      p.template store<WHOLE>(y + col, a.d - col);
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = t + u * step < a.T ? t + u * step : t;
+      id[u] = a.ids64 ? static_cast<const int64_t*>(a.ids)[at] : (int64_t)static_cast<const int32_t*>(a.ids)[at];
+    }
+    for (int col = lane * V; col < a.d; col += lanes * V) {
+      Piece<T, V> p[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        p[u].template load<WHOLE>(static_cast<const T*>(a.w) + (id[u] >= 0 && id[u] < a.V ? id[u] : 0) * a.sw + col, a.d - col);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool there = id[u] >= 0 && id[u] < a.V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) p[u].v[i] = (T)(there ? (float)p[u].v[i] * a.scale : __builtin_nanf(""));
+        if (t + u * step < a.T) p[u].template store<WHOLE>(static_cast<T*>(a.out) + (t + u * step) * a.d + col, a.d - col);
+      }
     }
   }
 }
 
 // ---- sorting ----
 
-// Each token's place: how many come before it. A workgroup ranks 64 tokens, each of its 16 waves against a sixteenth.
+// Each token's place: how many come before it. A workgroup ranks 16 tokens; keys go through LDS, 4096 at a time. A wave
+// compares its tokens (lane & 15) with 16 keys at a time, 4 for each group of 16 lanes; those before the workgroup's
+// own 16 count where they are equal, too.
+constexpr int kRankTile = 4096;
 __global__ void __launch_bounds__(1024) embedding_rank_kernel(EmbeddingArgs a) {
+  typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
+  __shared__ __attribute__((aligned(16))) int32_t keys[kRankTile];
   __shared__ int counts[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int T = (int)a.T, t = blockIdx.x * 64 + lane;
-  const int32_t mine = t < T ? key_of(a, t) : 0;
-  const int per = (T + 15) / 16, from = wave * per, end = from + per < T ? from + per : T;
+  const int lane = threadIdx.x & 63, group = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int T = (int)a.T, t0 = blockIdx.x * 16, t = t0 + (lane & 15);
+  const int32_t mine = key_of(a, t < T ? t : T - 1);
   int before = 0;
-  for (int base = from; base < end; base += 64) {
-    const int32_t theirs = base + lane < end ? key_of(a, base + lane) : 0;
-    const int n = end - base < 64 ? end - base : 64;
-    for (int k = 0; k < n; ++k) {
-      const int32_t other = __builtin_amdgcn_readlane(theirs, k);
-      before += other < mine || (other == mine && base + k < t) ? 1 : 0;
+  for (int base = 0; base < T; base += kRankTile) {
+    __syncthreads();
+#pragma unroll
+    for (int k = threadIdx.x; k < kRankTile; k += 1024) keys[k] = base + k < T ? key_of(a, base + k) : INT32_MAX;
+    __syncthreads();
+    const int end = T - base < kRankTile ? T - base : kRankTile;
+    for (int k = wave * 16; k < end; k += 256) {
+      const i32x4_t other = *reinterpret_cast<const i32x4_t*>(keys + k + 4 * group);
+      const int at = base + k;  // uniform
+      if (at == t0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) before += other[i] < mine || (other[i] == mine && at + 4 * group + i < t) ? 1 : 0;
+      } else {
+        const int32_t bound = at < t0 ? mine + 1 : mine;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) before += other[i] < bound ? 1 : 0;
+      }
     }
   }
   counts[wave][lane] = before;
   __syncthreads();
-  if (wave == 0 && t < T) {
+  if (threadIdx.x < 16 && t < T) {
     int place = 0;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) place += counts[w][lane];
+    for (int w = 0; w < 16; ++w)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) place += counts[w][g * 16 + threadIdx.x];
     a.keys[place] = mine;
     a.order[place] = t;
   }
@@ -174,7 +203,8 @@ __global__ void __launch_bounds__(1024) embedding_place_kernel(EmbeddingArgs a, 
 // ---- sums ----
 
 // Workgroups before `sums` add up stretches, a wave a stretch of one block of 64 pieces of columns; the others write
-// the rows of ids that do not occur, 256 ids each.
+// the rows of ids that do not occur, kRows ids each: few, so that the workgroups at work write one stretch of memory
+// between them (131072 ids of 2 KB, hardly one of them there: 256 ids a workgroup 159 us, 32 RATE us).
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(256) embedding_sum_kernel(EmbeddingArgs a, uint32_t sums, int blocks) {
   constexpr int V = 16 / sizeof(T);
@@ -182,19 +212,21 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(EmbeddingArgs a, uin
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   T* out = static_cast<T*>(a.out);
   if (blockIdx.x >= sums) {
-    __shared__ uint8_t absent[256];
-    const int64_t v0 = (int64_t)(blockIdx.x - sums) * 256, v = v0 + threadIdx.x;
-    int64_t lo = 0, hi = a.T;  // the first token whose key is v or more
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (a.keys[mid] < v) lo = mid + 1; else hi = mid;
+    __shared__ uint8_t absent[kRows];
+    const int64_t v0 = (int64_t)(blockIdx.x - sums) * kRows, v = v0 + threadIdx.x;
+    if (threadIdx.x < kRows) {
+      int64_t lo = 0, hi = a.T;  // the first token whose key is v or more
+      while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (a.keys[mid] < v) lo = mid + 1; else hi = mid;
+      }
+      absent[threadIdx.x] = v < a.V && (lo == a.T || a.keys[lo] != v);
     }
-    absent[threadIdx.x] = v < a.V && (lo == a.T || a.keys[lo] != v);
     __syncthreads();
     Piece<T, V> zero;
 #pragma unroll
     for (int i = 0; i < V; ++i) zero.v[i] = T(0.0f);
-    for (int r = wave; r < 256; r += 4) {
+    for (int r = wave; r < kRows; r += 4) {
       if (!absent[r]) continue;
       for (int col = lane * V; col < a.d; col += 64 * V) zero.template store<WHOLE>(out + (v0 + r) * a.d + col, a.d - col);
     }
@@ -251,43 +283,69 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(EmbeddingArgs a, uin
   }
 }
 
-// Ids that go past a stretch's end: a workgroup for each stretch that such an id begins in (the others leave), and
-// 256 columns; the waves add every sixteenth partial sum, and then the waves' sums.
+// Ids that go past a stretch's end: a wave for each stretch that such an id may begin in, and 256 columns, adds the id's
+// partial sums. Those of more than kLong the sixteen waves of a workgroup add together, every sixteenth each, and then
+// the waves' sums.
+constexpr int kLong = 24;
 template <typename T>
 __global__ void __launch_bounds__(1024) embedding_join_kernel(EmbeddingArgs a, int pitch) {
   __shared__ __attribute__((aligned(16))) f32x4_t sums[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t stretch = blockIdx.x, end = (stretch + 1) * kStretch;
-  if (end >= a.T) return;
-  const int32_t key = a.keys[end - 1];
-  if (key >= a.V || a.keys[end] != key) return;
-  if (a.keys[stretch * kStretch] == key && stretch > 0 && a.keys[stretch * kStretch - 1] == key) return;  // began before
-  // the stretches after this one that begin with the id
-  int64_t more = 0;
-  for (;;) {
-    const int64_t at = (stretch + 1 + more + lane) * kStretch;
-    const uint64_t same = __ballot(at < a.T && a.keys[at < a.T ? at : 0] == key);
-    const int n = same == ~(uint64_t)0 ? 64 : __builtin_ctzll(~same);
-    more += n;
-    if (n < 64) break;
-  }
+  __shared__ int64_t longs[16];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t stretch = (int64_t)blockIdx.x * 16 + wave, end = (stretch + 1) * kStretch;
   const int col = blockIdx.y * 256 + lane * 4;
-  f32x4_t s = {0.f, 0.f, 0.f, 0.f};
-  if (col < pitch) {
-    const float* part = a.part + col;
-#pragma unroll 4
-    for (int64_t q = wave; q <= more; q += 16)
-      s += *reinterpret_cast<const f32x4_t*>(part + ((stretch + q) * 2 + (q == 0 ? 1 : 0)) * pitch);
+  // the stretches after this one that begin with the id that goes on from it; 0: none begins here and goes on
+  int64_t more = 0;
+  int32_t key = 0;
+  if (end < a.T) {
+    const int32_t first = a.keys[stretch * kStretch], last = stretch > 0 ? a.keys[stretch * kStretch - 1] : -1,
+                  next = a.keys[end];
+    key = a.keys[end - 1];
+    if (key < a.V && next == key && !(first == key && last == key)) {
+      for (;;) {
+        const int64_t at = (stretch + 1 + more + lane) * kStretch;
+        const uint64_t same = __ballot(at < a.T && a.keys[at < a.T ? at : 0] == key);
+        const int n = same == ~(uint64_t)0 ? 64 : __builtin_ctzll(~same);
+        more += n;
+        if (n < 64) break;
+      }
+    }
   }
-  sums[wave][lane] = s;
+  // every `step`-th partial sum of an id that begins in stretch `at`, from number q on
+  auto add = [&](int64_t at, int64_t q, int64_t more, int step) {
+    f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+    if (col < pitch) {
+      const float* part = a.part + col;
+#pragma unroll 4
+      for (; q <= more; q += step)
+        s += *reinterpret_cast<const f32x4_t*>(part + ((at + q) * 2 + (q == 0 ? 1 : 0)) * pitch);
+    }
+    return s;
+  };
+  auto write = [&](int32_t key, const f32x4_t& s) {
+    T* out = static_cast<T*>(a.out) + (int64_t)key * a.d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col + i < a.d) out[col + i] = (T)(s[i] * a.scale);
+  };
+  if (more > 0 && more <= kLong) write(key, add(stretch, 0, more, 1));
+  if (lane == 0) longs[wave] = more > kLong ? more : 0;
   __syncthreads();
-  if (wave > 0) return;
+  for (int k = 0; k < 16; ++k) {
+    const int64_t n = longs[k];
+    if (n == 0) continue;
+    const int64_t at = (int64_t)blockIdx.x * 16 + k;
+    f32x4_t s = add(at, wave, n, 16);
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0) {
 #pragma unroll
-  for (int w = 1; w < 16; ++w) s += sums[w][lane];
-  T* out = static_cast<T*>(a.out) + (int64_t)key * a.d;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (col + i < a.d) out[col + i] = (T)(s[i] * a.scale);
+      for (int w = 1; w < 16; ++w) s += sums[w][lane];
+      write(a.keys[at * kStretch + kStretch - 1], s);
+    }
+    __syncthreads();
+  }
 }
 
 template <typename T>
@@ -354,20 +412,20 @@ hipError_t gradient(int kind, EmbeddingArgs a, char* ws, hipStream_t s) {
       shift += b;
     }
   } else if (a.T > 0) {
-    embedding_rank_kernel<<<(unsigned)((a.T + 63) / 64), 1024, 0, s>>>(a);
+    embedding_rank_kernel<<<(unsigned)((a.T + 15) / 16), 1024, 0, s>>>(a);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   a.part = reinterpret_cast<float*>(ws + l.total - l.part);
   const int blocks = (int)((a.d + 64 * V - 1) / (64 * V));
-  const uint32_t sums = (uint32_t)((stretches_of(a.T) * blocks + 3) / 4), rows = (uint32_t)((a.V + 255) / 256);
+  const uint32_t sums = (uint32_t)((stretches_of(a.T) * blocks + 3) / 4), rows = (uint32_t)((a.V + kRows - 1) / kRows);
   if (a.d % V == 0)
     embedding_sum_kernel<T, true><<<sums + rows, 256, 0, s>>>(a, sums, blocks);
   else
     embedding_sum_kernel<T, false><<<sums + rows, 256, 0, s>>>(a, sums, blocks);
   e = hipGetLastError();
   if (e != hipSuccess || a.T <= kStretch) return e;
-  embedding_join_kernel<T><<<dim3((unsigned)(stretches_of(a.T) - 1), (unsigned)((a.d + 255) / 256)), 1024, 0, s>>>(
+  embedding_join_kernel<T><<<dim3((unsigned)((stretches_of(a.T) + 14) / 16), (unsigned)((a.d + 255) / 256)), 1024, 0, s>>>(
       a, blocks * 64 * V);
   return hipGetLastError();
 }

@@ -138,8 +138,10 @@ int check_muon(int dtype, int grad_dtype, const fmx_muon_matrix* matrices, int64
                double c, double eps, bool step, bool* copies) {
   if (count < 0) return fail(FMX_ERR_INVALID, "invalid count=%lld", (long long)count);
   if (steps < 1 || steps > 100) return fail(FMX_ERR_INVALID, "steps=%d must be in 1 .. 100", steps);
-  if (!(eps > 0) || !isfinite(eps) || !isfinite(a) || !isfinite(b) || !isfinite(c))
-    return fail(FMX_ERR_INVALID, "eps must be > 0 and finite, the coefficients finite");
+  if (!(eps > 0) || !isfinite(eps)) return fail(FMX_ERR_INVALID, "eps must be > 0 and finite");
+  if (!(fabs(a) <= FMX_MUON_MAX_COEFFICIENT) || !(fabs(b) <= FMX_MUON_MAX_COEFFICIENT) ||
+      !(fabs(c) <= FMX_MUON_MAX_COEFFICIENT))
+    return fail(FMX_ERR_INVALID, "coefficients must be within +-%d", FMX_MUON_MAX_COEFFICIENT);
   if (count > 0 && !matrices) return fail(FMX_ERR_INVALID, "matrices must be non-null");
   for (int64_t i = 0; i < count; ++i) {
     const fmx_muon_matrix& x = matrices[i];

@@ -1,19 +1,23 @@
 // Orthogonalised updates (as the Muon optimiser makes them), many matrices in one launch.
 //
 //   m = mu m + (1 - mu) g,   u = (1 - mu) g + mu m  (or m),   X = u / |u|_F, its shorter side first
-//   steps times:  A = X X^T,  B = b A + c A^2,  X = a X + B X
+//   steps times:  A = X X^T,  B = a I + b A + c A^2,  X = B X
 //   p = p (1 - lr decay) - rate X
 //
 // Every singular value s of X goes to a s + b s^3 + c s^5, towards 1 from anywhere; a is large, so that small
 // ones grow quickly: five steps with a = 3.44 multiply them by up to 485, and with them whatever error lies in
 // their directions. Products run on fp16 MFMA with float32 sums. Where an error comes in, and what it costs
-// (relative distance of the result from 64 bits, matrices from Gaussian to eight singular values over nothing):
-//   X rounded to fp16        1.4e-3 to 4e-2: its rounding lies in all directions and grows 485-fold with them
+// (relative distance of the result from 64 bits; matrices of falling, flat and few singular values):
+//   X rounded to fp16        1.2e-3 to 4e-2: its rounding lies in all directions and grows 485-fold with them
 //   (bf16 for everything     1e-2 to 3e-1)
-//   X as a pair of fp16      2e-4 to 2e-3: the linear term a X takes both, the products only the upper half. What
-//                            the lower half would add there is B times it, and B is small but where X is large
-// so X lies in memory as two fp16 arrays, of which the lower one is read and written by the epilogue alone: no
-// product more. X is held times 2^8, A and B times 2^10: their small elements stay clear of fp16's subnormal ones.
+//   X as a pair of fp16      2e-4 to 3.5e-3: the linear term a X takes both, the products only the upper half. What
+//                            the lower half would add there is (B - a I) times it, which is small but where X is large
+//   a I within B             4e-4 to 2.3e-3: the upper half's linear term is part of its product, exact but for the
+//                            rounding of B's diagonal, which scales rows and does not grow
+// so X lies in memory as two fp16 arrays, of which the lower one is read and written by the epilogue alone (X = B X_upper +
+// a X_lower): no product more. The last form saves the epilogue X's upper half (24 matrices of 1024 x 4096: 302 us a
+// launch, 364 with it read; B's diagonal's rest as a product of its own in the loop 448). X is held times
+// 2^8, A and B times 2^10: their small elements stay clear of fp16's subnormal ones.
 //
 // A and B are symmetric: tiles on and below the diagonal are computed, and a tile that lies below leaves LDS
 // twice, the second time through transposing reads. Matrices taller than wide are transposed when X is made, and the
@@ -362,12 +366,23 @@ __global__ void __launch_bounds__(WI* WJ * 64) muon_kernel(Table t, int copy_bf)
   const int64_t iw = i0 + wi * FI * 16, jw = j0 + wj * FJ * 16;
   if (jw >= width) return;  // sides are multiples of 64 and a wave's block begins at one of FJ * 16
 
+  // 16-bit rows of the block in LDS, 16 bytes at a time, and from there to memory as whole lines
+  auto spot = [&](int r, int ch) __attribute__((always_inline)) { return mine + r * ROW + ((ch ^ (r & (ROW / 16 - 1))) << 4); };
+  auto put = [&](int x, int ch, const u32x4_t& w) __attribute__((always_inline)) {
+    *reinterpret_cast<u32x4_t*>(spot(x * 16 + c, ch)) = w;
+  };
+  auto flush = [&](int x, uint16_t* out) __attribute__((always_inline)) {
+    constexpr int CH = ROW / 16;  // of a row
+#pragma unroll
+    for (int h = 0; h < 16 * CH / 64; ++h) {
+      const int r = x * 16 + h * (64 / CH) + lane / CH, ch = lane % CH;
+      store_raw(out, (iw + r) * width + jw + ch * 8, 8, *reinterpret_cast<const u32x4_t*>(spot(r, ch)));
+    }
+  };
+
   if constexpr (SYM) {
     uint16_t* out = FORM == kGram ? a_of(t, e) : b_of(t, e);
     const uint16_t* in = a_of(t, e);
-    auto spot = [&](int r, int ch) __attribute__((always_inline)) {  // of 16 bytes
-      return mine + r * ROW + ((ch ^ (r & (ROW / 16 - 1))) << 4);
-    };
 #pragma unroll
     for (int x = 0; x < FI; ++x) {
       if (iw + x * 16 >= e.n) break;
@@ -384,11 +399,13 @@ __global__ void __launch_bounds__(WI* WJ * 64) muon_kernel(Table t, int copy_bf)
           load16(w, in, at, 8, false);
 #pragma unroll
           for (int k = 0; k < 8; ++k) v[k] = t.b * w[k] + (t.c / kA) * v[k];
+          const int64_t off = iw + x * 16 + c - (jw + y * 16 + of);  // of the diagonal among the 8
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] += k == off ? t.a * kA : 0.0f;
         }
-        const u32x4_t h = pack8(v, false);
-        store_raw(out, at, 8, h);
-        *reinterpret_cast<u32x4_t*>(spot(x * 16 + c, y * 2 + of / 8)) = h;
+        put(x, y * 2 + of / 8, pack8(v, false));
       }
+      flush(x, out);
     }
     if (row == col) return;  // the whole tile is there
     // column j of the block: its 8 rows i .. i + 7 a lane, read as two 4 x 16 blocks turned round
@@ -407,29 +424,36 @@ __global__ void __launch_bounds__(WI* WJ * 64) muon_kernel(Table t, int copy_bf)
       }
     }
   } else {
-    const uint16_t* xh = x_of(t, e, t.from);
     uint16_t* xl = low_of(t, e);
     const bool tall = e.rows > e.cols;
     float* turn = reinterpret_cast<float*>(mine);  // kLast of a tall parameter: [FJ * 16][17], a 16-row block turned round
+    // everything that is read, before the first store: loads behind stores would wait for them
+    u32x4_t low[FI][FJ / 2];
 #pragma unroll
     for (int x = 0; x < FI; ++x) {
       if (iw + x * 16 >= e.n) break;
 #pragma unroll
+      for (int y = 0; y < FJ; y += 2) low[x][y / 2] = load_raw(xl, (iw + x * 16 + c) * e.m + jw + y * 16 + of, 8);
+    }
+#pragma unroll
+    for (int x = 0; x < FI; ++x) {
+      if (iw + x * 16 >= e.n) break;
+      u32x4_t down[FJ / 2];
+#pragma unroll
       for (int y = 0; y < FJ; y += 2) {
         float v[8], hi[8], lo[8];
         pair(x, y, v);
-        const int64_t i = iw + x * 16 + c, j = jw + y * 16 + of, at = i * e.m + j;
-        load16(hi, xh, at, 8, false);
-        load16(lo, xl, at, 8, false);
+        const int64_t i = iw + x * 16 + c, j = jw + y * 16 + of;
+        unpack8(lo, low[x][y / 2], false);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = t.a * (hi[k] + lo[k]) + v[k] * (1.0f / kA);
+        for (int k = 0; k < 8; ++k) v[k] = t.a * lo[k] + v[k] * (1.0f / kA);
         if constexpr (FORM == kNext) {
           const u32x4_t h = pack8(v, false);
           unpack8(hi, h, false);
 #pragma unroll
           for (int k = 0; k < 8; ++k) v[k] -= hi[k];
-          store_raw(x_of(t, e, t.from ^ 1), at, 8, h);
-          store_raw(xl, at, 8, pack8(v, false));
+          put(x, y * 2 + of / 8, h);
+          down[y / 2] = pack8(v, false);
         } else {
 #pragma unroll
           for (int k = 0; k < 8; ++k) v[k] *= 1.0f / kX;
@@ -441,6 +465,12 @@ __global__ void __launch_bounds__(WI* WJ * 64) muon_kernel(Table t, int copy_bf)
             for (int k = 0; k < 8; ++k) turn[(y * 16 + of + k) * 17 + c] = v[k];
           }
         }
+      }
+      if constexpr (FORM == kNext) {
+        flush(x, x_of(t, e, t.from ^ 1));
+#pragma unroll
+        for (int y = 0; y < FJ; y += 2) put(x, y * 2 + of / 8, down[y / 2]);
+        flush(x, xl);
       }
       if constexpr (FORM == kLast) {
         if (tall) {
@@ -557,9 +587,10 @@ Entry entry(const MuonMatrix& x) {
   return e;
 }
 
-// Matrices worked on together: until their X's tiles of 128 are this many, which keeps the compute units busy, or the
-// table is full. More would only need more workspace (and leave the last-level cache).
-constexpr int64_t kEnough = 2048;
+// Matrices worked on together: until their X's tiles of 128 are this many, or the table is full. (25 matrices of
+// 1024 x 4096 in groups of 1024 tiles 4.1 ms, of 2048 3.3, all at once 3.1: a launch of more tiles has less of a last
+// round.)
+constexpr int64_t kEnough = 16384;
 
 // Calls f(first, end) for each group of matrices.
 template <class F>

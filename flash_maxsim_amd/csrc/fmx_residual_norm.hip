@@ -236,45 +236,51 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) total[s][j][i] = 0.0f;
-  typename C::Row x, r, g, dh, dy, nx, nr, ng, ndh, ndy;
-  f32x4_t st, nst;
-  int64_t row = (int64_t)blockIdx.x * NG + wave / NW;
-  auto load = [&](typename C::Row& x, typename C::Row& r, typename C::Row& g, typename C::Row& dh, typename C::Row& dy,
-                  f32x4_t& st, int64_t at) __attribute__((always_inline)) {
-    const bool have = at < a.M;
-    c.load(x, a.x, at * a.sx, have);
-    c.load(r, a.r, at * a.sr, have);
-    if (a.gate) c.load(g, a.gate, at * a.sg, have);
-    if (a.dh) c.load(dh, a.dh, at * a.sdh, have);
-    if (a.dy) c.load(dy, a.dy, at * a.sdy, have);
-    st = have ? reinterpret_cast<const f32x4_t*>(a.stats)[at] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+  struct Rows {
+    typename C::Row x, r, g, dh, dy;
+    f32x4_t st;
   };
-  load(x, r, g, dh, dy, st, row);
+  auto load = [&](Rows& o, int64_t at) __attribute__((always_inline)) {
+    const bool have = at < a.M;
+    c.load(o.x, a.x, at * a.sx, have);
+    c.load(o.r, a.r, at * a.sr, have);
+    if (a.gate) c.load(o.g, a.gate, at * a.sg, have);
+    if (a.dh) c.load(o.dh, a.dh, at * a.sdh, have);
+    if (a.dy) c.load(o.dy, a.dy, at * a.sdy, have);
+    o.st = have ? reinterpret_cast<const f32x4_t*>(a.stats)[at] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+  };
+  // AHEAD rows are loaded while this one is summed
+  constexpr int AHEAD = NV == 1 ? 2 : 1;
+  Rows rows[AHEAD + 1];
+  int64_t row = (int64_t)blockIdx.x * NG + wave / NW;
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) load(rows[i], row + i * step);
   int par = 0;
   for (int64_t base = (int64_t)blockIdx.x * NG; base < a.M; base += step, row += step) {
-    load(nx, nr, ng, ndh, ndy, nst, row + step);
+    load(rows[AHEAD], row + AHEAD * step);
+    auto &x = rows[0].x, &r = rows[0].r, &g = rows[0].g, &dh = rows[0].dh, &dy = rows[0].dy;
+    const f32x4_t st = rows[0].st;
     const float mu1 = st[0], rs1 = st[1], mu2 = st[2], rs2 = st[3];
     const bool have = row < a.M;
-    float hh[NV][V], t[NV][V];  // hh: norm(h), then g
+    // Without a row all of these are zeros. Past a row's end dy, dh and what is added up are zeros, too, but for g, which
+    // the row's means would enter: it is the one that is masked.
+    float hh[NV][V], xh[NV][V], o[NV][V];  // hh: norm(h), then g; xh: norm(x), or x
+    auto block = [&](int j, int i) { return POST ? xh[j][i] * pw[j][i] + pb[j][i] : xh[j][i]; };  // t
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float v = (float)x[j].v[i];
-        if constexpr (POST) v = (v - mu1) * rs1 * pw[j][i] + pb[j][i];
-        t[j][i] = v;
+        xh[j][i] = (float)x[j].v[i];
+        if constexpr (POST) xh[j][i] = (xh[j][i] - mu1) * rs1;
         const float q = a.gate ? k[j][i] * (float)g[j].v[i] : k[j][i];
-        const float h = a.alpha * (float)r[j].v[i] + q * v;
-        // past the row, and without one, nothing is added: what is there may be made of a row that is not finite
-        const bool in = c.in(j, i) && have;
-        const float n = in ? (h - mu2) * rs2 : 0.0f;
+        const float n = (a.alpha * (float)r[j].v[i] + q * block(j, i) - mu2) * rs2;
         hh[j][i] = n;
         if (a.dy) {
           const float d = (float)dy[j].v[i], wdy = d * w[j][i];
           s1 += wdy;
-          s2 += in ? wdy * n : 0.0f;
-          total[kDw][j][i] += in ? d * n : 0.0f;
+          s2 += wdy * n;
+          total[kDw][j][i] += d * n;
           total[kDb][j][i] += d;
         }
       }
@@ -283,7 +289,6 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
       par ^= 1;
     }
     const float c1 = a.rms ? 0.0f : s1 * inv, c2 = s2 * inv;
-    float o[NV][V];
     s1 = s2 = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -291,19 +296,19 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
       for (int i = 0; i < V; ++i) {
         float e = a.dh ? (float)dh[j].v[i] : 0.0f;
         if (a.dy) e += rs2 * ((float)dy[j].v[i] * w[j][i] - c1 - hh[j][i] * c2);
-        const bool in = c.in(j, i) && have;
-        e = in ? e : 0.0f;
+        e = c.in(j, i) ? e : 0.0f;
         hh[j][i] = e;
-        const float gate = a.gate ? (float)g[j].v[i] : 1.0f, f = e * gate, q = f * k[j][i];
-        total[kDscale][j][i] += in ? f * t[j][i] : 0.0f;
+        const float f = a.gate ? e * (float)g[j].v[i] : e, q = f * k[j][i];
+        total[kDscale][j][i] += f * block(j, i);
         if constexpr (POST) {
-          const float xh = in ? ((float)x[j].v[i] - mu1) * rs1 : 0.0f;
-          total[kDpw][j][i] += q * xh;
+          total[kDpw][j][i] += q * xh[j][i];
           total[kDpb][j][i] += q;
-          s1 += q * pw[j][i];
-          s2 += q * pw[j][i] * xh;
+          o[j][i] = q * pw[j][i];
+          s1 += o[j][i];
+          s2 += o[j][i] * xh[j][i];
+        } else {
+          o[j][i] = q;
         }
-        o[j][i] = q;
       }
     if (POST && a.dx) {
       row_sum2<NW>(s1, s2, red[par], wave);
@@ -312,10 +317,7 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float xh = ((float)x[j].v[i] - mu1) * rs1;
-          o[j][i] = rs1 * (o[j][i] * pw[j][i] - e1 - xh * e2);
-        }
+        for (int i = 0; i < V; ++i) o[j][i] = rs1 * (o[j][i] - e1 - xh[j][i] * e2);
     }
     if (have) {
       if (a.dx) c.store(a.dx, row * a.d, o);
@@ -323,7 +325,7 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int i = 0; i < V; ++i) o[j][i] = hh[j][i] * k[j][i] * t[j][i];
+          for (int i = 0; i < V; ++i) o[j][i] = hh[j][i] * k[j][i] * block(j, i);
         c.store(a.dgate, row * a.d, o);
       }
       if (a.dr) {
@@ -335,14 +337,7 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
       }
     }
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      x[j] = nx[j];
-      r[j] = nr[j];
-      if (a.gate) g[j] = ng[j];
-      if (a.dh) dh[j] = ndh[j];
-      if (a.dy) dy[j] = ndy[j];
-    }
-    st = nst;
+    for (int i = 0; i < AHEAD; ++i) rows[i] = rows[i + 1];
   }
   if (!a.part) return;
   // wanted sums one behind the other, [parts][wanted][d]

@@ -3,22 +3,26 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <stdint.h>
 
 namespace fmx {
 namespace {
 
-// V consecutive elements of type T as they lie in memory.
+// V consecutive elements of type T as they lie in memory. (They move as one vector: stores of the array itself, of
+// zeros for one, came apart into stores of elements; 268 MB of zeros 160 us, 46 as vectors.)
 template <typename T, int V>
 struct Piece {
+  typedef uint32_t words_t __attribute__((ext_vector_type(sizeof(T) * V / 4)));
   T v[V];
   // `left` of them are there, the others are zeros
   template <bool WHOLE>
   __device__ __forceinline__ void load(const T* p, int left) {
+    words_t w = {};
     if (WHOLE ? left > 0 : left >= V) {
-      __builtin_memcpy(v, p, sizeof(v));
+      __builtin_memcpy(&w, p, sizeof(w));
+      set(w);
     } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = T(0.0f);
+      set(w);
       if constexpr (!WHOLE) {
 #pragma unroll
         for (int i = 0; i < V - 1; ++i)
@@ -29,13 +33,16 @@ struct Piece {
   template <bool WHOLE>
   __device__ __forceinline__ void store(T* p, int left) const {
     if (WHOLE ? left > 0 : left >= V) {
-      __builtin_memcpy(p, v, sizeof(v));
+      words_t w;
+      __builtin_memcpy(&w, v, sizeof(w));
+      __builtin_memcpy(p, &w, sizeof(w));
     } else if constexpr (!WHOLE) {
 #pragma unroll
       for (int i = 0; i < V - 1; ++i)
         if (i < left) p[i] = v[i];
     }
   }
+  __device__ __forceinline__ void set(const words_t& w) { __builtin_memcpy(v, &w, sizeof(v)); }
 };
 
 }  // namespace

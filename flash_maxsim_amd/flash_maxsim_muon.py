@@ -9,7 +9,7 @@ goes to a s + b s^3 + c s^5 a few times, which brings all of them near one: thre
 products a step on matrix instructions, over all matrices in one launch. Products
 take fp16 operands and float32 sums; the iterate is held as a pair of fp16
 values, so that small singular values, which grow by hundreds, do not drown in
-its rounding. The result is within about 2e-3 (of its norm) of the formula's.
+its rounding. The result is within about 2.5e-3 (of its norm) of the formula's.
 Sums have a fixed order: the same inputs give the same bits.
 
 muon_step updates lists of matrices in place; Muon is the optimizer class over
@@ -62,7 +62,7 @@ def orthogonalize(updates, steps: int = 5, coefficients=COEFFICIENTS, eps: float
 
     Each is divided by the root of its squares' sum (at least eps), then
     X = a X + (b X X^T + c (X X^T)^2) X `steps` times with (a, b, c) =
-    coefficients. Types may differ from matrix to matrix. No gradients.
+    coefficients, each within +-20. Types may differ from matrix to matrix. No gradients.
     """
     one = isinstance(updates, torch.Tensor)
     updates = [updates] if one else list(updates)

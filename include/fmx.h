@@ -601,6 +601,8 @@ typedef struct fmx_muon_matrix {
 /* the most of a matrix's shorter and of its longer side */
 #define FMX_MUON_MAX_SHORT (1 << 14)
 #define FMX_MUON_MAX_LONG (1 << 20)
+/* of a, b and c in absolute value: a I + b A + c A^2 is held in fp16, times 2^10, for singular values up to one */
+#define FMX_MUON_MAX_COEFFICIENT 20
 
 /*
  * An orthogonalised step over `count` matrices (a host array, read before the call returns):
@@ -608,7 +610,7 @@ typedef struct fmx_muon_matrix {
  *   u = (1 - momentum) g + momentum m with nesterov, else m;  X = u / max(|u|, eps), |u| the root of its squares' sum
  *   `steps` times, X's shorter side first:  X = a X + (b X X^T + c (X X^T)^2) X
  *   p = p (1 - lr weight_decay) - lr f X,  f = sqrt(max(1, rows / cols)), with match_rms 0.2 sqrt(max(rows, cols))
- * Products on fp16 MFMA with fp32 sums, X held as a pair of fp16 values (the result is within about 2e-3 of the
+ * Products on fp16 MFMA with fp32 sums, X held as a pair of fp16 values (the result is within about 2.5e-3 of the
  * formula's, by the root of the squares), everything else in fp32 (|u| in 64 bits); p is rounded once. Types as
  * fmx_adamw's. Deterministic. Workspace: fmx_muon_workspace_bytes, 256-byte aligned.
  */

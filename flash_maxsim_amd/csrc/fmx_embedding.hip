@@ -203,8 +203,7 @@ __global__ void __launch_bounds__(1024) embedding_place_kernel(EmbeddingArgs a, 
 // ---- sums ----
 
 // Workgroups before `sums` add up stretches, a wave a stretch of one block of 64 pieces of columns; the others write
-// the rows of ids that do not occur, kRows ids each: few, so that the workgroups at work write one stretch of memory
-// between them (131072 ids of 2 KB, hardly one of them there: 256 ids a workgroup 159 us, 32 RATE us).
+// the rows of ids that do not occur, kRows ids each: as many as keep its search short.
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(256) embedding_sum_kernel(EmbeddingArgs a, uint32_t sums, int blocks) {
   constexpr int V = 16 / sizeof(T);

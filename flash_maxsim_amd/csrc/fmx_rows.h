@@ -9,7 +9,7 @@ namespace fmx {
 namespace {
 
 // V consecutive elements of type T as they lie in memory. (They move as one vector: stores of the array itself, of
-// zeros for one, came apart into stores of elements; 268 MB of zeros 160 us, 46 as vectors.)
+// zeros for one, came apart into stores of elements; 268 MB of zeros 160 us.)
 template <typename T, int V>
 struct Piece {
   typedef uint32_t words_t __attribute__((ext_vector_type(sizeof(T) * V / 4)));

@@ -95,9 +95,13 @@ struct LinearArgs {
   int64_t split_k, band;
   int splits;
   int act;
-  const void* B2;         // dx of a gated layer: rows of B for the first `half` stages of k, then those of B2, kb of each
+  // a gated layer's backward (else null): dx reads rows of B for the first `half` stages of k, then those of B2, kb of
+  // each; dw makes y from A and y2 from A2
+  const void* B2;
   int64_t sb2;
-  int half, kb;
+  const void* A2;
+  void* y2;
+  int half, kb;           // dw: half is set by launch_linear
 };
 
 struct LinearPlan {
@@ -106,8 +110,9 @@ struct LinearPlan {
   int splits;
   int64_t ti, tj, split_k, band;
 };
-LinearPlan linear_plan(LinearForm form, int64_t I, int64_t J, int64_t K);
-size_t linear_part_bytes(const LinearPlan& p, int64_t I, int64_t J);
+// pair: two products of these sizes in one launch (dw of a gated layer)
+LinearPlan linear_plan(LinearForm form, int64_t I, int64_t J, int64_t K, bool pair = false);
+size_t linear_part_bytes(const LinearPlan& p, int64_t I, int64_t J, bool pair = false);
 // Whether the dw product of this plan adds up its A's columns beside it (its registers hold no more at 256 x 256).
 inline bool linear_sums_columns(const LinearPlan& p) { return p.tile != kTile256; }
 hipError_t launch_linear(bool bf16, LinearForm form, LinearArgs a, const LinearPlan& p, hipStream_t s);

@@ -84,8 +84,8 @@ int check_gated(int dtype, int64_t x_stride, int64_t wg_stride, int64_t wu_strid
   return check_linear(dtype, x_stride, wu_stride, act, M, N, K);
 }
 
-// Backward workspace: dg and du beside each other, their column sums, the partial products of dx and of one weight's
-// gradient (used one after the other).
+// Backward workspace: dg and du beside each other, their column sums, the partial products of dx and of the
+// weights' gradients (used one after the other).
 struct GatedBwdWs {
   size_t dz, sums, part;
   size_t total() const { return dz + sums + part; }
@@ -97,7 +97,10 @@ GatedBwdWs gated_bwd_ws(int64_t M, int64_t N, int64_t K) {
   w.dz = round256((size_t)M * (size_t)np * 4);
   w.sums = round256((size_t)fmx::gated_dz_parts(M, N) * 2 * (size_t)N * sizeof(float));
   const size_t px = fmx::linear_part_bytes(fmx::linear_plan(fmx::kLinearInput, M, K, 2 * np), M, K);
-  const size_t pw = fmx::linear_part_bytes(fmx::linear_plan(fmx::kLinearWeight, N, K, M), N, K);
+  // both weights' gradients together, or one alone
+  const size_t two = fmx::linear_part_bytes(fmx::linear_plan(fmx::kLinearWeight, N, K, M, true), N, K, true);
+  const size_t one = fmx::linear_part_bytes(fmx::linear_plan(fmx::kLinearWeight, N, K, M), N, K);
+  const size_t pw = one > two ? one : two;
   w.part = round256(px > pw ? px : pw);
   return w;
 }
@@ -416,19 +419,18 @@ int fmx_gated_bwd(int dtype, const void* x, int64_t x_stride, const void* wg, in
     if (e != hipSuccess) return hip_status(e, "fmx_gated_bwd launch");
     a.B2 = nullptr;
   }
-  const fmx::LinearPlan plan_w = fmx::linear_plan(fmx::kLinearWeight, N, K, M);
-  for (int up = 0; up < 2; ++up) {
-    void* dw = up ? dwu : dwg;
-    if (!dw) continue;
-    a.A = base + (up ? np * 2 : 0);
+  if (weights) {
+    const bool both = dwg && dwu;
+    a.A = base + (dwg ? 0 : np * 2);
+    a.A2 = both ? base + np * 2 : nullptr;
     a.B = x;
     a.sb = x_stride;
     a.I = N;
     a.J = K;
     a.K = M;
-    a.y = dw;
-    e = fmx::launch_linear(bf, fmx::kLinearWeight, a, plan_w, s);
-    if (e != hipSuccess) return hip_status(e, "fmx_gated_bwd launch");
+    a.y = dwg ? dwg : dwu;
+    a.y2 = both ? dwu : nullptr;
+    e = fmx::launch_linear(bf, fmx::kLinearWeight, a, fmx::linear_plan(fmx::kLinearWeight, N, K, M, both), s);
   }
   return hip_status(e, "fmx_gated_bwd launch");
 }

@@ -74,7 +74,7 @@ __device__ __forceinline__ u32x4_t slopes8(const float (&s)[8]) {
 
 // Products in v (the bias added already) to their place: the activation, its slope, the residual in `res`, y.
 template <bool BF, int EPI>
-__device__ __forceinline__ void finish(const LinearArgs& a, int64_t i, int64_t j, int left, float (&v)[8],
+__device__ __forceinline__ void finish(const LinearArgs& a, void* out, int64_t i, int64_t j, int left, float (&v)[8],
                                        const u32x4_t& res) {
   if constexpr (EPI != kNoEpilogue) {
     if constexpr (EPI != FMX_ACT_NONE) {
@@ -93,13 +93,13 @@ __device__ __forceinline__ void finish(const LinearArgs& a, int64_t i, int64_t j
       for (int k = 0; k < 8; ++k) v[k] += r[k];
     }
   }
-  store16(a.y, i * a.J + j, left, v, BF);
+  store16(out, i * a.J + j, left, v, BF);
 }
 
 // ---- the product ----
 
-// PAIRED (dx of a gated layer): k runs over the rows of B and then over those of B2, which A's columns meet after
-// `half` stages.
+// PAIRED (a gated layer's backward): in dx k runs over the rows of B and then over those of B2, which A's columns meet
+// after `half` stages; dw makes y from A and y2 from A2, whose tiles follow each other.
 template <bool BF, bool AMAJ, bool BMAJ, int WI, int WJ, int FI, int FJ, int NS, int EPI, bool PAIRED>
 __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
   constexpr int TI = WI * FI * 16, TJ = WJ * FJ * 16, NT = WI * WJ * 64;
@@ -118,14 +118,17 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
 
   const Place at(blockIdx.x, (uint32_t)a.ti, (uint32_t)a.tj, (uint32_t)a.splits, (uint32_t)a.band);
   const uint32_t split = at.split;
-  const int64_t i0 = (int64_t)at.row * TI, j0 = (int64_t)at.col * TJ;
+  const bool second = PAIRED && AMAJ && at.row >= (uint32_t)a.half;
+  const int64_t i0 = (int64_t)(second ? at.row - (uint32_t)a.half : at.row) * TI, j0 = (int64_t)at.col * TJ;
+  void* const out = second ? a.y2 : a.y;
   const int64_t k0 = (int64_t)split * a.split_k;
   const int64_t kn = a.K - k0 < a.split_k ? a.K - k0 : a.split_k;
   const int nit = (int)((kn + BK - 1) / BK);
 
-  const SideA sa(a.A, a.sa, i0, a.I, k0, tid);
-  const SideB sb(a.B, a.sb, j0, a.Jr, PAIRED ? 0 : k0, tid);
-  const SideB sb2(PAIRED ? a.B2 : a.B, PAIRED ? a.sb2 : a.sb, j0, a.Jr, PAIRED ? 0 : k0, tid);
+  constexpr bool TURNS = PAIRED && !AMAJ;
+  const SideA sa(second ? a.A2 : a.A, a.sa, i0, a.I, k0, tid);
+  const SideB sb(a.B, a.sb, j0, a.Jr, TURNS ? 0 : k0, tid);
+  const SideB sb2(TURNS ? a.B2 : a.B, TURNS ? a.sb2 : a.sb, j0, a.Jr, TURNS ? 0 : k0, tid);
   const Frags<AMAJ, false, TI> fa(wi * FI * 16, lane);
   const Frags<BMAJ, !BMAJ, TJ> fb(wj * FJ * 16, lane);
 
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
   auto issue = [&](unsigned char* lds, int it) __attribute__((always_inline)) {
     const int left = (int)kn - it * BK;
     sa.issue(lds, it, left, wave);
-    if constexpr (PAIRED) {
+    if constexpr (TURNS) {
       const int stage = (int)(k0 / BK) + it, own = stage < a.half ? stage : stage - a.half;
       if (stage < a.half)
         sb.issue(lds + TI * BK * 2, own, a.kb - own * BK, wave);
@@ -280,7 +283,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
       }
       put(x, 0, pack8(v[0], BF));
       put(x, 1, pack8(v[1], BF));
-      flush(x, a.y);
+      flush(x, out);
     }
     return;
   }
@@ -308,13 +311,14 @@ __global__ void __launch_bounds__(WI* WJ * 64) linear_kernel(LinearArgs a) {
       pair(x, y, v);  // by all lanes: the exchange reads its partners' registers
       if (i >= a.I || left <= 0) continue;
       if (a.splits > 1) {
-        float* p = a.part + ((int64_t)split * a.I + i) * a.Jp + j;  // Jp: J rounded up to 8
+        const int64_t plane = PAIRED && AMAJ ? (int64_t)split * 2 + second : (int64_t)split;
+        float* p = a.part + (plane * a.I + i) * a.Jp + j;  // Jp: J rounded up to 8
         *reinterpret_cast<f32x4_t*>(p) = f32x4_t{v[0], v[1], v[2], v[3]};
         *reinterpret_cast<f32x4_t*>(p + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] += b[k];
-        finish<BF, EPI>(a, i, j, left, v, res[x]);
+        finish<BF, EPI>(a, out, i, j, left, v, res[x]);
       }
     }
   }
@@ -344,7 +348,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a, int grou
     }
     return;
   }
-  const int64_t per = a.Jp / 8, n = a.I * per;
+  const int64_t per = a.Jp / 8, rows = a.y2 ? 2 * a.I : a.I, n = rows * per;
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)groups * 256) {
     const int64_t i = t / per, j = (t - i * per) * 8;
     const float* p = a.part + i * a.Jp + j;
@@ -356,8 +360,8 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a, int grou
     f32x4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
-      s0 += *reinterpret_cast<const f32x4_t*>(p + s * a.I * a.Jp);
-      s1 += *reinterpret_cast<const f32x4_t*>(p + s * a.I * a.Jp + 4);
+      s0 += *reinterpret_cast<const f32x4_t*>(p + s * rows * a.Jp);
+      s1 += *reinterpret_cast<const f32x4_t*>(p + s * rows * a.Jp + 4);
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -365,7 +369,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs a, int grou
       v[4 + k] += s1[k];
     }
     const u32x4_t res = EPI != kNoEpilogue && a.res ? load_raw(a.res, i * a.sres + j, left) : u32x4_t{0u, 0u, 0u, 0u};
-    finish<BF, EPI>(a, i, j, left, v, res);
+    finish<BF, EPI>(a, i < a.I ? a.y : a.y2, i < a.I ? i : i - a.I, j, left, v, res);
   }
 }
 
@@ -431,7 +435,7 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
         v[k] += s0[k];
         v[4 + k] += s1[k];
       }
-      finish<BF, kAnyAct>(a, i, j, left, v, res);
+      finish<BF, kAnyAct>(a, a.y, i, j, left, v, res);
     }
   }
 }
@@ -517,8 +521,8 @@ hipError_t launch(const LinearArgs& a, int tile, hipStream_t s) {
   constexpr int kJoin = FORWARD ? kAnyAct : kNoEpilogue;
   if constexpr (!FORWARD) {
     bool done = false;
-    if constexpr (!AMAJ && BMAJ) {
-      if (a.B2) {
+    if constexpr (BMAJ) {
+      if (a.B2 || a.y2) {
         run_tile<BF, AMAJ, BMAJ, kNoEpilogue, true>(a, tile, grid, s);
         done = true;
       }
@@ -535,7 +539,7 @@ hipError_t launch(const LinearArgs& a, int tile, hipStream_t s) {
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  const int64_t need = (a.I * (a.Jp / 8) + 255) / 256;
+  const int64_t need = ((a.y2 ? 2 * a.I : a.I) * (a.Jp / 8) + 255) / 256;
   const int groups = (int)(need < 4096 ? need : 4096);
   linear_join_kernel<BF, kJoin><<<groups + (a.db ? (int)((a.I + 15) / 16) : 0), 256, 0, s>>>(a, groups);
   return hipGetLastError();
@@ -559,8 +563,10 @@ constexpr TileCost kCosts[] = {{kTile256, 256, 1, 1.45, 1.45, 8.5},
                                {kTile128Deep, 128, 1, 0.58, 0.58, 4.0},
                                {kTile64, 64, 2, 0.33, 0.43, 3.0}};
 
-LinearPlan linear_plan(LinearForm form, int64_t I, int64_t J, int64_t K) {
+LinearPlan linear_plan(LinearForm form, int64_t I, int64_t J, int64_t K, bool pair) {
   const int64_t cus = layer_cus();
+  static constexpr int kParts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+  static constexpr int kPairParts[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 24};
   LinearPlan best = {};
   // Few rows straight from memory: every workgroup reads all of x, which costs more than the tiles' waits once
   // x is large (us, few / tiles; 32 x 768 -> 128 4.4 / 7.0, 64 x 1024 -> 4096 7.4 / 9.6, 16 x 4096 -> 1024 9.6 / 9.1,
@@ -575,8 +581,8 @@ LinearPlan linear_plan(LinearForm form, int64_t I, int64_t J, int64_t K) {
     // The rows of a K-major tile are reached by 32-bit offsets below 2^31 from its first one. x and W have strides
     // below 2^22, which all tiles hold; dz has N's, below 2^24: tiles of 256 rows to N = 4.2 million, of 128 to 8.4.
     if (form != kLinearWeight && (c.size - 1) * K * 2 + BK * 2 > 0x7fffffff) continue;
-    const int64_t ti = (I + c.size - 1) / c.size, tj = (J + c.size - 1) / c.size, slots = cus * c.per_cu;
-    for (int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+    const int64_t ti = (I + c.size - 1) / c.size * (pair ? 2 : 1), tj = (J + c.size - 1) / c.size, slots = cus * c.per_cu;
+    for (int want : pair ? kPairParts : kParts) {
       int64_t per = ((K + want - 1) / want + BK - 1) / BK * BK;
       if (want > 1 && per < 4 * BK) break;  // a part shorter than its loads' latency
       const int64_t splits = (K + per - 1) / per, n = ti * tj * splits, whole = n / slots, left = n % slots;
@@ -584,7 +590,7 @@ LinearPlan linear_plan(LinearForm form, int64_t I, int64_t J, int64_t K) {
       double us = whole * (stages * c.full + c.rest);
       if (left) us += stages * (left > cus ? c.full : c.alone) + c.rest;
       // partial products written and read, mostly in the caches, and the second kernel
-      if (splits > 1) us += 2.5 + (double)splits * (double)I * (double)J * 8.0 / 8e6;
+      if (splits > 1) us += 2.5 + (double)splits * (double)I * (double)J * (pair ? 16.0 : 8.0) / 8e6;
       if (best.splits == 0 || us < least) {
         least = us;
         best.tile = c.tile;
@@ -602,8 +608,8 @@ LinearPlan linear_plan(LinearForm form, int64_t I, int64_t J, int64_t K) {
   return best;
 }
 
-size_t linear_part_bytes(const LinearPlan& p, int64_t I, int64_t J) {
-  return p.splits > 1 ? (size_t)p.splits * (size_t)I * (size_t)((J + 7) / 8 * 8) * sizeof(float) : 0;
+size_t linear_part_bytes(const LinearPlan& p, int64_t I, int64_t J, bool pair) {
+  return p.splits > 1 ? (pair ? 2 : 1) * (size_t)p.splits * (size_t)I * (size_t)((J + 7) / 8 * 8) * sizeof(float) : 0;
 }
 
 hipError_t launch_linear(bool bf16, LinearForm form, LinearArgs a, const LinearPlan& p, hipStream_t s) {
@@ -631,6 +637,7 @@ hipError_t launch_linear(bool bf16, LinearForm form, LinearArgs a, const LinearP
   a.band = p.band;
   a.Jp = (a.J + 7) / 8 * 8;
   a.Jr = form == kLinearForward ? a.J : a.Jp;  // row-major B: whole chunks of 8 columns
+  if (a.y2) a.half = (int)(p.ti / 2);
   if (p.tile == kFewRows) return bf16 ? launch_few<true>(a, s) : launch_few<false>(a, s);
   switch (form) {
     case kLinearForward:

@@ -249,17 +249,11 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
     if (a.dy) c.load(o.dy, a.dy, at * a.sdy, have);
     o.st = have ? reinterpret_cast<const f32x4_t*>(a.stats)[at] : f32x4_t{0.f, 0.f, 0.f, 0.f};
   };
-  // AHEAD rows are loaded while this one is summed
-  constexpr int AHEAD = NV == 1 ? 2 : 1;
-  Rows rows[AHEAD + 1];
   int64_t row = (int64_t)blockIdx.x * NG + wave / NW;
-#pragma unroll
-  for (int i = 0; i < AHEAD; ++i) load(rows[i], row + i * step);
   int par = 0;
-  for (int64_t base = (int64_t)blockIdx.x * NG; base < a.M; base += step, row += step) {
-    load(rows[AHEAD], row + AHEAD * step);
-    auto &x = rows[0].x, &r = rows[0].r, &g = rows[0].g, &dh = rows[0].dh, &dy = rows[0].dy;
-    const f32x4_t st = rows[0].st;
+  auto sums = [&](const Rows& rows) __attribute__((always_inline)) {
+    const auto &x = rows.x, &r = rows.r, &g = rows.g, &dh = rows.dh, &dy = rows.dy;
+    const f32x4_t st = rows.st;
     const float mu1 = st[0], rs1 = st[1], mu2 = st[2], rs2 = st[3];
     const bool have = row < a.M;
     // Without a row all of these are zeros. Past a row's end dy, dh and what is added up are zeros, too, but for g, which
@@ -336,8 +330,35 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
         c.store(a.dr, row * a.d, o);
       }
     }
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) rows[i] = rows[i + 1];
+  };
+  // Rows are loaded while others are summed: two ahead in three sets of registers, one ahead where a lane has 16 elements.
+  // (The sets take turns by name: handing registers on would wait for their loads.)
+  int64_t base = (int64_t)blockIdx.x * NG;
+  if constexpr (NV == 1) {
+    Rows r0, r1, r2;
+    load(r0, row);
+    load(r1, row + step);
+    auto turn = [&](Rows& now, Rows& next) __attribute__((always_inline)) {
+      load(next, row + 2 * step);
+      sums(now);
+      base += step;
+      row += step;
+      return base < a.M;  // the same for all rows of the workgroup, and so is the number of barriers
+    };
+    while (turn(r0, r2) && turn(r1, r0) && turn(r2, r1)) {
+    }
+  } else {
+    Rows r0, r1;
+    load(r0, row);
+    auto turn = [&](Rows& now, Rows& next) __attribute__((always_inline)) {
+      load(next, row + step);
+      sums(now);
+      base += step;
+      row += step;
+      return base < a.M;
+    };
+    while (turn(r0, r1) && turn(r1, r0)) {
+    }
   }
   if (!a.part) return;
   // wanted sums one behind the other, [parts][wanted][d]

@@ -178,8 +178,8 @@ struct MuonMatrix {
 };
 
 struct MuonScalars {
-  double lr;
-  float mu, omu, eps, keep;  // omu: 1 - mu; keep: 1 - lr * weight decay
+  double lr, eps;
+  float mu, omu, keep;       // omu: 1 - mu; keep: 1 - lr * weight decay
   float a, b, c;
   int steps, nesterov, by_rms, apply;
   const float* grad_scale;   // one value, or null

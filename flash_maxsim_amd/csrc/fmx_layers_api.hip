@@ -114,7 +114,7 @@ int check_residual_norm(int dtype, int w_dtype, int64_t x_stride, int64_t r_stri
     return fail(FMX_ERR_INVALID, "invalid sizes M=%lld d=%lld or strides", (long long)M, (long long)d);
   if (d > FMX_RESIDUAL_NORM_MAX_D)
     return fail(FMX_ERR_UNSUPPORTED, "d=%lld exceeds FMX_RESIDUAL_NORM_MAX_D=%d", (long long)d, FMX_RESIDUAL_NORM_MAX_D);
-  if (!isfinite(alpha)) return fail(FMX_ERR_INVALID, "alpha must be finite");
+  if (!isfinite((float)alpha)) return fail(FMX_ERR_INVALID, "alpha must be finite in fp32");
   return FMX_OK;
 }
 
@@ -126,7 +126,7 @@ int check_embedding(int dtype, int ids_bits, int64_t stride, double scale, int64
                 (long long)stride);
   if (T > FMX_EMBEDDING_MAX_TOKENS || V > FMX_EMBEDDING_MAX_ROWS || d > FMX_MAX_D)
     return fail(FMX_ERR_UNSUPPORTED, "T=%lld V=%lld d=%lld too large", (long long)T, (long long)V, (long long)d);
-  if (!isfinite(scale)) return fail(FMX_ERR_INVALID, "scale must be finite");
+  if (!isfinite((float)scale)) return fail(FMX_ERR_INVALID, "scale must be finite in fp32");
   return FMX_OK;
 }
 
@@ -169,7 +169,7 @@ int run_muon(int pd, int gd, int cd, const fmx_muon_matrix* matrices, int64_t co
   sc.a = (float)a;
   sc.b = (float)b;
   sc.c = (float)c;
-  sc.eps = (float)eps;
+  sc.eps = eps;
   const fmx::MuonMatrix* list = reinterpret_cast<const fmx::MuonMatrix*>(matrices);
   const size_t need = fmx::muon_workspace_bytes(list, count);
   if (need > 0 && (!workspace || bytes < need || !aligned(workspace, 256)))

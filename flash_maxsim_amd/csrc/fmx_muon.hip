@@ -55,7 +55,8 @@ struct Entry {
 struct Table {
   char* ws;
   const float* grad_scale;
-  float mu, omu, eps, keep;     // omu: 1 - mu
+  double eps;
+  float mu, omu, keep;          // omu: 1 - mu
   float a, b, c;
   int nesterov, apply;          // apply: parameters move; else the result is written
   uint32_t total;               // workgroups
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(256) muon_start_kernel(Table t) {
     __syncthreads();
   }
   const double norm = sqrt(sums[0]);
-  const double by = (double)kX / (norm <= (double)t.eps ? (double)t.eps : norm);  // a norm that is NaN stays so
+  const double by = (double)kX / (norm <= t.eps ? t.eps : norm);  // a norm that is NaN stays so
   const float scale = t.grad_scale ? *t.grad_scale : 1.0f;
   const bool tall = e.rows > e.cols;
   const int row = threadIdx.x >> 2, part = (threadIdx.x & 3) * 16;

@@ -28,6 +28,7 @@ from . import _lib
 from .flash_maxsim import _check_devices, _device_guard
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+MAX_SHORT, MAX_LONG = 1 << 14, 1 << 20
 ADJUST = {"original": 0, "match_rms_adamw": 1}
 
 _CODES = {torch.float16: _lib.FMX_DTYPE_F16, torch.bfloat16: _lib.FMX_DTYPE_BF16, torch.float32: _lib.FMX_DTYPE_F32}
@@ -48,6 +49,22 @@ def _coefficients(c) -> tuple[float, float, float]:
 def _workspace(lib, table, count: int, dev) -> tuple[torch.Tensor | None, int]:
     nbytes = lib.fmx_muon_workspace_bytes(table, count)
     return _lib.workspace(nbytes, dev), nbytes
+
+
+def _check_sides(t: torch.Tensor) -> None:
+    if min(t.shape) > MAX_SHORT or max(t.shape) > MAX_LONG:
+        raise ValueError(f"a matrix of {tuple(t.shape)}: its sides are at most {MAX_SHORT} and {MAX_LONG}")
+
+
+def _apart(written, read) -> None:
+    """No memory that is written is also another tensor's: a step reads gradients again after it has written momenta."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), w)
+             for ts, w in ((written, True), (read, False)) for t in ts if t.numel() and t.is_contiguous()]
+    end, end_written = 0, 0  # of all before, and of those that are written
+    for first, last, w in sorted(spans):
+        if first < (end if w else end_written):
+            raise ValueError("params, momenta and copies must not share memory with each other or with gradients")
+        end, end_written = max(end, last), max(end_written, last) if w else end_written
 
 
 def _no_tangents(tensors) -> None:
@@ -73,6 +90,7 @@ def orthogonalize(updates, steps: int = 5, coefficients=COEFFICIENTS, eps: float
     keep = []  # contiguous copies, until the launches
     for i, u in enumerate(updates):
         assert u.ndim == 2, "an update is a matrix"
+        _check_sides(u)
         if u.dtype not in _CODES:
             raise TypeError(f"updates must be float16, bfloat16 or float32, got {u.dtype}")
         dev = _check_devices(u)
@@ -106,7 +124,7 @@ def muon_step(params, grads, momenta, lr: float = 1e-3, momentum: float = 0.95, 
     parameters' shapes. grad_scale, a float32 value on the GPU, multiplies every
     gradient without a read back. copies, a list with a float16 or bfloat16 tensor
     (or None) for each parameter, receives the new float32 parameters rounded.
-    No tensor may appear twice among params, momenta and copies.
+    params, momenta and copies share no memory with each other or with gradients.
     """
     if adjust not in ADJUST:
         raise ValueError(f"adjust={adjust!r} must be one of {list(ADJUST)}")
@@ -121,9 +139,7 @@ def muon_step(params, grads, momenta, lr: float = 1e-3, momentum: float = 0.95, 
         if grad_scale.dtype != torch.float32:
             raise TypeError(f"grad_scale must be float32, got {grad_scale.dtype}")
     _no_tangents([*params, *grads, *momenta])
-    written = [t.data_ptr() for t in (*params, *momenta, *copies) if t is not None and t.numel()]
-    if len(set(written)) != len(written):
-        raise ValueError("a tensor appears twice among params, momenta and copies")
+    _apart([t for t in (*params, *momenta, *copies) if t is not None], grads)
     batches: dict = {}
     keep = []  # contiguous copies of gradients, until the launches
     for p, g, m, c in zip(params, grads, momenta, copies):
@@ -138,6 +154,7 @@ def muon_step(params, grads, momenta, lr: float = 1e-3, momentum: float = 0.95, 
         if m.dtype != torch.float32:
             raise TypeError(f"momenta must be float32, got {m.dtype}")
         assert p.ndim == 2, "a parameter is a matrix"
+        _check_sides(p)
         assert g.shape == p.shape and m.shape == p.shape and (c is None or c.shape == p.shape), \
             "gradient, momentum and copy have their parameter's shape"
         if any(t is not None and (t.is_neg() or not t.is_contiguous()) for t in (p, m, c)):

@@ -109,6 +109,7 @@ def test_scales():
         check(fm.orthogonalize((u * by).cuda(), eps=1e-30), u)
     check(fm.orthogonalize((u * 1e-12).cuda()), u * 1e-12)  # norm below eps
     check(fm.orthogonalize(u.cuda(), eps=1e3), u, eps=1e3)
+    assert not fm.orthogonalize(torch.zeros(8, 8, device="cuda"), eps=1e-60).any()
 
 
 def test_steps_and_coefficients():
@@ -342,7 +343,7 @@ def test_refusals():
     g = torch.ones(4, 8, device="cuda")
     ok = dict(params=[p], grads=[g], momenta=[m])
     for bad in (dict(adjust="other"), dict(grads=[]), dict(params=[p.t().contiguous().t()]), dict(coefficients=(1.0, 2.0)),
-                dict(momenta=[p]), dict(params=[p, p], grads=[g, g], momenta=[m, m.clone()])):
+                dict(momenta=[p]), dict(momenta=[g]), dict(grads=[p]), dict(params=[p, p], grads=[g, g], momenta=[m, m.clone()])):
         with pytest.raises(ValueError):
             fm.muon_step(**(ok | bad))
     for bad in (dict(grads=[g[:3]]), dict(momenta=[m.view(8, 4)]), dict(params=[p[0]], grads=[g[0]], momenta=[m[0]]),
@@ -360,6 +361,15 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             fm.muon_step(**(ok | bad))
     assert not p.any() and not m.any()
+    flat = torch.zeros(96, device="cuda")
+    with pytest.raises(ValueError, match="share"):  # the momentum's last row is the parameter's first
+        fm.muon_step([flat[24:56].view(4, 8)], [g], [flat[:32].view(4, 8)])
+    fm.muon_step([flat[:32].view(4, 8)], [flat[64:].view(4, 8)], [flat[32:64].view(4, 8)])  # side by side
+    # one matrix past the limits among others of another type: none is moved
+    q, big = torch.ones(4, 8, device="cuda", dtype=torch.half), torch.zeros((1 << 20) + 1, 1, device="cuda")
+    with pytest.raises(ValueError, match="sides"):
+        fm.muon_step([q, big], [torch.ones_like(q), big + 1], [m.clone(), big + 2])
+    assert (q == 1).all()
     with pytest.raises(AssertionError):
         fm.orthogonalize(p[0])
     with pytest.raises(TypeError):

@@ -6,8 +6,11 @@
 // order, and the sorted list is cut into stretches of kStretch tokens whatever their ids: a wave sums a stretch's
 // rows in registers and writes the ids that begin and end in it to dW; of an id that goes on past the
 // stretch's end it writes a float32 partial sum, and a second kernel adds an id's partial sums in order. So an id that
-// makes up half of the tokens costs no more than others. Rows of ids that do not occur get zeros from other workgroups of
-// the first kernel, which look for their ids in the sorted list.
+// makes up half of the tokens costs no more than others.
+//
+// Rows of ids that do not occur get zeros from workgroups of their own, beside the radix sort's few (which leave the GPU
+// idle) or, where there is none, beside the sums. Which ids occur the first kernel notes: seen[id] is one of the
+// id's tokens, whichever was stored last. The list is never cleared: an entry counts only if it names a token that has the id.
 //
 // Sorting: up to kRankMost tokens each counts the tokens before it (T^2 comparisons, one launch: 1024 tokens 3, 16384 16 us);
 // more go through passes of a radix sort, of 2 launches each, by digits of up to 10 bits.
@@ -22,7 +25,7 @@ namespace {
 
 constexpr int kStretch = 32;         // sorted tokens that a wave sums
 constexpr int64_t kRankMost = 16384;
-constexpr int kRows = 32;            // ids of a workgroup that writes zeros
+constexpr int kRows = 64;            // ids of a workgroup that writes zeros
 constexpr int kBits = 10;            // of a digit, at most
 constexpr int kTile = 4096;          // tokens of a workgroup of the radix sort
 
@@ -63,6 +66,35 @@ __global__ void __launch_bounds__(256) embedding_kernel(EmbeddingArgs a, int lan
   }
 }
 
+// ---- rows of ids that do not occur ----
+
+__device__ __forceinline__ void note(const EmbeddingArgs& a, int32_t key, int64_t t) {
+  if (key < a.V) a.seen[key] = (int32_t)t;
+}
+
+// Zeros to the rows of kRows ids from v0 on that do not occur, by all threads of a workgroup.
+template <int THREADS>
+__device__ __forceinline__ void write_zeros(const EmbeddingArgs& a, int64_t v0) {
+  __shared__ uint8_t absent[kRows];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (threadIdx.x < kRows) {
+    const int64_t v = v0 + threadIdx.x;
+    // without tokens there is neither a list nor an id
+    const int64_t t = v < a.V && a.T > 0 ? (int64_t)(uint32_t)a.seen[v] : a.T;
+    absent[threadIdx.x] = v < a.V && (t >= a.T || key_of(a, t) != v);
+  }
+  __syncthreads();
+  const int64_t bytes = (int64_t)a.d * a.size;
+  for (int r = wave; r < kRows; r += THREADS / 64) {
+    if (!absent[r]) continue;
+    char* row = static_cast<char*>(a.out) + (v0 + r) * bytes;
+    const u32x4_t zero = {0u, 0u, 0u, 0u};
+    for (int64_t at = lane * 16; at + 16 <= bytes; at += 64 * 16) __builtin_memcpy(row + at, &zero, 16);
+    const int64_t rest = bytes & ~(int64_t)15;  // elements of 2 or 4 bytes, a pair of bytes a lane
+    if (rest + lane * 2 < bytes) *reinterpret_cast<uint16_t*>(row + rest + lane * 2) = 0;
+  }
+}
+
 // ---- sorting ----
 
 // Each token's place: how many come before it. A workgroup ranks 16 tokens; keys go through LDS, 4096 at a time. A wave
@@ -77,6 +109,7 @@ __global__ void __launch_bounds__(1024) embedding_rank_kernel(EmbeddingArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int T = (int)a.T, t0 = blockIdx.x * 16, t = t0 + (lane & 15);
   const int32_t mine = key_of(a, t < T ? t : T - 1);
+  if (threadIdx.x < 16 && t < T) note(a, mine, t);
   int before = 0;
   for (int base = 0; base < T; base += kRankTile) {
     __syncthreads();
@@ -121,18 +154,23 @@ __global__ void __launch_bounds__(1024) embedding_count_kernel(EmbeddingArgs a, 
 #pragma unroll
   for (int k = 0; k < kTile / 1024; ++k) {
     const int64_t t = (int64_t)blockIdx.x * kTile + k * 1024 + threadIdx.x;
-    if (t < a.T) atomicAdd(&hist[((FIRST ? key_of(a, t) : keys[t]) >> shift) & (digits - 1)], 1);
+    if (t >= a.T) break;
+    const int32_t key = FIRST ? key_of(a, t) : keys[t];
+    if (FIRST) note(a, key, t);
+    atomicAdd(&hist[(key >> shift) & (digits - 1)], 1);
   }
   __syncthreads();
   if ((int)threadIdx.x < digits) counts[(int64_t)blockIdx.x * digits + threadIdx.x] = hist[threadIdx.x];
 }
 
 // Tokens to their places of this pass, in their order before it: digits before, workgroups before, waves before (a
-// wave has kTile / 16 neighbouring tokens), tokens of the wave before.
+// wave has kTile / 16 neighbouring tokens), tokens of the wave before. The workgroups after those of the tokens write
+// zeros, to the ids from `zeros` on.
 template <bool FIRST>
 __global__ void __launch_bounds__(1024) embedding_place_kernel(EmbeddingArgs a, int shift, int bits, const int32_t* keys,
                                                               const int32_t* order, const int32_t* counts, int groups,
-                                                              int32_t* keys_out, int32_t* order_out) {
+                                                              int32_t* keys_out, int32_t* order_out, int64_t zeros) {
+  if ((int)blockIdx.x >= groups) return write_zeros<1024>(a, zeros + (int64_t)((int)blockIdx.x - groups) * kRows);
   __shared__ int32_t mine[16][1 << kBits];
   __shared__ int32_t sums[16];
   const int digits = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -203,34 +241,14 @@ __global__ void __launch_bounds__(1024) embedding_place_kernel(EmbeddingArgs a, 
 // ---- sums ----
 
 // Workgroups before `sums` add up stretches, a wave a stretch of one block of 64 pieces of columns; the others write
-// the rows of ids that do not occur, kRows ids each: as many as keep its search short.
+// the rows of ids that do not occur, kRows ids each.
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(256) embedding_sum_kernel(EmbeddingArgs a, uint32_t sums, int blocks) {
   constexpr int V = 16 / sizeof(T);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   T* out = static_cast<T*>(a.out);
-  if (blockIdx.x >= sums) {
-    __shared__ uint8_t absent[kRows];
-    const int64_t v0 = (int64_t)(blockIdx.x - sums) * kRows, v = v0 + threadIdx.x;
-    if (threadIdx.x < kRows) {
-      int64_t lo = 0, hi = a.T;  // the first token whose key is v or more
-      while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (a.keys[mid] < v) lo = mid + 1; else hi = mid;
-      }
-      absent[threadIdx.x] = v < a.V && (lo == a.T || a.keys[lo] != v);
-    }
-    __syncthreads();
-    Piece<T, V> zero;
-#pragma unroll
-    for (int i = 0; i < V; ++i) zero.v[i] = T(0.0f);
-    for (int r = wave; r < kRows; r += 4) {
-      if (!absent[r]) continue;
-      for (int col = lane * V; col < a.d; col += 64 * V) zero.template store<WHOLE>(out + (v0 + r) * a.d + col, a.d - col);
-    }
-    return;
-  }
+  if (blockIdx.x >= sums) return write_zeros<256>(a, (int64_t)(blockIdx.x - sums) * kRows);
   const int64_t id = (int64_t)blockIdx.x * 4 + wave, stretch = id / blocks;
   const int col = (int)(id - stretch * blocks) * 64 * V + lane * V;
   const int64_t from = stretch * kStretch;
@@ -370,7 +388,7 @@ int bits_of(int64_t V) {  // of the keys 0 .. V
 int64_t stretches_of(int64_t T) { return (T + kStretch - 1) / kStretch; }
 
 struct Layout {
-  int64_t keys, counts, part, total;  // bytes: two lists of keys and of tokens; digits' counts; partial sums
+  int64_t keys, counts, seen, part, total;  // bytes: lists of keys and of tokens; digits' counts; partial sums
 };
 Layout layout(int kind, int64_t T, int64_t V, int64_t d) {
   const int64_t per = 64 * (kind == FMX_DTYPE_F32 ? 4 : 8), pitch = (d + per - 1) / per * per;
@@ -378,8 +396,9 @@ Layout layout(int kind, int64_t T, int64_t V, int64_t d) {
   Layout l;
   l.keys = (T * 4 + 255) / 256 * 256;
   l.counts = radix ? (T + kTile - 1) / kTile * (4 << kBits) : 0;
+  l.seen = T ? (V * 4 + 255) / 256 * 256 : 0;
   l.part = stretches_of(T) * 2 * pitch * 4;
-  l.total = (radix ? 4 : 2) * l.keys + l.counts + l.part;
+  l.total = (radix ? 4 : 2) * l.keys + l.counts + l.seen + l.part;
   return l;
 }
 
@@ -391,20 +410,26 @@ hipError_t gradient(int kind, EmbeddingArgs a, char* ws, hipStream_t s) {
   for (int i = 0; i < 4; ++i) lists[i] = reinterpret_cast<int32_t*>(ws + (i < 2 || a.T > kRankMost ? i * l.keys : 0));
   a.keys = lists[0];
   a.order = lists[1];
+  a.seen = reinterpret_cast<int32_t*>(ws + l.total - l.part - l.seen);
+  a.size = (int)sizeof(T);
+  const int64_t rows = (a.V + kRows - 1) / kRows;  // workgroups that write zeros
   if (a.T > kRankMost) {
     int32_t* counts = reinterpret_cast<int32_t*>(ws + 4 * l.keys);
     const int bits = bits_of(a.V), passes = (bits + kBits - 1) / kBits, groups = (int)((a.T + kTile - 1) / kTile);
     int shift = 0;
     for (int p = 0; p < passes; ++p) {  // the bits left over the passes left
       const int b = (bits - shift + passes - p - 1) / (passes - p), to = (p & 1) * 2, from = 2 - to;
+      const int64_t z0 = rows * p / passes, zn = rows * (p + 1) / passes - z0;
+      const unsigned grid = (unsigned)(groups + zn);
       if (p == 0) {
         embedding_count_kernel<true><<<groups, 1024, 0, s>>>(a, shift, b, nullptr, counts);
         embedding_place_kernel<true>
-            <<<groups, 1024, 0, s>>>(a, shift, b, nullptr, nullptr, counts, groups, lists[to], lists[to + 1]);
+            <<<grid, 1024, 0, s>>>(a, shift, b, nullptr, nullptr, counts, groups, lists[to], lists[to + 1], z0 * kRows);
       } else {
         embedding_count_kernel<false><<<groups, 1024, 0, s>>>(a, shift, b, lists[from], counts);
         embedding_place_kernel<false>
-            <<<groups, 1024, 0, s>>>(a, shift, b, lists[from], lists[from + 1], counts, groups, lists[to], lists[to + 1]);
+            <<<grid, 1024, 0, s>>>(a, shift, b, lists[from], lists[from + 1], counts, groups, lists[to], lists[to + 1],
+                                   z0 * kRows);
       }
       a.keys = lists[to];
       a.order = lists[to + 1];
@@ -417,11 +442,12 @@ hipError_t gradient(int kind, EmbeddingArgs a, char* ws, hipStream_t s) {
   if (e != hipSuccess) return e;
   a.part = reinterpret_cast<float*>(ws + l.total - l.part);
   const int blocks = (int)((a.d + 64 * V - 1) / (64 * V));
-  const uint32_t sums = (uint32_t)((stretches_of(a.T) * blocks + 3) / 4), rows = (uint32_t)((a.V + kRows - 1) / kRows);
+  const uint32_t sums = (uint32_t)((stretches_of(a.T) * blocks + 3) / 4);
+  const uint32_t grid = sums + (a.T > kRankMost ? 0u : (uint32_t)rows);
   if (a.d % V == 0)
-    embedding_sum_kernel<T, true><<<sums + rows, 256, 0, s>>>(a, sums, blocks);
+    embedding_sum_kernel<T, true><<<grid, 256, 0, s>>>(a, sums, blocks);
   else
-    embedding_sum_kernel<T, false><<<sums + rows, 256, 0, s>>>(a, sums, blocks);
+    embedding_sum_kernel<T, false><<<grid, 256, 0, s>>>(a, sums, blocks);
   e = hipGetLastError();
   if (e != hipSuccess || a.T <= kStretch) return e;
   embedding_join_kernel<T><<<dim3((unsigned)((stretches_of(a.T) + 14) / 16), (unsigned)((a.d + 255) / 256)), 1024, 0, s>>>(

@@ -222,11 +222,13 @@ struct EmbeddingArgs {
   void* out;             // forward: [T, d], backward: dw [V, d]; contiguous
   int32_t* keys;         // backward, in the workspace: the ids sorted, and the tokens in their order
   int32_t* order;
+  int32_t* seen;         // [V]: a token of each id that occurs, anything for others
   float* part;           // backward: [stretches][2][columns] sums of ids that go on
   int64_t T, V, sw, sdy;
   int64_t padding;       // the id without a gradient, or -1
   int d;
   int ids64;
+  int size;              // bytes of an element (set by launch_embedding_bwd)
   float scale;
 };
 

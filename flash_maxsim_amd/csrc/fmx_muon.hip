@@ -48,8 +48,8 @@ struct Entry {
   int64_t at;           // of its part of the workspace, bytes
   int32_t rows, cols;   // of the parameter
   int32_t n, m;         // of X, padded: n the shorter side
-  uint32_t first;       // its first workgroup of the launch
   float rate;
+  int32_t unused;
 };
 
 struct Table {
@@ -61,6 +61,7 @@ struct Table {
   int nesterov, apply;          // apply: parameters move; else the result is written
   uint32_t total;               // workgroups
   int count, from;              // from: which of the two X is read
+  uint32_t first[kMost];        // an entry's first workgroup of the launch; past the last one: all ones
   Entry e[kMost];
 };
 static_assert(sizeof(Table) <= 4096, "kernel arguments");
@@ -82,14 +83,12 @@ __device__ __forceinline__ double* squares_of(const Table& t, const Entry& e) {
   return reinterpret_cast<double*>(t.ws + e.at + 3 * x_bytes(e) + 2 * a_bytes(e));
 }
 
-// The entry that workgroup `id` works for: the last one whose first workgroup is not past it.
+// The entry that workgroup `id` works for: the last one whose first workgroup is not past it. One load for all: a search
+// waits for the arguments' memory once for every step (a step over four small matrices, 17 launches, 102 us by a search, 97).
 __device__ __forceinline__ int entry_of(const Table& t, uint32_t id) {
-  int lo = 0, hi = t.count;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (t.e[mid].first <= id) lo = mid; else hi = mid;
-  }
-  return lo;
+  const int lane = threadIdx.x & 63;
+  const uint32_t first = t.first[lane < kMost ? lane : kMost - 1];
+  return __builtin_popcountll(__ballot(lane < kMost && first <= id)) - 1;
 }
 
 // 8 consecutive values from element `at` of a row-major array, `left` of them there (at least 1; none: zeros).
@@ -142,23 +141,24 @@ __device__ __forceinline__ void direction(float (&u)[8], const float (&g)[8], co
 template <int G>
 __global__ void __launch_bounds__(256) muon_momentum_kernel(Table t) {
   __shared__ double sums[256];
-  const Entry& e = t.e[entry_of(t, blockIdx.x)];
-  const uint32_t chunk = blockIdx.x - e.first;
+  const int at = entry_of(t, blockIdx.x);
+  const Entry& e = t.e[at];
+  const uint32_t chunk = blockIdx.x - t.first[at];
   const int64_t size = (int64_t)e.rows * e.cols;
   const float scale = t.grad_scale ? *t.grad_scale : 1.0f;
   double sum = 0.0;
 #pragma unroll
   for (int v = 0; v < kChunk / 2048; ++v) {
-    const int64_t at = (int64_t)chunk * kChunk + v * 2048 + threadIdx.x * 8;
-    if (at >= size) break;
-    const int left = size - at < 8 ? (int)(size - at) : 8;
+    const int64_t from = (int64_t)chunk * kChunk + v * 2048 + threadIdx.x * 8;
+    if (from >= size) break;
+    const int left = size - from < 8 ? (int)(size - from) : 8;
     float g[8], m[8], u[8];
-    load8<G>(g, e.grad, at, left);
+    load8<G>(g, e.grad, from, left);
     if (e.momentum) {
-      load8<FMX_DTYPE_F32>(m, e.momentum, at, left);
+      load8<FMX_DTYPE_F32>(m, e.momentum, from, left);
 #pragma unroll
       for (int k = 0; k < 8; ++k) m[k] = t.mu * m[k] + t.omu * (g[k] * scale);
-      store8<FMX_DTYPE_F32>(e.momentum, at, left, m);
+      store8<FMX_DTYPE_F32>(e.momentum, from, left, m);
     }
     direction(u, g, m, t, e.momentum != nullptr, scale);
 #pragma unroll
@@ -178,8 +178,9 @@ template <int G>
 __global__ void __launch_bounds__(256) muon_start_kernel(Table t) {
   __shared__ double sums[256];
   __shared__ float tile[64][65];
-  const Entry& e = t.e[entry_of(t, blockIdx.x)];
-  const uint32_t id = blockIdx.x - e.first, tj = (uint32_t)e.m / 64, ti = id / tj;
+  const int at = entry_of(t, blockIdx.x);
+  const Entry& e = t.e[at];
+  const uint32_t id = blockIdx.x - t.first[at], tj = (uint32_t)e.m / 64, ti = id / tj;
   const int i0 = (int)ti * 64, j0 = (int)(id - ti * tj) * 64;
   const int64_t size = (int64_t)e.rows * e.cols, chunks = (size + kChunk - 1) / kChunk;
   double sum = 0.0;
@@ -279,8 +280,9 @@ __global__ void __launch_bounds__(WI* WJ * 64) muon_kernel(Table t, int copy_bf)
     const uint32_t per = t.total / 8, x = id & 7, rest = t.total & 7;
     id = (id >> 3) + x * per + (x < rest ? x : rest);
   }
-  const Entry& e = t.e[entry_of(t, id)];
-  id -= e.first;
+  const int at = entry_of(t, id);
+  const Entry& e = t.e[at];
+  id -= t.first[at];
   uint32_t row, col;
   if constexpr (SYM) {  // row r of the triangle begins at r (r + 1) / 2
     row = (uint32_t)((sqrtf(8.0f * (float)id + 1.0f) - 1.0f) * 0.5f);
@@ -538,7 +540,7 @@ hipError_t run_form(Table t, int copy_bf, hipStream_t s) {
   const int size = choose(t, FORM);
   uint32_t total = 0;
   for (int i = 0; i < t.count; ++i) {
-    t.e[i].first = total;
+    t.first[i] = total;
     total += (uint32_t)tiles_of(t.e[i], FORM, kSizes[size]);
   }
   t.total = total;
@@ -554,7 +556,7 @@ template <int G>
 hipError_t run_start(Table t, hipStream_t s) {
   uint32_t total = 0;
   for (int i = 0; i < t.count; ++i) {
-    t.e[i].first = total;
+    t.first[i] = total;
     total += (uint32_t)(((int64_t)t.e[i].rows * t.e[i].cols + kChunk - 1) / kChunk);
   }
   muon_momentum_kernel<G><<<total, 256, 0, s>>>(t);
@@ -562,7 +564,7 @@ hipError_t run_start(Table t, hipStream_t s) {
   if (e != hipSuccess) return e;
   total = 0;
   for (int i = 0; i < t.count; ++i) {
-    t.e[i].first = total;
+    t.first[i] = total;
     total += (uint32_t)((int64_t)(t.e[i].n / 64) * (t.e[i].m / 64));
   }
   muon_start_kernel<G><<<total, 256, 0, s>>>(t);
@@ -628,6 +630,7 @@ hipError_t launch_muon(int pkind, int gkind, int ckind, const MuonMatrix* x, int
   groups(x, count, [&](int64_t from, int64_t end) {
     if (e != hipSuccess) return;
     Table t = {};
+    for (uint32_t& f : t.first) f = ~0u;
     t.ws = static_cast<char*>(ws);
     t.grad_scale = sc.grad_scale;
     t.mu = sc.mu;

@@ -478,6 +478,7 @@ void run_tile(const GatedArgs& a, int tile, hipStream_t s) {
   const unsigned grid = (unsigned)(a.ti * a.tj * a.splits);
   switch (tile) {
     case kTile256: gated_kernel<BF, 4, 2, 4, 4, 2, ACT><<<grid, 512, 0, s>>>(a); break;
+    case kTile192: gated_kernel<BF, 4, 1, 3, 4, 2, ACT><<<grid, 256, 0, s>>>(a); break;
     case kTile128: gated_kernel<BF, 2, 2, 4, 2, 2, ACT><<<grid, 256, 0, s>>>(a); break;
     case kTile128Deep: gated_kernel<BF, 2, 2, 4, 2, 4, ACT><<<grid, 256, 0, s>>>(a); break;
     default: gated_kernel<BF, 2, 2, 2, 2, 4, ACT><<<grid, 256, 0, s>>>(a); break;
@@ -523,7 +524,7 @@ constexpr GatedCost kGatedCosts[] = {{kTile256, 256, 128, 1, 1.45, 1.45, 8.5},
                                      {kTile128Deep, 128, 64, 1, 0.58, 0.58, 4.0},
                                      {kTile64, 64, 64, 1, 0.40, 0.40, 3.0}};
 
-GatedPlan gated_plan(int64_t I, int64_t J, int64_t K) {
+GatedPlan gated_plan(int64_t I, int64_t J, int64_t K, bool keep) {
   const int64_t cus = layer_cus();
   GatedPlan best = {};
   if (I <= 64 && (I + 15) / 16 * K <= 4096) {  // as for the linear layer
@@ -553,6 +554,17 @@ GatedPlan gated_plan(int64_t I, int64_t J, int64_t K) {
         best.band = 1024 / c.rows;
       }
     }
+  }
+  // Where the factors are kept as well, three times the output, two workgroups a unit that cover each other's stores are
+  // the better large tile (us, 256 x 128 / 192 x 64: training step 16384 x 1024 -> 2816 682 / 666, its forward alone
+  // 208 / 209: the power saved goes to the products after it; 8192 x 1024 -> 4096 without factors 124 / 130). The
+  // tile alone changes, not the parts of k: y has the same bits with and without the factors.
+  if (keep && best.tile == kTile256 && best.splits == 1) {
+    best.tile = kTile192;
+    best.rows = 192;
+    best.ti = (I + 191) / 192;
+    best.tj = (J + 63) / 64;
+    best.band = 5;
   }
   return best;
 }

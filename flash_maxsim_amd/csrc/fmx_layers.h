@@ -71,7 +71,7 @@ hipError_t launch_adamw_decode(const void* codes, bool second, const float* scal
 // ---- linear (fmx_linear.hip) ----
 
 enum LinearForm { kLinearForward, kLinearInput, kLinearWeight };  // y, dx, dw
-enum LinearTile { kTile64, kTile128, kTile128Deep, kTile256, kFewRows };  // deep: four stages in LDS, not two
+enum LinearTile { kTile64, kTile128, kTile128Deep, kTile256, kFewRows, kTile192 };  // deep: four stages in LDS, not two
 
 // C[I, J] = sum over k < K of A(i, k) B(j, k); see fmx_linear.hip for the operands of each form.
 struct LinearArgs {
@@ -152,7 +152,8 @@ struct GatedPlan {
   int tile, rows, splits;
   int64_t ti, tj, split_k, band;
 };
-GatedPlan gated_plan(int64_t I, int64_t J, int64_t K);
+// keep: the backward's factors are written
+GatedPlan gated_plan(int64_t I, int64_t J, int64_t K, bool keep);
 size_t gated_part_bytes(const GatedPlan& p, int64_t I, int64_t J);
 hipError_t launch_gated(bool bf16, GatedArgs a, const GatedPlan& p, hipStream_t s);
 

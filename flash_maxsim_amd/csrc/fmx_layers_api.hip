@@ -311,7 +311,7 @@ int fmx_linear_bwd(int dtype, const void* x, int64_t x_stride, const void* w, in
 
 size_t fmx_gated_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (M < 1 || N < 1 || K < 1) return 0;
-  return fmx::gated_part_bytes(fmx::gated_plan(M, N, (K + 7) / 8 * 8), M, N);
+  return fmx::gated_part_bytes(fmx::gated_plan(M, N, (K + 7) / 8 * 8, false), M, N);
 }
 
 int fmx_gated(int dtype, const void* x, int64_t x_stride, const void* wg, int64_t wg_stride, const void* wu,
@@ -341,7 +341,7 @@ int fmx_gated(int dtype, const void* x, int64_t x_stride, const void* wg, int64_
   a.keep = factors;
   a.act = act;
   a.part = static_cast<float*>(workspace);
-  const fmx::GatedPlan p = fmx::gated_plan(M, N, a.K);
+  const fmx::GatedPlan p = fmx::gated_plan(M, N, a.K, factors != nullptr);
   const size_t need = fmx::gated_part_bytes(p, M, N);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(FMX_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace_bytes);

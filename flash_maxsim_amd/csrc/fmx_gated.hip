@@ -25,31 +25,36 @@ namespace {
 // times as far from 64 bits as ones rounded once, where dg's and the result's roundings alone make 1.41. So it is kept
 // with more bits than they have:
 //   bf16  16 bits: sign, and a measure of |v|'s logarithm (its float32 bits) in steps of 2^-9 of a power of two from 2^-16
-//         to 2^32, of 2^-7 from there down to 2^-80: off by 2^-10 (2^-8) of the factor at most, 1.44 times. 0 is
-//         exact, what is smaller than 2^-80 becomes 0, from 2^32 on and NaN: NaN.
+//         to 2^16, of 2^-7 from there down to 2^-80 and up to 2^79.9: off by 2^-10 (2^-8) of the factor at most, 1.44
+//         times. 0 is exact, what is smaller than 2^-80 becomes 0, what is larger than 2^79.9 and NaN: NaN.
 //   fp16  24 bits: float32 without its last 8, off by 2^-16: 1.41 times. The low bytes of both factors make a plane
 //         of their own.
 template <bool BF>
 struct FactorCode {
-  static constexpr int kKnee = (127 - 16) << 23, kFine = (kKnee >> 14) - 8192, kCoarse = (kKnee >> 16) - 8192;
+  // The three lines meet where the steps change: a code's value is the middle one of them, and so is a value's code.
+  static constexpr int kLow = (127 - 16) << 23, kHigh = (127 + 16) << 23;
+  static constexpr int kFine = (kLow >> 14) - 8192, kBelow = (kLow >> 16) - 8192, kAbove = (kHigh >> 16) - 24576;
+  static __device__ __forceinline__ int middle(int below, int fine, int above) {
+    const int v = fine < above ? fine : above;
+    return v > below ? v : below;  // below < above
+  }
   static __device__ __forceinline__ uint32_t encode(float v) {
     const uint32_t b = __builtin_bit_cast(uint32_t, v);
     if constexpr (!BF) return b + 0x80u;  // its upper 24 bits
-    const int m = (int)(b & 0x7fffffffu);
-    int c = ((m + 0x2000) >> 14) - kFine;
-    const int low = ((m + 0x8000) >> 16) - kCoarse;
-    c = c > low ? c : low;  // the fine steps are the steeper line, the larger one above the knee
+    const uint32_t m = b & 0x7fffffffu;
+    const int coarse = (int)((m + 0x8000u) >> 16);
+    int c = middle(coarse - kBelow, (int)((m + 0x2000u) >> 14) - kFine, coarse - kAbove);
     c = c > 0 ? c : 0;
     c = c < 32767 ? c : 32767;
     return (uint32_t)c | ((b >> 16) & 0x8000u);
   }
   static __device__ __forceinline__ float decode(uint32_t hi, uint32_t lo) {
     if constexpr (!BF) return __builtin_bit_cast(float, (hi << 16) | (lo << 8));
-    const uint32_t c = hi & 0x7fffu;
-    uint32_t m = (c + (uint32_t)kFine) << 14;
-    const uint32_t low = (c + (uint32_t)kCoarse) << 16;
-    m = m < low ? m : low;
-    m = c == 0 ? 0u : c == 32767u ? 0x7fc00000u : m;
+    const int c = (int)(hi & 0x7fffu);
+    // The lines the other way round: the coarse ones are the steeper. The one of small values passes 2^31 and is negative
+    // from code 26752 on; the middle one is that of large values there all the same.
+    uint32_t m = (uint32_t)middle((c + kAbove) * 65536, (c + kFine) * 16384, (int)((uint32_t)(c + kBelow) << 16));
+    m = c == 0 ? 0u : c == 32767 ? 0x7fc00000u : m;
     return __builtin_bit_cast(float, m | ((hi & 0x8000u) << 16));
   }
 };

@@ -9,7 +9,7 @@ and y is rounded once: neither product reaches memory. The backward rounds
 dg = dy u act'(g) and du = dy act(g) to the operands' type, as MFMA takes them; the
 factors u act'(g) and act(g) are kept between the passes in codes of more bits than
 the operands have (bfloat16: 16, fp16: 24; off by 2^-10 and 2^-16 of the factor at
-most, from 2^-16 to 2^32). Bias gradients sum the unrounded dg and du. Sums have
+most; bfloat16 outside 2^-16 .. 2^16 by 2^-8, and beyond 2^79 a factor is NaN). Bias gradients sum the unrounded dg and du. Sums have
 a fixed order: the same inputs give the same bits.
 
 x and the weights are read in place when their rows are 16-byte aligned and K is a

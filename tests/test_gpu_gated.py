@@ -219,6 +219,27 @@ def test_arguments_far_out(name, dtype):
         verify({**s, "x": x.repeat(9, 1), "dy": s["dy"].repeat(9, 1)}, name)
 
 
+@pytest.mark.parametrize("exponent", [12, 15, 16, 17, 30, 33, 45, 60, 70])
+def test_large_factors(exponent):
+    """bfloat16 factors of 2^16 and more are off by 2^-8 at most, one of the roundings that u counts: products of
+    a row of x has one element, so that the products are exact but for a rounding, whatever their size."""
+    g = torch.Generator().manual_seed(exponent)
+    M, N, K = 40, 24, 8
+    one = torch.zeros(M, K)
+    one[torch.arange(M), torch.arange(M) % K] = torch.rand(M, generator=g) + 1.0
+    s = {"x": one.bfloat16(), "wg": (torch.rand(N, K, generator=g) + 0.5).bfloat16(),
+         "wu": ((torch.rand(N, K, generator=g) - 0.5) * 2.0 ** exponent).bfloat16(), "bg": None, "bu": None,
+         "dy": (torch.randn(M, N, generator=g) * 2.0 ** -exponent).bfloat16()}
+    got = run(s, None)
+    x, wg, wu, dy = (s[k].double() for k in ("x", "wg", "wu", "dy"))
+    dg, du = dy * (x @ wu.t()), dy * (x @ wg.t())
+    u_ = 2.0 ** -8  # of the code, of dg or du, and of the result; terms of float32 sums besides
+    step = (1 + u_) ** 3 * (1 + F32 * 2 * M) - 1
+    for k, terms in (("dwg", (dg.t().abs() @ x.abs(), dg.t() @ x)), ("dwu", (du.t().abs() @ x.abs(), du.t() @ x)),
+                     ("dx", (dg.abs() @ wg.abs() + du.abs() @ wu.abs(), dg @ wg + du @ wu))):
+        assert ((got[k].cpu().double() - terms[1]).abs() <= step * terms[0] + TINY[torch.bfloat16]).all(), k
+
+
 def test_small_factors_reach_the_weights():
     """A unit whose arguments all lie at -20, where SiLU is -4e-8: its gradients are those of the formula."""
     M, K = 256, 16

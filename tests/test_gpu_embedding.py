@@ -71,7 +71,7 @@ def verify(ids, w, dy, scale=1.0, padding=None):
 
 # tokens around the stretches of 32 and the sorts' limits, ids around digits' limits, widths around the pieces
 SIZES = [(1, 1, 1), (1, 5, 3), (2, 300, 8), (31, 7, 9), (32, 7, 16), (33, 2, 64), (64, 1000, 100), (65, 3, 513), (200, 50, 1030),
-         (1000, 1023, 24), (1025, 1024, 40), (3000, 1025, 77), (5001, 1009, 300), (16384, 70, 33), (16385, 70, 33),
+         (1000, 1023, 24), (1025, 1024, 40), (3000, 1025, 77), (5001, 1009, 300), (14336, 70, 33), (14337, 70, 33), (16384, 70, 33), (16385, 70, 33),
          (16400, 1, 8), (20000, 1024, 17), (20480, 100000, 8), (30001, 1048576, 3), (70000, 4097, 64)]
 
 

@@ -33,6 +33,10 @@ constexpr int64_t kRankMost = 14336;
 constexpr int kRows = 64;            // ids of a workgroup that writes zeros
 constexpr int kBits = 10;            // of a digit, at most
 constexpr int kTile = 4096;          // tokens of a workgroup of the radix sort
+// A gradient of at least this many bytes is stored past the caches, which cannot hold it for its next reader (rows of 1024
+// bf16 elements, the gradient alone and with a reader after it, us, through the caches / past them: 49152 rows 51 and 80 / 51
+// and 82, 98304 59 and 135 / 65 and 141, 131072 118 and 209 / 92 and 195).
+constexpr int64_t kPast = 224 << 20;
 
 // The id of token t as a key of the sort: V for tokens without a gradient (outside 0 .. V - 1, or the padding id).
 __device__ __forceinline__ int32_t key_of(const EmbeddingArgs& a, int64_t t) {
@@ -94,7 +98,13 @@ __device__ __forceinline__ void write_zeros(const EmbeddingArgs& a, int64_t v0) 
     if (!absent[r]) continue;
     char* row = static_cast<char*>(a.out) + (v0 + r) * bytes;
     const u32x4_t zero = {0u, 0u, 0u, 0u};
-    for (int64_t at = lane * 16; at + 16 <= bytes; at += 64 * 16) __builtin_memcpy(row + at, &zero, 16);
+    if (a.past) {
+      typedef u32x4_t loose_t __attribute__((aligned(2)));
+      for (int64_t at = lane * 16; at + 16 <= bytes; at += 64 * 16)
+        __builtin_nontemporal_store(zero, reinterpret_cast<loose_t*>(row + at));
+    } else {
+      for (int64_t at = lane * 16; at + 16 <= bytes; at += 64 * 16) __builtin_memcpy(row + at, &zero, 16);
+    }
     const int64_t rest = bytes & ~(int64_t)15;  // elements of 2 or 4 bytes, a pair of bytes a lane
     if (rest + lane * 2 < bytes) *reinterpret_cast<uint16_t*>(row + rest + lane * 2) = 0;
   }
@@ -291,7 +301,10 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(EmbeddingArgs a, uin
           Piece<T, V> o;
 #pragma unroll
           for (int i = 0; i < V; ++i) o.v[i] = (T)(s[i] * a.scale);
-          o.template store<WHOLE>(out + (int64_t)key * a.d + col, a.d - col);
+          if (a.past)
+            o.template store<WHOLE, true>(out + (int64_t)key * a.d + col, a.d - col);
+          else
+            o.template store<WHOLE>(out + (int64_t)key * a.d + col, a.d - col);
         } else {
           // an id that goes on: its first stretch's sum in slot 1, the later ones' in slot 0
           float* part = a.part + ((stretch * 2 + (begins ? 1 : 0)) * blocks) * 64 * V + col;
@@ -417,6 +430,7 @@ hipError_t gradient(int kind, EmbeddingArgs a, char* ws, hipStream_t s) {
   a.order = lists[1];
   a.seen = reinterpret_cast<int32_t*>(ws + l.total - l.part - l.seen);
   a.size = (int)sizeof(T);
+  a.past = a.V * a.d * a.size >= kPast;
   const int64_t rows = (a.V + kRows - 1) / kRows;  // workgroups that write zeros
   if (a.T > kRankMost) {
     int32_t* counts = reinterpret_cast<int32_t*>(ws + 4 * l.keys);

@@ -229,7 +229,8 @@ struct EmbeddingArgs {
   int64_t padding;       // the id without a gradient, or -1
   int d;
   int ids64;
-  int size;              // bytes of an element (set by launch_embedding_bwd)
+  int size;              // bytes of an element (set by launch_embedding_bwd, as is the next)
+  int past;              // dw is stored past the caches
   float scale;
 };
 

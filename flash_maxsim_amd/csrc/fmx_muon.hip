@@ -127,6 +127,18 @@ __device__ __forceinline__ void store8(void* base, int64_t at, int left, const f
   }
 }
 
+// 8 float32 values past the caches, which are left to what is read again: the momentum is next read whole. (24 matrices of
+// 1024 x 4096 224 -> 175 us for the launch; steps over 4 to 36 of them 1 to 3 % less, so too over 12 of 512 x 2048.)
+__device__ __forceinline__ void store_past(float* p, int left, const float (&v)[8]) {
+  if (left >= 8) {
+    typedef f32x4_t loose_t __attribute__((aligned(4)));
+    __builtin_nontemporal_store(f32x4_t{v[0], v[1], v[2], v[3]}, reinterpret_cast<loose_t*>(p));
+    __builtin_nontemporal_store(f32x4_t{v[4], v[5], v[6], v[7]}, reinterpret_cast<loose_t*>(p + 4));
+  } else {
+    store8<FMX_DTYPE_F32>(p, 0, left, v);
+  }
+}
+
 // u of 8 elements from the gradient and the (new) momentum.
 __device__ __forceinline__ void direction(float (&u)[8], const float (&g)[8], const float (&m)[8], const Table& t,
                                           bool momentum, float scale) {
@@ -158,7 +170,7 @@ __global__ void __launch_bounds__(256) muon_momentum_kernel(Table t) {
       load8<FMX_DTYPE_F32>(m, e.momentum, from, left);
 #pragma unroll
       for (int k = 0; k < 8; ++k) m[k] = t.mu * m[k] + t.omu * (g[k] * scale);
-      store8<FMX_DTYPE_F32>(e.momentum, from, left, m);
+      store_past(e.momentum + from, left, m);
     }
     direction(u, g, m, t, e.momentum != nullptr, scale);
 #pragma unroll
@@ -195,13 +207,14 @@ __global__ void __launch_bounds__(256) muon_start_kernel(Table t) {
   const double by = (double)kX / (norm <= t.eps ? t.eps : norm);  // a norm that is NaN stays so
   const float scale = t.grad_scale ? *t.grad_scale : 1.0f;
   const bool tall = e.rows > e.cols;
-  const int row = threadIdx.x >> 2, part = (threadIdx.x & 3) * 16;
+  // 8 lanes a row, a line of memory; rows r and r + 32 of the tile
+  const int row = threadIdx.x >> 3, part = (threadIdx.x & 7) * 8;
   // the tile's rows as the parameter has them: of i, or of j
   const int r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;
   float x[2][8];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int r = r0 + row, c = c0 + part + 8 * h;
+    const int r = r0 + row + 32 * h, c = c0 + part;
     const int left = r < e.rows ? (e.cols - c < 8 ? e.cols - c : 8) : 0;
     float g[8], m[8];
 #pragma unroll
@@ -219,16 +232,16 @@ __global__ void __launch_bounds__(256) muon_start_kernel(Table t) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) tile[part + 8 * h + k][row] = x[h][k];
+      for (int k = 0; k < 8; ++k) tile[part + k][row + 32 * h] = x[h][k];
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[h][k] = tile[row][part + 8 * h + k];
+      for (int k = 0; k < 8; ++k) x[h][k] = tile[row + 32 * h][part + k];
   }
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int64_t at = (int64_t)(i0 + row) * e.m + j0 + part + 8 * h;
+    const int64_t at = (int64_t)(i0 + row + 32 * h) * e.m + j0 + part;
     const u32x4_t hi = pack8(x[h], false);
     float up[8];
     unpack8(up, hi, false);
@@ -254,6 +267,114 @@ __device__ __forceinline__ void move8(const Table& t, const Entry& e, int64_t at
   }
   store8<P>(e.param, at, left, x);
   if (P == FMX_DTYPE_F32 && e.copy) store16(e.copy, at, left, x, copy_bf);
+}
+
+// A lane's 8 neighbouring columns of a pair of j fragments; of a row-major operand the lanes exchange halves.
+template <bool BMAJ>
+__device__ __forceinline__ void pair_of(const f32x4_t& a, const f32x4_t& b, float (&v)[8]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[k] = a[k];
+    v[4 + k] = b[k];
+    if constexpr (BMAJ) {
+      const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v[k]),
+                                                      __builtin_bit_cast(uint32_t, v[4 + k]), false, false);
+      const uint32_t r0 = r[0], r1 = r[1];
+      v[k] = __builtin_bit_cast(float, r0);
+      v[4 + k] = __builtin_bit_cast(float, r1);
+    }
+  }
+}
+
+// From a wave's products of FI x FJ fragments, from row iw and column jw on, to the next X and its lower half (kNext) or to
+// the parameter (kLast; P: its type), in whole lines: `mine` is LDS of the wave's own, kTurn bytes. What lies outside of X
+// is left out.
+constexpr int kTurn = 4096;
+template <int FORM, int P, int FI, int FJ>
+__device__ __forceinline__ void finish_x(const Table& t, const Entry& e, const f32x4_t (&acc)[FI][FJ], int64_t iw, int64_t jw,
+                                         unsigned char* mine, int lane, int copy_bf) {
+  constexpr int ROW = FJ * 32, CH = ROW / 16;  // bytes of a 16-bit row of the block, 16-byte pieces of it
+  static_assert(16 * ROW <= kTurn && FJ * 16 * 16 * 4 <= kTurn, "a wave's block");
+  const int c = lane & 15, g = lane >> 4, of = (g & 1) * 16 + (g >> 1) * 8;
+  auto spot = [&](int r, int ch) __attribute__((always_inline)) { return mine + r * ROW + ((ch ^ (r & (CH - 1))) << 4); };
+  auto put = [&](int ch, const u32x4_t& w) __attribute__((always_inline)) { *reinterpret_cast<u32x4_t*>(spot(c, ch)) = w; };
+  // the block's first element: its others lie within 128 rows of at most 2^21 bytes, below 2^31
+  const int64_t first = iw * e.m + jw;
+  const int pitch = e.m * 2, rows = jw < e.m ? (int)(e.n - iw) : 0;
+  const uint32_t out_at = (uint32_t)((lane / CH) * pitch + (lane % CH) * 16), in_at = (uint32_t)(c * pitch + of * 2);
+  auto flush = [&](int x, rsrc_t out) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 16 * CH / 64; ++h) {
+      const u32x4_t w = *reinterpret_cast<const u32x4_t*>(spot(h * (64 / CH) + lane / CH, lane % CH));
+      __builtin_amdgcn_raw_buffer_store_b128(w, out, x * 16 < rows ? out_at : kOOB, (x * 16 + h * (64 / CH)) * pitch, 0);
+    }
+  };
+  const rsrc_t rl = make_rsrc(low_of(t, e) + first, 0x7fffffffu);
+  const rsrc_t rx = make_rsrc(x_of(t, e, t.from ^ 1) + first, 0x7fffffffu);
+  const bool tall = e.rows > e.cols;
+  // kLast of a tall parameter: [FJ * 16][16], a 16-row block turned round, its columns swizzled
+  float* turn = reinterpret_cast<float*>(mine);
+  auto turned = [&](int j, int i) __attribute__((always_inline)) { return j * 16 + (i ^ (j & 15)); };
+  // Everything that is read, before the first store: loads behind stores would wait for them. (No branches: rows past X's
+  // read as zeros, and what is stored to them goes nowhere.)
+  u32x4_t low[FI][FJ / 2];
+#pragma unroll
+  for (int x = 0; x < FI; ++x)
+#pragma unroll
+    for (int y = 0; y < FJ; y += 2)
+      low[x][y / 2] = __builtin_amdgcn_raw_buffer_load_b128(rl, x * 16 < rows ? in_at + y * 32 : kOOB, x * 16 * pitch, 0);
+#pragma unroll
+  for (int x = 0; x < FI; ++x) {
+    u32x4_t down[FJ / 2];
+#pragma unroll
+    for (int y = 0; y < FJ; y += 2) {
+      float v[8], hi[8], lo[8];
+      pair_of<true>(acc[x][y], acc[x][y + 1], v);
+      const int64_t i = iw + x * 16 + c, j = jw + y * 16 + of;
+      unpack8(lo, low[x][y / 2], false);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = t.a * lo[k] + v[k] * (1.0f / kA);
+      if constexpr (FORM == kNext) {
+        const u32x4_t h = pack8(v, false);
+        unpack8(hi, h, false);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] -= hi[k];
+        put(y * 2 + of / 8, h);
+        down[y / 2] = pack8(v, false);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= 1.0f / kX;
+        if (!tall) {
+          const int left = e.cols - j < 8 ? (int)(e.cols - j) : 8;
+          if (i < e.rows && left > 0) move8<P>(t, e, i * e.cols + j, left, v, copy_bf);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) turn[turned(y * 16 + of + k, c)] = v[k];
+        }
+      }
+    }
+    if constexpr (FORM == kNext) {
+      flush(x, rx);
+#pragma unroll
+      for (int y = 0; y < FJ; y += 2) put(y * 2 + of / 8, down[y / 2]);
+      flush(x, rl);
+    }
+    if constexpr (FORM == kLast) {
+      if (tall) {
+        // row j of the parameter, its elements i .. i + 7
+#pragma unroll
+        for (int h = 0; h < FJ / 2; ++h) {
+          const int jr = h * 32 + (lane >> 1), part = (lane & 1) * 8;
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = turn[turned(jr, part + k)];
+          const int64_t j = jw + jr, i = iw + x * 16 + part;
+          const int left = e.cols - i < 8 ? (int)(e.cols - i) : 8;
+          if (j < e.rows && left > 0) move8<P>(t, e, j * e.cols + i, left, v, copy_bf);
+        }
+      }
+    }
+  }
 }
 
 // P: the parameters' type (kLast)
@@ -346,28 +467,13 @@ __global__ void __launch_bounds__(WI* WJ * 64) muon_kernel(Table t, int copy_bf)
   run_stages<NS, LOADS, FJ*(BMAJ ? 2 : 1) + FI, FI * FJ>(nit, buffer, issue, read, multiply, [](auto) {});
 
   // A lane's results: row c of each i fragment, and of a pair of j fragments 8 columns, from column `of` of the pair's 32 on.
-  const int c = lane & 15, g = lane >> 4;
-  const int of = BMAJ ? (g & 1) * 16 + (g >> 1) * 8 : 8 * g;
-  auto pair = [&](int x, int y, float (&v)[8]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[k] = acc[x][y][k];
-      v[4 + k] = acc[x][y + 1][k];
-      if constexpr (BMAJ) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v[k]),
-                                                        __builtin_bit_cast(uint32_t, v[4 + k]), false, false);
-        const uint32_t r0 = r[0], r1 = r[1];
-        v[k] = __builtin_bit_cast(float, r0);
-        v[4 + k] = __builtin_bit_cast(float, r1);
-      }
-    }
-  };
+  const int c = lane & 15, g = lane >> 4, of = 8 * g;
   stage_barrier();  // LDS is free: nothing is loaded into it or read from it any more
   constexpr int ROW = FJ * 32;  // bytes of a wave's 16-bit row
   unsigned char* mine = (wave < WI * WJ / 2 ? lds0 : lds1) + (wave % (WI * WJ / 2)) * (BYTES / (WI * WJ / 2));
-  static_assert(BYTES / (WI * WJ / 2) >= FI * 16 * ROW && BYTES / (WI * WJ / 2) >= FJ * 16 * 17 * 4, "a wave's block");
+  static_assert(BYTES / (WI * WJ / 2) >= FI * 16 * ROW && BYTES / (WI * WJ / 2) >= kTurn, "a wave's block");
   const int64_t iw = i0 + wi * FI * 16, jw = j0 + wj * FJ * 16;
-  if (jw >= width) return;  // sides are multiples of 64 and a wave's block begins at one of FJ * 16
+  if (jw >= width || iw >= e.n) return;  // sides are multiples of 64 and a wave's block begins at one of 32 at least
 
   // 16-bit rows of the block in LDS, 16 bytes at a time, and from there to memory as whole lines
   auto spot = [&](int r, int ch) __attribute__((always_inline)) { return mine + r * ROW + ((ch ^ (r & (ROW / 16 - 1))) << 4); };
@@ -392,7 +498,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) muon_kernel(Table t, int copy_bf)
 #pragma unroll
       for (int y = 0; y < FJ; y += 2) {
         float v[8];
-        pair(x, y, v);
+        pair_of<false>(acc[x][y], acc[x][y + 1], v);
         const int64_t at = (iw + x * 16 + c) * e.n + jw + y * 16 + of;
         if constexpr (FORM == kGram) {
 #pragma unroll
@@ -427,71 +533,169 @@ __global__ void __launch_bounds__(WI* WJ * 64) muon_kernel(Table t, int copy_bf)
       }
     }
   } else {
-    uint16_t* xl = low_of(t, e);
-    const bool tall = e.rows > e.cols;
-    float* turn = reinterpret_cast<float*>(mine);  // kLast of a tall parameter: [FJ * 16][17], a 16-row block turned round
-    // everything that is read, before the first store: loads behind stores would wait for them
-    u32x4_t low[FI][FJ / 2];
-#pragma unroll
-    for (int x = 0; x < FI; ++x) {
-      if (iw + x * 16 >= e.n) break;
-#pragma unroll
-      for (int y = 0; y < FJ; y += 2) low[x][y / 2] = load_raw(xl, (iw + x * 16 + c) * e.m + jw + y * 16 + of, 8);
-    }
-#pragma unroll
-    for (int x = 0; x < FI; ++x) {
-      if (iw + x * 16 >= e.n) break;
-      u32x4_t down[FJ / 2];
-#pragma unroll
-      for (int y = 0; y < FJ; y += 2) {
-        float v[8], hi[8], lo[8];
-        pair(x, y, v);
-        const int64_t i = iw + x * 16 + c, j = jw + y * 16 + of;
-        unpack8(lo, low[x][y / 2], false);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = t.a * lo[k] + v[k] * (1.0f / kA);
-        if constexpr (FORM == kNext) {
-          const u32x4_t h = pack8(v, false);
-          unpack8(hi, h, false);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] -= hi[k];
-          put(x, y * 2 + of / 8, h);
-          down[y / 2] = pack8(v, false);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] *= 1.0f / kX;
-          if (!tall) {
-            const int left = e.cols - j < 8 ? (int)(e.cols - j) : 8;
-            if (i < e.rows && left > 0) move8<P>(t, e, i * e.cols + j, left, v, copy_bf);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) turn[(y * 16 + of + k) * 17 + c] = v[k];
-          }
-        }
-      }
-      if constexpr (FORM == kNext) {
-        flush(x, x_of(t, e, t.from ^ 1));
-#pragma unroll
-        for (int y = 0; y < FJ; y += 2) put(x, y * 2 + of / 8, down[y / 2]);
-        flush(x, xl);
-      }
-      if constexpr (FORM == kLast) {
-        if (tall) {
-          // row j of the parameter, its elements i .. i + 7
-#pragma unroll
-          for (int h = 0; h < FJ / 2; ++h) {
-            const int jr = h * 32 + (lane >> 1), part = (lane & 1) * 8;
-            float v[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = turn[jr * 17 + part + k];
-            const int64_t j = jw + jr, i = iw + x * 16 + part;
-            const int left = e.cols - i < 8 ? (int)(e.cols - i) : 8;
-            if (j < e.rows && left > 0) move8<P>(t, e, j * e.cols + i, left, v, copy_bf);
-          }
-        }
-      }
-    }
+    finish_x<FORM, P, FI, FJ>(t, e, acc, iw, jw, mine, lane, copy_bf);
   }
+}
+
+// X's products in tiles of 256 x 256: a workgroup on each compute unit takes tile after tile, the next one's first two stages
+// are loaded before a tile is finished, and its stores drain while the next tile's first stage is multiplied. (24 matrices of
+// 1024 x 4096 311 -> 294 us. The products alone take 206 of them, what is read and written besides 150: they share the unit's
+// path to the caches, and of the 990 MB that HBM moves 400 are stores. Not waiting for those in the first stage took
+// registers that spilled, 305; starting the units at different times and storing past the caches gained nothing.)
+template <int FORM, int P>
+__global__ void __launch_bounds__(512) muon_next_kernel(Table t, int copy_bf) {
+  constexpr int WI = 2, FI = 8, FJ = 4, TI = 256, NT = 512, BYTES = 2 * TI * BK * 2;
+  using SideA = Side<false, false, TI, NT>;
+  using SideB = Side<true, false, TI, NT>;
+  constexpr int LOADS = SideA::kLoads + SideB::kLoads, READS = 2 * FJ + FI;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds0[BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds1[BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char own[8 * kTurn];
+
+  int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wi = wave % WI, wj = wave / WI;
+  Frags<false, false, TI> fa(wi * FI * 16, tid & 63);
+  Frags<true, false, TI> fb(wj * FJ * 16, tid & 63);
+  // Addresses made of these are made anew for every tile, and hold no registers where they are not used.
+  auto fresh = [](auto& v) __attribute__((always_inline)) { __asm__ volatile("" : "+v"(v)); };
+  struct Tile {
+    int at, i0;
+    int64_t j0;
+  };
+  auto place = [&](uint32_t id) __attribute__((always_inline)) {
+    // workgroups go to the eight XCDs in turn; each XCD takes a run of consecutive tiles
+    const uint32_t per = t.total / 8, x = id & 7, rest = t.total & 7;
+    return (id >> 3) + x * per + (x < rest ? x : rest);
+  };
+  auto locate = [&](uint32_t id, int at) __attribute__((always_inline)) {
+    Tile o;
+    o.at = at;
+    const Entry& e = t.e[o.at];
+    id -= t.first[o.at];
+    // the rows of a column of tiles, which read the same columns of X, one after the other
+    const uint32_t ti = (uint32_t)(e.n + TI - 1) / TI, col = id / ti;
+    o.i0 = (int)(id - col * ti) * TI;
+    o.j0 = (int64_t)col * TI;
+    return o;
+  };
+  // What a tile's stages are loaded from, as Side loads them, with what all lanes share in scalar registers: a thread's
+  // chunks of B lie 64 rows apart, those of X 16, and sides are multiples of 64.
+  const char *pa, *pb;
+  int depth, rows, pitch;
+  uint32_t va_at, vb_at;
+  auto begin = [&](const Tile& o) __attribute__((always_inline)) {
+    const Entry& e = t.e[o.at];
+    pa = reinterpret_cast<const char*>(b_of(t, e) + (int64_t)o.i0 * e.n);
+    pb = reinterpret_cast<const char*>(x_of(t, e, t.from) + o.j0);
+    depth = e.n;
+    rows = e.n - o.i0;
+    pitch = e.m * 2;
+    const int ra = tid / 8, rb = tid / 32;
+    const int ca = (tid % 8) ^ SideA::key(ra), cb = (tid % 32) ^ SideB::key(rb);
+    va_at = (uint32_t)(ra * depth * 2 + ca * 16);
+    vb_at = o.j0 + cb * 8 < e.m ? (uint32_t)(rb * pitch + cb * 16) : kOOB;
+  };
+  const uint32_t first = place(blockIdx.x);
+  Tile o = locate(first, __builtin_amdgcn_readfirstlane(entry_of(t, first)));
+  begin(o);
+  f32x4_t acc[FI][FJ];
+  u32x4_t va[2][FI], vb[2][FJ];
+  // stage `it`; past the last one zeros
+  auto issue = [&](unsigned char* lds, int it) __attribute__((always_inline)) {
+    const bool have = it * BK < depth;
+    const char *a = pa + it * BK * 2, *b = pb + (int64_t)it * BK * pitch;
+#pragma unroll
+    for (int n = 0; n < SideA::kLoads; ++n)
+      dma16_lds<false>(make_rsrc(a + (int64_t)(n * 64) * depth * 2, 0x7fffffffu), lds + (n * NT + wave * 64) * 16,
+                       have && n * 64 < rows ? va_at : kOOB);
+#pragma unroll
+    for (int n = 0; n < SideB::kLoads; ++n)
+      dma16_lds<false>(make_rsrc(b + (int64_t)(n * 16) * pitch, 0x7fffffffu), lds + TI * BK * 2 + (n * NT + wave * 64) * 16,
+                       have ? vb_at : kOOB);
+  };
+  auto read = [&](auto set, const unsigned char* lds, int kk) __attribute__((always_inline)) {
+    constexpr int Z = decltype(set)::value;
+#pragma unroll
+    for (int y = 0; y < FJ; ++y) vb[Z][y] = fb.read(lds + TI * BK * 2, y, kk);
+    fresh(fa.at[kk]);
+#pragma unroll
+    for (int x = 0; x < FI; ++x) va[Z][x] = fa.read(lds, x, kk);
+  };
+  auto multiply = [&](auto set) __attribute__((always_inline)) {
+    constexpr int Z = decltype(set)::value;
+#pragma unroll
+    for (int x = 0; x < FI; ++x)
+#pragma unroll
+      for (int y = 0; y < FJ; ++y) acc[x][y] = mfma16x16x32<false>(vb[Z][y], va[Z][x], acc[x][y]);
+  };
+  // The stage in `lds`, while stage `it` (of this tile or the next) is loaded behind it and, unless it is the tile's last,
+  // the first fragments of the one in `other` are read: run_stages' order.
+  auto stage = [&](unsigned char* lds, const unsigned char* other, int it, auto last) __attribute__((always_inline)) {
+    read(set1, lds, 1);
+    multiply(set0);
+    wait_vmem<0>();
+    stage_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    issue(lds, it);
+    if constexpr (!decltype(last)::value) read(set0, other, 0);
+    multiply(set1);
+#pragma unroll
+    for (int n = 0; n < LOADS; ++n) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    }
+    if constexpr (!decltype(last)::value) {
+#pragma unroll
+      for (int n = 0; n < READS / 2; ++n) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, FI * FJ, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr std::false_type more_follow{};
+  constexpr std::true_type last_one{};
+  issue(lds0, 0);
+  issue(lds1, 1);
+  wait_vmem<LOADS>();
+  stage_barrier();
+  for (uint32_t id = blockIdx.x;; id += gridDim.x) {
+    fresh(fb.at[0]);
+    read(set0, lds0, 0);
+#pragma unroll
+    for (int x = 0; x < FI; ++x)
+#pragma unroll
+      for (int y = 0; y < FJ; ++y) acc[x][y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    const int nit = (depth + 2 * BK - 1) / (2 * BK) * 2;  // in pairs: a tile begins in lds0 (a stage past the end is zeros)
+    for (int it = 2; it < nit; it += 2) {
+      stage(lds0, lds1, it, more_follow);
+      stage(lds1, lds0, it + 1, more_follow);
+    }
+    const Tile now = o;
+    const bool more = id + gridDim.x < t.total;
+    fresh(tid);
+    if (more) {
+      // from the last tile's entry on, by scalar loads: entry_of's would wait for the stages in flight
+      const uint32_t next = place(id + gridDim.x);
+      int at = o.at;
+      while (at + 1 < t.count && t.first[at + 1] <= next) ++at;
+      while (t.first[at] > next) --at;
+      o = locate(next, at);
+      begin(o);
+    } else {
+      depth = 0;  // nothing is read, zeros reach LDS
+    }
+    stage(lds0, lds1, 0, more_follow);
+    stage(lds1, lds0, 1, last_one);
+    const Entry& e = t.e[now.at];
+    const int64_t jw = now.j0 + wj * FJ * 16;
+    fresh(tid);
+    finish_x<FORM, P, FI, FJ>(t, e, acc, now.i0 + wi * FI * 16, jw, own + wave * kTurn, tid & 63, copy_bf);
+    if (!more) break;
+  }
+  wait_vmem<0>();  // the empty stages' DMA writes no longer reach LDS after this wave ends
 }
 
 constexpr int kSizes[] = {256, 128, 64};  // of tiles
@@ -545,7 +749,14 @@ hipError_t run_form(Table t, int copy_bf, hipStream_t s) {
   }
   t.total = total;
   switch (size) {
-    case 0: muon_kernel<FORM, P, 2, 4, 8, 4, 2><<<total, 512, 0, s>>>(t, copy_bf); break;
+    case 0:
+      if constexpr (FORM == kGram || FORM == kPolynomial) {
+        muon_kernel<FORM, P, 2, 4, 8, 4, 2><<<total, 512, 0, s>>>(t, copy_bf);
+      } else {
+        const uint32_t cus = (uint32_t)layer_cus();
+        muon_next_kernel<FORM, P><<<total < cus ? total : cus, 512, 0, s>>>(t, copy_bf);
+      }
+      break;
     case 1: muon_kernel<FORM, P, 2, 2, 4, 4, 2><<<total, 256, 0, s>>>(t, copy_bf); break;
     default: muon_kernel<FORM, P, 2, 2, 2, 2, 4><<<total, 256, 0, s>>>(t, copy_bf); break;
   }

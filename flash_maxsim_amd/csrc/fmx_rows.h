@@ -30,12 +30,18 @@ struct Piece {
       }
     }
   }
-  template <bool WHOLE>
+  // PAST: past the caches, for what is too large to be found in them
+  template <bool WHOLE, bool PAST = false>
   __device__ __forceinline__ void store(T* p, int left) const {
     if (WHOLE ? left > 0 : left >= V) {
       words_t w;
       __builtin_memcpy(&w, v, sizeof(w));
-      __builtin_memcpy(p, &w, sizeof(w));
+      if constexpr (PAST) {
+        typedef words_t loose_t __attribute__((aligned(sizeof(T))));
+        __builtin_nontemporal_store(w, reinterpret_cast<loose_t*>(p));
+      } else {
+        __builtin_memcpy(p, &w, sizeof(w));
+      }
     } else if constexpr (!WHOLE) {
 #pragma unroll
       for (int i = 0; i < V - 1; ++i)

@@ -23,7 +23,8 @@
 // twice, the second time through transposing reads. Matrices taller than wide are transposed when X is made, and the
 // last product's epilogue, which moves the parameters, transposes back.
 //
-// A launch walks the tiles of up to kMost matrices of any shapes, from a table in its arguments.
+// A launch walks the tiles of up to kMost matrices of any shapes, from a table in its arguments: two for the momentum and X, three
+// a step (A, B, X), two where the matrices are small.
 #include <math.h>
 
 #include "fmx_device.h"
@@ -84,7 +85,7 @@ __device__ __forceinline__ double* squares_of(const Table& t, const Entry& e) {
 }
 
 // The entry that workgroup `id` works for: the last one whose first workgroup is not past it. One load for all: a search
-// waits for the arguments' memory once for every step (a step over four small matrices, 17 launches, 102 us by a search, 97).
+// waits for the arguments' memory once for every step (17 launches over four small matrices 102 -> 97 us).
 __device__ __forceinline__ int entry_of(const Table& t, uint32_t id) {
   const int lane = threadIdx.x & 63;
   const uint32_t first = t.first[lane < kMost ? lane : kMost - 1];
@@ -263,10 +264,16 @@ __device__ __forceinline__ void move8(const Table& t, const Entry& e, int64_t at
     float p[8];
     load8<P>(p, e.param, at, left);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = p[k] * t.keep - e.rate * x[k];
+    for (int k = 0; k < 8; ++k) x[k] = __builtin_fmaf(-e.rate, x[k], p[k] * t.keep);
   }
   store8<P>(e.param, at, left, x);
   if (P == FMX_DTYPE_F32 && e.copy) store16(e.copy, at, left, x, copy_bf);
+}
+
+// b A + c A^2 of an element, as B is held. (Multiplications and additions are fused as written here and in finish_x: a matrix
+// has the same bits by whichever kernel.)
+__device__ __forceinline__ float polynomial(const Table& t, float a, float square) {
+  return __builtin_fmaf(t.b, a, t.c / kA * square);
 }
 
 // A lane's 8 neighbouring columns of a pair of j fragments; of a row-major operand the lanes exchange halves.
@@ -333,7 +340,7 @@ __device__ __forceinline__ void finish_x(const Table& t, const Entry& e, const f
       const int64_t i = iw + x * 16 + c, j = jw + y * 16 + of;
       unpack8(lo, low[x][y / 2], false);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = t.a * lo[k] + v[k] * (1.0f / kA);
+      for (int k = 0; k < 8; ++k) v[k] = __builtin_fmaf(t.a, lo[k], v[k] * (1.0f / kA));
       if constexpr (FORM == kNext) {
         const u32x4_t h = pack8(v, false);
         unpack8(hi, h, false);
@@ -507,7 +514,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) muon_kernel(Table t, int copy_bf)
           float w[8];
           load16(w, in, at, 8, false);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = t.b * w[k] + (t.c / kA) * v[k];
+          for (int k = 0; k < 8; ++k) v[k] = polynomial(t, w[k], v[k]);
           const int64_t off = iw + x * 16 + c - (jw + y * 16 + of);  // of the diagonal among the 8
 #pragma unroll
           for (int k = 0; k < 8; ++k) v[k] += k == off ? t.a * kA : 0.0f;
@@ -698,6 +705,126 @@ __global__ void __launch_bounds__(512) muon_next_kernel(Table t, int copy_bf) {
   wait_vmem<0>();  // the empty stages' DMA writes no longer reach LDS after this wave ends
 }
 
+// Small matrices (n up to kSmall, all tiles of a launch at once): a product's launch for X makes its rows of B itself, from
+// all of A in LDS, and B has no launch of its own: 64 x 64 of X a workgroup, 64 x n of B before. (Five steps over matrices of,
+// us: 64 x 1024 82 -> 67, 128 x 768 83 -> 66, 256 x 256 80 -> 69, four of 256 x 1024 101 -> 92; launch by launch of those 4.7 and
+// 5.4 -> 8.1. Eight stages in LDS for their Gram matrices: 256 x 4096 159 -> 148, 256 x 1024 the same, 256 x 256 69 -> 71: not kept.)
+constexpr int kSmall = 256;
+template <int FORM, int P>
+__global__ void __launch_bounds__(256) muon_small_kernel(Table t, int copy_bf) {
+  constexpr int FI = 2, FJ = 2, BLOCK = 64 * BK * 2, NB = kSmall / 64;  // 64 x 64 elements of 16 bits
+  using SideA = Side<false, false, 64, 256>;
+  using SideX = Side<true, false, 64, 256>;
+  __shared__ __attribute__((aligned(1024))) unsigned char all[NB * NB * BLOCK];  // A by blocks, then X's columns
+  __shared__ __attribute__((aligned(1024))) unsigned char panel[NB * BLOCK];     // B's rows
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wi = wave & 1, wj = wave >> 1;
+  // workgroups go to the eight XCDs in turn; each XCD takes a run of consecutive tiles
+  uint32_t id = blockIdx.x;
+  {
+    const uint32_t per = t.total / 8, x = id & 7, rest = t.total & 7;
+    id = (id >> 3) + x * per + (x < rest ? x : rest);
+  }
+  const int at = __builtin_amdgcn_readfirstlane(entry_of(t, id));
+  const Entry& e = t.e[at];
+  id -= t.first[at];
+  const int nb = e.n / 64;
+  const int col = (int)id / nb, row = (int)id - col * nb;
+  const int64_t j0 = (int64_t)col * 64;
+
+  const int r = tid >> 3, ch = tid & 7;  // a thread's 16 bytes of 32 rows of 128
+  const rsrc_t ra = make_rsrc(a_of(t, e), 0x7fffffffu);
+  for (int b = 0; b < nb; ++b)
+    for (int k = 0; k < nb; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        dma16_lds<false>(ra, all + (b * nb + k) * BLOCK + (h * 256 + wave * 64) * 16,
+                         (uint32_t)(((b * 64 + h * 32 + r) * e.n + k * 64 + (ch ^ SideA::key(r)) * 8) * 2));
+  // X's columns wait in registers until A's place is free
+  const rsrc_t rx = make_rsrc(x_of(t, e, t.from) + j0, 0x7fffffffu);
+  u32x4_t x[2 * NB];
+#pragma unroll
+  for (int q = 0; q < 2 * NB; ++q)
+    x[q] = ld16(rx, q * 32 < e.n ? (uint32_t)(((q * 32 + r) * (int64_t)e.m + ch * 8) * 2) : kOOB);
+  wait_vmem<2 * NB>();
+  stage_barrier();
+
+  const Frags<false, false, 64> fi(wi * 32, lane), fj(wj * 32, lane);
+  // of row i of a block of B and columns j .. j + 3 of it: where they lie in A's and the panel's blocks
+  auto spot = [&](int i, int j) __attribute__((always_inline)) { return i * 128 + (((j >> 3) ^ (i & 7)) << 4) + (j & 4) * 2; };
+  f32x4_t acc[FI][FJ];
+  auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int a = 0; a < FI; ++a)
+#pragma unroll
+      for (int b = 0; b < FJ; ++b) acc[a][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  };
+  auto multiply = [&](const u32x4_t (&vi)[FI], const u32x4_t (&vj)[FJ]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int a = 0; a < FI; ++a)
+#pragma unroll
+      for (int b = 0; b < FJ; ++b) acc[a][b] = mfma16x16x32<false>(vj[b], vi[a], acc[a][b]);
+  };
+  // Both products for a count of blocks that the compiler knows: fragments are then read well ahead of their multiplication,
+  // and those of the panel's own rows once.
+  auto products = [&](auto blocks) __attribute__((always_inline)) {
+    constexpr int N = decltype(blocks)::value;
+    u32x4_t vi[2 * N][FI];
+#pragma unroll
+    for (int k = 0; k < 2 * N; ++k)
+#pragma unroll
+      for (int a = 0; a < FI; ++a) vi[k][a] = fi.read(all + (row * N + k / 2) * BLOCK, a, k & 1);
+#pragma unroll 1
+    for (int jb = 0; jb < N; ++jb) {
+      clear();
+#pragma unroll
+      for (int k = 0; k < 2 * N; ++k) {
+        const unsigned char* aj = all + (jb * N + k / 2) * BLOCK;
+        const u32x4_t vj[FJ] = {fj.read(aj, 0, k & 1), fj.read(aj, 1, k & 1)};
+        multiply(vi[k], vj);
+      }
+#pragma unroll
+      for (int a = 0; a < FI; ++a)
+#pragma unroll
+        for (int b = 0; b < FJ; ++b) {
+          const int i = wi * 32 + a * 16 + c, j = wj * 32 + b * 16 + 4 * g;
+          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(all + (row * N + jb) * BLOCK + spot(i, j));
+          float v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            v[k] = polynomial(t, unpack((k & 1) ? w[k / 2] >> 16 : w[k / 2] & 0xffffu, false), acc[a][b][k]);
+            v[k] += row == jb && i == j + k ? t.a * kA : 0.0f;
+          }
+          *reinterpret_cast<u32x2_t*>(panel + jb * BLOCK + spot(i, j)) =
+              u32x2_t{pack2(v[0], v[1], false), pack2(v[2], v[3], false)};
+        }
+    }
+    stage_barrier();  // A is not read any more
+#pragma unroll
+    for (int q = 0; q < 2 * N; ++q)
+      *reinterpret_cast<u32x4_t*>(all + (q * 32 + r) * 128 + ((ch ^ SideX::key(r)) << 4)) = x[q];
+    stage_barrier();
+    const Frags<true, false, 64> fx(wj * 32, lane);
+    clear();
+#pragma unroll
+    for (int k = 0; k < 2 * N; ++k) {
+      const unsigned char *bi = panel + (k / 2) * BLOCK, *xj = all + (k / 2) * BLOCK;
+      const u32x4_t vb[FI] = {fi.read(bi, 0, k & 1), fi.read(bi, 1, k & 1)}, vx[FJ] = {fx.read(xj, 0, k & 1), fx.read(xj, 1, k & 1)};
+      multiply(vb, vx);
+    }
+  };
+  switch (nb) {
+    case 1: products(std::integral_constant<int, 1>{}); break;
+    case 2: products(std::integral_constant<int, 2>{}); break;
+    case 3: products(std::integral_constant<int, 3>{}); break;
+    default: products(std::integral_constant<int, NB>{}); break;
+  }
+  // past X's columns there is room in A's place
+  static_assert(NB * BLOCK + 4 * kTurn <= NB * NB * BLOCK, "LDS of the waves' own");
+  finish_x<FORM, P, FI, FJ>(t, e, acc, row * 64 + wi * 32, j0 + wj * 32, all + NB * BLOCK + wave * kTurn, lane, copy_bf);
+}
+
 constexpr int kSizes[] = {256, 128, 64};  // of tiles
 
 // Tiles of a product and the time of their rounds over the compute units, from the linear layer's stages (us): rounds of
@@ -761,6 +888,33 @@ hipError_t run_form(Table t, int copy_bf, hipStream_t s) {
     default: muon_kernel<FORM, P, 2, 2, 2, 2, 4><<<total, 256, 0, s>>>(t, copy_bf); break;
   }
   return hipGetLastError();
+}
+
+// Whether muon_small_kernel takes a launch's matrices.
+bool small(const Table& t) {
+  int64_t tiles = 0;
+  for (int i = 0; i < t.count; ++i) {
+    if (t.e[i].n > kSmall) return false;
+    tiles += tiles_of(t.e[i], kNext, 64);
+  }
+  return tiles <= layer_cus();
+}
+
+template <int FORM, int P>
+hipError_t run_small(Table t, int copy_bf, hipStream_t s) {
+  t.total = 0;
+  for (int i = 0; i < t.count; ++i) {
+    t.first[i] = t.total;
+    t.total += (uint32_t)tiles_of(t.e[i], FORM, 64);
+  }
+  muon_small_kernel<FORM, P><<<t.total, 256, 0, s>>>(t, copy_bf);
+  return hipGetLastError();
+}
+
+// The next X, or (kLast) the parameters.
+template <int FORM, int P>
+hipError_t run_x(const Table& t, bool few, int copy_bf, hipStream_t s) {
+  return few ? run_small<FORM, P>(t, copy_bf, s) : run_form<FORM, P>(t, copy_bf, s);
 }
 
 template <int G>
@@ -869,20 +1023,21 @@ hipError_t launch_muon(int pkind, int gkind, int ckind, const MuonMatrix* x, int
     }
     e = gkind == FMX_DTYPE_F32 ? run_start<FMX_DTYPE_F32>(t, s) : gkind == FMX_DTYPE_BF16 ? run_start<FMX_DTYPE_BF16>(t, s)
                                                                                      : run_start<FMX_DTYPE_F16>(t, s);
+    const bool few = small(t);
     for (int k = 0; k < sc.steps && e == hipSuccess; ++k) {
       t.from = k & 1;
       e = run_form<kGram, 0>(t, 0, s);
-      if (e == hipSuccess) e = run_form<kPolynomial, 0>(t, 0, s);
+      if (e == hipSuccess && !few) e = run_form<kPolynomial, 0>(t, 0, s);
       if (e != hipSuccess) return;
       const int bf = ckind == FMX_DTYPE_BF16;
       if (k + 1 < sc.steps)
-        e = run_form<kNext, 0>(t, 0, s);
+        e = run_x<kNext, 0>(t, few, 0, s);
       else if (pkind == FMX_DTYPE_F32)
-        e = run_form<kLast, FMX_DTYPE_F32>(t, bf, s);
+        e = run_x<kLast, FMX_DTYPE_F32>(t, few, bf, s);
       else if (pkind == FMX_DTYPE_BF16)
-        e = run_form<kLast, FMX_DTYPE_BF16>(t, bf, s);
+        e = run_x<kLast, FMX_DTYPE_BF16>(t, few, bf, s);
       else
-        e = run_form<kLast, FMX_DTYPE_F16>(t, bf, s);
+        e = run_x<kLast, FMX_DTYPE_F16>(t, few, bf, s);
     }
   });
   return e;

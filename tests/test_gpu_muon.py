@@ -102,6 +102,29 @@ def test_large_tiles(rows, cols, count):
         assert (got.double() - want).norm() <= (2e-3 + 2.0 ** -8) * want.norm()
 
 
+def test_tiles_of_many_shapes_one_after_the_other():
+    """Workgroups that go from tile to tile through matrices of other sizes: sides that end inside a tile, an odd count of
+    stages, tall ones, one too small for the tile; one of them three times."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    sizes = [(1024, 4096)] * 3 + [(320, 20000), (5000, 450), (40, 3000), (700, 9000), (1000, 130)]
+    us = [torch.randn(*s, generator=g, device="cuda") for s in sizes]
+    us += [us[4]] * 2
+    results = fm.orthogonalize(us)
+    for u, got in zip(us, results):
+        want, tol = tolerance(u)
+        assert (got.double() - want).norm() <= tol + UNIT[got.dtype] * want.norm(), u.shape
+    assert torch.equal(results[4], results[-1]) and torch.equal(results[4], results[-2])
+
+
+@pytest.mark.parametrize("rows,cols", [(64, 1000), (100, 600), (190, 300), (256, 1024), (1000, 200), (250, 70)])
+def test_small_matrices_alone_and_among_many(rows, cols):
+    """Alone, B has no launch of its own; among forty it has. The same bits."""
+    u = matrix(rows, cols, "falling", 8).cuda()
+    alone = fm.orthogonalize(u)
+    check(alone, u)
+    assert all(torch.equal(o, alone) for o in fm.orthogonalize([u] * 40))
+
+
 def test_scales():
     """The result does not depend on the update's size, until its norm is below eps."""
     u = matrix(60, 90, "gauss", 5)

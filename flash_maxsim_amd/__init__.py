@@ -12,7 +12,11 @@ flash_maxsim_batched_topk, flash_maxsim_int8_topk), and training with doc
 lengths (flash_maxsim_train's doc_lengths) or several queries
 (flash_maxsim_train_batched). The layers that such training moves: layer norm
 (layer_norm), a linear layer with bias, activation and residual (linear), and
-AdamW with moments in 32 or 8 bits (AdamW, adamw_step).
+AdamW with moments in 32 or 8 bits (AdamW, adamw_step). The encoder block around
+them: ids to hidden states (embedding), the gated feed-forward's first half
+(gated_linear; linear is the second), the step between two blocks
+(residual_norm), and orthogonalised updates of its matrices (Muon, muon_step,
+orthogonalize).
 """
 
 __version__ = "0.1.0"

@@ -16,9 +16,9 @@
 // of a radix sort, of 2 launches each, by digits of up to 10 bits. Both for the whole gradient of a 30522 x 128 bf16 table,
 // us: 1024 tokens 19 / 31, 4096 22 / 41, 8192 27 / 43, 12288 37 / 44, 16384 48 / 45.
 //
-// 65536 tokens of a 131072 x 1024 bf16 table, few ids most of the tokens, us: the lookup 45 (134 MB written, 2.9 TB/s, the
-// few ids' rows out of the caches), the gradient 121: the sums 62 (134 MB of dy read row by row in the ids' order), the sort
-// 51, with 224 MB of zeros beside it (4.4 TB/s), the join 9. 32 tokens of 768: the lookup 3.4, a launch's own time.
+// 65536 tokens of a 131072 x 1024 bf16 table, few ids most of the tokens, us: the lookup 41 (134 MB written, 3.3 TB/s, the
+// few ids' rows out of the caches), the gradient 111: the sums 44 (134 MB of dy read row by row in the ids' order, 47 MB written,
+// 4.1 TB/s), the sort 57, with 224 MB of zeros beside it, the join 9. 32 tokens of 768: the lookup 3.4, a launch's own time.
 #include "fmx_device.h"
 #include "fmx_layers.h"
 #include "fmx_rows.h"

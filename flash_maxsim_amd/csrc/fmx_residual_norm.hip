@@ -14,10 +14,13 @@
 //
 // A row lives in the registers of one to eight waves between its sums and its outputs, 8 elements a lane in the backward
 // (its five column sums, four vectors of weights and two rows of five arrays spill at 16, which only rows of more than
-// 4096 elements take) and up to 16 in the forward; a workgroup's eight waves walk the rows in strides of the launch, the next row
-// (in the backward: two) loaded while this one is summed. 65536 x 1024 bf16 with both norms, gate and scale: forward 124 us (5.3 TB/s),
-// backward 207 (5.1 TB/s; one row ahead 243, in workgroups of four waves 278), the join of its sums 5. 32 x 768: 3.9. Variances are those of centred values, from registers. Rows may begin at any element: accesses of
-// 16 bytes need no more than an element's alignment here, and the last piece of an odd row is taken element by element.
+// 4096 elements take) and up to 16 in the forward; a workgroup's eight waves walk the rows in strides of the launch, the
+// next row (in the backward: the next two) loaded while this one is summed. Variances are those of centred values, from
+// registers. Rows may begin at any element: accesses of 16 bytes need no more than an element's alignment here, and the
+// last piece of an odd row is taken element by element.
+//
+// 65536 x 1024 bf16 with both norms, gate and scale: forward 124 us (5.3 TB/s), backward 207 (5.1 TB/s; loads one row ahead
+// 243, workgroups of four waves then 278), the join of its sums 5. 32 x 768: 3.9, a launch's own time.
 //
 // Weight gradients: a workgroup adds its waves' sums in LDS in the waves' order and writes one row of partial sums; a
 // second kernel adds those rows in a fixed order. No atomics.

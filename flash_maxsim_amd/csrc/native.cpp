@@ -22,6 +22,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
@@ -773,7 +774,24 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-struct GatedLinearBackward : public torch::autograd::Node {
+// A captured backward pass cannot hand gradients to nodes of the default stream, such as a leaf's that a graph built outside of
+// the capture keeps alive: the engine would make that stream wait for the capture, which ends the process. Refused before.
+struct BlockNode : public torch::autograd::Node {
+  void check_capture() const {
+    for (size_t i = 0; i < num_outputs(); ++i) {
+      const auto& to = next_edge(i).function;
+      if (!to || !task_should_compute_output(i)) continue;
+      const auto stream = to->stream();
+      if (!stream || stream->id() != 0) continue;  // 0: the default stream's
+      TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
+                  "flash_maxsim_amd: a backward pass is captured into a graph while a graph of the same tensors that was built on "
+                  "the default stream still lives; free it before the capture, or build it on another stream");
+      return;
+    }
+  }
+};
+
+struct GatedLinearBackward : public BlockNode {
   // x and the weights as the kernels read them; each is there where a wanted gradient needs it
   torch::autograd::SavedVariable x, wg, wu, factors;
   std::vector<int64_t> x_sizes;
@@ -783,6 +801,7 @@ struct GatedLinearBackward : public torch::autograd::Node {
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     const Tensor dy0 = grads[0];
     if (!dy0.defined()) return torch::autograd::variable_list(5);
+    check_capture();
     const bool again = c10::GradMode::is_enabled();
     Tensor keep, d[5];
     {
@@ -823,7 +842,7 @@ struct GatedLinearBackward : public torch::autograd::Node {
   std::string name() const override { return "FlashMaxSimGatedLinearBackward"; }
 };
 
-struct ResidualNormBackward : public torch::autograd::Node {
+struct ResidualNormBackward : public BlockNode {
   torch::autograd::SavedVariable rows[3], vectors[4], stats;  // x, residual, gate; weight, post weight, post bias, scale
   bool has[7];
   std::vector<int64_t> sizes;
@@ -836,6 +855,7 @@ struct ResidualNormBackward : public torch::autograd::Node {
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     const Tensor dh0 = grads[0], dy0 = grads[1];
     if (!dh0.defined() && !dy0.defined()) return torch::autograd::variable_list(8);
+    check_capture();
     const Tensor& like = dh0.defined() ? dh0 : dy0;
     const bool again = c10::GradMode::is_enabled();
     Tensor keep[2], out[8];
@@ -880,7 +900,7 @@ struct ResidualNormBackward : public torch::autograd::Node {
   std::string name() const override { return "FlashMaxSimResidualNormBackward"; }
 };
 
-struct EmbeddingBackward : public torch::autograd::Node {
+struct EmbeddingBackward : public BlockNode {
   torch::autograd::SavedVariable ids;
   at::ScalarType ids_type;
   int64_t T, V, d, padding;
@@ -890,6 +910,7 @@ struct EmbeddingBackward : public torch::autograd::Node {
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     const Tensor dy0 = grads[0];
     if (!dy0.defined() || !task_should_compute_output(0)) return torch::autograd::variable_list(1);
+    check_capture();
     const bool again = c10::GradMode::is_enabled();
     Tensor keep, dw;
     {

@@ -130,3 +130,36 @@ def test_one_block_and_its_step_in_a_graph(example):
         for name in captured[0].w:
             assert torch.equal(captured[0].master[name], eager[0].master[name]), name
             assert torch.equal(captured[0].w[name], eager[0].w[name]), name
+
+
+def test_captured_backward_beside_an_eager_graph():
+    """A leaf whose eager graph, built on the default stream, still lives: the captured backward is refused, and works once
+    that graph is gone. Gradients that are not wanted do not count."""
+    rows = lambda: torch.randn(8, 64, device="cuda", dtype=torch.float16)  # noqa: E731
+    x, w, table = rows(), rows(), torch.randn(20, 64, device="cuda")
+    ids = torch.randint(0, 20, (8,), device="cuda")
+    calls = {"gated": (lambda a, b: fm.gated_linear(a, b, b), rows(), w), "norm": (lambda a, b: fm.residual_norm(a, b)[1], rows(), x),
+             "embedding": (lambda a, b: fm.embedding(ids, a), table, w)}
+    for name, (call, leaf, other) in calls.items():
+        leaf, other = leaf.requires_grad_(True), other.detach().clone().requires_grad_(True)
+        dy = torch.ones_like(call(leaf, other))
+
+        def backward(leaf=leaf, call=call, other=other, dy=dy):
+            return torch.autograd.grad(call(leaf, other), leaf, dy)[0]
+
+        want = backward()
+        eager = call(leaf, other)
+        with pytest.raises(RuntimeError, match="still lives"), torch.cuda.graph(torch.cuda.CUDAGraph()):
+            backward()
+        assert torch.equal(backward(), want), name
+        del eager
+        only = call(leaf.detach(), other) if name != "embedding" else None  # holds the other's gradient alone
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = backward()
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), name
+            assert torch.equal(backward(), want), name
+        del only

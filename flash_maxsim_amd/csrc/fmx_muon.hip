@@ -747,7 +747,7 @@ __global__ void __launch_bounds__(256) muon_small_kernel(Table t, int copy_bf) {
 #pragma unroll
   for (int q = 0; q < 2 * NB; ++q)
     x[q] = ld16(rx, q * 32 < e.n ? (uint32_t)(((q * 32 + r) * (int64_t)e.m + ch * 8) * 2) : kOOB);
-  wait_vmem<2 * NB>();
+  wait_vmem<0>();
   stage_barrier();
 
   const Frags<false, false, 64> fi(wi * 32, lane), fj(wj * 32, lane);

@@ -139,7 +139,6 @@ def muon_step(params, grads, momenta, lr: float = 1e-3, momentum: float = 0.95, 
         if grad_scale.dtype != torch.float32:
             raise TypeError(f"grad_scale must be float32, got {grad_scale.dtype}")
     _no_tangents([*params, *grads, *momenta])
-    _apart([t for t in (*params, *momenta, *copies) if t is not None], grads)
     batches: dict = {}
     keep = []  # contiguous copies of gradients, until the launches
     for p, g, m, c in zip(params, grads, momenta, copies):
@@ -165,6 +164,7 @@ def muon_step(params, grads, momenta, lr: float = 1e-3, momentum: float = 0.95, 
             keep.append(g)
         row = _Matrix(p.data_ptr(), g.data_ptr(), m.data_ptr(), _lib.ptr(c), *p.shape)
         batches.setdefault((dev, p.dtype, g.dtype, None if c is None else c.dtype), []).append(row)
+    _apart([t for t in (*params, *momenta, *copies) if t is not None], grads)
     lib = _lib.load()
     for (dev, pt, gt, ct), rows in batches.items():
         table = (_Matrix * len(rows))(*rows)

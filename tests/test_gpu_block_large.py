@@ -96,6 +96,24 @@ def test_embedding():
     assert torch.equal(dw[:50], dy[:50]) and not any(t.any() for t in dw[50:V - 3000].split(1 << 20))
 
 
+@pytest.mark.parametrize("T", [9, 5000, 40000])
+@pytest.mark.parametrize("d,dtype", [(601, torch.float16), (299, torch.float32), (608, torch.bfloat16)])
+def test_embedding_gradient_past_the_caches(T, d, dtype):
+    """Tables whose gradient is stored past the caches, rows at any element."""
+    V = 200003
+    g = torch.Generator(device=DEV).manual_seed(T + d)
+    ids = torch.randint(V - 20000, V, (T,), generator=g, device=DEV)
+    ids[: T // 3] = 7
+    w = torch.empty(V, d, device=DEV, dtype=dtype).requires_grad_(True)
+    dy = torch.randn(T, d, generator=g, device=DEV).to(dtype)
+    (dw,) = torch.autograd.grad(fm.embedding(ids, w), w, dy)
+    want = torch.zeros(V, d, dtype=torch.float64, device=DEV).index_add_(0, ids, dy.double())
+    size = torch.zeros(V, d, dtype=torch.float64, device=DEV).index_add_(0, ids, dy.double().abs())
+    # the result's rounding, and float32 sums of fewer than T terms
+    u = torch.finfo(dtype).eps / 2
+    assert ((dw.double() - want).abs() <= u * want.abs() + F32 * T * size + 2.0 ** -25).all()
+
+
 def test_embedding_of_many_tokens():
     """T x d past 2^32: rows of dy and of y."""
     T, V, d = (1 << 22) + 333, 500, 1032

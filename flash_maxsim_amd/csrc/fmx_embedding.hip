@@ -46,17 +46,18 @@ __device__ __forceinline__ int32_t key_of(const EmbeddingArgs& a, int64_t t) {
 
 // ---- lookup ----
 
-// U rows of a thread at a time: their ids, then their rows, then the stores, each in flight together.
+// kAhead rows of a thread at a time: their ids, then their rows, then the stores, each in flight together. A workgroup's are
+// neighbours (4096 x 1024 bf16 6.5 -> 4.4 us, 16384 x 768 11.0 -> 9.3, larger ones equal, against rows a launch apart).
+constexpr int kAhead = 4;
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(256) embedding_kernel(EmbeddingArgs a, int lanes) {
-  constexpr int V = 16 / sizeof(T), U = 4;
+  constexpr int V = 16 / sizeof(T), U = kAhead;
   const int lane = threadIdx.x & (lanes - 1), rows = 256 / lanes;
-  const int64_t step = (int64_t)gridDim.x * rows;
-  for (int64_t t = (int64_t)blockIdx.x * rows + threadIdx.x / lanes; t < a.T; t += U * step) {
+  for (int64_t t = (int64_t)blockIdx.x * rows * U + threadIdx.x / lanes; t < a.T; t += (int64_t)gridDim.x * rows * U) {
     int64_t id[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t at = t + u * step < a.T ? t + u * step : t;
+      const int64_t at = t + u * rows < a.T ? t + u * rows : t;
       id[u] = a.ids64 ? static_cast<const int64_t*>(a.ids)[at] : (int64_t)static_cast<const int32_t*>(a.ids)[at];
     }
     for (int col = lane * V; col < a.d; col += lanes * V) {
@@ -69,7 +70,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(EmbeddingArgs a, int lan
         const bool there = id[u] >= 0 && id[u] < a.V;
 #pragma unroll
         for (int i = 0; i < V; ++i) p[u].v[i] = (T)(there ? (float)p[u].v[i] * a.scale : __builtin_nanf(""));
-        if (t + u * step < a.T) p[u].template store<WHOLE>(static_cast<T*>(a.out) + (t + u * step) * a.d + col, a.d - col);
+        if (t + u * rows < a.T) p[u].template store<WHOLE>(static_cast<T*>(a.out) + (t + u * rows) * a.d + col, a.d - col);
       }
     }
   }
@@ -388,7 +389,7 @@ hipError_t lookup(const EmbeddingArgs& a, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
   int lanes = 1;
   while (lanes < 256 && lanes * V < a.d) lanes *= 2;
-  const int64_t rows = 256 / lanes, want = (a.T + rows - 1) / rows, most = (int64_t)layer_cus() * 16;
+  const int64_t rows = 256 / lanes, want = (a.T + rows * kAhead - 1) / (rows * kAhead), most = (int64_t)layer_cus() * 16;
   const unsigned grid = (unsigned)(want < most ? want : most);
   if (a.d % V == 0)
     embedding_kernel<T, true><<<grid, 256, 0, s>>>(a, lanes);

@@ -18,7 +18,7 @@
 //
 // 65536 tokens of a 131072 x 1024 bf16 table, few ids most of the tokens, us: the lookup 41 (134 MB written, 3.3 TB/s, the
 // few ids' rows out of the caches), the gradient 111: the sums 44 (134 MB of dy read row by row in the ids' order, 47 MB written,
-// 4.1 TB/s), the sort 57, with 224 MB of zeros beside it, the join 9. 32 tokens of 768: the lookup 3.4, a launch's own time.
+// 4.1 TB/s), the sort 57, with 224 MB of zeros beside it, the join 9. 32 tokens of 768: the lookup 3.2, a launch's own time.
 #include "fmx_device.h"
 #include "fmx_layers.h"
 #include "fmx_rows.h"

@@ -16,8 +16,7 @@
 // (its five column sums, four vectors of weights and two rows of five arrays spill at 16, which only rows of more than
 // 4096 elements take) and up to 16 in the forward; a workgroup's eight waves walk the rows in strides of the launch, the
 // next row (in the backward: the next two) loaded while this one is summed. Variances are those of centred values, from
-// registers. Rows may begin at any element: accesses of 16 bytes need no more than an element's alignment here, and the
-// last piece of an odd row is taken element by element.
+// registers. Rows may begin at any element: accesses of 16 bytes need no more than an element's alignment here.
 //
 // 65536 x 1024 bf16 with both norms, gate and scale: forward 124 us (5.3 TB/s), backward 207 (5.1 TB/s; loads one row ahead
 // 243, workgroups of four waves then 278), the join of its sums 5. 32 x 768: 3.9, a launch's own time.
@@ -59,20 +58,43 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int wav
 }
 
 // Where a lane's elements lie: piece j of V elements at column ((j * NW + sub) * 64 + lane) * V, sub the wave's place
-// among the NW of its row. WHOLE: d is a multiple of V, no piece ends early.
+// among the NW of its row. WHOLE: d is a multiple of V, no piece ends early. Else the last piece begins at d - V and has some
+// of the columns of the one before it: both lanes compute the same there and store the same, and `in` leaves them out of
+// sums, by a factor (pieces that ended early, element by element, took twice as long: 65536 x 771 fp16, layer norms, forward
+// 182 us, backward 355; now 108 and 209, and 90 and 172 of 768 columns).
+// Rows of less than a piece end early.
 template <typename T, int NV, int NW, bool WHOLE>
 struct Cols {
   static constexpr int V = 16 / sizeof(T);
   using Row = Piece<T, V>[NV];
-  int col[NV], left[NV];
+  // the first half of the pieces is there in every lane: narrower rows have fewer waves or pieces (waves_of)
+  static constexpr int kFull = NV * V == 16 || NW > 1 ? NV / 2 : 0;
+  int col[NV], left[NV], again[WHOLE ? 1 : NV];  // again: of the columns before it
+  float mine[WHOLE ? 1 : NV - kFull][V];         // 1 where a column of these pieces is there and the lane's own, else 0
   __device__ __forceinline__ Cols(int wave, int lane, int d) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       col[j] = ((j * NW + wave % NW) * 64 + lane) * V;
       left[j] = d - col[j];
+      if constexpr (!WHOLE) {
+        again[j] = d >= V && left[j] > 0 && left[j] < V ? V - left[j] : 0;
+        col[j] -= again[j];
+        left[j] += again[j];
+        if (j >= kFull) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) mine[j - kFull][i] = in(j, i) ? 1.0f : 0.0f;
+        }
+      }
     }
   }
-  __device__ __forceinline__ bool in(int j, int i) const { return WHOLE ? left[j] > 0 : i < left[j]; }
+  // whether a column is there, and whether it is the lane's own
+  __device__ __forceinline__ bool has(int j, int i) const { return j < kFull || (WHOLE ? left[j] > 0 : i < left[j]); }
+  __device__ __forceinline__ bool in(int j, int i) const { return has(j, i) && (WHOLE || i >= again[j]); }
+  // A value as a row's sum takes it: zero where `in` is not. (Of a WHOLE row the caller's are zeros there, or it asks.)
+  __device__ __forceinline__ float own(int j, int i, float v) const {
+    if constexpr (WHOLE) return v;
+    return j < kFull ? v : v * mine[j < kFull ? 0 : j - kFull][i];
+  }
   // a row's elements; zeros past it, and everywhere without a row
   __device__ __forceinline__ void load(Row& x, const void* base, int64_t at, bool have) const {
     const T* row = static_cast<const T*>(base) + at;
@@ -97,7 +119,7 @@ struct Cols {
       Piece<W, V> p;
       p.template load<WHOLE>(w + col[j], left[j]);
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[j][i] = in(j, i) ? (float)p.v[i] : other;
+      for (int i = 0; i < V; ++i) o[j][i] = has(j, i) ? (float)p.v[i] : other;
     }
   }
   __device__ __forceinline__ void weights(float (&o)[NV][V], const void* w, int w32, float other) const {
@@ -153,7 +175,7 @@ __global__ void __launch_bounds__(kThreads) residual_norm_fwd_kernel(ResidualNor
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < V; ++i) s += h[j][i];
+        for (int i = 0; i < V; ++i) s += c.own(j, i, h[j][i]);
       mu = sum(s) * inv;
     }
     float sq = 0.0f;
@@ -161,8 +183,8 @@ __global__ void __launch_bounds__(kThreads) residual_norm_fwd_kernel(ResidualNor
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float e = h[j][i] - mu;
-        sq += c.in(j, i) ? e * e : 0.0f;
+        const float e = c.own(j, i, h[j][i] - mu);
+        sq += !WHOLE || c.has(j, i) ? e * e : 0.0f;
       }
     rs = 1.0f / sqrtf(sum(sq) * inv + a.eps);
   };
@@ -189,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) residual_norm_fwd_kernel(ResidualNor
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float q = a.gate ? k[j][i] * (float)g[j].v[i] : k[j][i];
-        h[j][i] = c.in(j, i) ? a.alpha * (float)r[j].v[i] + q * h[j][i] : 0.0f;
+        h[j][i] = !WHOLE || c.has(j, i) ? a.alpha * (float)r[j].v[i] + q * h[j][i] : 0.0f;
       }
     moments(mu2, rs2);
     if (row < a.M) {
@@ -261,7 +283,7 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
     const float mu1 = st[0], rs1 = st[1], mu2 = st[2], rs2 = st[3];
     const bool have = row < a.M;
     // Without a row all of these are zeros. Past a row's end dy, dh and what is added up are zeros, too, but for g, which
-    // the row's means would enter: it is the one that is masked.
+    // the row's means would enter: it is the one that is masked (of rows that are not WHOLE, what goes into sums is).
     float hh[NV][V], xh[NV][V], o[NV][V];  // hh: norm(h), then g; xh: norm(x), or x
     auto block = [&](int j, int i) { return POST ? xh[j][i] * pw[j][i] + pb[j][i] : xh[j][i]; };  // t
     float s1 = 0.0f, s2 = 0.0f;
@@ -275,7 +297,7 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
         const float n = (a.alpha * (float)r[j].v[i] + q * block(j, i) - mu2) * rs2;
         hh[j][i] = n;
         if (a.dy) {
-          const float d = (float)dy[j].v[i], wdy = d * w[j][i];
+          const float d = (float)dy[j].v[i], wdy = c.own(j, i, d * w[j][i]);
           s1 += wdy;
           s2 += wdy * n;
           total[kDw][j][i] += d * n;
@@ -294,7 +316,7 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
       for (int i = 0; i < V; ++i) {
         float e = a.dh ? (float)dh[j].v[i] : 0.0f;
         if (a.dy) e += rs2 * ((float)dy[j].v[i] * w[j][i] - c1 - hh[j][i] * c2);
-        e = c.in(j, i) ? e : 0.0f;
+        e = !WHOLE || c.has(j, i) ? e : 0.0f;
         hh[j][i] = e;
         const float f = a.gate ? e * (float)g[j].v[i] : e, q = f * k[j][i];
         total[kDscale][j][i] += f * block(j, i);
@@ -302,8 +324,9 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
           total[kDpw][j][i] += q * xh[j][i];
           total[kDpb][j][i] += q;
           o[j][i] = q * pw[j][i];
-          s1 += o[j][i];
-          s2 += o[j][i] * xh[j][i];
+          const float p = c.own(j, i, o[j][i]);
+          s1 += p;
+          s2 += p * xh[j][i];
         } else {
           o[j][i] = q;
         }
@@ -378,7 +401,7 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
 #pragma unroll
             for (int i = 0; i < V; ++i) {
               const int at = c.col[j] + i;
-              fold[at] = q ? fold[at] + total[s][j][i] : total[s][j][i];
+              if (WHOLE || c.in(j, i)) fold[at] = q ? fold[at] + total[s][j][i] : total[s][j][i];
             }
         }
         __syncthreads();

@@ -18,11 +18,12 @@
 // next row (in the backward: the next two) loaded while this one is summed. Variances are those of centred values, from
 // registers. Rows may begin at any element: accesses of 16 bytes need no more than an element's alignment here.
 //
-// 65536 x 1024 bf16 with both norms, gate and scale: forward 124 us (5.3 TB/s), backward 207 (5.1 TB/s; loads one row ahead
+// 65536 x 1024 bf16 with both norms, gate and scale: forward 124 us (5.3 TB/s), backward 205 (5.2 TB/s; loads one row ahead
 // 243, workgroups of four waves then 278), the join of its sums 5. 32 x 768: 3.9, a launch's own time.
 //
 // Weight gradients: a workgroup adds its waves' sums in LDS in the waves' order and writes one row of partial sums; a
-// second kernel adds those rows in a fixed order. No atomics.
+// second kernel adds those rows in a fixed order. No atomics. (The waves one after the other, in the columns' order with its
+// bank conflicts, took 11 of 24 us of 1537 x 771 fp16; now 16.5.)
 #include "fmx_device.h"
 #include "fmx_layers.h"
 #include "fmx_rows.h"
@@ -61,7 +62,7 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int wav
 // among the NW of its row. WHOLE: d is a multiple of V, no piece ends early. Else the last piece begins at d - V and has some
 // of the columns of the one before it: both lanes compute the same there and store the same, and `in` leaves them out of
 // sums, by a factor (pieces that ended early, element by element, took twice as long: 65536 x 771 fp16, layer norms, forward
-// 182 us, backward 355; now 108 and 209, and 90 and 172 of 768 columns).
+// 182 us, backward 355; now 108 and 203, and 90 and 170 of 768 columns).
 // Rows of less than a piece end early.
 template <typename T, int NV, int NW, bool WHOLE>
 struct Cols {
@@ -240,10 +241,12 @@ template <typename T, int NV, int NW, bool POST, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNormArgs a) {
   using C = Cols<T, NV, NW, WHOLE>;
   constexpr int V = C::V, NG = kWaves / NW;
-  constexpr int W = 64 * V * NV * NW;  // columns that the registers of a row hold
   constexpr int S = POST ? kSums : kDscale + 1;
+  // The workgroup's rows' sums meet in LDS: of each piece V rows of 64 lanes, 64 / V apart in banks, so that neither the lanes
+  // that write a row nor the threads that read columns in order fall in the same ones. Two sums take turns.
+  constexpr int P = 64 + 64 / V, PIECE = V * P, ROW = NV * NW * PIECE;
   __shared__ float red[2][2 * kWaves];
-  __shared__ float fold[NG > 1 ? W : 1];  // the workgroup's rows' sums meet here, one after the other
+  __shared__ float fold[2][NG > 1 ? NG * ROW : 1];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const C c(wave, lane, a.d);
@@ -390,24 +393,28 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
   if (!a.part) return;
   // wanted sums one behind the other, [parts][wanted][d]
   float* part = a.part + (int64_t)blockIdx.x * a.wanted * a.d;
+  int turn = 0;
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     if (!a.sums[s]) continue;
     if constexpr (NG > 1) {
-      for (int q = 0; q < NG; ++q) {
-        if (wave / NW == q) {
+      float* f = fold[turn & 1];
+      ++turn;
 #pragma unroll
-          for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const int at = c.col[j] + i;
-              if (WHOLE || c.in(j, i)) fold[at] = q ? fold[at] + total[s][j][i] : total[s][j][i];
-            }
-        }
-        __syncthreads();
-      }
-      for (int at = threadIdx.x; at < a.d; at += kThreads) part[at] = fold[at];
+        for (int i = 0; i < V; ++i)
+          f[wave / NW * ROW + (j * NW + wave % NW) * PIECE + i * P + lane] = total[s][j][i];
       __syncthreads();
+      for (int k = threadIdx.x; k < a.d; k += kThreads) {
+        const int piece = k / V, left = a.d - piece * V;
+        const int i = k % V + (!WHOLE && a.d >= V && left < V ? V - left : 0);  // in the lane that has it as its own
+        const float* at = f + piece / 64 * PIECE + i * P + piece % 64;
+        float t = at[0];
+#pragma unroll
+        for (int q = 1; q < NG; ++q) t += at[q * ROW];
+        part[k] = t;
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < NV; ++j)

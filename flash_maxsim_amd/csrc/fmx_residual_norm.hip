@@ -60,9 +60,10 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int wav
 
 // Where a lane's elements lie: piece j of V elements at column ((j * NW + sub) * 64 + lane) * V, sub the wave's place
 // among the NW of its row. WHOLE: d is a multiple of V, no piece ends early. Else the last piece begins at d - V and has some
-// of the columns of the one before it: both lanes compute the same there and store the same, and `in` leaves them out of
-// sums, by a factor (pieces that ended early, element by element, took twice as long: 65536 x 771 fp16, layer norms, forward
-// 182 us, backward 355; now 108 and 203, and 90 and 170 of 768 columns).
+// of the columns of the one before it: both lanes compute the same there and store the same, and `own` leaves them out of
+// sums by a mask of a value's bits: a factor of zero would make NaN of an infinity. (Pieces that ended early, element by
+// element: 65536 x 771 fp16, layer norms, forward 182 us, backward 355; with a factor 104 and 196, with the mask 109 and 200;
+// 82 and 147 of 768 columns.)
 // Rows of less than a piece end early.
 template <typename T, int NV, int NW, bool WHOLE>
 struct Cols {
@@ -71,7 +72,7 @@ struct Cols {
   // the first half of the pieces is there in every lane: narrower rows have fewer waves or pieces (waves_of)
   static constexpr int kFull = NV * V == 16 || NW > 1 ? NV / 2 : 0;
   int col[NV], left[NV], again[WHOLE ? 1 : NV];  // again: of the columns before it
-  float mine[WHOLE ? 1 : NV - kFull][V];         // 1 where a column of these pieces is there and the lane's own, else 0
+  uint32_t mine[WHOLE ? 1 : NV - kFull][V];      // all ones where a column of these pieces is there and the lane's own, else 0
   __device__ __forceinline__ Cols(int wave, int lane, int d) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -83,7 +84,7 @@ struct Cols {
         left[j] += again[j];
         if (j >= kFull) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) mine[j - kFull][i] = in(j, i) ? 1.0f : 0.0f;
+          for (int i = 0; i < V; ++i) mine[j - kFull][i] = in(j, i) ? ~0u : 0u;
         }
       }
     }
@@ -94,7 +95,8 @@ struct Cols {
   // A value as a row's sum takes it: zero where `in` is not. (Of a WHOLE row the caller's are zeros there, or it asks.)
   __device__ __forceinline__ float own(int j, int i, float v) const {
     if constexpr (WHOLE) return v;
-    return j < kFull ? v : v * mine[j < kFull ? 0 : j - kFull][i];
+    if (j < kFull) return v;
+    return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & mine[j < kFull ? 0 : j - kFull][i]);
   }
   // a row's elements; zeros past it, and everywhere without a row
   __device__ __forceinline__ void load(Row& x, const void* base, int64_t at, bool have) const {
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
         if (a.dy) {
           const float d = (float)dy[j].v[i], wdy = c.own(j, i, d * w[j][i]);
           s1 += wdy;
-          s2 += wdy * n;
+          s2 += wdy * c.own(j, i, n);
           total[kDw][j][i] += d * n;
           total[kDb][j][i] += d;
         }
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(kThreads) residual_norm_bwd_kernel(ResidualNor
           o[j][i] = q * pw[j][i];
           const float p = c.own(j, i, o[j][i]);
           s1 += p;
-          s2 += p * xh[j][i];
+          s2 += p * c.own(j, i, xh[j][i]);
         } else {
           o[j][i] = q;
         }

@@ -1064,7 +1064,7 @@ PyObject* residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// embedding(ids [...], weight [V, d], scale, padding): y [..., d]
+// embedding(ids [...], weight [V, d], scale, padding): y [..., d]; padding is a row of the table, or -1
 PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   FMX_ARGS(4);
@@ -1073,10 +1073,15 @@ PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int dtype = code_of(*w);
   const double scale = PyFloat_AS_DOUBLE(args[2]);
   const int64_t padding = PyLong_AsLongLong(args[3]), T = t->numel();
+  if (padding == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
   FMX_ORDINARY(dtype >= 0 && (t->scalar_type() == at::kLong || t->scalar_type() == at::kInt) && T > 0 && t->is_contiguous() &&
                w->dim() == 2 && w->size(0) >= 1 && w->size(1) >= 1 && (w->size(1) == 1 || w->stride(1) == 1) &&
                w->stride(0) >= 0 && t->device() == w->device() && here(*w) && !has_tangent(w));
   const int64_t V = w->size(0), d = w->size(1);
+  FMX_ORDINARY(padding >= -1 && padding < V);
   const bool grad = grad_wanted({w});
   auto sizes = t->sizes().vec();
   sizes.push_back(d);

@@ -88,8 +88,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
     rows of NaN (a launch cannot raise) and no gradient. Differentiable in
     weight, with a dense gradient; tokens of padding_idx add nothing to it.
     """
-    if padding_idx is None and math.isfinite(scale):
-        out = _lib.native().embedding(ids, weight, float(scale), -1)
+    if math.isfinite(scale) and (padding_idx is None or (type(padding_idx) is int and padding_idx >= 0)):
+        out = _lib.native().embedding(ids, weight, float(scale), -1 if padding_idx is None else padding_idx)
         if out is not None:
             return out
     _check(ids, weight, scale, padding_idx)

@@ -28,6 +28,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/python_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
@@ -561,6 +562,33 @@ Tensor given_back(const torch::autograd::SavedVariable& saved, const Tensor& dy,
   return t.clone(at::MemoryFormat::Contiguous);
 }
 
+// A captured backward pass cannot hand gradients to nodes of the default stream, such as a leaf's that a graph built outside of
+// the capture keeps alive: the engine would make that stream wait for the capture, which ends the process. Each backward calls
+// this before anything else, with its own node.
+void check_capture(const torch::autograd::Node& node) {
+  for (size_t i = 0; i < node.num_outputs(); ++i) {
+    const auto& to = node.next_edge(i).function;
+    if (!to || !node.task_should_compute_output(i)) continue;
+    const auto stream = to->stream();
+    if (!stream || stream->id() != 0) continue;  // 0: the default stream's
+    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
+                "flash_maxsim_amd: a backward pass is captured into a graph while a graph of the same tensors that was built on "
+                "the default stream still lives; free it before the capture, or build it on another stream");
+    return;
+  }
+}
+
+// refuse_capture(ctx): the same for an autograd function in Python, whose ctx is its node.
+PyObject* refuse_capture(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  FMX_ARGS(1);
+  TORCH_CHECK_TYPE(THPFunction_Check(args[0]), "refuse_capture takes an autograd function's ctx");
+  const auto node = reinterpret_cast<THPFunction*>(args[0])->cdata.lock();
+  if (node) check_capture(*node);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 struct LinearBackward : public torch::autograd::Node {
   // x and w as the kernels read them; each is there where a wanted gradient needs it: x for dw, w for dx
   torch::autograd::SavedVariable x, w, slope;
@@ -571,6 +599,7 @@ struct LinearBackward : public torch::autograd::Node {
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     const Tensor dy0 = grads[0];
     if (!dy0.defined()) return torch::autograd::variable_list(4);
+    check_capture(*this);
     const bool again = c10::GradMode::is_enabled();
     Tensor keep, dx, dw, db;
     {
@@ -621,6 +650,7 @@ struct LayerNormBackward : public torch::autograd::Node {
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     const Tensor dy0 = grads[0];
     if (!dy0.defined()) return torch::autograd::variable_list(3);
+    check_capture(*this);
     const bool again = c10::GradMode::is_enabled();
     Tensor keep, dx, dw, db;
     {
@@ -774,24 +804,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// A captured backward pass cannot hand gradients to nodes of the default stream, such as a leaf's that a graph built outside of
-// the capture keeps alive: the engine would make that stream wait for the capture, which ends the process. Refused before.
-struct BlockNode : public torch::autograd::Node {
-  void check_capture() const {
-    for (size_t i = 0; i < num_outputs(); ++i) {
-      const auto& to = next_edge(i).function;
-      if (!to || !task_should_compute_output(i)) continue;
-      const auto stream = to->stream();
-      if (!stream || stream->id() != 0) continue;  // 0: the default stream's
-      TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
-                  "flash_maxsim_amd: a backward pass is captured into a graph while a graph of the same tensors that was built on "
-                  "the default stream still lives; free it before the capture, or build it on another stream");
-      return;
-    }
-  }
-};
-
-struct GatedLinearBackward : public BlockNode {
+struct GatedLinearBackward : public torch::autograd::Node {
   // x and the weights as the kernels read them; each is there where a wanted gradient needs it
   torch::autograd::SavedVariable x, wg, wu, factors;
   std::vector<int64_t> x_sizes;
@@ -801,7 +814,7 @@ struct GatedLinearBackward : public BlockNode {
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     const Tensor dy0 = grads[0];
     if (!dy0.defined()) return torch::autograd::variable_list(5);
-    check_capture();
+    check_capture(*this);
     const bool again = c10::GradMode::is_enabled();
     Tensor keep, d[5];
     {
@@ -842,7 +855,7 @@ struct GatedLinearBackward : public BlockNode {
   std::string name() const override { return "FlashMaxSimGatedLinearBackward"; }
 };
 
-struct ResidualNormBackward : public BlockNode {
+struct ResidualNormBackward : public torch::autograd::Node {
   torch::autograd::SavedVariable rows[3], vectors[4], stats;  // x, residual, gate; weight, post weight, post bias, scale
   bool has[7];
   std::vector<int64_t> sizes;
@@ -855,7 +868,7 @@ struct ResidualNormBackward : public BlockNode {
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     const Tensor dh0 = grads[0], dy0 = grads[1];
     if (!dh0.defined() && !dy0.defined()) return torch::autograd::variable_list(8);
-    check_capture();
+    check_capture(*this);
     const Tensor& like = dh0.defined() ? dh0 : dy0;
     const bool again = c10::GradMode::is_enabled();
     Tensor keep[2], out[8];
@@ -900,7 +913,7 @@ struct ResidualNormBackward : public BlockNode {
   std::string name() const override { return "FlashMaxSimResidualNormBackward"; }
 };
 
-struct EmbeddingBackward : public BlockNode {
+struct EmbeddingBackward : public torch::autograd::Node {
   torch::autograd::SavedVariable ids;
   at::ScalarType ids_type;
   int64_t T, V, d, padding;
@@ -910,7 +923,7 @@ struct EmbeddingBackward : public BlockNode {
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     const Tensor dy0 = grads[0];
     if (!dy0.defined() || !task_should_compute_output(0)) return torch::autograd::variable_list(1);
-    check_capture();
+    check_capture(*this);
     const bool again = c10::GradMode::is_enabled();
     Tensor keep, dw;
     {
@@ -1216,7 +1229,7 @@ PyMethodDef methods[] = {FMX_METHOD(score),   FMX_METHOD(batched), FMX_METHOD(sp
                          FMX_METHOD(int8_packed), FMX_METHOD(forward), FMX_METHOD(backward),
                          FMX_METHOD(linear),  FMX_METHOD(layer_norm), FMX_METHOD(adamw),
                          FMX_METHOD(adamw_decode), FMX_METHOD(gated_linear), FMX_METHOD(residual_norm),
-                         FMX_METHOD(embedding),
+                         FMX_METHOD(embedding), FMX_METHOD(refuse_capture),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

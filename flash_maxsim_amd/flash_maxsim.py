@@ -204,6 +204,7 @@ class _FlashMaxSimFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_scores):
+        _lib.native().refuse_capture(ctx)
         Qk, Dk, argmax, lengths = ctx.saved_tensors
         d = ctx.d
         Nq, Lq = Qk.shape[:2]

@@ -63,6 +63,7 @@ class _EmbeddingFn(torch.autograd.Function):
     def backward(ctx, dy):
         if not ctx.needs_input_grad[1]:
             return None, None, None, None
+        _lib.native().refuse_capture(ctx)
         (ids,) = ctx.saved_tensors
         ids = ids.resolve_neg().contiguous()
         V, d = ctx.shape

@@ -82,6 +82,7 @@ class _GatedLinearFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _lib.native().refuse_capture(ctx)
         *operands, factors = ctx.saved_tensors
         # hooks on saved tensors may give them back in another layout
         xk, wg, wu = (None if t is None else _operand(t) for t in operands)

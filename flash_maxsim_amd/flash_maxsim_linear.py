@@ -90,6 +90,7 @@ class _LinearFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _lib.native().refuse_capture(ctx)
         xk, wk, slope = ctx.saved_tensors
         # hooks on saved tensors may give them back in another layout
         xk, wk = (None if t is None else _operand(t) for t in (xk, wk))

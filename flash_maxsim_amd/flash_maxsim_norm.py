@@ -83,6 +83,7 @@ class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _lib.native().refuse_capture(ctx)
         rows, weight, mean, rstd = ctx.saved_tensors
         M, d = rows.shape
         # hooks on saved tensors may give them back in another layout

@@ -96,6 +96,7 @@ class _ResidualNormFn(torch.autograd.Function):
     def backward(ctx, dh, dy):
         if dh is None and dy is None:
             return (None,) * 12
+        _lib.native().refuse_capture(ctx)
         x, r, g, w, pw, pb, scale, stats = ctx.saved_tensors
         d, (post, alpha, rms) = ctx.shape[-1], ctx.how
         # hooks on saved tensors may give them back in another layout

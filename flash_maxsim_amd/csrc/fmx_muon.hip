@@ -39,7 +39,11 @@ namespace {
 constexpr float kX = 256.0f, kA = 1024.0f;  // what X, and A and B, are held times
 constexpr int kMost = 40;                   // matrices of a launch: their table fits a kernel's arguments
 constexpr int kPad = 64;                    // X's sides in the workspace are multiples of this, the rest is zeros
-constexpr int kChunk = 8192;                // elements whose squares one workgroup adds up
+constexpr int kChunk = 8192;                // elements whose squares one workgroup adds up, or a multiple (chunk_of)
+// Sums of squares of a matrix at most: every workgroup that makes a tile of X adds all of them, 16 KB, four bytes an element of
+// the tile. (Without a bound the work grows with the square of the elements: all before the first step 931 us for
+// 8192 x 28672 bf16 and 268 ms for 4104 x 2^20; so 277 us and 7.2 ms.)
+constexpr int kSums = 2048;
 
 struct Entry {
   void* param;          // or the orthogonalised result
@@ -50,7 +54,7 @@ struct Entry {
   int32_t rows, cols;   // of the parameter
   int32_t n, m;         // of X, padded: n the shorter side
   float rate;
-  int32_t unused;
+  int32_t chunk;        // elements of a sum of squares
 };
 
 struct Table {
@@ -160,22 +164,24 @@ __global__ void __launch_bounds__(256) muon_momentum_kernel(Table t) {
   const int64_t size = (int64_t)e.rows * e.cols;
   const float scale = t.grad_scale ? *t.grad_scale : 1.0f;
   double sum = 0.0;
+  for (int part = 0; part < e.chunk; part += kChunk) {
 #pragma unroll
-  for (int v = 0; v < kChunk / 2048; ++v) {
-    const int64_t from = (int64_t)chunk * kChunk + v * 2048 + threadIdx.x * 8;
-    if (from >= size) break;
-    const int left = size - from < 8 ? (int)(size - from) : 8;
-    float g[8], m[8], u[8];
-    load8<G>(g, e.grad, from, left);
-    if (e.momentum) {
-      load8<FMX_DTYPE_F32>(m, e.momentum, from, left);
+    for (int v = 0; v < kChunk / 2048; ++v) {
+      const int64_t from = (int64_t)chunk * e.chunk + part + v * 2048 + threadIdx.x * 8;
+      if (from >= size) break;
+      const int left = size - from < 8 ? (int)(size - from) : 8;
+      float g[8], m[8], u[8];
+      load8<G>(g, e.grad, from, left);
+      if (e.momentum) {
+        load8<FMX_DTYPE_F32>(m, e.momentum, from, left);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m[k] = t.mu * m[k] + t.omu * (g[k] * scale);
-      store_past(e.momentum + from, left, m);
+        for (int k = 0; k < 8; ++k) m[k] = t.mu * m[k] + t.omu * (g[k] * scale);
+        store_past(e.momentum + from, left, m);
+      }
+      direction(u, g, m, t, e.momentum != nullptr, scale);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += k < left ? (double)u[k] * (double)u[k] : 0.0;
     }
-    direction(u, g, m, t, e.momentum != nullptr, scale);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) sum += k < left ? (double)u[k] * (double)u[k] : 0.0;
   }
   sums[threadIdx.x] = sum;
   __syncthreads();
@@ -195,7 +201,7 @@ __global__ void __launch_bounds__(256) muon_start_kernel(Table t) {
   const Entry& e = t.e[at];
   const uint32_t id = blockIdx.x - t.first[at], tj = (uint32_t)e.m / 64, ti = id / tj;
   const int i0 = (int)ti * 64, j0 = (int)(id - ti * tj) * 64;
-  const int64_t size = (int64_t)e.rows * e.cols, chunks = (size + kChunk - 1) / kChunk;
+  const int64_t size = (int64_t)e.rows * e.cols, chunks = (size + e.chunk - 1) / e.chunk;
   double sum = 0.0;
   for (int64_t k = threadIdx.x; k < chunks; k += 256) sum += squares_of(t, e)[k];
   sums[threadIdx.x] = sum;
@@ -917,12 +923,16 @@ hipError_t run_x(const Table& t, bool few, int copy_bf, hipStream_t s) {
   return few ? run_small<FORM, P>(t, copy_bf, s) : run_form<FORM, P>(t, copy_bf, s);
 }
 
+// Elements of a matrix's sum of squares: kChunk, or as many times that as keep to kSums sums.
+int32_t chunk_of(int64_t size) { return (int32_t)((size + (int64_t)kChunk * kSums - 1) / ((int64_t)kChunk * kSums) * kChunk); }
+int64_t chunks_of(const Entry& e) { return ((int64_t)e.rows * e.cols + e.chunk - 1) / e.chunk; }
+
 template <int G>
 hipError_t run_start(Table t, hipStream_t s) {
   uint32_t total = 0;
   for (int i = 0; i < t.count; ++i) {
     t.first[i] = total;
-    total += (uint32_t)(((int64_t)t.e[i].rows * t.e[i].cols + kChunk - 1) / kChunk);
+    total += (uint32_t)chunks_of(t.e[i]);
   }
   muon_momentum_kernel<G><<<total, 256, 0, s>>>(t);
   const hipError_t e = hipGetLastError();
@@ -937,8 +947,7 @@ hipError_t run_start(Table t, hipStream_t s) {
 }
 
 int64_t region(const Entry& e) {
-  const int64_t chunks = ((int64_t)e.rows * e.cols + kChunk - 1) / kChunk;
-  return (3 * x_bytes(e) + 2 * a_bytes(e) + chunks * 8 + 255) / 256 * 256;
+  return (3 * x_bytes(e) + 2 * a_bytes(e) + chunks_of(e) * 8 + 255) / 256 * 256;
 }
 
 Entry entry(const MuonMatrix& x) {
@@ -952,6 +961,7 @@ Entry entry(const MuonMatrix& x) {
   const int64_t n = x.rows < x.cols ? x.rows : x.cols, m = x.rows < x.cols ? x.cols : x.rows;
   e.n = (int32_t)((n + kPad - 1) / kPad * kPad);
   e.m = (int32_t)((m + kPad - 1) / kPad * kPad);
+  e.chunk = chunk_of(x.rows * x.cols);
   return e;
 }
 

@@ -111,3 +111,15 @@ def test_alone_and_among_others():
         alone = fm.orthogonalize(u)
         for others in (2, 9, 30):
             assert all(torch.equal(o, alone) for o in fm.orthogonalize([u] * others)), (shape, others)
+
+
+@pytest.mark.parametrize("shapes", [[(301, 60001)], [(60001, 301), (64, 300000)], [(130, 140000), (100, 30)]])
+def test_sums_of_squares_over_longer_chunks(shapes):
+    """More than 2^24 elements: a workgroup adds up the squares of several chunks, the last one's end early."""
+    for dtype, grad_dtype in ((torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32)):
+        kw = dict(lr=0.02, momentum=0.95, weight_decay=0.1, nesterov=True, adjust="original")
+        p, g, m = inputs(shapes, dtype, grad_dtype, 4)
+        P, M = [t.clone() for t in p], [t.clone() for t in m]
+        fm.muon_step(P, g, M, **kw)
+        for i in range(len(shapes)):
+            check(p[i], g[i], m[i], P[i], M[i], **kw)

@@ -13,7 +13,7 @@
 // id's tokens, whichever was stored last. The list is never cleared: an entry counts only if it names a token that has the id.
 //
 // Sorting: up to kRankMost tokens each counts the tokens before it (T^2 comparisons, one launch); more go through passes
-// of a radix sort, of 2 launches each, by digits of up to 10 bits. Both for the whole gradient of a 30522 x 128 bf16 table,
+// of a radix sort, of 2 launches each (3 of more than 2^18 tokens), by digits of up to 10 bits. Both for the whole gradient of a 30522 x 128 bf16 table,
 // us: 1024 tokens 19 / 31, 4096 22 / 41, 8192 27 / 43, 12288 37 / 44, 16384 48 / 45.
 //
 // 65536 tokens of a 131072 x 1024 bf16 table, few ids most of the tokens, us: the lookup 41 (134 MB written, 3.3 TB/s, the
@@ -33,6 +33,10 @@ constexpr int64_t kRankMost = 14336;
 constexpr int kRows = 64;            // ids of a workgroup that writes zeros
 constexpr int kBits = 10;            // of a digit, at most
 constexpr int kTile = 4096;          // tokens of a workgroup of the radix sort
+// A pass of more workgroups than this adds up their digits' counts in a launch of its own, fewer each for themselves, work that
+// grows with their square (rows of 8 bf16 elements, 100000 ids, each for itself / a launch, us: 2^15 tokens 46 / 52, 2^17 55 / 60,
+// 2^18 69 / 70, 2^19 98 / 95, 2^22 687 / 489, 2^24 5070 / 1810; 1000 ids, 2^26 tokens 81 ms / 6.2).
+constexpr int kScanFrom = 64;
 // A gradient of at least this many bytes is stored past the caches, which cannot hold it for its next reader (rows of 1024
 // bf16 elements, the gradient alone and with a reader after it, us, through the caches / past them: 49152 rows 51 and 80 / 51
 // and 82, 98304 59 and 135 / 65 and 141, 131072 118 and 209 / 92 and 195).
@@ -188,6 +192,36 @@ __global__ void __launch_bounds__(1024) embedding_count_kernel(EmbeddingArgs a, 
   if ((int)threadIdx.x < digits) counts[(int64_t)blockIdx.x * digits + threadIdx.x] = hist[threadIdx.x];
 }
 
+// The counts of each digit, [groups][digits], to those of the workgroups before, and their sum to the row behind them. A
+// workgroup has 32 digits, its threads 32 stretches of the groups.
+__global__ void __launch_bounds__(1024) embedding_scan_kernel(int32_t* counts, int groups, int digits) {
+  __shared__ int32_t sums[32][33];
+  const int digit = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
+  const int per = (groups + 31) / 32, from = part * per, end = from + per < groups ? from + per : groups;
+  int sum = 0;
+  if (digit < digits) {
+#pragma unroll 8
+    for (int g = from; g < end; ++g) sum += counts[(int64_t)g * digits + digit];
+  }
+  sums[part][threadIdx.x & 31] = sum;
+  __syncthreads();
+  if (digit >= digits) return;
+  int before = 0;
+  for (int p = 0; p < part; ++p) before += sums[p][threadIdx.x & 31];
+  constexpr int U = 8;  // counts in flight
+  for (int g = from; g < end; g += U) {
+    int n[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) n[u] = g + u < end ? counts[(int64_t)(g + u) * digits + digit] : 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (g + u < end) counts[(int64_t)(g + u) * digits + digit] = before;
+      before += n[u];
+    }
+  }
+  if (part == 31) counts[(int64_t)groups * digits + digit] = before;
+}
+
 // Tokens to their places of this pass, in their order before it: digits before, workgroups before, waves before (a
 // wave has kTile / 16 neighbouring tokens), tokens of the wave before. The workgroups after those of the tokens write
 // zeros, to the ids from `zeros` on.
@@ -201,7 +235,10 @@ __global__ void __launch_bounds__(1024) embedding_place_kernel(EmbeddingArgs a, 
   const int digits = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // how many tokens lie before this workgroup's of digit threadIdx.x
   int total = 0, before = 0;
-  if ((int)threadIdx.x < digits) {
+  if ((int)threadIdx.x < digits && groups > kScanFrom) {
+    total = counts[(int64_t)groups * digits + threadIdx.x];
+    before = counts[(int64_t)blockIdx.x * digits + threadIdx.x];
+  } else if ((int)threadIdx.x < digits) {
 #pragma unroll 8
     for (int g = 0; g < groups; ++g) {
       const int n = counts[(int64_t)g * digits + threadIdx.x];
@@ -425,7 +462,7 @@ Layout layout(int kind, int64_t T, int64_t V, int64_t d) {
   const bool radix = T > kRankMost;
   Layout l;
   l.keys = (T * 4 + 255) / 256 * 256;
-  l.counts = radix ? (T + kTile - 1) / kTile * (4 << kBits) : 0;
+  l.counts = radix ? ((T + kTile - 1) / kTile + 1) * (4 << kBits) : 0;
   l.seen = T ? (V * 4 + 255) / 256 * 256 : 0;
   l.part = stretches_of(T) * 2 * pitch * 4;
   l.total = (radix ? 4 : 2) * l.keys + l.counts + l.seen + l.part;
@@ -452,16 +489,19 @@ hipError_t gradient(int kind, EmbeddingArgs a, char* ws, hipStream_t s) {
       const int b = (bits - shift + passes - p - 1) / (passes - p), to = (p & 1) * 2, from = 2 - to;
       const int64_t z0 = rows * p / passes, zn = rows * (p + 1) / passes - z0;
       const unsigned grid = (unsigned)(groups + zn);
-      if (p == 0) {
+      if (p == 0)
         embedding_count_kernel<true><<<groups, 1024, 0, s>>>(a, shift, b, nullptr, counts);
+      else
+        embedding_count_kernel<false><<<groups, 1024, 0, s>>>(a, shift, b, lists[from], counts);
+      if (groups > kScanFrom)
+        embedding_scan_kernel<<<(unsigned)(((1 << b) + 31) / 32), 1024, 0, s>>>(counts, groups, 1 << b);
+      if (p == 0)
         embedding_place_kernel<true>
             <<<grid, 1024, 0, s>>>(a, shift, b, nullptr, nullptr, counts, groups, lists[to], lists[to + 1], z0 * kRows);
-      } else {
-        embedding_count_kernel<false><<<groups, 1024, 0, s>>>(a, shift, b, lists[from], counts);
+      else
         embedding_place_kernel<false>
             <<<grid, 1024, 0, s>>>(a, shift, b, lists[from], lists[from + 1], counts, groups, lists[to], lists[to + 1],
                                    z0 * kRows);
-      }
       a.keys = lists[to];
       a.order = lists[to + 1];
       shift += b;

@@ -11,6 +11,8 @@ from __future__ import annotations
 import pytest
 import torch
 
+import flash_maxsim_amd as fm
+from launches import launches
 from test_gpu_embedding import F32, SIZES, TYPES, UNIT, make, run
 
 pytestmark = pytest.mark.gpu
@@ -73,3 +75,24 @@ def test_whole_numbers_past_the_caches(T, d, dtype):
     want = torch.zeros(V, d, dtype=torch.float32, device="cuda").index_add_(0, ids, dy.float())  # exact, below 2^24
     assert want.abs().max() < 1 << 22
     assert torch.equal(run(ids, torch.zeros(V, d, dtype=dtype), dy)[1], want.to(dtype))
+
+
+@pytest.mark.parametrize("T,V,d,padding", [(262144, 1000, 8, None), (262145, 1000, 8, 3), (262145, 1, 5, None), (300001, 2, 4, 1),
+                                           (700000, 100000, 4, 7), (1000003, 3000000, 2, None), (4500000, 40, 2, 39)])
+def test_whole_numbers_of_many_tokens(T, V, d, padding):
+    """Around the count of tokens from which digits are added up in a launch of their own, one to three digits."""
+    ids = make(T, V, d, torch.float32, T + V, "frequent")[0]
+    dy = torch.randint(-4, 5, (T, d), generator=torch.Generator().manual_seed(T)).float()
+    keep = ids >= 0 if padding is None else ids != padding
+    want = torch.zeros(V, d, dtype=torch.int64).index_add_(0, ids[keep], dy[keep].long())
+    assert want.abs().max() < 1 << 22
+    assert torch.equal(run(ids, torch.zeros(V, d), dy, 1.0, padding)[1].cpu().long(), want)
+
+
+def test_digits_of_many_tokens_are_added_up_once(tmp_path):
+    """Not by every workgroup of a pass for itself: a launch in each of the two passes."""
+    for T, times in ((262144, 0), (262145, 2)):
+        ids, w = torch.arange(T, device="cuda") % 5000, torch.zeros(5000, 4, device="cuda", requires_grad=True)
+        dy = torch.ones(T, 4, device="cuda")
+        ran = launches(lambda: torch.autograd.grad(fm.embedding(ids, w), w, dy), tmp_path)
+        assert sum("embedding_scan_kernel" in name for name, _ in ran) == times

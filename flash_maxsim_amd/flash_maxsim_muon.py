@@ -57,13 +57,14 @@ def _check_sides(t: torch.Tensor) -> None:
 
 
 def _apart(written, read) -> None:
-    """No memory that is written is also another tensor's: a step reads gradients again after it has written momenta."""
+    """No memory that is written is also another tensor's: a step reads gradients and their scale again after it has
+    written momenta."""
     spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), w)
              for ts, w in ((written, True), (read, False)) for t in ts if t.numel() and t.is_contiguous()]
     end, end_written = 0, 0  # of all before, and of those that are written
     for first, last, w in sorted(spans):
         if first < (end if w else end_written):
-            raise ValueError("params, momenta and copies must not share memory with each other or with gradients")
+            raise ValueError("params, momenta and copies must not share memory with each other, with gradients or grad_scale")
         end, end_written = max(end, last), max(end_written, last) if w else end_written
 
 
@@ -124,7 +125,7 @@ def muon_step(params, grads, momenta, lr: float = 1e-3, momentum: float = 0.95, 
     parameters' shapes. grad_scale, a float32 value on the GPU, multiplies every
     gradient without a read back. copies, a list with a float16 or bfloat16 tensor
     (or None) for each parameter, receives the new float32 parameters rounded.
-    params, momenta and copies share no memory with each other or with gradients.
+    params, momenta and copies share no memory with each other, with gradients or with grad_scale.
     """
     if adjust not in ADJUST:
         raise ValueError(f"adjust={adjust!r} must be one of {list(ADJUST)}")
@@ -164,7 +165,7 @@ def muon_step(params, grads, momenta, lr: float = 1e-3, momentum: float = 0.95, 
             keep.append(g)
         row = _Matrix(p.data_ptr(), g.data_ptr(), m.data_ptr(), _lib.ptr(c), *p.shape)
         batches.setdefault((dev, p.dtype, g.dtype, None if c is None else c.dtype), []).append(row)
-    _apart([t for t in (*params, *momenta, *copies) if t is not None], grads)
+    _apart([t for t in (*params, *momenta, *copies) if t is not None], [*grads, *([] if grad_scale is None else [grad_scale])])
     lib = _lib.load()
     for (dev, pt, gt, ct), rows in batches.items():
         table = (_Matrix * len(rows))(*rows)

@@ -5,8 +5,10 @@
 // The gradient has no atomics on values: tokens are sorted by id (stable), so that the rows of an id lie in a fixed
 // order, and the sorted list is cut into stretches of kStretch tokens whatever their ids: a wave sums a stretch's
 // rows in registers and writes the ids that begin and end in it to dW; of an id that goes on past the
-// stretch's end it writes a float32 partial sum, and a second kernel adds an id's partial sums in order. So an id that
-// makes up half of the tokens costs no more than others.
+// stretch's end it writes a float32 partial sum, and a second kernel adds an id's partial sums in order. The sums so cost the
+// same whatever ids repeat; the join does not, for an id's partial sums are a workgroup's for each 256 columns (100000 x 1024
+// bf16, us of which the join, no id frequent / one id half of the tokens / all: 65536 tokens 104, 6 / 132, 31 / 145, 56;
+// 2^20 tokens 665, 99 / 1108, 515 / 1719, 1095).
 //
 // Rows of ids that do not occur get zeros from workgroups of their own, beside the radix sort's few (which leave the GPU
 // idle) or, where there is none, beside the sums. Which ids occur the first kernel notes: seen[id] is one of the

@@ -567,7 +567,9 @@ GatedPlan gated_plan(int64_t I, int64_t J, int64_t K, bool keep) {
   }
   // Where the factors are kept as well, three times the output, two workgroups a unit that cover each other's stores are
   // the better large tile (us, 256 x 128 / 192 x 64: training step 16384 x 1024 -> 2816 682 / 666, its forward alone
-  // 208 / 209: the power saved goes to the products after it; 8192 x 1024 -> 4096 without factors 124 / 130). The
+  // 208 / 209: the power saved goes to the products after it; 8192 x 1024 -> 4096 without factors 124 / 130; other training
+  // steps 8192 x 1024 -> 4096 492 / 476, 32768 x 768 -> 2304 915 / 891, 32768 x 768 -> 1152 483 / 464, 4096 x 2048 -> 5632
+  // 573 / 559, 65536 x 384 -> 1536 fp16 871 / 865, 8192 x 4096 -> 4096 1339 / 1358). The
   // tile alone changes, not the parts of k: y has the same bits with and without the factors.
   if (keep && best.tile == kTile256 && best.splits == 1) {
     best.tile = kTile192;

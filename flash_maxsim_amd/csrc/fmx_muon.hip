@@ -23,6 +23,9 @@
 // twice, the second time through transposing reads. Matrices taller than wide are transposed when X is made, and the
 // last product's epilogue, which moves the parameters, transposes back.
 //
+// 25 matrices, 24 of 1024 x 4096, a step: 2.63 ms with bf16 parameters and gradients, 2.93 with float32 parameters, bf16
+// gradients and copies, 2.98 with float32 gradients.
+//
 // A launch walks the tiles of up to kMost matrices of any shapes, from a table in its arguments: two for the momentum and X, three
 // a step (A, B, X), two where the matrices are small.
 #include <math.h>

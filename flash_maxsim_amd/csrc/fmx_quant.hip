@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(256) quantize_wide_kernel(QuantArgs a) {
 // non-temporal loads pass by (30 MB: d = 768 11.6 / 14.0, 1024 11.5 / 14.0, 4096 17.5 /
 // 22.4; 60 MB: d = 768 23 / 18, 1024 22 / 19), and from d = 1032 to 2048 at every size
 // measured (160 MB and 1 GB: d = 1536 34 / 49 and 223 / 264, 2048 35 / 47 and 213 / 252;
-// but d = 3072 1 GB 535 / 440).
+// wider rows 1 GB 535 / 440).
 template <int SRC>
 hipError_t dispatch_q(const QuantArgs& a, hipStream_t s) {
   const int chunks = (int)((a.d + 7) / 8);

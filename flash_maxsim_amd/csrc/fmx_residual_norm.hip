@@ -19,11 +19,13 @@
 // registers. Rows may begin at any element: accesses of 16 bytes need no more than an element's alignment here.
 //
 // 65536 x 1024 bf16 with both norms, gate and scale: forward 124 us (5.3 TB/s), backward 205 (5.2 TB/s; loads one row ahead
-// 243, workgroups of four waves then 278), the join of its sums 5. 32 x 768: 3.9, a launch's own time.
+// 243, workgroups of four waves then 278), the join of its sums 5. 32 x 768: 3.9, a launch's own time. 65536 x 768 without a
+// gate: fp16 82 and 147 us (4.9 and 4.1 TB/s: the backward's rows of 513 to 1023 columns have two waves with room for 1024), float32
+// 154 and 224 (5.2 and 5.4 TB/s).
 //
 // Weight gradients: a workgroup adds its waves' sums in LDS in the waves' order and writes one row of partial sums; a
 // second kernel adds those rows in a fixed order. No atomics. (The waves one after the other, in the columns' order with its
-// bank conflicts, took 11 of 24 us of 1537 x 771 fp16; now 16.5.)
+// bank conflicts, took 11 of 24 us of 1537 x 771 fp16; now 16.6.)
 #include "fmx_device.h"
 #include "fmx_layers.h"
 #include "fmx_rows.h"

@@ -14,6 +14,8 @@
 //                            the lower half would add there is (B - a I) times it, which is small but where X is large
 //   a I within B             4e-4 to 2.3e-3: the upper half's linear term is part of its product, exact but for the
 //                            rounding of B's diagonal, which scales rows and does not grow
+//                            (thousands of matrices of 1 to 8 rows, whose few errors do not average out: median 1.5e-3 to
+//                            2.6e-3, the largest 1.4e-2, of 2 x 2; of 16 rows and more 2.6e-3 at most)
 // so X lies in memory as two fp16 arrays, of which the lower one is read and written by the epilogue alone (X = B X_upper +
 // a X_lower): no product more. The last form saves the epilogue X's upper half (24 matrices of 1024 x 4096: 302 us a
 // launch, 364 with it read; B's diagonal's rest as a product of its own in the loop 448). X is held times

@@ -9,7 +9,9 @@ goes to a s + b s^3 + c s^5 a few times, which brings all of them near one: thre
 products a step on matrix instructions, over all matrices in one launch. Products
 take fp16 operands and float32 sums; the iterate is held as a pair of fp16
 values, so that small singular values, which grow by hundreds, do not drown in
-its rounding. The result is within about 2.5e-3 (of its norm) of the formula's.
+its rounding. The result is within about 2.5e-3 (of its norm) of the formula's where the
+shorter side is 16 or more; of shorter ones, whose few singular values' errors do not
+average out, the median is 2e-3 and the worst of some thousands 1.4e-2.
 Sums have a fixed order: the same inputs give the same bits.
 
 muon_step updates lists of matrices in place; Muon is the optimizer class over

@@ -611,8 +611,8 @@ typedef struct fmx_muon_matrix {
  *   `steps` times, X's shorter side first:  X = a X + (b X X^T + c (X X^T)^2) X
  *   p = p (1 - lr weight_decay) - lr f X,  f = sqrt(max(1, rows / cols)), with match_rms 0.2 sqrt(max(rows, cols))
  * Products on fp16 MFMA with fp32 sums, X held as a pair of fp16 values (the result is within about 2.5e-3 of the
- * formula's, by the root of the squares), everything else in fp32 (|u| in 64 bits); p is rounded once. Types as
- * fmx_adamw's. Deterministic. Workspace: fmx_muon_workspace_bytes, 256-byte aligned.
+ * formula's, by the root of the squares; where the shorter side is below 16 at times up to 1.4e-2), everything else in fp32
+ * (|u| in 64 bits); p is rounded once. Types as fmx_adamw's. Deterministic. Workspace: fmx_muon_workspace_bytes, 256-byte aligned.
  */
 int fmx_muon(int param_dtype, int grad_dtype, int copy_dtype, const fmx_muon_matrix* matrices, int64_t count, double lr,
              double momentum, int nesterov, double weight_decay, int steps, double a, double b, double c, double eps,
